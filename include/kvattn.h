@@ -1,6 +1,6 @@
 /*
  * kvattn.h — C ABI of libkvattn.so, the MI355X (gfx950) full-attention
- * KV-cache path: paged FP16 K/V cache, fused QK-RMSNorm + RoPE + K/V append,
+ * KV-cache path: paged FP16 or 8-bit K/V cache, fused QK-RMSNorm + RoPE + K/V append,
  * split-K GQA decode, chunked causal prefill and tree-verify attention.
  *
  * Conventions (the reference's host wrappers use the same ones):
@@ -59,6 +59,27 @@ enum {
 
 /* Cache flags. */
 #define KVA_FLAG_HOST_ONLY 0x1u /* no device memory: host bookkeeping only  */
+/* An 8-bit cache: half the memory, and half the bytes of an attention step.
+ * A full block (a KV head's share of a page: 16 rows of 256 values, K and V
+ * apart) is held as codes c in [-127, 127] and one scale s; a value is c*s.
+ * s is the smallest m*2^e with m in 8..15 and e >= -24 for which 127*s covers
+ * the block's largest magnitude, at most 512, and c is x/s rounded to the
+ * nearest (ties to even): c*s is an fp16 number, at most s/2 from x while
+ * |x| <= 65024.  A sequence's last page, until its sixteenth row arrives, is
+ * held in fp16 as it came (32 KB per sequence slot, KV head and layer), so
+ * codes depend on a page's rows alone, not on the steps that they came in.
+ * A row of a head in which K or V is not finite reads as NaN keys and zero
+ * values, and once its page is full every row of that block has NaN keys:
+ * attention that sees such a row gives NaN.  All calls of a step are the same
+ * as on an fp16 cache but those that address or move rows, which return
+ * KVA_ERR_UNSUPPORTED: kva_layer_pools, kva_row_ptr, tree_bits in
+ * kva_step_begin, kva_tree_verify, a kva_rollback that moves rows, and
+ * kva_timeline_enable.  kva_seq_set_len goes up only to rows that were
+ * written; set back into a full page, that page's rows continue from the
+ * values its codes stand for.  kva_seq_set_blocks leaves a last page that is
+ * not full with the sequence.  Recorded appends take one new token per
+ * sequence.                                                                 */
+#define KVA_FLAG_INT8 0x2u
 
 /*
  * Cache configuration.  Replaces the constructor arguments of
@@ -164,6 +185,20 @@ int kva_append_qknorm_rope(kva_cache *cache, int32_t layer, void *q, void *k,
                            const void *v, const void *q_norm_w, const void *k_norm_w,
                            const void *cos_tab, const void *sin_tab, int32_t table_rows,
                            kva_stream_t stream);
+/* The step's K/V rows as they are: k, v [T, num_kv_heads, 256] fp16 in step
+ * token order (normalised and rotated already, e.g. rows that kva_read_rows
+ * gave, of this cache or another), only read.  The reference's append_kv_gpu
+ * (engine.py:199-218) for all rows of a step.                              */
+int kva_append_rows(kva_cache *cache, int32_t layer, const void *k, const void *v, kva_stream_t stream);
+/* Rows [first[b], first[b] + count[b]) of each sequence seq_ids[b], packed in
+ * that order: k_out, v_out [sum of count, num_kv_heads, 256] fp16, the values
+ * that the cache holds (16-byte aligned).  No counterpart in the reference,
+ * whose callers read the contiguous cache by address.  The index arrays are
+ * host arrays; a sequence may be listed more than once.  Needs no step; not
+ * while a graph is recorded.                                               */
+int kva_read_rows(kva_cache *cache, int32_t layer, int32_t n_seqs, const int32_t *seq_ids,
+                  const int32_t *first, const int32_t *count, void *k_out, void *v_out,
+                  kva_stream_t stream);
 /* The Q/K/V projection of every new token of the step, fused with the
  * append above: the producer side of the cache.  Replaces the FP16
  * attention projections (gemv_fp16_v2, gemv_fp16_v2.hip:22-85) launched at

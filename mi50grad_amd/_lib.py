@@ -18,6 +18,7 @@ LIB_PATH = Path(os.environ["KVA_LIB"]).resolve() if os.environ.get("KVA_LIB") \
     else Path(__file__).resolve().with_name("libkvattn.so")
 
 KVA_FLAG_HOST_ONLY = 0x1
+KVA_FLAG_INT8 = 0x2
 ERROR_NAMES = {
     -1: "KVA_ERR_INVALID_ARG", -2: "KVA_ERR_UNSUPPORTED", -3: "KVA_ERR_NO_DEVICE",
     -4: "KVA_ERR_OUT_OF_BLOCKS", -5: "KVA_ERR_CAPACITY", -6: "KVA_ERR_BAD_SEQ",
@@ -71,6 +72,8 @@ SIGNATURES = {
     "kva_sync_tables": [_P, _P],
     "kva_step_begin": [_P, _I, _PI, _PI, _PI, POINTER(c_uint64), _P],
     "kva_append_qknorm_rope": [_P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _P],
+    "kva_append_rows": [_P, _I, _P, _P, _P],
+    "kva_read_rows": [_P, _I, _I, _PI, _PI, _PI, _P, _P, _P],
     "kva_project_append": [_P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P],
     "kva_out_project": [_P, _P, _I, _I, _P, _I, _P, _P, _P],
     "kva_decode": [_P, _I, _P, _P, _P],

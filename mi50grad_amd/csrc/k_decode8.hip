@@ -1,0 +1,300 @@
+// GQA decode attention over the 8-bit cache (gfx950).
+//
+// out = softmax(q K^T / 16) V per query head over the values that the cache
+// stands for (k_page8.h), as decode over the FP16 cache, with half its bytes.
+// Stream-K over pages as there (k_walk.h): workgroup w walks the w-th share of
+// the pages of all sequences, one wave per KV head; a sequence that the share
+// holds whole is written out, a cut one leaves partials for the merge.
+//
+// A block is 8 KB in operand order, so a wave brings it in as eight 1 KB loads
+// that write LDS directly (and one of its scales), through a ring of its own:
+// no wave waits for another, and no register is held by a load in flight.
+//   QK: S^T = K Q^T on 16x16x32 products, the codes as A (integers, exact),
+//       the G query rows as columns of B; the block's scale goes into the
+//       softmax's factor;
+//   softmax: on the C layout (lane: head column l % 16, rows 4 (l / 16) .. + 3),
+//       where four probabilities are already the B operand of
+//   PV: O^T[dim][head] += V^T P^T on 16x16x16 products, V as values (code times
+//       scale, exact in FP16).
+// Both products run on the matrix unit: on the vector unit, as the FP16
+// decode's PV, the conversion of the codes would come on top of six heads' sums.
+#include "k_common.h"
+#include "k_page8.h"
+#include "k_walk.h"
+#include "kva_internal.h"
+
+namespace kva {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kQkScale = kLog2e / 16.0f;
+// A column's reference max moves only when a block's passes it by more than
+// this (log2 units): probabilities stay below 2^8, which FP16 holds to the same
+// relative precision, and the accumulators are rescaled rarely.
+constexpr float kSlack = 8.0f;
+constexpr int kRing = 4;                              // blocks of LDS per wave
+constexpr int kSlotBytes = 2 * kPageElems + 256;      // K, V, scales (one dword a lane)
+constexpr int kLoads = 9;                             // vector loads of a block
+
+__device__ __forceinline__ half8_t as_h8(uint4 v) { return __builtin_bit_cast(half8_t, v); }
+__device__ __forceinline__ half4_t as_h4(uint2 v) { return __builtin_bit_cast(half4_t, v); }
+
+// m: the reference max of this lane's head column, in log2 units; l: the
+// FP16 probabilities of this lane's rows summed; acc: dims 16 t + 4 (l / 16) .. +
+// 3 of the column's head.
+struct State {
+    float m, l;
+    float4_t acc[16];
+};
+__device__ __forceinline__ void reset(State &st) {
+    st.m = -INFINITY;
+    st.l = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 16; ++t) st.acc[t] = float4_t{0.f, 0.f, 0.f, 0.f};
+}
+
+// Scores x (log2 units, masked ones -inf) of this lane's four rows to
+// probabilities as the B operand.
+__device__ __forceinline__ half4_t fold_scores(State &st, const float4_t &x) {
+    constexpr uint32_t kOnes = 0x3c003c00u;  // FP16 pair (1, 1)
+    const float mx = group4_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+    const bool jump = mx > st.m + kSlack;
+    if (__builtin_amdgcn_ballot_w64(jump)) {
+        const float mn = jump ? mx : st.m;
+        // From -inf, acc and l are zero; a column of NaN scores stays at -inf.
+        const float corr = st.m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.m - mn);
+        st.l *= corr;
+#pragma unroll
+        for (int t = 0; t < 16; ++t) st.acc[t] *= corr;
+        st.m = mn;
+    }
+    const float mu = st.m == -INFINITY ? 0.0f : st.m;
+    const uint32_t p0 = pack_p2(__builtin_amdgcn_exp2f(x[0] - mu), __builtin_amdgcn_exp2f(x[1] - mu));
+    const uint32_t p1 = pack_p2(__builtin_amdgcn_exp2f(x[2] - mu), __builtin_amdgcn_exp2f(x[3] - mu));
+    st.l = dot2(p1, kOnes, dot2(p0, kOnes, st.l));  // l sums the FP16 probabilities PV uses
+    return as_h4(make_uint2(p0, p1));
+}
+
+// A full block from LDS.
+__device__ __forceinline__ void fold_block(State &st, const uint8_t *slot, const uint4 (&qb)[8], int lane) {
+    const float2 sc = *reinterpret_cast<const float2 *>(slot + 2 * kPageElems);
+    float4_t s[2] = {float4_t{0.f, 0.f, 0.f, 0.f}, float4_t{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(slot + 1024 * i + 16 * lane);
+        s[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(codes8(w.x, w.y)), as_h8(qb[2 * i]), s[0], 0, 0, 0);
+        s[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(codes8(w.z, w.w)), as_h8(qb[2 * i + 1]), s[1], 0, 0, 0);
+    }
+    const half4_t p = fold_scores(st, (s[0] + s[1]) * (sc.x * kQkScale));
+    const uint32_t vs = scale_h2(sc.y);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(slot + kPageElems + 1024 * j + 16 * lane);
+        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            st.acc[4 * j + t] = __builtin_amdgcn_mfma_f32_16x16x16f16(as_h4(values4(ws[t], vs)), p, st.acc[4 * j + t], 0, 0, 0);
+    }
+}
+
+// The open block: `lim` FP16 rows (1..15) in page order; what lies behind them
+// is stale, so its scores are masked and its values zeroed.
+__device__ __forceinline__ void fold_open(State &st, const uint16_t *open, const uint4 (&qb)[8], int lane, int lim) {
+    const int grp = lane >> 4;
+    float4_t s[2] = {float4_t{0.f, 0.f, 0.f, 0.f}, float4_t{0.f, 0.f, 0.f, 0.f}};
+    uint4 k[8], v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) k[i] = ld16(open + 1024 * (i >> 1) + 16 * lane + 8 * (i & 1));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = ld16(open + kPageElems + 1024 * (i >> 1) + 16 * lane + 8 * (i & 1));
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        s[i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(k[i]), as_h8(qb[i]), s[i & 1], 0, 0, 0);
+    float4_t x = (s[0] + s[1]) * kQkScale;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = 4 * grp + i < lim ? x[i] : -INFINITY;
+    const half4_t p = fold_scores(st, x);
+    const uint32_t m0 = (4 * grp < lim ? 0xffffu : 0u) | (4 * grp + 1 < lim ? 0xffff0000u : 0u);
+    const uint32_t m1 = (4 * grp + 2 < lim ? 0xffffu : 0u) | (4 * grp + 3 < lim ? 0xffff0000u : 0u);
+#pragma unroll
+    for (int t = 0; t < 16; ++t) {
+        const uint4 w = v[t >> 1];  // dim tiles 2i, 2i + 1
+        const uint2 y = (t & 1) ? make_uint2(w.z & m0, w.w & m1) : make_uint2(w.x & m0, w.y & m1);
+        st.acc[t] = __builtin_amdgcn_mfma_f32_16x16x16f16(as_h4(y), p, st.acc[t], 0, 0, 0);
+    }
+}
+
+// B operand: query head col of the group (zero past G), k-step 2i + e holding
+// dims 64 i + 16 (l / 16) + 8 e .. + 7.
+__device__ __forceinline__ void load_query(uint4 (&qb)[8], const uint16_t *q, int G, int lane) {
+    const int col = lane & 15, grp = lane >> 4;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+        qb[k] = col < G ? ld16(q + col * kHeadDim + 64 * (k >> 1) + 16 * grp + 8 * (k & 1)) : make_uint4(0, 0, 0, 0);
+}
+
+// Eight loads of a block and one of its scales to a slot; off: the same
+// loads through empty resources.
+__device__ __forceinline__ void issue_block(uint32_t slot, const uint8_t *k, const uint8_t *v, const float *scales,
+                                            bool on, int lane) {
+    const auto rk = ro_rsrc(k, on ? kPageElems : 0u), rv = ro_rsrc(v, on ? kPageElems : 0u);
+    const auto rs = ro_rsrc(scales, on ? 8u : 0u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) load_to_lds_at(rk, slot + 1024 * i, 16 * lane, 1024 * i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) load_to_lds_at(rv, slot + kPageElems + 1024 * i, 16 * lane, 1024 * i);
+    touch_line(rs, slot + 2 * kPageElems, 4 * (lane & 1), 0);
+}
+
+__global__ __launch_bounds__(64 * kDecodeHeadsPerWg) void decode8_kernel(Decode8Args e) {
+    const DecodeArgs &a = e.d;
+    extern __shared__ __attribute__((aligned(16))) uint8_t ring[];  // [waves][kRing][kSlotBytes]
+    const int w = blockIdx.x;
+    int P, W;
+    stream_k_shape(a, P, W);
+    if (w >= W) return;
+    const int p_begin = wg_start(w, P, W);
+    const int p_end = wg_start(w + 1, P, W);
+    if (p_begin >= p_end) return;
+    const int hkv = a.num_kv_heads, nh = a.num_heads, G = nh / hkv;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int h = __builtin_amdgcn_readfirstlane(blockIdx.y * (blockDim.x >> 6) + wave);
+    const int lane = threadIdx.x & 63;
+    const int col = lane & 15, grp = lane >> 4;
+    uint8_t *mine = ring + static_cast<size_t>(wave) * kRing * kSlotBytes;
+
+    // The first sequence of the share: the last with pages before it <= p_begin.
+    int b0 = 0;
+    for (int c0 = 0; c0 < a.n_seqs; c0 += 64) {
+        const int i = c0 + lane;
+        const uint64_t before = __ballot((i < a.n_seqs ? a.pre_seq[i + 1] : INT32_MAX) <= p_begin);
+        b0 += __popcll(before);
+        if (before != ~0ull) break;
+    }
+    b0 = __builtin_amdgcn_readfirstlane(b0);
+    SeqWindow win;
+    load_window(win, a, b0, lane);
+
+    auto next = [&](Cursor c) -> Cursor {
+        if (!c.ok) return c;
+        if (c.base + c.pg + 1 >= p_end) {
+            c.ok = false;
+            return c;
+        }
+        if (c.pg + 1 < c.npg) {
+            ++c.pg;
+            return c;
+        }
+        int b = c.b;
+        do {
+            ++b;
+            if (b - win.b0 >= 64) load_window(win, a, b, lane);
+            c = seq_cursor(win, b);
+        } while (c.npg == 0);
+        return c;
+    };
+    auto page_id = [&](const Cursor &c) -> int {
+        return ld_uniform(a.table + static_cast<size_t>(c.sid) * a.table_stride + c.pg);
+    };
+    auto is_open = [](const Cursor &c) { return c.pg == (c.ctx >> 4); };  // rows ctx & 15 > 0 of it
+    auto issue = [&](int slot, const Cursor &c, int id) {
+        const size_t blk = static_cast<size_t>(id) * hkv + h;
+        issue_block(lds_addr(mine + slot * kSlotBytes), e.k8 + blk * kPageElems, e.v8 + blk * kPageElems,
+                    e.scales + 2 * blk, c.ok && !is_open(c), lane);
+    };
+
+    uint4 qb[8];
+    auto query = [&](int b) { load_query(qb, a.q + (static_cast<size_t>(b) * nh + h * G) * kHeadDim, G, lane); };
+    State st;
+    reset(st);
+    auto finish = [&](const Cursor &c) {
+        const float lt = group4_sum(st.l);  // the four lane groups hold disjoint rows
+        if (col >= G) return;
+        if (c.base >= p_begin && c.base + c.npg <= p_end) {
+            const float inv = 1.0f / lt;
+            uint16_t *o = a.out + (static_cast<size_t>(c.b) * nh + h * G + col) * kHeadDim + 4 * grp;
+            const uint16_t *g =
+                a.gate ? a.gate + static_cast<int64_t>(c.b) * a.gate_stride + (h * G + col) * kHeadDim + 4 * grp : nullptr;
+#pragma unroll
+            for (int t = 0; t < 16; ++t)
+                *reinterpret_cast<uint2 *>(o + 16 * t) =
+                    out_fp16x4(st.acc[t][0] * inv, st.acc[t][1] * inv, st.acc[t][2] * inv, st.acc[t][3] * inv,
+                               g ? g + 16 * t : nullptr);
+        } else {
+            const int slot = 2 * w + (c.b == b0 ? 0 : 1);
+            const size_t u = (static_cast<size_t>(slot) * hkv + h) * G + col;
+#pragma unroll
+            for (int t = 0; t < 16; ++t)
+                *reinterpret_cast<float4_t *>(a.ws_acc + u * kHeadDim + 16 * t + 4 * grp) = st.acc[t];
+            if (grp == 0) {
+                a.ws_ml[u * 2] = st.m;
+                a.ws_ml[u * 2 + 1] = lt;
+            }
+        }
+    };
+
+    // Cursors cq[0] (folded in now) .. cq[kRing - 1] (issued now), and the
+    // page after that, whose id is fetched a block ahead.
+    Cursor cq[kRing];
+    cq[0] = seq_cursor(win, b0);
+    cq[0].pg = p_begin - cq[0].base;
+    query(b0);
+#pragma unroll
+    for (int i = 1; i < kRing; ++i) cq[i] = next(cq[i - 1]);
+    int id = page_id(cq[0]);
+#pragma unroll
+    for (int i = 0; i + 1 < kRing; ++i) {
+        issue(i, cq[i], id);
+        if (cq[i + 1].ok) id = page_id(cq[i + 1]);
+    }
+    int n = 0;
+    while (true) {
+        // Slot n - 1's last reads have returned: it is issued over.
+        __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));  // lgkmcnt(0)
+        __builtin_amdgcn_sched_barrier(0);
+        issue((n + kRing - 1) % kRing, cq[kRing - 1], id);
+        const Cursor after = next(cq[kRing - 1]);
+        if (after.ok) id = page_id(after);
+        wait_vm<kLoads * (kRing - 1)>();
+        __builtin_amdgcn_sched_barrier(0);
+        const Cursor cur = cq[0];
+        if (is_open(cur))
+            fold_open(st, e.open + (static_cast<size_t>(cur.sid) * hkv + h) * 2 * kPageElems, qb, lane, cur.ctx & 15);
+        else
+            fold_block(st, mine + (n % kRing) * kSlotBytes, qb, lane);
+        const bool more = cq[1].ok;
+        if (!more || cq[1].b != cur.b) {
+            finish(cur);
+            if (!more) break;
+            query(cq[1].b);
+            reset(st);
+        }
+#pragma unroll
+        for (int i = 0; i + 1 < kRing; ++i) cq[i] = cq[i + 1];
+        cq[kRing - 1] = after;
+        ++n;
+    }
+    // Loads past the share write LDS too: none may land after it is handed on.
+    __builtin_amdgcn_s_waitcnt(0);
+}
+
+}  // namespace
+
+hipError_t launch_decode8(const Decode8Args &a, hipStream_t s) {
+    const DecodeArgs &d = a.d;
+    if (d.n_seqs <= 0) return hipSuccess;
+    int hpw = d.num_kv_heads <= kDecodeHeadsPerWg ? d.num_kv_heads : kDecodeHeadsPerWg;
+    while (d.num_kv_heads % hpw) --hpw;
+    const size_t lds = static_cast<size_t>(hpw) * kRing * kSlotBytes;
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(decode8_kernel),
+                                       hipFuncAttributeMaxDynamicSharedMemorySize,
+                                       kDecodeHeadsPerWg * kRing * kSlotBytes);
+    if (e != hipSuccess) return e;
+    if (d.ev_before && (e = hipEventRecord(d.ev_before, s)) != hipSuccess) return e;
+    hipLaunchKernelGGL(decode8_kernel, dim3(d.n_wg, d.num_kv_heads / hpw), dim3(64 * hpw), lds, s, a);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    if (d.ev_after && (e = hipEventRecord(d.ev_after, s)) != hipSuccess) return e;
+    return launch_decode_merge(d, s);
+}
+
+}  // namespace kva

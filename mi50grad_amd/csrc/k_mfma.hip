@@ -46,7 +46,16 @@
 //       ds_read_b64_tr_b16 from the row-major V tile; 16 dim tiles).
 // The k-index permutation of P^T (keys 4g..4g+3 and 16+4g..16+4g+3 in lane
 // group g) is matched by the V^T reads, so the sum is over the right pairs.
+//
+// Over the 8-bit cache (Q8; causal steps) the same, but a block comes in
+// through registers: its codes (half the bytes, k_page8.h) are converted once
+// per workgroup, each wave its share, and put into LDS as operands, K as integers
+// (the blocks' scales go to the scores), V as values.  Two stages: while block i
+// is multiplied, block i+1's conversion has been written and block i+2's codes
+// are on their way.  Page order makes every access linear, so nothing is padded
+// or swapped and V needs no transposing read.
 #include "k_common.h"
+#include "k_page8.h"
 #include "kva_internal.h"
 
 namespace kva {
@@ -103,6 +112,7 @@ struct Unit {
     int b, h, tile;       // sequence (index in the step), kv head, query tile
     int ctx, ns, tok, T;  // keys visible, first new slot, first token, new tokens
     const int32_t *trow;  // block-table row
+    int sid;              // cache slot of the sequence
 };
 
 // Units are head-major: unit u is tile r = u % U1 of head u / U1 (U1 =
@@ -126,7 +136,8 @@ __device__ __forceinline__ Unit load_unit(const MultiQueryArgs &a, int u, int b)
     x.ns = ld_uniform(a.new_start + b);
     x.tok = ld_uniform(a.tok_off + b);
     x.T = ld_uniform(a.tok_off + b + 1) - x.tok;
-    x.trow = a.table + static_cast<size_t>(ld_uniform(a.seq_ids + b)) * a.table_stride;
+    x.sid = ld_uniform(a.seq_ids + b);
+    x.trow = a.table + static_cast<size_t>(x.sid) * a.table_stride;
     return x;
 }
 
@@ -217,10 +228,11 @@ __device__ __forceinline__ int mq_share_of(int i, int W) {
 // the page of the next block).
 constexpr int kQkAhead = 3, kPvAhead = 3;
 
-template <int NT, int WAVES, bool TREE, int KEYS>
+template <int NT, int WAVES, bool TREE, int KEYS, bool Q8 = false>
 __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
-    constexpr int kRing = ring_stages<KEYS>();
-    constexpr int kTileBytes = tile_bytes<KEYS>();
+    static_assert(!Q8 || (!TREE && KEYS == 8 * WAVES), "a wave converts an eighth (a quarter) of a block");
+    constexpr int kRing = Q8 ? 2 : ring_stages<KEYS>();
+    constexpr int kTileBytes = Q8 ? KEYS * kRowBytes : tile_bytes<KEYS>();
     // Keys folded in at a time: a block's, or with two row tiles per wave
     // half of a 64-key block's (the scores of all would not fit the
     // registers beside two tiles' accumulators).
@@ -229,6 +241,7 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
     constexpr int kKS = kFold / 32;  // 32-key steps of a fold (PV)
     __shared__ __attribute__((aligned(16))) uint8_t ring[kRing][2 * kTileBytes];
     __shared__ __attribute__((aligned(16))) uint8_t strips[WAVES][16 * kStripRow];  // the epilogue's, per wave
+    __shared__ float factor[2][Q8 ? KEYS / 16 : 1];  // Q8: what a stage's scores are multiplied by, per page
     const int w = mq_share_of(blockIdx.x, a.n_wg);  // this workgroup's share (and partial slots)
     const int W = a.n_wg;
     const int NB = a.total_blocks;
@@ -244,7 +257,7 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
     const int G = nh / hkv;
     const int Q = a.q_tile;
     const int row_bytes = hkv * kRowBytes;
-    const float scale = kLog2e / 16.0f;
+    const float scale = Q8 ? 1.0f : kLog2e / 16.0f;
 
     // The token of this lane's query row in each of the wave's NT tiles.
     int iq[NT];
@@ -283,14 +296,113 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
             ig = iu.ub;
         }
     };
+    // Q8: ids8 requests the page ids of the next block (lane l: page l % pages
+    // of a block), load8 its codes and scales into registers (and moves on to the
+    // block after it), put8 converts what load8 brought and writes it to a stage.
+    // Wave wv takes chunk groups 2 (wv % 2), + 1 of K page wv / 2 and tile group
+    // wv % 4 of V pages 2 (wv / 4), + 1.  Pages past the sequence are zeros, the
+    // open page is FP16 rows, of which the stale ones are masked (K) or zeroed (V).
+    constexpr int kPages = KEYS / 16;
+    const int nt8 = wv >> 1, ih8 = wv & 1, ks8 = wv >> 2, j8 = wv & 3;
+    [[maybe_unused]] uint4 rk[2], rv[2];
+    [[maybe_unused]] float rsc = 0.0f;  // lane l: scale of page l % kPages, of V where l & kPages
+    [[maybe_unused]] int pg8 = 0, open8 = -1, lim8 = 0, sid8 = 0, h8 = 0;
+    [[maybe_unused]] bool on8 = false;
+    [[maybe_unused]] auto ids8 = [&]() {
+        const int p0 = (ig - iu.ub) * kPages;
+        vpage = ig < q1 ? iu.trow[min(p0 + (lane & (kPages - 1)), (iu.ctx - 1) >> 4)] : 0;
+    };
+    [[maybe_unused]] auto load8 = [&]() {
+        on8 = ig < q1;
+        pg8 = (ig - iu.ub) * kPages;
+        open8 = (iu.ctx & 15) ? iu.ctx >> 4 : -1;
+        lim8 = iu.ctx & 15;
+        sid8 = iu.sid;
+        h8 = iu.h;
+        const int full = on8 ? iu.ctx >> 4 : 0;  // full pages of the sequence
+        auto codes = [&](const uint8_t *base, int p) {
+            const int id = __builtin_amdgcn_readlane(vpage, p);
+            return ro_rsrc(base + (static_cast<size_t>(id) * hkv + iu.h) * kPageElems, pg8 + p < full ? kPageElems : 0u);
+        };
+        auto load = [&](__amdgpu_buffer_rsrc_t r, int ofs) {
+            const auto x = __builtin_amdgcn_raw_buffer_load_b128(r, 16 * lane, ofs, 0);
+            return make_uint4(x[0], x[1], x[2], x[3]);
+        };
+        const auto k = codes(a.k8, nt8), v0 = codes(a.v8, 2 * ks8), v1 = codes(a.v8, 2 * ks8 + 1);
+        rk[0] = load(k, 2048 * ih8);
+        rk[1] = load(k, 2048 * ih8 + 1024);
+        rv[0] = load(v0, 1024 * j8);
+        rv[1] = load(v1, 1024 * j8);
+        const float sc = a.scales[(static_cast<size_t>(vpage) * hkv + iu.h) * 2 + ((lane & kPages) ? 1 : 0)];
+        rsc = pg8 + (lane & (kPages - 1)) < full ? sc : 0.0f;
+        if (on8 && ++ig < q1 && ig >= iu.ue) {
+            iu = load_unit<KEYS>(a, iu.u + 1, iu.b);
+            ig = iu.ub;
+        }
+    };
+    [[maybe_unused]] auto put8 = [&](int st) {
+        if (!on8) return;  // uniform over the workgroup
+        const uint16_t *open = a.open + (static_cast<size_t>(sid8) * hkv + h8) * 2 * kPageElems;
+        auto scale_of = [&](int lane_of) {
+            return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, rsc), lane_of));
+        };
+        uint8_t *kd = ring[st] + ((nt8 * 8 + 4 * ih8) * 64 + lane) * 16;
+        const bool k_open = pg8 + nt8 == open8;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            uint4 lo, hi;
+            if (k_open) {
+                const uint16_t *src = open + 1024 * (2 * ih8 + e) + 16 * lane;
+                lo = ld16(src);
+                hi = ld16(src + 8);
+            } else {
+                lo = codes8(rk[e].x, rk[e].y);
+                hi = codes8(rk[e].z, rk[e].w);
+            }
+            *reinterpret_cast<uint4 *>(kd + 2048 * e) = lo;
+            *reinterpret_cast<uint4 *>(kd + 2048 * e + 1024) = hi;
+        }
+        if (ih8 == 0 && lane == 0) factor[st][nt8] = (k_open ? 1.0f : scale_of(nt8)) * (kLog2e / 16.0f);
+        uint8_t *vd = ring[st] + kTileBytes + ((ks8 * 16 + 4 * j8) * 64 + lane) * 16;
+        uint2 part[2][4];
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            const uint32_t w[4] = {rv[p].x, rv[p].y, rv[p].z, rv[p].w};
+            const uint32_t s2 = scale_h2(scale_of(kPages + 2 * ks8 + p));
+            if (pg8 + 2 * ks8 + p == open8) {
+                const uint32_t m0 = (4 * grp < lim8 ? 0xffffu : 0u) | (4 * grp + 1 < lim8 ? 0xffff0000u : 0u);
+                const uint32_t m1 = (4 * grp + 2 < lim8 ? 0xffffu : 0u) | (4 * grp + 3 < lim8 ? 0xffff0000u : 0u);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const uint2 x = ld8(open + kPageElems + 1024 * j8 + 16 * lane + 4 * q);
+                    part[p][q] = make_uint2(x.x & m0, x.y & m1);
+                }
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) part[p][q] = values4(w[q], s2);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<uint4 *>(vd + 1024 * q) = make_uint4(part[0][q].x, part[0][q].y, part[1][q].x, part[1][q].y);
+    };
     Unit cu = iu;
     int g = ig;
+    if constexpr (Q8) {
+        ids8();
+        load8();
+        ids8();
+        put8(0);
+        load8();
+        ids8();
+    } else {
 #pragma unroll
-    for (int s = 0; s + 1 < kRing; ++s) {
-        fetch_page();
-        issue(s);
+        for (int s = 0; s + 1 < kRing; ++s) {
+            fetch_page();
+            issue(s);
+        }
+        if constexpr (kPageAhead) page_ahead();
     }
-    if constexpr (kPageAhead) page_ahead();
 
     int n_done = 0;  // blocks computed by this workgroup (ring position)
     while (true) {
@@ -304,7 +416,7 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
         bool qvalid[NT];
         int qslot[NT];
         uint64_t qbits[NT];
-        uint4 qb[NT][8];  // B operand Q^T: dims 32*kk + 8*grp .. +8
+        uint4 qb[NT][8];  // B operand Q^T: dims 32*kk + 8*grp .. +8 (Q8: 64*(kk/2) + 16*grp + 8*(kk%2) .. +8)
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const int qi = cu.tile * Q + iq[t];
@@ -317,9 +429,9 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
             const uint16_t *qr = a.q +
                                  (static_cast<size_t>(cu.tok + (has ? ql : 0)) * nh + cu.h * G + (has ? rl - il * G : 0)) *
                                      kHeadDim +
-                                 8 * (lane & 3);
+                                 (Q8 ? 16 : 8) * (lane & 3);
 #pragma unroll
-            for (int kk = 0; kk < 8; ++kk) qb[t][kk] = ld16(qr + 32 * kk);
+            for (int kk = 0; kk < 8; ++kk) qb[t][kk] = ld16(qr + (Q8 ? 64 * (kk >> 1) + 8 * (kk & 1) : 32 * kk));
             const int from = 4 * (4 * col + grp);  // bytes: the lane that holds this lane's pieces
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk) {
@@ -351,19 +463,30 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
         }
 
         for (; g < seg_end; ++g) {
-            wait_block<WAVES, KEYS>();
-            __builtin_amdgcn_s_barrier();
-            __builtin_amdgcn_sched_barrier(0);
-            if constexpr (kPageAhead)
-                ipage = __builtin_amdgcn_readfirstlane(vpage);
-            else
-                fetch_page();
-            issue((n_done + kRing - 1) % kRing);
-            if constexpr (kPageAhead) page_ahead();
-            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (Q8) {
+                wait_vm_lds<63>();  // this wave's part of the stage is written (LDS only)
+                __builtin_amdgcn_s_barrier();
+                __builtin_amdgcn_sched_barrier(0);
+                put8((n_done + 1) & 1);
+                load8();
+                ids8();
+                __builtin_amdgcn_sched_barrier(0);
+            } else {
+                wait_block<WAVES, KEYS>();
+                __builtin_amdgcn_s_barrier();
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (kPageAhead)
+                    ipage = __builtin_amdgcn_readfirstlane(vpage);
+                else
+                    fetch_page();
+                issue((n_done + kRing - 1) % kRing);
+                if constexpr (kPageAhead) page_ahead();
+                __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll 1
             for (int fold = 0; fold < KEYS / kFold; ++fold) {
-                const uint8_t *kt = ring[n_done % kRing] + fold * (kFold / 2) * kPairBytes;
+                // Q8: operands of 1 KB, [16-key tile][k-step] and [32-key step][dim tile].
+                const uint8_t *kt = ring[n_done % kRing] + fold * (Q8 ? kFold * kRowBytes : (kFold / 2) * kPairBytes);
                 const uint8_t *kbase = kt + key_off(col) + 16 * k_granule(col, grp);
                 const int key0 = (g - cu.ub) * KEYS + fold * kFold;
 
@@ -376,6 +499,8 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
                 // Operand i: key tile i % kKT (key 16*nt + col), k-step i / kKT
                 // (granule 4*kk + grp): kbase + nt*8 pairs + 64*kk.
                 auto read_k = [&](int i) -> uint4 {
+                    if constexpr (Q8)
+                        return *reinterpret_cast<const uint4 *>(kt + ((i % kKT) * 8 + i / kKT) * 1024 + 16 * lane);
                     return *reinterpret_cast<const uint4 *>(kbase + 8 * (i % kKT) * kPairBytes + 64 * (i / kKT));
                 };
                 uint4 ka[kQkAhead];
@@ -390,6 +515,14 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
                                                                               s[t][i % kKT], 0, 0, 0);
                     if (i + kQkAhead < 8 * kKT) ka[i % kQkAhead] = read_k(i + kQkAhead);
                     __builtin_amdgcn_sched_barrier(0);
+                }
+                if constexpr (Q8) {
+#pragma unroll
+                    for (int nt = 0; nt < kKT; ++nt) {
+                        const float f = factor[n_done % kRing][fold * kKT + nt];
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) s[t][nt] *= f;
+                    }
                 }
                 half8_t pb[NT][kKS];
                 float corr[NT];
@@ -479,6 +612,9 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
                 const uint8_t *vbase[2] = {vb + 64 * (vr & 1), vb - 64 * (vr & 1)};
                 // Operand i: dim tile i / kKS, keys 32*(i % kKS) .. (16 pairs on).
                 auto read_v = [&](int i) -> half8_t {
+                    if constexpr (Q8)
+                        return as_h8(*reinterpret_cast<const uint4 *>(kt + kTileBytes + ((i % kKS) * 16 + i / kKS) * 1024 +
+                                                                      16 * lane));
                     short4_t part[2];
 #pragma unroll
                     for (int hh = 0; hh < 2; ++hh) {
@@ -660,6 +796,7 @@ __global__ __launch_bounds__(64 * kMqCombineRows) void mq_combine_kernel(MultiQu
 
 template <int NT, int WAVES>
 hipError_t launch_mq(const MultiQueryArgs &a, hipStream_t s) {
+    if (a.k8 && (NT > 1 || a.tree || a.keys != 8 * WAVES)) return hipErrorInvalidValue;
     // 64-key blocks only for eight-wave causal tiles (mq_keys_for).
     const bool k64 = a.keys == 64 && WAVES == 8 && !a.tree;
     if (a.keys != 32 && !k64) return hipErrorInvalidValue;
@@ -667,7 +804,10 @@ hipError_t launch_mq(const MultiQueryArgs &a, hipStream_t s) {
         const hipError_t e = hipEventRecord(a.ev_before, s);
         if (e != hipSuccess) return e;
     }
-    if constexpr (NT > 1) {  // long prefill steps only
+    if (a.k8) {
+        if constexpr (NT == 1)
+            hipLaunchKernelGGL((mq_kernel<NT, WAVES, false, 8 * WAVES, true>), dim3(a.n_wg), dim3(64 * WAVES), 0, s, a);
+    } else if constexpr (NT > 1) {  // long prefill steps only
         hipLaunchKernelGGL((mq_kernel<NT, WAVES, false, 64>), dim3(a.n_wg), dim3(64 * WAVES), 0, s, a);
     } else if (a.tree) {
         hipLaunchKernelGGL((mq_kernel<NT, WAVES, true, 32>), dim3(a.n_wg), dim3(64 * WAVES), 0, s, a);

@@ -72,6 +72,16 @@ struct kva_cache {
     // device memory
     uint16_t *d_k = nullptr;
     uint16_t *d_v = nullptr;
+    // An 8-bit cache (KVA_FLAG_INT8) has these instead of the FP16 pools:
+    // codes, scales and open blocks as in kva::Store8Args, of all layers; rows
+    // that a projection leaves for the append, [2][max_step_tokens][Hkv][256];
+    // and the numbers 0, 1, 2, ... as that projection's slots and page ids.
+    bool int8 = false;
+    uint8_t *d_k8 = nullptr, *d_v8 = nullptr;
+    float *d_scales = nullptr;
+    uint16_t *d_open = nullptr, *d_stage = nullptr;
+    int32_t *d_count = nullptr;
+    size_t layer_codes = 0, layer_scales = 0, layer_open = 0;  // elements
     int32_t *d_table = nullptr;
     uint8_t *d_step = nullptr;
     size_t step_bytes = 0;
@@ -105,6 +115,9 @@ struct kva_cache {
     std::vector<int32_t> nblk;    // blocks held per sequence
     std::vector<int32_t> len;     // committed length per sequence
     std::vector<uint8_t> freed;   // sequence released by kva_seq_free
+    // 8-bit cache: the page whose rows a sequence's open block holds (-1:
+    // none), and the rows that its pages and open block hold.
+    std::vector<int32_t> open_page, held;
     std::vector<uint8_t> used;    // per block
     std::vector<int32_t> free_list;
     std::vector<int32_t> patches; // pending (seq, idx, block) triples
@@ -125,7 +138,8 @@ struct kva_cache {
     bool st_all_one = false, st_has_bits = false;
     std::vector<int32_t> st_pre;  // pages of the step's earlier sequences, [n_seqs + 1]
     size_t off_seq = 0, off_ctx = 0, off_start = 0, off_tokoff = 0, off_tseq = 0,
-           off_tslot = 0, off_tpos = 0, off_bits = 0, off_pre = 0, off_pids = 0, off_cut = 0;
+           off_tslot = 0, off_tpos = 0, off_bits = 0, off_pre = 0, off_pids = 0, off_cut = 0, off_touch = 0;
+    int32_t st_touch = 0;  // 8-bit cache: pages that the step's rows go to
 
     // Caller's timing events around the dominant kernel of each hot call
     // (kva_kernel_events); null: none.
@@ -150,7 +164,7 @@ struct kva_graph {
     hipGraphExec_t exec = nullptr;
     int32_t n_seqs = 0, n_tok = 0, table_rows = 0;
     bool all_one = false, has_bits = false;
-    size_t offs[12] = {};
+    size_t offs[13] = {};
 };
 
 namespace {
@@ -300,9 +314,47 @@ int32_t choose_wg(const kva_cache *c, int64_t pages) {
     return static_cast<int32_t>(std::max<int64_t>(1, w));
 }
 
+// An 8-bit cache keeps values, not rows at addresses.
+int refuse_int8(const kva_cache *c, const char *what) {
+    if (c->int8) return fail(KVA_ERR_UNSUPPORTED, "%s is not available on an 8-bit cache", what);
+    return KVA_OK;
+}
+
+// `layer`'s codes, scales and open blocks for a launch's arguments.
+template <class Args>
+void set_layer8(const kva_cache *c, int32_t layer, Args &a) {
+    a.k8 = c->d_k8 + c->layer_codes * layer;
+    a.v8 = c->d_v8 + c->layer_codes * layer;
+    a.scales = c->d_scales + c->layer_scales * layer;
+    a.open = c->d_open + c->layer_open * layer;
+}
+
+// Touch records (kva::kTouchWords each) to the device through the staging
+// ring, in chunks that fit it, `launch` called for each with its device address
+// and count.
+template <class Launch>
+int upload_touches(kva_cache *c, const std::vector<int32_t> &touches, hipStream_t s, Launch launch) {
+    constexpr size_t kBytes = kva::kTouchWords * sizeof(int32_t);
+    const size_t per_chunk = c->aux_bytes / kBytes, total = touches.size() / kva::kTouchWords;
+    for (size_t done = 0; done < total;) {
+        const size_t n = std::min(per_chunk, total - done);
+        uint8_t *h;
+        int idx;
+        int rc = acquire_stage(c, &h, &idx);
+        if (rc) return rc;
+        std::memcpy(h, touches.data() + done * kva::kTouchWords, n * kBytes);
+        KVA_HIP(hipMemcpyAsync(c->d_aux, h, n * kBytes, hipMemcpyHostToDevice, s));
+        if ((rc = release_stage(c, idx, s))) return rc;
+        KVA_HIP(launch(reinterpret_cast<const int32_t *>(c->d_aux), static_cast<int32_t>(n)));
+        done += n;
+    }
+    return KVA_OK;
+}
+
 // Whether any step of this cache can be long enough for two row tiles per
 // wave: every tile of the longest step at the longest sequence.
 bool may_take_two_tiles(const kva_cache *c) {
+    if (c->int8) return false;
     const int32_t q = kva::mq_tile_tokens(c->group, 8, 1);
     const int64_t tiles = (static_cast<int64_t>(c->cfg.max_step_tokens) / q + c->cfg.max_seqs) * c->cfg.num_kv_heads;
     const int64_t blocks = static_cast<int64_t>(c->cfg.max_blocks_per_seq) * kva::kBlockTokens / 64 + 1;
@@ -345,6 +397,7 @@ int kva_create(const kva_config *cfg, kva_cache **out) {
     if (rc) return rc;
     kva_cache *c = new kva_cache();
     c->cfg = *cfg;
+    c->int8 = (cfg->flags & KVA_FLAG_INT8) != 0;
     c->host_only = (cfg->flags & KVA_FLAG_HOST_ONLY) != 0;
     c->group = cfg->num_heads / cfg->num_kv_heads;
     c->row_elems = static_cast<size_t>(cfg->num_kv_heads) * cfg->head_dim;
@@ -354,6 +407,12 @@ int kva_create(const kva_config *cfg, kva_cache **out) {
     c->nblk.assign(cfg->max_seqs, 0);
     c->len.assign(cfg->max_seqs, 0);
     c->freed.assign(cfg->max_seqs, 0);
+    c->open_page.assign(cfg->max_seqs, -1);
+    c->held.assign(cfg->max_seqs, 0);
+    const size_t block_heads = static_cast<size_t>(cfg->max_blocks) * cfg->num_kv_heads;
+    c->layer_codes = block_heads * kva::kPageElems;
+    c->layer_scales = block_heads * 2;
+    c->layer_open = static_cast<size_t>(cfg->max_seqs) * cfg->num_kv_heads * 2 * kva::kPageElems;
     c->used.assign(cfg->max_blocks, 0);
     c->free_list.resize(cfg->max_blocks);
     for (int32_t i = 0; i < cfg->max_blocks; ++i) c->free_list[i] = cfg->max_blocks - 1 - i;
@@ -370,6 +429,11 @@ int kva_create(const kva_config *cfg, kva_cache **out) {
                     round_up(sizeof(uint64_t) * static_cast<size_t>(cfg->max_step_tokens), 256) +
                     round_up(sizeof(int32_t) * kva::kPlanPages * static_cast<size_t>(cfg->max_seqs), 256) +
                     round_up(sizeof(int32_t) * kva::kMqCutWords * max_units, 256) + 1024;
+    if (c->int8)  // a sequence's n new rows lie in at most n / 16 + 2 pages
+        c->step_bytes += round_up(sizeof(int32_t) * kva::kTouchWords *
+                                      (static_cast<size_t>(cfg->max_step_tokens) / kva::kBlockTokens +
+                                       2 * static_cast<size_t>(cfg->max_seqs)),
+                                  256);
     const size_t patch_cap = std::max<size_t>(4096, cfg->max_seqs + cfg->max_step_tokens);
     c->aux_bytes = round_up(std::max(patch_cap * 3 * sizeof(int32_t),
                                      (static_cast<size_t>(cfg->max_step_tokens) * 3 + cfg->max_seqs + 1) *
@@ -394,12 +458,36 @@ int kva_create(const kva_config *cfg, kva_cache **out) {
             return code;
         };
         hipError_t e;
-        const size_t pool_bytes = c->layer_elems * cfg->n_layers * sizeof(uint16_t);
-        if ((e = hipMalloc(&c->d_k, pool_bytes)) != hipSuccess) return cleanup(hip_fail(e, "hipMalloc(K pool)"));
-        if ((e = hipMalloc(&c->d_v, pool_bytes)) != hipSuccess) return cleanup(hip_fail(e, "hipMalloc(V pool)"));
         // Zeroed pools: rows never written read as finite zeros.
-        if ((e = hipMemset(c->d_k, 0, pool_bytes)) != hipSuccess) return cleanup(hip_fail(e, "hipMemset(K)"));
-        if ((e = hipMemset(c->d_v, 0, pool_bytes)) != hipSuccess) return cleanup(hip_fail(e, "hipMemset(V)"));
+        auto filled = [&](auto **p, size_t n, int byte) {
+            const hipError_t rc = hipMalloc(p, n * sizeof(**p));
+            return rc != hipSuccess ? rc : hipMemset(*p, byte, n * sizeof(**p));
+        };
+        const size_t layers = cfg->n_layers;
+        if (c->int8) {
+            if ((e = filled(&c->d_k8, c->layer_codes * layers, 128)) != hipSuccess)
+                return cleanup(hip_fail(e, "hipMalloc(K codes)"));
+            if ((e = filled(&c->d_v8, c->layer_codes * layers, 128)) != hipSuccess)
+                return cleanup(hip_fail(e, "hipMalloc(V codes)"));
+            if ((e = filled(&c->d_scales, c->layer_scales * layers, 0)) != hipSuccess)
+                return cleanup(hip_fail(e, "hipMalloc(scales)"));
+            if ((e = filled(&c->d_open, c->layer_open * layers, 0)) != hipSuccess)
+                return cleanup(hip_fail(e, "hipMalloc(open blocks)"));
+            const size_t step_rows = static_cast<size_t>(cfg->max_step_tokens) * c->row_elems;
+            if ((e = hipMalloc(&c->d_stage, 2 * step_rows * sizeof(uint16_t))) != hipSuccess)
+                return cleanup(hip_fail(e, "hipMalloc(projected rows)"));
+            std::vector<int32_t> count(cfg->max_step_tokens);
+            for (int32_t i = 0; i < cfg->max_step_tokens; ++i) count[i] = i;
+            if ((e = hipMalloc(&c->d_count, count.size() * sizeof(int32_t))) != hipSuccess ||
+                (e = hipMemcpy(c->d_count, count.data(), count.size() * sizeof(int32_t), hipMemcpyHostToDevice)) !=
+                    hipSuccess)
+                return cleanup(hip_fail(e, "hipMalloc(row numbers)"));
+        } else {
+            if ((e = filled(&c->d_k, c->layer_elems * layers, 0)) != hipSuccess)
+                return cleanup(hip_fail(e, "hipMalloc(K pool)"));
+            if ((e = filled(&c->d_v, c->layer_elems * layers, 0)) != hipSuccess)
+                return cleanup(hip_fail(e, "hipMalloc(V pool)"));
+        }
         const size_t tbytes = c->table.size() * sizeof(int32_t);
         if ((e = hipMalloc(&c->d_table, tbytes)) != hipSuccess) return cleanup(hip_fail(e, "hipMalloc(table)"));
         if ((e = hipMemset(c->d_table, 0, tbytes)) != hipSuccess) return cleanup(hip_fail(e, "hipMemset(table)"));
@@ -453,6 +541,12 @@ int kva_destroy(kva_cache *c) {
         }
         (void)hipFree(c->d_k);
         (void)hipFree(c->d_v);
+        (void)hipFree(c->d_k8);
+        (void)hipFree(c->d_v8);
+        (void)hipFree(c->d_scales);
+        (void)hipFree(c->d_open);
+        (void)hipFree(c->d_stage);
+        (void)hipFree(c->d_count);
         (void)hipFree(c->d_table);
         (void)hipFree(c->d_step);
         (void)hipFree(c->d_aux);
@@ -469,9 +563,9 @@ int kva_destroy(kva_cache *c) {
 
 int kva_get_layout(const kva_cache *c, kva_layout *out) {
     if (!c || !out) return fail(KVA_ERR_INVALID_ARG, "NULL argument");
-    out->row_bytes = c->row_elems * sizeof(uint16_t);
+    out->row_bytes = c->row_elems * (c->int8 ? 1 : sizeof(uint16_t));
     out->block_bytes = out->row_bytes * kva::kBlockTokens;
-    out->layer_bytes = c->layer_elems * sizeof(uint16_t);
+    out->layer_bytes = c->layer_elems * (c->int8 ? 1 : sizeof(uint16_t));
     out->block_tokens = kva::kBlockTokens;
     out->max_blocks_per_seq = c->cfg.max_blocks_per_seq;
     return KVA_OK;
@@ -481,6 +575,7 @@ int kva_layer_pools(const kva_cache *c, int32_t layer, void **k_pool, void **v_p
     int rc = require_device(c);
     if (rc) return rc;
     if ((rc = check_layer(c, layer))) return rc;
+    if ((rc = refuse_int8(c, "kva_layer_pools"))) return rc;
     if (!k_pool || !v_pool) return fail(KVA_ERR_INVALID_ARG, "NULL output pointer");
     *k_pool = c->d_k + c->layer_elems * layer;
     *v_pool = c->d_v + c->layer_elems * layer;
@@ -543,6 +638,8 @@ int kva_seq_free(kva_cache *c, int32_t seq) {
     if (c->freed[seq]) return fail(KVA_ERR_DOUBLE_FREE, "sequence %d already freed", seq);
     release_blocks(c, seq);
     c->len[seq] = 0;
+    c->open_page[seq] = -1;
+    c->held[seq] = 0;
     c->freed[seq] = 1;
     c->step_valid = false;
     return KVA_OK;
@@ -564,6 +661,8 @@ int kva_seq_set_len(kva_cache *c, int32_t seq, int32_t len) {
     if (static_cast<int64_t>(len) > static_cast<int64_t>(c->nblk[seq]) * kva::kBlockTokens)
         return fail(KVA_ERR_CAPACITY, "length %d exceeds reserved capacity %d", len,
                     c->nblk[seq] * kva::kBlockTokens);
+    if (c->int8 && len > c->held[seq])
+        return fail(KVA_ERR_STATE, "length %d: an 8-bit cache holds %d rows of sequence %d", len, c->held[seq], seq);
     c->len[seq] = len;
     c->step_valid = false;
     return KVA_OK;
@@ -593,6 +692,7 @@ int kva_row_ptr(const kva_cache *c, int32_t layer, int32_t seq, int32_t slot, vo
     if (rc) return rc;
     if ((rc = check_layer(c, layer))) return rc;
     if ((rc = check_seq(c, seq))) return rc;
+    if ((rc = refuse_int8(c, "kva_row_ptr"))) return rc;
     if (!k_row || !v_row) return fail(KVA_ERR_INVALID_ARG, "NULL output pointer");
     if (slot < 0 || slot >= c->nblk[seq] * kva::kBlockTokens)
         return fail(KVA_ERR_CAPACITY, "slot %d outside the %d reserved rows of sequence %d", slot,
@@ -647,6 +747,7 @@ int kva_step_begin(kva_cache *c, int32_t n_seqs, const int32_t *seq_ids, const i
         for (int64_t i = 0; i < n_tok; ++i)
             if (rope_pos[i] < 0) return fail(KVA_ERR_INVALID_ARG, "rope_pos[%lld] < 0", static_cast<long long>(i));
     if (tree_bits) {
+        if (int rc = refuse_int8(c, "a step with tree_bits")) return rc;
         int64_t t = 0;
         for (int32_t b = 0; b < n_seqs; ++b) {
             if (n_new[b] > 64) return fail(KVA_ERR_UNSUPPORTED, "tree of %d nodes > 64", n_new[b]);
@@ -698,7 +799,28 @@ int kva_step_begin(kva_cache *c, int32_t n_seqs, const int32_t *seq_ids, const i
     const size_t o_tpos = round_up(o_tslot + sizeof(int32_t) * n_tok, 16);
     const size_t o_bits = round_up(o_tpos + sizeof(int32_t) * n_tok, 16);
     const size_t o_pids = round_up(o_bits + (tree_bits ? sizeof(uint64_t) * n_tok : 0), 16);
-    const size_t o_cut = round_up(o_pids + sizeof(int32_t) * kva::kPlanPages * n_seqs, 16);
+    const size_t o_touch = round_up(o_pids + sizeof(int32_t) * kva::kPlanPages * n_seqs, 16);
+    // 8-bit cache: the pages that the step's rows go to, a record each; and the
+    // sequences whose length was set back into a full page, whose rows become
+    // the open block's again.
+    std::vector<int32_t> touches, reopened;
+    if (c->int8) {
+        int32_t tok = 0;
+        for (int32_t b = 0; b < n_seqs; ++b) {
+            const int32_t s = seq_ids[b], start = c->len[s], end = start + n_new[b];
+            if (start % kva::kBlockTokens && c->open_page[s] != start / kva::kBlockTokens)
+                reopened.insert(reopened.end(), {s, start / kva::kBlockTokens, 0, 0, 0, 0, 0, 0});
+            c->open_page[s] = end % kva::kBlockTokens ? end / kva::kBlockTokens : -1;
+            c->held[s] = end;
+            for (int32_t at = start; at < end;) {
+                const int32_t r0 = at % kva::kBlockTokens, n = std::min(end - at, kva::kBlockTokens - r0);
+                touches.insert(touches.end(), {s, at / kva::kBlockTokens, tok, r0, n, 0, 0, 0});
+                at += n;
+                tok += n;
+            }
+        }
+    }
+    const size_t o_cut = o_touch + touches.size() * sizeof(int32_t);
     // The cut-unit records (below) take at most one per unit; only those
     // written are uploaded.
     const size_t total_max = o_cut + sizeof(int32_t) * kva::kMqCutWords * n_units;
@@ -784,6 +906,7 @@ int kva_step_begin(kva_cache *c, int32_t n_seqs, const int32_t *seq_ids, const i
     }
     p_mqpre[units] = static_cast<int32_t>(blocks);
     if (tree_bits) std::memcpy(h + o_bits, tree_bits, sizeof(uint64_t) * n_tok);
+    if (!touches.empty()) std::memcpy(h + o_touch, touches.data(), touches.size() * sizeof(int32_t));
     // The units the multi-query launch will cut across workgroups (the same
     // shares: kva::mq_wg_count workgroups over the unit positions), one
     // record each for its combine: head, the tile's first new token, its
@@ -835,9 +958,23 @@ int kva_step_begin(kva_cache *c, int32_t n_seqs, const int32_t *seq_ids, const i
         int rc = release_stage(c, idx, s);
         if (rc) return rc;
         if ((rc = flush_patches(c, s))) return rc;
+        kva::ReopenArgs ro{};
+        set_layer8(c, 0, ro);
+        ro.table = c->d_table;
+        ro.table_stride = c->cfg.max_blocks_per_seq;
+        ro.layer_codes = c->layer_codes;
+        ro.layer_scales = c->layer_scales;
+        ro.layer_open = c->layer_open;
+        rc = upload_touches(c, reopened, s, [&](const int32_t *recs, int32_t n) {
+            ro.touch = recs;
+            return kva::launch_reopen(ro, n, c->cfg.num_kv_heads, c->cfg.n_layers, s);
+        });
+        if (rc) return rc;
     } else {
         c->patches.clear();
     }
+    c->off_touch = o_touch;
+    c->st_touch = static_cast<int32_t>(touches.size() / kva::kTouchWords);
     c->off_seq = o_seq;
     c->off_ctx = o_ctx;
     c->off_start = o_start;
@@ -872,6 +1009,22 @@ int kva_step_begin(kva_cache *c, int32_t n_seqs, const int32_t *seq_ids, const i
     return KVA_OK;
 }
 
+// Where the step's rows go, for an append's launch.
+static void set_append_plan(const kva_cache *c, int32_t layer, kva::AppendArgs &a) {
+    if (!c->int8) {
+        a.k_pool = c->d_k + c->layer_elems * layer;
+        a.v_pool = c->d_v + c->layer_elems * layer;
+    }
+    a.table = c->d_table;
+    a.table_stride = c->cfg.max_blocks_per_seq;
+    a.tok_seq = at<int32_t>(c->d_step, c->off_tseq);
+    a.tok_slot = at<int32_t>(c->d_step, c->off_tslot);
+    a.tok_pos = at<int32_t>(c->d_step, c->off_tpos);
+    a.n_tok = c->st_n_tok;
+    a.num_heads = c->cfg.num_heads;
+    a.num_kv_heads = c->cfg.num_kv_heads;
+}
+
 // Check an append's operands (the step already begun) and fill its launch
 // arguments.
 static int make_append(kva_cache *c, int32_t layer, void *q, void *k, const void *v, const void *q_norm_w,
@@ -895,18 +1048,29 @@ static int make_append(kva_cache *c, int32_t layer, void *q, void *k, const void
     a.k_w = static_cast<const uint16_t *>(k_norm_w);
     a.cos_tab = static_cast<const uint16_t *>(cos_tab);
     a.sin_tab = static_cast<const uint16_t *>(sin_tab);
-    a.k_pool = c->d_k + c->layer_elems * layer;
-    a.v_pool = c->d_v + c->layer_elems * layer;
-    a.table = c->d_table;
-    a.table_stride = c->cfg.max_blocks_per_seq;
-    a.tok_seq = at<int32_t>(c->d_step, c->off_tseq);
-    a.tok_slot = at<int32_t>(c->d_step, c->off_tslot);
-    a.tok_pos = at<int32_t>(c->d_step, c->off_tpos);
-    a.n_tok = c->st_n_tok;
-    a.num_heads = c->cfg.num_heads;
-    a.num_kv_heads = c->cfg.num_kv_heads;
     a.half_rot = half_rot;
     a.eps = c->cfg.eps;
+    set_append_plan(c, layer, a);
+    return KVA_OK;
+}
+
+// The step's rows into the cache: norm, else ap.k and ap.v as they are.
+static hipError_t launch_rows(kva_cache *c, int32_t layer, const kva::AppendArgs &ap, bool norm, hipStream_t s) {
+    if (!c->int8) return norm ? kva::launch_append(ap, s) : kva::launch_copy_rows(ap, s);
+    kva::Store8Args a{};
+    a.ap = ap;
+    a.norm = norm;
+    a.touch = at<int32_t>(c->d_step, c->off_touch);
+    a.n_touch = c->st_touch;
+    set_layer8(c, layer, a);
+    return kva::launch_store8(a, s);
+}
+
+// A recorded append into an 8-bit cache has a workgroup per page that the step
+// touches, which later steps share only with one new token per sequence.
+static int check_rows8_capture(const kva_cache *c) {
+    if (c->int8 && c->capturing && !c->st_all_one)
+        return fail(KVA_ERR_STATE, "an 8-bit cache records appends of one new token per sequence only");
     return KVA_OK;
 }
 
@@ -920,8 +1084,28 @@ static int append_impl(kva_cache *c, int32_t layer, void *q, void *k, const void
     if (c->st_n_tok == 0) return require_device(c);
     kva::AppendArgs a;
     if ((rc = make_append(c, layer, q, k, v, q_norm_w, k_norm_w, cos_tab, sin_tab, table_rows, a))) return rc;
+    if ((rc = check_rows8_capture(c))) return rc;
     if ((rc = require_device(c))) return rc;
-    KVA_HIP(kva::launch_append(a, static_cast<hipStream_t>(stream)));
+    KVA_HIP(launch_rows(c, layer, a, true, static_cast<hipStream_t>(stream)));
+    return KVA_OK;
+}
+
+static int append_rows_impl(kva_cache *c, int32_t layer, const void *k, const void *v, kva_stream_t stream) {
+    if (!c) return fail(KVA_ERR_INVALID_ARG, "cache is NULL");
+    int rc = check_layer(c, layer);
+    if (rc) return rc;
+    if (!c->step_valid) return fail(KVA_ERR_STATE, "no step begun (kva_step_begin)");
+    if (c->st_n_tok == 0) return require_device(c);
+    if (!k || !v) return fail(KVA_ERR_INVALID_ARG, "NULL tensor pointer");
+    if (!aligned16(k) || !aligned16(v)) return fail(KVA_ERR_MISALIGNED, "k and v must be 16-byte aligned");
+    if ((rc = check_rows8_capture(c))) return rc;
+    if ((rc = require_device(c))) return rc;
+    kva::AppendArgs a{};
+    a.k = static_cast<uint16_t *>(const_cast<void *>(k));  // only read
+    a.v = static_cast<const uint16_t *>(v);
+    a.keep_k = 1;
+    set_append_plan(c, layer, a);
+    KVA_HIP(launch_rows(c, layer, a, false, static_cast<hipStream_t>(stream)));
     return KVA_OK;
 }
 
@@ -1012,22 +1196,39 @@ static int project_impl(kva_cache *c, int32_t layer, const void *x, int32_t hidd
     kva::ProductPlan plan{};
     bool planned = kva::plan_product(a, true, c->n_cu, c->part_floats, plan);
     c->last_product = plan;
+    if ((rc = check_rows8_capture(c))) return rc;
     if ((rc = require_device(c))) return rc;
-    a.k_pool = c->d_k + c->layer_elems * layer;
-    a.v_pool = c->d_v + c->layer_elems * layer;
+    // Onto an 8-bit cache the projection leaves its rows in token order (token t
+    // in slot t of a sequence whose i-th page is block i) and an append of rows
+    // takes them from there.
+    uint16_t *staged_v = c->int8 ? c->d_stage + static_cast<size_t>(c->cfg.max_step_tokens) * c->row_elems : nullptr;
+    a.k_pool = c->int8 ? c->d_stage : c->d_k + c->layer_elems * layer;
+    a.v_pool = c->int8 ? staged_v : c->d_v + c->layer_elems * layer;
+    if (c->int8) {
+        a.table = c->d_count;
+        a.table_stride = 0;
+    }
     for (int32_t t0 = 0; t0 < c->st_n_tok; t0 += per) {
         a.x = static_cast<const uint16_t *>(x) + t0 * h;
         a.q_out = static_cast<uint16_t *>(q_out) + t0 * q_row;
         a.gate_out = q_gate_out ? static_cast<uint16_t *>(q_gate_out) + t0 * q_row : nullptr;
         a.kv_out = kv_out ? static_cast<uint16_t *>(kv_out) + t0 * kv_row : nullptr;
         a.tok_seq = at<int32_t>(c->d_step, c->off_tseq) + t0;
-        a.tok_slot = at<int32_t>(c->d_step, c->off_tslot) + t0;
+        a.tok_slot = (c->int8 ? c->d_count : at<int32_t>(c->d_step, c->off_tslot)) + t0;
         a.tok_pos = at<int32_t>(c->d_step, c->off_tpos) + t0;
         if (const int32_t n = std::min(per, c->st_n_tok - t0); n != a.n_tok) {
             a.n_tok = n;
             planned = kva::plan_product(a, true, c->n_cu, c->part_floats, plan);
         }
         KVA_HIP(planned ? kva::launch_project(a, plan, static_cast<hipStream_t>(stream)) : hipErrorInvalidValue);
+    }
+    if (c->int8) {
+        kva::AppendArgs rows{};
+        rows.k = c->d_stage;
+        rows.v = staged_v;
+        rows.keep_k = 1;
+        set_append_plan(c, layer, rows);
+        KVA_HIP(launch_rows(c, layer, rows, false, static_cast<hipStream_t>(stream)));
     }
     c->last_proj_path = c->st_n_tok > kva::kProjTokens ? KVA_PROJECT_PREFILL_GEMM : KVA_PROJECT_KERNELS;
     return KVA_OK;
@@ -1086,6 +1287,7 @@ int kva_timeline_enable(kva_cache *c, int32_t on) {
     if (!c) return fail(KVA_ERR_INVALID_ARG, "cache is NULL");
     if (int rc = require_device(c)) return rc;
     if (int rc = refuse_while_capturing(c, "kva_timeline_enable")) return rc;
+    if (int rc = refuse_int8(c, "the decode timeline")) return rc;
     if (!on) {
         if (c->d_timeline) KVA_HIP(hipFree(c->d_timeline));
         c->d_timeline = nullptr;
@@ -1225,8 +1427,10 @@ static int decode_impl(kva_cache *c, int32_t layer, const void *q, const void *g
     a.gate = static_cast<const uint16_t *>(gate);
     a.gate_stride = gate_stride;
     a.q = static_cast<const uint16_t *>(q);
-    a.k_pool = c->d_k + c->layer_elems * layer;
-    a.v_pool = c->d_v + c->layer_elems * layer;
+    if (!c->int8) {
+        a.k_pool = c->d_k + c->layer_elems * layer;
+        a.v_pool = c->d_v + c->layer_elems * layer;
+    }
     a.table = c->d_table;
     a.table_stride = c->cfg.max_blocks_per_seq;
     a.seq_ids = at<int32_t>(c->d_step, c->off_seq);
@@ -1237,8 +1441,9 @@ static int decode_impl(kva_cache *c, int32_t layer, const void *q, const void *g
     a.num_heads = c->cfg.num_heads;
     a.num_kv_heads = c->cfg.num_kv_heads;
     set_stream_k(c, a, c->st_total_pages, c->cfg.num_heads);
-    if ((a.whole = use_whole(c, c->split_user, c->st_max_ctx, c->st_n_seqs, c->cfg.num_heads,
-                             c->cfg.num_kv_heads, c->n_cu))) {
+    c->last_whole = false;
+    if (!c->int8 && (a.whole = use_whole(c, c->split_user, c->st_max_ctx, c->st_n_seqs, c->cfg.num_heads,
+                                         c->cfg.num_kv_heads, c->n_cu))) {
         // Every launch of this form reads the lengths from the step plan: a
         // recorded one stays correct when they grow.
     } else if (c->capturing) {
@@ -1265,8 +1470,15 @@ static int decode_impl(kva_cache *c, int32_t layer, const void *q, const void *g
             a.fused = 1;
             a.app = ap;
         } else {
-            KVA_HIP(kva::launch_append(ap, static_cast<hipStream_t>(stream)));
+            KVA_HIP(launch_rows(c, layer, ap, true, static_cast<hipStream_t>(stream)));
         }
+    }
+    if (c->int8) {
+        kva::Decode8Args d{};
+        d.d = a;
+        set_layer8(c, layer, d);
+        KVA_HIP(kva::launch_decode8(d, static_cast<hipStream_t>(stream)));
+        return KVA_OK;
     }
     KVA_HIP(kva::launch_decode(a, static_cast<hipStream_t>(stream)));
     return KVA_OK;
@@ -1323,6 +1535,67 @@ int kva_append_qknorm_rope(kva_cache *c, int32_t layer, void *q, void *k, const 
     if (rc == KVA_OK && c->capturing && c->st_n_tok > 0)
         c->cap_table_rows = c->cap_table_rows ? std::min(c->cap_table_rows, table_rows) : table_rows;
     return capture_note(c, rc);
+}
+
+int kva_append_rows(kva_cache *c, int32_t layer, const void *k, const void *v, kva_stream_t stream) {
+    int rc = capture_check(c, stream);
+    if (rc) return capture_note(c, rc);
+    return capture_note(c, append_rows_impl(c, layer, k, v, stream));
+}
+
+int kva_read_rows(kva_cache *c, int32_t layer, int32_t n_seqs, const int32_t *seq_ids, const int32_t *first,
+                  const int32_t *count, void *k_out, void *v_out, kva_stream_t stream) {
+    if (!c) return fail(KVA_ERR_INVALID_ARG, "cache is NULL");
+    if (int rc = refuse_while_capturing(c, "kva_read_rows")) return rc;
+    int rc = check_layer(c, layer);
+    if (rc) return rc;
+    if (n_seqs < 0) return fail(KVA_ERR_INVALID_ARG, "n_seqs %d < 0", n_seqs);
+    if (n_seqs > 0 && (!seq_ids || !first || !count)) return fail(KVA_ERR_INVALID_ARG, "NULL index array");
+    std::vector<int32_t> touches;
+    int64_t rows = 0;
+    for (int32_t b = 0; b < n_seqs; ++b) {
+        const int32_t s = seq_ids[b];
+        if ((rc = check_seq(c, s))) return rc;
+        if (first[b] < 0 || count[b] < 0 || static_cast<int64_t>(first[b]) + count[b] > c->len[s])
+            return fail(KVA_ERR_INVALID_ARG, "sequence %d: rows [%d, %d + %d) outside its %d", s, first[b], first[b],
+                        count[b], c->len[s]);
+        if (rows + count[b] > INT32_MAX) return fail(KVA_ERR_INVALID_ARG, "more than %d rows", INT32_MAX);
+        const int32_t end = first[b] + count[b];
+        for (int32_t at = first[b]; at < end;) {
+            const int32_t page = at / kva::kBlockTokens, r0 = at % kva::kBlockTokens;
+            const int32_t n = std::min(end - at, kva::kBlockTokens - r0);
+            const int32_t open = c->int8 && c->open_page[s] == page;
+            touches.insert(touches.end(), {s, page, static_cast<int32_t>(rows), r0, n, open, 0, 0});
+            at += n;
+            rows += n;
+        }
+    }
+    if (rows > 0) {
+        if (!k_out || !v_out) return fail(KVA_ERR_INVALID_ARG, "NULL tensor pointer");
+        if (!aligned16(k_out) || !aligned16(v_out))
+            return fail(KVA_ERR_MISALIGNED, "k_out and v_out must be 16-byte aligned");
+    }
+    if ((rc = require_device(c))) return rc;
+    if (rows == 0) return KVA_OK;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if ((rc = flush_patches(c, s))) return rc;
+    kva::ReadRowsArgs a{};
+    a.num_kv_heads = c->cfg.num_kv_heads;
+    a.table = c->d_table;
+    a.table_stride = c->cfg.max_blocks_per_seq;
+    if (c->int8) {
+        set_layer8(c, layer, a);
+    } else {
+        a.k_pool = c->d_k + c->layer_elems * layer;
+        a.v_pool = c->d_v + c->layer_elems * layer;
+    }
+    a.k_out = static_cast<uint16_t *>(k_out);
+    a.v_out = static_cast<uint16_t *>(v_out);
+    return upload_touches(c, touches, s, [&](const int32_t *recs, int32_t n) {
+        a.touch = recs;
+        a.n_touch = n;
+        return kva::launch_read_rows(a, s);
+    });
 }
 
 int kva_project_append(kva_cache *c, int32_t layer, const void *x, int32_t hidden, const void *w_q_fused,
@@ -1424,20 +1697,25 @@ static int multi_query(kva_cache *c, int32_t layer, const void *q, void *out, kv
     int rc = check_layer(c, layer);
     if (rc) return rc;
     if (!c->step_valid) return fail(KVA_ERR_STATE, "no step begun (kva_step_begin)");
+    if (tree && (rc = refuse_int8(c, "kva_tree_verify"))) return rc;
     if (tree && !c->st_has_bits) return fail(KVA_ERR_STATE, "tree verify needs tree_bits in kva_step_begin");
     if (!q || !out) return fail(KVA_ERR_INVALID_ARG, "NULL tensor pointer");
     if (!aligned16(q) || !aligned16(out)) return fail(KVA_ERR_MISALIGNED, "q/out must be 16-byte aligned");
     if ((rc = check_gate(gate, gate_stride, c->cfg.num_heads))) return rc;
     if ((rc = require_device(c))) return rc;
     if (c->st_n_tok == 0) return KVA_OK;
-    if (append) KVA_HIP(kva::launch_append(*append, static_cast<hipStream_t>(stream)));
+    if (append) KVA_HIP(launch_rows(c, layer, *append, true, static_cast<hipStream_t>(stream)));
     kva::MultiQueryArgs a{};
     a.gate = static_cast<const uint16_t *>(gate);
     a.gate_stride = gate_stride;
     a.q = static_cast<const uint16_t *>(q);
     a.out = static_cast<uint16_t *>(out);
-    a.k_pool = c->d_k + c->layer_elems * layer;
-    a.v_pool = c->d_v + c->layer_elems * layer;
+    if (c->int8) {
+        set_layer8(c, layer, a);
+    } else {
+        a.k_pool = c->d_k + c->layer_elems * layer;
+        a.v_pool = c->d_v + c->layer_elems * layer;
+    }
     a.table = c->d_table;
     a.table_stride = c->cfg.max_blocks_per_seq;
     a.seq_ids = at<int32_t>(c->d_step, c->off_seq);
@@ -1569,6 +1847,8 @@ int kva_rollback(kva_cache *c, int32_t n_seqs, const int32_t *seq_ids, const int
         round_up(n_moves_all * 3 * sizeof(int32_t), 16) + (n_groups_all + 1) * sizeof(int32_t) > c->aux_bytes)
         return fail(KVA_ERR_CAPACITY, "rollback moves %zu rows, more than the staging area holds (%zu bytes)",
                     n_moves_all, c->aux_bytes);
+    if (n_moves_all > 0)
+        if (int rc = refuse_int8(c, "a rollback that moves rows")) return rc;
     for (int32_t b = 0; b < n_seqs; ++b) {
         const int32_t s = seq_ids[b];
         const int32_t n = keep_off[b + 1] - keep_off[b];
@@ -1652,8 +1932,9 @@ int kva_graph_capture_end(kva_cache *c, kva_stream_t stream, kva_graph **out) {
     g->table_rows = c->cap_table_rows;
     g->all_one = c->st_all_one;
     g->has_bits = c->st_has_bits;
-    const size_t offs[12] = {c->off_seq,  c->off_ctx,  c->off_start, c->off_tokoff, c->off_tseq,  c->off_tslot,
-                             c->off_tpos, c->off_bits, c->off_pre,   c->off_upre,   c->off_mqpre, c->off_pids};
+    const size_t offs[13] = {c->off_seq,  c->off_ctx,  c->off_start, c->off_tokoff, c->off_tseq,
+                             c->off_tslot, c->off_tpos, c->off_bits, c->off_pre,    c->off_upre,
+                             c->off_mqpre, c->off_pids, c->off_touch};
     std::memcpy(g->offs, offs, sizeof(offs));
     *out = g;
     return KVA_OK;
@@ -1664,8 +1945,9 @@ int kva_graph_launch(kva_graph *g, kva_stream_t stream) {
     kva_cache *c = g->cache;
     if (c->capturing) return fail(KVA_ERR_STATE, "a graph is being recorded");
     if (!c->step_valid) return fail(KVA_ERR_STATE, "no step begun (kva_step_begin)");
-    const size_t offs[12] = {c->off_seq,  c->off_ctx,  c->off_start, c->off_tokoff, c->off_tseq,  c->off_tslot,
-                             c->off_tpos, c->off_bits, c->off_pre,   c->off_upre,   c->off_mqpre, c->off_pids};
+    const size_t offs[13] = {c->off_seq,  c->off_ctx,  c->off_start, c->off_tokoff, c->off_tseq,
+                             c->off_tslot, c->off_tpos, c->off_bits, c->off_pre,    c->off_upre,
+                             c->off_mqpre, c->off_pids, c->off_touch};
     if (c->st_n_seqs != g->n_seqs || c->st_n_tok != g->n_tok || c->st_all_one != g->all_one ||
         c->st_has_bits != g->has_bits || std::memcmp(offs, g->offs, sizeof(offs)) != 0)
         return fail(KVA_ERR_STATE, "the current step (%d sequences, %d tokens) is not the recorded shape (%d, %d)",

@@ -17,6 +17,12 @@ constexpr int kSplitQuantum = 16; // decode split sizes are whole pages
 constexpr int kCombineRecs = 64;  // sequences whose combine facts travel in the decode arguments
 constexpr int kPlanPages = 64;    // page ids per sequence in the step plan (one per lane)
 constexpr int kCombineChunk = 16; // decode partials a combine wave requests together
+constexpr size_t kPageElems = kBlockTokens * kHeadDim;  // values of a block: a KV head's share of a page, K or V
+// A touch: the rows of one page that a step writes or a read wants.  int32
+// words: sequence, page of it, first row's place among the step's tokens (or
+// the output's rows), first row within the page, rows, 1 if the page is the
+// sequence's open block; two spare.
+constexpr int kTouchWords = 8;
 
 // Fused QK-RMSNorm + RoPE + K/V append over all new tokens of a step.
 struct AppendArgs {
@@ -219,6 +225,8 @@ struct DecodeArgs {
 constexpr int kTimelineWords = 4;
 constexpr int kWholeWaves = 8;  // waves per whole-sequence decode workgroup
 hipError_t launch_decode(const DecodeArgs &a, hipStream_t s);
+// The merge of a stream-K launch's partials by itself.
+hipError_t launch_decode_merge(const DecodeArgs &a, hipStream_t s);
 
 // Static device scratch of kva_legacy_decode_noalloc (k_noalloc.hip): the
 // decode partial slots [2*n_wg][H][256] floats, then [2*n_wg][H][2].
@@ -299,6 +307,11 @@ struct MultiQueryArgs {
     int64_t gate_stride;
     // Events around mq_kernel itself (null: none), as in DecodeArgs.
     hipEvent_t ev_before, ev_after;
+    // 8-bit cache (k8 null: FP16): this layer's codes, scales and open blocks,
+    // as in Store8Args.
+    const uint8_t *k8, *v8;
+    const float *scales;
+    const uint16_t *open;
 };
 // Keys per multi-query block.  64 for a step of eight-wave prefill tiles
 // (half the barriers, page lookups and softmax reductions per key, two LDS
@@ -346,5 +359,56 @@ constexpr int mq_waves_for(int G, int max_new) { return max_new * G <= 64 ? 4 : 
 // 512 after 4000 (26) 83 + 15 against 80 + 11.
 constexpr bool mq_two_tiles(int64_t blocks, int32_t wgs) { return blocks >= 48 * static_cast<int64_t>(wgs); }
 hipError_t launch_multi_query(const MultiQueryArgs &a, hipStream_t s);
+
+// ---- the 8-bit cache (page order, scales, codes: k_page8.h) ----
+
+// Append into an 8-bit cache.  norm: ap.q and ap.k as in launch_append; else
+// ap.k and ap.v are rows as the cache takes them, and ap.q is not touched.
+struct Store8Args {
+    AppendArgs ap;
+    const int32_t *touch;     // device [n_touch][kTouchWords]
+    int32_t n_touch;
+    int32_t norm;
+    uint8_t *k8, *v8;         // this layer's codes [blocks][Hkv][kPageElems]
+    float *scales;            // [blocks][Hkv][2]: K's, V's
+    uint16_t *open;           // open blocks [max_seqs][Hkv][2][kPageElems]
+};
+hipError_t launch_store8(const Store8Args &a, hipStream_t s);
+// append_rows on an FP16 cache: ap.k, ap.v to their slots as they are.
+hipError_t launch_copy_rows(const AppendArgs &a, hipStream_t s);
+// Decode over an 8-bit cache: d as in launch_decode, on its paged stream-K
+// path, but for the pools.
+struct Decode8Args {
+    DecodeArgs d;
+    const uint8_t *k8, *v8;   // as in Store8Args
+    const float *scales;
+    const uint16_t *open;
+};
+hipError_t launch_decode8(const Decode8Args &a, hipStream_t s);
+// Rows as FP16, from an FP16 cache (k8 null) or an 8-bit one.
+struct ReadRowsArgs {
+    const int32_t *touch;
+    int32_t n_touch;
+    int32_t num_kv_heads;
+    const int32_t *table;
+    int32_t table_stride;
+    const uint16_t *k_pool, *v_pool;
+    const uint8_t *k8, *v8;
+    const float *scales;
+    const uint16_t *open;
+    uint16_t *k_out, *v_out;  // [rows][Hkv][256]
+};
+hipError_t launch_read_rows(const ReadRowsArgs &a, hipStream_t s);
+// Open blocks from their pages' codes, in every layer (bases of layer 0).
+struct ReopenArgs {
+    const int32_t *touch;     // device [n][kTouchWords]: sequence, page
+    const int32_t *table;
+    int32_t table_stride;
+    const uint8_t *k8, *v8;
+    const float *scales;
+    uint16_t *open;
+    size_t layer_codes, layer_scales, layer_open;  // elements between layers
+};
+hipError_t launch_reopen(const ReopenArgs &a, int32_t n, int32_t num_kv_heads, int32_t n_layers, hipStream_t s);
 
 }  // namespace kva

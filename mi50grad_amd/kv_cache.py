@@ -1,4 +1,4 @@
-"""Paged FP16 KV cache (libkvattn) and the reference-compatible ``KVCache``.
+"""Paged FP16 or 8-bit KV cache (libkvattn) and the reference-compatible ``KVCache``.
 
 ``PagedKVCache`` is the full interface: ragged per-sequence lengths, a block
 table per sequence, per-step plans shared by all layers, and the hot-path
@@ -37,10 +37,15 @@ class PagedKVCache:
     def __init__(self, n_layers: int, max_seqs: int, max_blocks: int, max_blocks_per_seq: int,
                  max_step_tokens: int = 4096, num_heads: int = 24, num_kv_heads: int = 4,
                  head_dim: int = HEAD_DIM, rotary_dim: int = 64, eps: float = 1e-6,
-                 host_only: bool = False):
+                 host_only: bool = False, kv_bits: int = 16):
+        """kv_bits: 16 (FP16 rows) or 8 (codes with a scale per page and KV
+        head, KVA_FLAG_INT8)."""
+        if kv_bits not in (8, 16):
+            raise ValueError(f"kv_bits {kv_bits}: 8 or 16")
         cfg = _lib.KvaConfig(n_layers, num_heads, num_kv_heads, head_dim, rotary_dim, BLOCK_TOKENS,
                              max_seqs, max_blocks, max_blocks_per_seq, max_step_tokens, eps,
-                             _lib.KVA_FLAG_HOST_ONLY if host_only else 0)
+                             (_lib.KVA_FLAG_HOST_ONLY if host_only else 0) |
+                             (_lib.KVA_FLAG_INT8 if kv_bits == 8 else 0))
         self.cfg = cfg
         h = ctypes.c_void_p()
         _lib.call("kva_create", ctypes.byref(cfg), ctypes.byref(h))
@@ -50,6 +55,7 @@ class PagedKVCache:
         self.num_kv_heads = num_kv_heads
         self.head_dim = head_dim
         self.host_only = host_only
+        self.kv_bits = kv_bits
         lay = _lib.KvaLayout()
         _lib.call("kva_get_layout", self.handle, ctypes.byref(lay))
         self.row_bytes = lay.row_bytes
@@ -147,6 +153,20 @@ class PagedKVCache:
                stream=None) -> None:
         _lib.call("kva_append_qknorm_rope", self.handle, layer, _ptr(q), _ptr(k), _ptr(v),
                   _ptr(q_norm_w), _ptr(k_norm_w), _ptr(cos_tab), _ptr(sin_tab), table_rows, stream)
+
+    def append_rows(self, layer: int, k, v, stream=None) -> None:
+        """The step's K/V rows as they are (normalised and rotated already):
+        k, v [T, Hkv, 256], only read."""
+        _lib.call("kva_append_rows", self.handle, layer, _ptr(k), _ptr(v), stream)
+
+    def read_rows(self, layer: int, seq_ids: Sequence[int], first: Sequence[int], count: Sequence[int], k_out, v_out,
+                  stream=None) -> None:
+        """Rows [first, first + count) of each sequence as FP16, packed:
+        k_out, v_out [sum of count, Hkv, 256], the values the cache holds."""
+        if not len(seq_ids) == len(first) == len(count):
+            raise ValueError("seq_ids, first and count differ in length")
+        _lib.call("kva_read_rows", self.handle, layer, len(seq_ids), _lib.int_array(seq_ids), _lib.int_array(first),
+                  _lib.int_array(count), _ptr(k_out), _ptr(v_out), stream)
 
     def append_decode(self, layer: int, q, k, v, q_norm_w, k_norm_w, cos_tab, sin_tab, table_rows: int, out,
                       stream=None, gate=None, gate_stride: int = 0) -> None:

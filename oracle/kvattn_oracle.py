@@ -434,3 +434,81 @@ def partial_softmax(q_row, k, v):
     m = np.max(s)
     e = np.exp(s - m)
     return m, e.sum(), e @ v.astype(np.float64)
+
+
+# ---- the 8-bit cache --------------------------------------------------------
+
+def int8_scale(amax: float) -> float:
+    """The scale of a block whose largest magnitude is `amax`: the smallest
+    m * 2^e with m in 8..15 and e >= -24 for which 127 scale >= amax, at most
+    512.  By search over whole numbers, so no rounding enters."""
+    from fractions import Fraction
+
+    a = Fraction(float(amax))
+    for e in range(-24, 7):
+        for m in range(8, 16):
+            s = Fraction(m) * Fraction(2) ** e
+            if 127 * s >= a or s == 512:
+                return float(s)
+    raise AssertionError
+
+
+def int8_block(x: np.ndarray) -> tuple[np.ndarray, float]:
+    """Codes and scale of one full block x [16, 256] (finite fp16)."""
+    x = np.asarray(x, np.float64)
+    s = int8_scale(np.max(np.abs(x)))
+    return np.clip(np.rint(x / s), -127, 127), s
+
+
+def int8_rows(k: np.ndarray, v: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
+    """What an 8-bit cache holds of a sequence's rows k, v [L, Hkv, 256] fp16
+    (as float64): full 16-row pages as codes times scale per KV head, the rows
+    behind the last full page as they are.  A row of a head with a value that
+    is not finite: NaN keys, zero values; in a full page every row of the head
+    gets NaN keys."""
+    k, v = np.array(k, np.float64), np.array(v, np.float64)
+    bad = ~(np.isfinite(k).all(-1) & np.isfinite(v).all(-1))  # [L, Hkv]
+    k[bad], v[bad] = np.nan, 0.0
+    for p in range(k.shape[0] // 16):
+        rows = slice(16 * p, 16 * p + 16)
+        for h in range(k.shape[1]):
+            c, s = int8_block(v[rows, h])
+            v[rows, h] = c * s
+            if bad[rows, h].any():
+                k[rows, h] = np.nan
+            else:
+                c, s = int8_block(k[rows, h])
+                k[rows, h] = c * s
+    return k, v
+
+
+def attention_bound(q, k, v, seen=None, gate=None):
+    """Causal or plain attention in float64 of q [n, H, 256] over k, v [L,
+    Hkv, 256] (seen: [n, L] bool), and how far a result may be off that sums in
+    float32, rounds its probabilities and its output to fp16 (each half a
+    step): the probabilities' rounding eps moves an output by sum p eps (v -
+    out), a score's error delta by as much times delta, the output's by itself."""
+    n, H, d = q.shape
+    hkv = k.shape[1]
+    G = H // hkv
+    q = np.asarray(q, np.float64)
+    half = np.finfo(np.float16).eps / 2
+    f32 = np.finfo(np.float32).eps / 2
+    out, tol = np.empty_like(q), np.empty_like(q)
+    for h in range(H):
+        kh, vh = k[:, h // G], v[:, h // G]
+        s = q[:, h] @ kh.T / 16.0
+        size = np.abs(q[:, h]) @ np.nan_to_num(np.abs(kh)).T / 16.0
+        delta = (d + 8) * f32 * size.max() + 16 * f32
+        if seen is not None:
+            s = np.where(seen, s, -np.inf)
+        p = np.exp(s - s.max(-1, keepdims=True))
+        p /= p.sum(-1, keepdims=True)
+        out[:, h] = p @ vh
+        # |v - out| <= |v| + |out|; the float32 sums of p and p v round as well
+        tol[:, h] = (half + 2 * delta + 64 * f32) * (p @ np.abs(vh) + np.abs(out[:, h]))
+    if gate is not None:
+        g = 1.0 / (1.0 + np.exp(-np.asarray(gate, np.float64)))
+        tol = tol * g + half * np.abs(out) * g  # the ungated output is rounded first
+        out = out * g
+    return out, tol + half * np.abs(out) + np.finfo(np.float16).smallest_subnormal

@@ -1,0 +1,131 @@
+"""The 8-bit cache without a GPU: its oracle against exact arithmetic, and what
+its calls refuse (a host-only cache reports every refusal)."""
+from fractions import Fraction
+
+import numpy as np
+import pytest
+
+from mi50grad_amd._lib import KvaError
+from mi50grad_amd.kv_cache import PagedKVCache
+from oracle import kvattn_oracle as orc
+
+UNSUPPORTED, STATE, INVALID, NO_DEVICE, MISALIGNED, BAD_SEQ = -2, -8, -1, -3, -10, -6
+
+
+def make(**kw):
+    args = dict(n_layers=2, max_seqs=4, max_blocks=20, max_blocks_per_seq=8, max_step_tokens=64, host_only=True,
+                kv_bits=8)
+    args.update(kw)
+    return PagedKVCache(**args)
+
+
+def refused(code, call, *args, **kw):
+    with pytest.raises(KvaError) as e:
+        call(*args, **kw)
+    assert e.value.code == code, e.value
+
+
+def test_scale_is_the_smallest_of_its_kind():
+    scales = sorted(m * 2.0 ** e for m in range(8, 16) for e in range(-24, 6)) + [512.0]
+    rng = np.random.default_rng(0)
+    tops = np.concatenate([[0.0, 2.0 ** -24, 65504.0, 65024.0, 1.0], np.exp(rng.uniform(-16, 11, 300))])
+    for top in tops.astype(np.float16).astype(np.float64):
+        want = next((s for s in scales if Fraction(127) * Fraction(s) >= Fraction(top)), 512.0)
+        assert orc.int8_scale(top) == want
+
+
+def test_values_are_fp16_numbers():
+    """Codes of every scale times the scale: exact in fp16."""
+    codes = np.arange(-127, 128, dtype=np.float64)
+    for e in range(-24, 7):
+        for m in range(8, 16):
+            s = m * 2.0 ** e
+            if s <= 512:
+                assert np.array_equal((codes * s).astype(np.float16).astype(np.float64), codes * s)
+
+
+def test_codes_do_not_depend_on_the_arithmetic():
+    """x / s in float32 rounds to the code that exact arithmetic gives, for
+    every fp16 magnitude of some binades and every significand of s."""
+    for m in range(8, 16):
+        s = m * 2.0 ** -9
+        x = np.arange(0x0001, 0x7c00, dtype=np.uint16).view(np.float16)
+        x = x[x.astype(np.float64) <= 127 * s]
+        got = np.rint(x.astype(np.float32) / np.float32(s)).astype(int)
+        num = [Fraction(float(v)) / Fraction(s) for v in x]
+        want = [int(n) + (1 if n - int(n) > Fraction(1, 2) or (n - int(n) == Fraction(1, 2) and int(n) % 2) else 0)
+                for n in num]
+        assert np.array_equal(got, want)
+
+
+def test_full_pages_only_are_rounded():
+    rng = np.random.default_rng(1)
+    k, v = [rng.standard_normal((20, 2, 256)).astype(np.float16) for _ in range(2)]
+    gk, gv = orc.int8_rows(k, v)
+    assert np.array_equal(gk[16:], k[16:]) and np.array_equal(gv[16:], v[16:])
+    assert not np.array_equal(gk[:16], k[:16])
+    assert np.array_equal(orc.int8_rows(k[:15], v[:15])[0], k[:15])
+
+
+def test_attention_bound_is_attention():
+    rng = np.random.default_rng(2)
+    q, k, v = rng.standard_normal((3, 6, 256)), rng.standard_normal((20, 2, 256)), rng.standard_normal((20, 2, 256))
+    seen = orc.chunk_visibility(17, 3)
+    out, tol = orc.attention_bound(q, k, v, seen)
+    want = orc.attention_fp32(q.astype(np.float32), k, v, seen)
+    assert np.abs(out - want).max() < 1e-5 and (tol > 0).all() and tol.max() < 5e-3
+
+
+def test_addresses_and_moves_are_refused():
+    c = make()
+    c.reserve(0, 32)
+    refused(NO_DEVICE, c.layer_pools, 0)
+    refused(UNSUPPORTED, c.begin_step, [0], [2], tree_bits=[1, 3])
+    c.begin_step([0], [20])
+    refused(UNSUPPORTED, c.tree_verify, 0, 16, 16)
+    refused(UNSUPPORTED, c.rollback, [0], [4], [[0, 2]])
+    assert c.seq_len(0) == 20
+    c.rollback([0], [4], [[0, 1, 2]])  # a prefix moves nothing
+    assert c.seq_len(0) == 7
+
+
+def test_length_goes_up_only_to_rows_written():
+    c = make()
+    c.reserve(0, 100)
+    refused(STATE, c.set_len, 0, 1)
+    c.begin_step([0], [40])
+    c.set_len(0, 10)
+    c.set_len(0, 40)
+    c.set_len(0, 20)
+    c.begin_step([0], [1])
+    refused(STATE, c.set_len, 0, 22)
+    c.free_seq(0)
+    c.reserve(0, 100)
+    refused(STATE, c.set_len, 0, 1)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_append_rows_and_read_rows_refuse(bits):
+    c = make(kv_bits=bits)
+    refused(STATE, c.append_rows, 0, 16, 16)
+    c.begin_step([1, 2], [3, 0])
+    refused(INVALID, c.append_rows, 2, 16, 16)
+    refused(INVALID, c.append_rows, 0, None, 16)
+    refused(MISALIGNED, c.append_rows, 0, 16, 24)
+    refused(NO_DEVICE, c.append_rows, 0, 16, 16)
+    refused(BAD_SEQ, c.read_rows, 0, [4], [0], [0], 16, 16)
+    refused(INVALID, c.read_rows, 0, [1], [1], [3], 16, 16)
+    refused(INVALID, c.read_rows, 0, [1], [-1], [1], 16, 16)
+    refused(INVALID, c.read_rows, 0, [1], [0], [-1], 16, 16)
+    refused(INVALID, c.read_rows, -1, [1], [0], [1], 16, 16)
+    refused(INVALID, c.read_rows, 0, [1], [0], [1], None, 16)
+    refused(MISALIGNED, c.read_rows, 0, [1], [0], [1], 16, 20)
+    refused(NO_DEVICE, c.read_rows, 0, [1], [0], [3], 16, 16)
+    with pytest.raises(ValueError):
+        c.read_rows(0, [1, 2], [0], [1], 16, 16)
+
+
+def test_kinds_of_cache():
+    with pytest.raises(ValueError):
+        make(kv_bits=4)
+    assert make().row_bytes * 2 == make(kv_bits=16).row_bytes
