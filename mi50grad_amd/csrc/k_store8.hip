@@ -7,7 +7,10 @@
 // the workgroup takes the rows that came earlier from the sequence's open
 // block and writes the page's codes: from FP16 rows always, so a page's codes do
 // not depend on the steps that its rows came in.  Otherwise the new rows join
-// the open block.  Query rows are normalised by further workgroups of the launch.
+// the open block.  Where a step closes the open page and leaves rows in a later
+// one, one workgroup does both: the open block's old rows have been read when
+// its new ones are written.  Query rows are normalised by further workgroups of
+// the launch.
 //
 // Bound by latency for a decode step (a touch is one row) and by memory
 // for a prompt.
@@ -41,33 +44,39 @@ __global__ __launch_bounds__(kThreads) void store8_kernel(Store8Args a) {
     const int u = blockIdx.x / hkv, h = blockIdx.x - u * hkv;
     const int32_t *rec = a.touch + static_cast<size_t>(u) * kTouchWords;
     const int seq = ld_uniform(rec), page = ld_uniform(rec + 1), tok0 = ld_uniform(rec + 2);
-    const int r0 = ld_uniform(rec + 3), n = ld_uniform(rec + 4);
+    const int r0 = ld_uniform(rec + 3), n = ld_uniform(rec + 4), tok1 = ld_uniform(rec + 5), n1 = ld_uniform(rec + 6);
     const bool closes = r0 + n == kBlockTokens;  // uniform over the workgroup
     uint16_t *open = a.open + (static_cast<size_t>(seq) * hkv + h) * 2 * kPageElems;
-    BlockRow x{};
-    const bool fresh = row >= r0 && row < r0 + n;
-    const int t = tok0 + row - r0;
-    if (fresh) {
-        const size_t at = (static_cast<size_t>(t) * hkv + h) * kHeadDim + 8 * l32;
-        x.k = ld16(ap.k + at);
-        x.v = ld16(ap.v + at);
-    } else if (closes) {  // row < r0
-        x = load_open_row(open, row, l32);
-    }
-    if (a.norm) {  // every half-wave runs the arithmetic, so its lane exchanges are whole
-        const int pos = fresh ? ap.tok_pos[t] : 0;
-        const NormRopeIn in = norm_rope_in<32>(ap.k_w, ap.cos_tab + static_cast<size_t>(pos) * ap.half_rot,
-                                               ap.sin_tab + static_cast<size_t>(pos) * ap.half_rot, ap.half_rot, l32);
-        const uint4 y = norm_rope_apply<32>(x.k, in, ap.half_rot, ap.eps, l32);
-        if (fresh) {
-            x.k = y;
-            if (!ap.keep_k) st16(ap.k + (static_cast<size_t>(t) * hkv + h) * kHeadDim + 8 * l32, y);
+    // Token t's row, as the cache takes it; every half-wave of a wave calls it
+    // (one without a row with t = -1), so the lane exchanges are whole.
+    auto fresh_row = [&](int t) -> BlockRow {
+        BlockRow x{};
+        const size_t at = (static_cast<size_t>(max(t, 0)) * hkv + h) * kHeadDim + 8 * l32;
+        if (t >= 0) {
+            x.k = ld16(ap.k + at);
+            x.v = ld16(ap.v + at);
         }
-    }
-    mend_row(x);  // an earlier row of the open block has been through this
+        if (a.norm) {
+            const int pos = t >= 0 ? ap.tok_pos[t] : 0;
+            const NormRopeIn in = norm_rope_in<32>(ap.k_w, ap.cos_tab + static_cast<size_t>(pos) * ap.half_rot,
+                                                   ap.sin_tab + static_cast<size_t>(pos) * ap.half_rot, ap.half_rot, l32);
+            x.k = norm_rope_apply<32>(x.k, in, ap.half_rot, ap.eps, l32);
+            if (t >= 0 && !ap.keep_k) st16(ap.k + at, x.k);
+        }
+        mend_row(x);
+        return x;
+    };
+    const bool fresh = row >= r0 && row < r0 + n;
+    BlockRow x = fresh_row(fresh ? tok0 + row - r0 : -1);
     if (!closes) {
         if (fresh) store_open_row(open, row, l32, x);
         return;
+    }
+    if (!fresh) x = load_open_row(open, row, l32);  // row < r0
+    if (n1 > 0) {
+        const BlockRow y = fresh_row(row < n1 ? tok1 + row : -1);
+        __syncthreads();
+        if (row < n1) store_open_row(open, row, l32, y);
     }
     const int blk = ld_uniform(ap.table + static_cast<size_t>(seq) * ap.table_stride + page);
     const size_t b = static_cast<size_t>(blk) * hkv + h;

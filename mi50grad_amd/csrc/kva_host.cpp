@@ -812,12 +812,20 @@ int kva_step_begin(kva_cache *c, int32_t n_seqs, const int32_t *seq_ids, const i
                 reopened.insert(reopened.end(), {s, start / kva::kBlockTokens, 0, 0, 0, 0, 0, 0});
             c->open_page[s] = end % kva::kBlockTokens ? end / kva::kBlockTokens : -1;
             c->held[s] = end;
-            for (int32_t at = start; at < end;) {
-                const int32_t r0 = at % kva::kBlockTokens, n = std::min(end - at, kva::kBlockTokens - r0);
-                touches.insert(touches.end(), {s, at / kva::kBlockTokens, tok, r0, n, 0, 0, 0});
+            // The open page, closed by this step, and the rows that are then open
+            // are one record: the open block holds both, one after the other.
+            const int32_t behind = end % kva::kBlockTokens;
+            const bool both = start % kva::kBlockTokens && behind && end / kva::kBlockTokens != start / kva::kBlockTokens;
+            const int32_t last = both ? end - behind : end;
+            for (int32_t at = start; at < last;) {
+                const int32_t r0 = at % kva::kBlockTokens, n = std::min(last - at, kva::kBlockTokens - r0);
+                const int32_t tok1 = tok + last - at;  // the first of the rows behind
+                touches.insert(touches.end(), {s, at / kva::kBlockTokens, tok, r0, n, r0 && both ? tok1 : 0,
+                                               r0 && both ? behind : 0, 0});
                 at += n;
                 tok += n;
             }
+            tok += end - last;
         }
     }
     const size_t o_cut = o_touch + touches.size() * sizeof(int32_t);

@@ -20,8 +20,9 @@ constexpr int kCombineChunk = 16; // decode partials a combine wave requests tog
 constexpr size_t kPageElems = kBlockTokens * kHeadDim;  // values of a block: a KV head's share of a page, K or V
 // A touch: the rows of one page that a step writes or a read wants.  int32
 // words: sequence, page of it, first row's place among the step's tokens (or
-// the output's rows), first row within the page, rows, 1 if the page is the
-// sequence's open block; two spare.
+// the output's rows), first row within the page, rows; then for a read 1 if the
+// page is the sequence's open block, for a write that closes the open page the
+// step's first row of the page that is open then, and its rows (0: none).
 constexpr int kTouchWords = 8;
 
 // Fused QK-RMSNorm + RoPE + K/V append over all new tokens of a step.

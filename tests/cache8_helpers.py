@@ -17,7 +17,7 @@ def rows(rng, n, kv, size=1.0):
     return (k * size).astype(np.float16), (v * size).astype(np.float16)
 
 
-def make(lens, heads=24, kv=4, layers=1, bits=8, extra=0, step=4096, spare=0, slots=None):
+def make(lens, heads=24, kv=4, layers=1, bits=8, extra=0, step=8192, spare=0, slots=None):
     """A cache with a permuted block list per sequence, room for `extra` rows
     behind each length."""
     need = [(n + extra + 15) // 16 for n in lens]

@@ -49,6 +49,26 @@ def test_rows_held(device, kv, how):
     cache.destroy()
 
 
+def test_rows_that_close_the_open_page_and_open_another(device):
+    """A sequence's open block is read for the page that closes and written for
+    the page that is open then, in one step, for many sequences and heads at once."""
+    say("close and open")
+    rng = np.random.default_rng(14)
+    kv, B = 8, 48
+    old = [int(x) for x in rng.integers(1, 16, B)]
+    new = [16 - o + 16 * int(p) + int(r) for o, p, r in zip(old, rng.integers(0, 3, B), rng.integers(1, 16, B))]
+    cache = make([o + n for o, n in zip(old, new)], heads=kv, kv=kv)
+    data = [rows(rng, o + n, kv) for o, n in zip(old, new)]
+    seqs = list(range(B))
+    put(device, cache, seqs, [d[0][:o] for d, o in zip(data, old)], [d[1][:o] for d, o in zip(data, old)])
+    put(device, cache, seqs, [d[0][o:] for d, o in zip(data, old)], [d[1][o:] for d, o in zip(data, old)])
+    got = held(device, cache, seqs)
+    want = [orc.int8_rows(*d) for d in data]
+    assert same_bits(got[0], np.concatenate([w[0] for w in want]))
+    assert same_bits(got[1], np.concatenate([w[1] for w in want]))
+    cache.destroy()
+
+
 @pytest.mark.parametrize("what", ["zeros", "tiny", "huge", "halfway", "borders", "one_large"])
 def test_rows_of_hard_values(device, what):
     """Magnitudes at the ends of the scales, values half-way between two codes,
