@@ -354,6 +354,44 @@ int kva_rollback(kva_cache *cache, int32_t n_seqs, const int32_t *seq_ids,
                  const int32_t *base_len, const int32_t *keep_off,
                  const int32_t *keep_rows, kva_stream_t stream);
 
+/* ---- eviction ------------------------------------------------------------ */
+/* What the step's tokens look at: for each sequence b of the step and each KV
+ * head h, with m = min(n_new, n_obs) of the sequence's last tokens,
+ *   weights[b][h][j] = decay * weights[b][h][j]
+ *                      + sum over those tokens and h's query heads of
+ *                        softmax(q K^T / 16)[j],     j in [0, len),
+ * each token seeing the rows up to its own, as in kva_decode / kva_prefill
+ * (call it after the step's append, with the same q).  weights: device fp32
+ * [n_seqs][num_kv_heads][w_stride] in step order, w_stride at least the
+ * longest length; entries from len on are left alone, and with decay 0 the
+ * old ones are not read.  A sequence without new tokens is only decayed.
+ * n_obs at most 32.  No counterpart in the reference.  Sums are in fp32 and in
+ * a fixed order.  Not for a step with tree_bits, not while a graph is recorded. */
+int kva_attn_weights(kva_cache *cache, int32_t layer, const void *q, int32_t n_obs, float decay,
+                     float *weights, int64_t w_stride, kva_stream_t stream);
+/* Keep keep[b] rows of each sequence src_ids[b], in every layer and KV head
+ * apart: the first `first`, the latest `recent`, and of the others those of
+ * largest weight (equal ones from the lowest slot on; NaN counts as -inf), in
+ * their order.  A sequence of at most keep[b] rows keeps all of them.  The
+ * rows become slots 0..keep-1 of dst_ids[b], in blocks of its own, and its
+ * length; what it held goes.  dst_ids NULL, or the source itself: the source is
+ * replaced (its blocks are released, in groups where the pool is short: the
+ * largest of the sequences has to find its new blocks free; one that keeps all
+ * its rows is left as it is); another sequence is a copy, the source stays.  Keys keep the positions that they were rotated
+ * to, so the steps that follow pass rope_pos.  On an 8-bit cache the values held
+ * are rounded once more, to their new page's scale.
+ * weights: device fp32 [n_layers][n_seqs][num_kv_heads][w_stride]; kept:
+ * device int32 [n_layers][n_seqs][num_kv_heads][kept_stride], gets the slots
+ * that stayed, ascending, and -1 behind them; weights_out (nullable): the
+ * layout of weights, gets the weights of the rows that stayed and zeros behind
+ * them, for a kva_attn_weights that goes on.  None may overlap.  Ends the
+ * current step.  src_ids, dst_ids and keep are host arrays; a sequence is
+ * listed once.  No counterpart in the reference, whose cache only grows.    */
+int kva_evict(kva_cache *cache, int32_t n_seqs, const int32_t *src_ids, const int32_t *dst_ids,
+              const int32_t *keep, int32_t first, int32_t recent, const float *weights,
+              float *weights_out, int64_t w_stride, int32_t *kept, int64_t kept_stride,
+              kva_stream_t stream);
+
 /* Split-K tuning for kva_decode: tokens per split (multiple of 16); 0 =
  * automatic.  Automatic runs a step whose longest sequence is at most 1024
  * rows in the whole-sequence form (each sequence walked whole by workgroups

@@ -74,6 +74,8 @@ SIGNATURES = {
     "kva_append_qknorm_rope": [_P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _P],
     "kva_append_rows": [_P, _I, _P, _P, _P],
     "kva_read_rows": [_P, _I, _I, _PI, _PI, _PI, _P, _P, _P],
+    "kva_attn_weights": [_P, _I, _P, _I, c_float, _P, c_int64, _P],
+    "kva_evict": [_P, _I, _PI, _PI, _PI, _I, _I, _P, _P, c_int64, _P, c_int64, _P],
     "kva_project_append": [_P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P],
     "kva_out_project": [_P, _P, _I, _I, _P, _I, _P, _P, _P],
     "kva_decode": [_P, _I, _P, _P, _P],

@@ -93,6 +93,7 @@ struct kva_cache {
     float *d_mq_acc = nullptr;  // multi-query partial slots [2*mq_max_wg][128 or 256 rows][256]
     float *d_mq_ml = nullptr;
     int32_t mq_max_wg = 0;
+    size_t mq_floats = 0;  // what d_mq_acc holds
     bool mq_two_tiles = false;  // a step may take two row tiles per wave (256-row slots)
     float *d_proj = nullptr;    // projection partials [splits][tokens][rows]
     size_t part_floats = 0;     // what it holds
@@ -452,6 +453,7 @@ int kva_create(const kva_config *cfg, kva_cache **out) {
     c->n_cu = kHostOnlyCus;
     c->mq_max_wg = c->n_cu;  // the device's CU count below
     c->mq_two_tiles = may_take_two_tiles(c);
+    c->mq_floats = static_cast<size_t>(2) * c->mq_max_wg * (c->mq_two_tiles ? 256 : 128) * kva::kHeadDim;
     if (!c->host_only) {
         auto cleanup = [&](int code) {
             kva_destroy(c);
@@ -511,7 +513,8 @@ int kva_create(const kva_config *cfg, kva_cache **out) {
         c->mq_max_wg = c->n_cu;
         c->mq_two_tiles = may_take_two_tiles(c);
         const size_t mq_rows = static_cast<size_t>(2) * c->mq_max_wg * (c->mq_two_tiles ? 256 : 128);
-        if ((e = hipMalloc(&c->d_mq_acc, mq_rows * kva::kHeadDim * sizeof(float))) != hipSuccess)
+        c->mq_floats = mq_rows * kva::kHeadDim;
+        if ((e = hipMalloc(&c->d_mq_acc, c->mq_floats * sizeof(float))) != hipSuccess)
             return cleanup(hip_fail(e, "hipMalloc(multi-query workspace)"));
         if ((e = hipMalloc(&c->d_mq_ml, mq_rows * 2 * sizeof(float))) != hipSuccess)
             return cleanup(hip_fail(e, "hipMalloc(multi-query workspace ml)"));
@@ -1604,6 +1607,222 @@ int kva_read_rows(kva_cache *c, int32_t layer, int32_t n_seqs, const int32_t *se
         a.n_touch = n;
         return kva::launch_read_rows(a, s);
     });
+}
+
+int kva_attn_weights(kva_cache *c, int32_t layer, const void *q, int32_t n_obs, float decay, float *weights,
+                     int64_t w_stride, kva_stream_t stream) {
+    if (!c) return fail(KVA_ERR_INVALID_ARG, "cache is NULL");
+    if (int rc = refuse_while_capturing(c, "kva_attn_weights")) return rc;
+    int rc = check_layer(c, layer);
+    if (rc) return rc;
+    if (!c->step_valid) return fail(KVA_ERR_STATE, "no step begun (kva_step_begin)");
+    if (c->st_has_bits) return fail(KVA_ERR_STATE, "the weights of a step with tree_bits are not defined");
+    if (!q || !weights) return fail(KVA_ERR_INVALID_ARG, "NULL tensor pointer");
+    if (!aligned16(q)) return fail(KVA_ERR_MISALIGNED, "q must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(weights) & 3u) return fail(KVA_ERR_MISALIGNED, "weights must be 4-byte aligned");
+    const int32_t group = c->group;
+    if (n_obs < 1 || n_obs > kva::kMaxObserved)
+        return fail(KVA_ERR_UNSUPPORTED, "n_obs %d outside [1, %d]", n_obs, kva::kMaxObserved);
+    if (!(decay - decay == 0.0f)) return fail(KVA_ERR_INVALID_ARG, "decay must be finite");
+    if (w_stride < c->st_max_ctx)
+        return fail(KVA_ERR_INVALID_ARG, "w_stride %lld is less than the longest sequence's %d rows",
+                    static_cast<long long>(w_stride), c->st_max_ctx);
+    kva::WeightArgs a{};
+    a.n_obs = std::min(n_obs, std::max(1, c->st_max_new));
+    a.part_rows = a.n_obs * group;
+    // Workgroups of four waves: as many as the chip holds of them, by the LDS
+    // that their query rows take, some more where a batch is ragged, and four
+    // pages each at least.
+    const int32_t tiles = (a.part_rows + 15) / 16;
+    const int64_t target = static_cast<int64_t>(c->n_cu) * (tiles <= 1 ? 8 : tiles <= 4 ? 4 : tiles <= 8 ? 2 : 1);
+    const int64_t units = static_cast<int64_t>(c->st_n_seqs) * c->cfg.num_kv_heads;
+    const int64_t pages = (c->st_max_ctx + kva::kBlockTokens - 1) / kva::kBlockTokens;
+    const int64_t fit = static_cast<int64_t>(c->mq_floats) / (2 * units * a.part_rows);
+    if (fit < 1)
+        return fail(KVA_ERR_CAPACITY, "%d sequences of %d query rows exceed the workspace", c->st_n_seqs, a.part_rows);
+    a.splits = static_cast<int32_t>(std::max<int64_t>(
+        1, std::min<int64_t>({(target + units - 1) / units, (pages + 3) / 4, fit, int64_t{256}})));
+    if ((rc = require_device(c))) return rc;
+    a.q = static_cast<const uint16_t *>(q);
+    a.seq_ids = at<int32_t>(c->d_step, c->off_seq);
+    a.ctx_lens = at<int32_t>(c->d_step, c->off_ctx);
+    a.tok_off = at<int32_t>(c->d_step, c->off_tokoff);
+    a.table = c->d_table;
+    a.table_stride = c->cfg.max_blocks_per_seq;
+    if (c->int8)
+        set_layer8(c, layer, a);
+    else
+        a.k_pool = c->d_k + c->layer_elems * layer;
+    a.n_seqs = c->st_n_seqs;
+    a.num_heads = c->cfg.num_heads;
+    a.num_kv_heads = c->cfg.num_kv_heads;
+    a.part = reinterpret_cast<float2 *>(c->d_mq_acc);
+    a.decay = decay;
+    a.weights = weights;
+    a.w_stride = w_stride;
+    KVA_HIP(kva::launch_weights(a, static_cast<hipStream_t>(stream)));
+    return KVA_OK;
+}
+
+int kva_evict(kva_cache *c, int32_t n_seqs, const int32_t *src_ids, const int32_t *dst_ids, const int32_t *keep,
+              int32_t first, int32_t recent, const float *weights, float *weights_out, int64_t w_stride,
+              int32_t *kept, int64_t kept_stride, kva_stream_t stream) {
+    if (!c) return fail(KVA_ERR_INVALID_ARG, "cache is NULL");
+    if (int rc = refuse_while_capturing(c, "kva_evict")) return rc;
+    if (n_seqs < 0 || n_seqs > c->cfg.max_seqs) return fail(KVA_ERR_INVALID_ARG, "bad n_seqs %d", n_seqs);
+    if (n_seqs == 0) return KVA_OK;
+    if (!src_ids || !keep) return fail(KVA_ERR_INVALID_ARG, "NULL index array");
+    if (!weights || !kept) return fail(KVA_ERR_INVALID_ARG, "NULL tensor pointer");
+    if ((reinterpret_cast<uintptr_t>(weights) | reinterpret_cast<uintptr_t>(weights_out) |
+         reinterpret_cast<uintptr_t>(kept)) & 3u)
+        return fail(KVA_ERR_MISALIGNED, "weights, weights_out and kept must be 4-byte aligned");
+    if (first < 0 || recent < 0) return fail(KVA_ERR_INVALID_ARG, "first %d or recent %d < 0", first, recent);
+    // Everything is checked before anything changes.
+    std::vector<uint8_t> role(c->cfg.max_seqs, 0);  // 1: a source, 2: a destination
+    std::vector<int32_t> n_keep(n_seqs);
+    int32_t longest = 0, most = 0;
+    for (int32_t b = 0; b < n_seqs; ++b) {
+        const int32_t s = src_ids[b];
+        if (int rc = check_seq(c, s)) return rc;
+        if (role[s]) return fail(KVA_ERR_INVALID_ARG, "sequence %d listed twice", s);
+        role[s] = 1;
+        if (keep[b] < 0) return fail(KVA_ERR_INVALID_ARG, "keep[%d] = %d < 0", b, keep[b]);
+        const int32_t len = c->len[s];
+        n_keep[b] = std::min(keep[b], len);
+        if (n_keep[b] < len && static_cast<int64_t>(first) + recent > n_keep[b])
+            return fail(KVA_ERR_INVALID_ARG, "sequence %d: %d rows cannot hold the first %d and the latest %d", s,
+                        keep[b], first, recent);
+        longest = std::max(longest, len);
+        most = std::max(most, n_keep[b]);
+    }
+    int64_t free_blocks = static_cast<int64_t>(c->free_list.size()), held_back = 0;
+    for (int32_t b = 0; b < n_seqs; ++b) {
+        const int32_t s = src_ids[b], d = dst_ids ? dst_ids[b] : s;
+        if (int rc = check_seq(c, d)) return rc;
+        if (d != s) {
+            if (role[d]) return fail(KVA_ERR_INVALID_ARG, "sequence %d is listed twice or is another's source", d);
+            role[d] = 2;
+            free_blocks += c->nblk[d];
+        } else if (n_keep[b] == c->len[s]) {
+            continue;  // nothing moves
+        }
+        const int64_t need = (static_cast<int64_t>(n_keep[b]) + kva::kBlockTokens - 1) / kva::kBlockTokens;
+        if (need > free_blocks) {  // the sequences before this one give up theirs first
+            free_blocks += held_back;
+            held_back = 0;
+        }
+        if (need > free_blocks)
+            return fail(KVA_ERR_OUT_OF_BLOCKS, "sequence %d: the rows that stay need %lld free blocks, %lld there", s,
+                        static_cast<long long>(need), static_cast<long long>(free_blocks));
+        free_blocks -= need;
+        if (d == s) held_back += c->nblk[s];
+    }
+    if (w_stride < longest || kept_stride < most)
+        return fail(KVA_ERR_INVALID_ARG, "w_stride %lld or kept_stride %lld is less than the %d rows or the %d that stay",
+                    static_cast<long long>(w_stride), static_cast<long long>(kept_stride), longest, most);
+    const size_t heads = static_cast<size_t>(c->cfg.n_layers) * n_seqs * c->cfg.num_kv_heads;
+    if (overlaps(weights_out, 2 * heads * w_stride, weights, 2 * heads * w_stride) ||
+        overlaps(kept, 2 * heads * kept_stride, weights, 2 * heads * w_stride) ||
+        overlaps(kept, 2 * heads * kept_stride, weights_out, 2 * heads * w_stride))
+        return fail(KVA_ERR_INVALID_ARG, "weights, weights_out and kept must not overlap");
+    if (int rc = require_device(c)) return rc;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    int rc = flush_patches(c, s);
+    if (rc) return rc;
+    c->step_valid = false;
+    {
+        kva::SelectArgs a{};
+        a.weights = weights;
+        a.weights_out = weights_out;
+        a.w_stride = w_stride;
+        a.kept = kept;
+        a.kept_stride = kept_stride;
+        a.num_kv_heads = c->cfg.num_kv_heads;
+        a.first = first;
+        a.recent = recent;
+        uint8_t *h;
+        int idx;
+        if ((rc = acquire_stage(c, &h, &idx))) return rc;
+        for (int32_t b = 0; b < n_seqs; ++b) {
+            at<int32_t>(h, 0)[2 * b] = c->len[src_ids[b]];
+            at<int32_t>(h, 0)[2 * b + 1] = n_keep[b];
+        }
+        KVA_HIP(hipMemcpyAsync(c->d_aux, h, 2 * sizeof(int32_t) * n_seqs, hipMemcpyHostToDevice, s));
+        if ((rc = release_stage(c, idx, s))) return rc;
+        a.seqs = reinterpret_cast<const int32_t *>(c->d_aux);
+        KVA_HIP(kva::launch_select(a, n_seqs, c->cfg.n_layers, longest, s));
+    }
+    kva::GatherArgs g{};
+    g.kept = kept;
+    g.kept_stride = kept_stride;
+    g.n_seqs = n_seqs;
+    g.table = c->d_table;
+    g.table_stride = c->cfg.max_blocks_per_seq;
+    g.k_pool = c->d_k;
+    g.v_pool = c->d_v;
+    g.layer_elems = c->layer_elems;
+    if (c->int8) set_layer8(c, 0, g);
+    g.layer_codes = c->layer_codes;
+    g.layer_scales = c->layer_scales;
+    g.layer_open = c->layer_open;
+    // Sequences in groups: a group's rows are copied in one launch, then its
+    // sources give up the blocks that they are replaced from.
+    std::vector<int32_t> recs;
+    std::vector<std::pair<int32_t, std::vector<int32_t>>> replaced;  // sequence, its new blocks
+    auto adopt = [&](int32_t seq, const std::vector<int32_t> &ids) {
+        const size_t base = static_cast<size_t>(seq) * c->cfg.max_blocks_per_seq;
+        for (size_t i = 0; i < ids.size(); ++i) {
+            c->table[base + i] = ids[i];
+            c->patches.insert(c->patches.end(), {seq, static_cast<int32_t>(i), ids[i]});
+        }
+        c->nblk[seq] = static_cast<int32_t>(ids.size());
+        c->freed[seq] = 0;
+    };
+    auto run_group = [&]() -> int {
+        const int rc = upload_touches(c, recs, s, [&](const int32_t *r, int32_t n) {
+            g.recs = r;
+            return kva::launch_gather(g, n, c->cfg.num_kv_heads, c->cfg.n_layers, s);
+        });
+        recs.clear();
+        for (auto &[seq, ids] : replaced) {
+            release_blocks(c, seq);
+            adopt(seq, ids);
+        }
+        replaced.clear();
+        return rc;
+    };
+    for (int32_t b = 0; b < n_seqs; ++b) {
+        const int32_t src = src_ids[b], dst = dst_ids ? dst_ids[b] : src, n = n_keep[b];
+        if (dst != src)
+            release_blocks(c, dst);
+        else if (n == c->len[src])
+            continue;
+        const int32_t need = (n + kva::kBlockTokens - 1) / kva::kBlockTokens;
+        if (static_cast<size_t>(need) > c->free_list.size() && (rc = run_group())) return rc;
+        std::vector<int32_t> ids(need);
+        for (int32_t &id : ids) {
+            id = c->free_list.back();
+            c->free_list.pop_back();
+            c->used[id] = 1;
+        }
+        const int32_t full = n / kva::kBlockTokens, behind = n % kva::kBlockTokens;
+        const int32_t src_open = c->int8 ? c->open_page[src] : -1;
+        for (int32_t p = 0; p < full; ++p) {
+            const bool last = p + 1 == full && behind;
+            recs.insert(recs.end(), {b, p, src, dst, ids[p], last ? ids[p + 1] : -1,
+                                     kva::kBlockTokens + (last ? behind : 0), src_open});
+        }
+        if (full == 0 && behind) recs.insert(recs.end(), {b, 0, src, dst, -1, ids[0], behind, src_open});
+        if (dst == src)
+            replaced.emplace_back(src, std::move(ids));
+        else
+            adopt(dst, ids);
+        c->len[dst] = n;
+        c->held[dst] = n;
+        c->open_page[dst] = behind ? full : -1;
+    }
+    if ((rc = run_group())) return rc;
+    return flush_patches(c, s);
 }
 
 int kva_project_append(kva_cache *c, int32_t layer, const void *x, int32_t hidden, const void *w_q_fused,

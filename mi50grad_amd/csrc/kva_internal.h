@@ -412,4 +412,65 @@ struct ReopenArgs {
 };
 hipError_t launch_reopen(const ReopenArgs &a, int32_t n, int32_t num_kv_heads, int32_t n_layers, hipStream_t s);
 
+// ---- eviction (k_evict.hip) ----
+
+constexpr int kMaxObserved = 32;     // query tokens per sequence that kva_attn_weights looks at, at most
+constexpr int kMaxWeightRows = 256;  // query rows (tokens x heads of a group), at most: 16 tiles
+struct WeightArgs {
+    const uint16_t *q;        // [T][H][256]
+    const int32_t *seq_ids;   // device, as in MultiQueryArgs
+    const int32_t *ctx_lens;
+    const int32_t *tok_off;
+    const int32_t *table;
+    int32_t table_stride;
+    const uint16_t *k_pool;   // FP16 cache
+    const uint8_t *k8;        // 8-bit cache (null: FP16); v8 unused
+    const uint8_t *v8;
+    const float *scales;
+    const uint16_t *open;
+    int32_t n_seqs, num_heads, num_kv_heads;
+    int32_t n_obs;
+    int32_t splits;           // workgroups that share a sequence's pages
+    int32_t part_rows;        // query rows at most
+    float2 *part;             // [n_seqs][Hkv][splits][part_rows]: max (log2 units), sum
+    float decay;
+    float *weights;           // [n_seqs][Hkv][w_stride]
+    int64_t w_stride;
+};
+hipError_t launch_weights(const WeightArgs &a, hipStream_t s);
+
+constexpr int kSelectLds = 32768;    // rows whose keys select_kernel holds in LDS, at most
+struct SelectArgs {
+    const int32_t *seqs;      // device [n_seqs][2]: rows, rows that stay
+    const float *weights;     // [layers][n_seqs][Hkv][w_stride]
+    float *weights_out;       // nullable
+    int64_t w_stride;
+    int32_t *kept;            // [layers][n_seqs][Hkv][kept_stride]
+    int64_t kept_stride;
+    int32_t num_kv_heads;
+    int32_t first, recent;
+};
+// most: rows of the longest sequence.
+hipError_t launch_select(const SelectArgs &a, int32_t n_seqs, int32_t n_layers, int32_t most, hipStream_t s);
+
+struct GatherArgs {
+    // Device [n][kTouchWords]: sequence's index in the call, destination page,
+    // source sequence, destination sequence, block of the page (-1: none full),
+    // block of the rows behind it (FP16 cache), rows of both, the source's open
+    // page (-1: none).
+    const int32_t *recs;
+    const int32_t *kept;
+    int64_t kept_stride;
+    int32_t n_seqs;           // of the call
+    const int32_t *table;
+    int32_t table_stride;
+    uint16_t *k_pool, *v_pool;  // layer 0
+    size_t layer_elems;
+    uint8_t *k8, *v8;
+    float *scales;
+    uint16_t *open;
+    size_t layer_codes, layer_scales, layer_open;
+};
+hipError_t launch_gather(const GatherArgs &a, int32_t n_recs, int32_t num_kv_heads, int32_t n_layers, hipStream_t s);
+
 }  // namespace kva

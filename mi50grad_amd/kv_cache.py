@@ -168,6 +168,28 @@ class PagedKVCache:
         _lib.call("kva_read_rows", self.handle, layer, len(seq_ids), _lib.int_array(seq_ids), _lib.int_array(first),
                   _lib.int_array(count), _ptr(k_out), _ptr(v_out), stream)
 
+    def attn_weights(self, layer: int, q, weights, w_stride: int, n_obs: int = 1, decay: float = 1.0,
+                     stream=None) -> None:
+        """weights[b][h][j] = decay * weights[b][h][j] + the softmax weights
+        that row j gets from the step's last n_obs tokens of sequence b and
+        the query heads of KV head h: weights [n_seqs, Hkv, w_stride] fp32."""
+        _lib.call("kva_attn_weights", self.handle, layer, _ptr(q), n_obs, decay, _ptr(weights), w_stride, stream)
+
+    def evict(self, seq_ids: Sequence[int], keep: Sequence[int], weights, w_stride: int, kept, kept_stride: int,
+              first: int = 0, recent: int = 0, dst_ids: Sequence[int] | None = None, weights_out=None,
+              stream=None) -> None:
+        """Keep keep[b] rows of each sequence, per layer and KV head: the
+        first `first`, the latest `recent` and those of largest weight
+        (kva_evict).  weights, weights_out [n_layers, n_seqs, Hkv, w_stride]
+        fp32; kept [n_layers, n_seqs, Hkv, kept_stride] int32.  dst_ids: the
+        sequences that get them (by default the sources themselves).  Later
+        steps pass rope_pos: slots are no positions any more."""
+        if len(keep) != len(seq_ids) or (dst_ids is not None and len(dst_ids) != len(seq_ids)):
+            raise ValueError("seq_ids, dst_ids and keep differ in length")
+        _lib.call("kva_evict", self.handle, len(seq_ids), _lib.int_array(seq_ids),
+                  None if dst_ids is None else _lib.int_array(dst_ids), _lib.int_array(keep), first, recent,
+                  _ptr(weights), _ptr(weights_out), w_stride, _ptr(kept), kept_stride, stream)
+
     def append_decode(self, layer: int, q, k, v, q_norm_w, k_norm_w, cos_tab, sin_tab, table_rows: int, out,
                       stream=None, gate=None, gate_stride: int = 0) -> None:
         """append() then decode() for a step of one token per sequence, in

@@ -129,3 +129,57 @@ def test_kinds_of_cache():
     with pytest.raises(ValueError):
         make(kv_bits=4)
     assert make().row_bytes * 2 == make(kv_bits=16).row_bytes
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_attn_weights_refuses(bits):
+    c = make(kv_bits=bits)
+    ok = (0, 16, 16, 100)
+    refused(STATE, c.attn_weights, *ok)
+    c.begin_step([1, 2], [30, 5])
+    refused(NO_DEVICE, c.attn_weights, *ok, n_obs=32)
+    refused(INVALID, c.attn_weights, 2, 16, 16, 100)
+    refused(INVALID, c.attn_weights, 0, None, 16, 100)
+    refused(INVALID, c.attn_weights, 0, 16, None, 100)
+    refused(MISALIGNED, c.attn_weights, 0, 24, 16, 100)
+    refused(MISALIGNED, c.attn_weights, 0, 16, 18, 100)
+    refused(INVALID, c.attn_weights, 0, 16, 16, 29)
+    for n in (0, -1, 33):
+        refused(UNSUPPORTED, c.attn_weights, *ok, n_obs=n)
+    for d in (float("nan"), float("inf")):
+        refused(INVALID, c.attn_weights, *ok, decay=d)
+    if bits == 16:
+        c.begin_step([3], [1], tree_bits=[1])
+        refused(STATE, c.attn_weights, *ok)
+
+
+def test_evict_refuses():
+    c = make()
+    c.begin_step([0, 1], [40, 20])
+    big = 1 << 20
+    ok = dict(weights=16, w_stride=40, kept=big, kept_stride=20)
+    call = lambda ids, keep, **kw: refused(kw.pop("code"), c.evict, ids, keep, **{**ok, **kw})  # noqa: E731
+    call([0, 1], [20, 20], code=NO_DEVICE)
+    call([0, 4], [20, 20], code=BAD_SEQ)
+    call([0, 0], [20, 20], code=INVALID)
+    call([0], [-1], code=INVALID)
+    call([0], [10], first=4, recent=7, code=INVALID)
+    call([0], [10], first=-1, code=INVALID)
+    call([0], [10], recent=-1, code=INVALID)
+    call([0, 1], [20, 20], dst_ids=[1, 0], code=INVALID)  # another's source
+    call([0, 1], [20, 20], dst_ids=[2, 2], code=INVALID)
+    call([0, 1], [20, 20], dst_ids=[2, 9], code=BAD_SEQ)
+    call([0], [20], weights=None, code=INVALID)
+    call([0], [20], kept=None, code=INVALID)
+    call([0], [20], kept=big + 2, code=MISALIGNED)
+    call([0], [20], w_stride=39, code=INVALID)
+    call([0], [20], kept_stride=19, code=INVALID)
+    call([0], [20], weights_out=16, code=INVALID)
+    call([0], [20], kept=32, code=INVALID)
+    with pytest.raises(ValueError):
+        c.evict([0, 1], [20], **ok)
+    assert c.seq_len(0) == 40 and c.seq_len(1) == 20
+    tight = make(max_blocks=6, max_step_tokens=128)
+    tight.begin_step([0, 1], [40, 40])
+    refused(-4, tight.evict, [0], [20], **ok)
+    refused(NO_DEVICE, tight.evict, [0, 1], [40, 40], 16, 40, big, 40)

@@ -1,0 +1,313 @@
+"""GPU: attention weights gathered over both kinds of cache, and eviction by
+them, against plain float64 forms."""
+import numpy as np
+import pytest
+
+from cache8_helpers import D, held, make, put, rows, same_bits, within
+from gpu_helpers import Tables, expected_norm, say
+from mi50grad_amd._lib import KvaError
+from oracle import kvattn_oracle as orc
+
+pytestmark = pytest.mark.gpu
+F32 = np.finfo(np.float32).eps / 2
+
+
+def _values(bits, k, v):
+    return orc.int8_rows(k, v) if bits == 8 else (k.astype(np.float64), v.astype(np.float64))
+
+
+def _weights(q, k, ctx, m, G):
+    """Sum of the softmax weights of the last m tokens of q [n, H, D] over k
+    [ctx, kv, D]: [kv, ctx], and how far float32 may be off: a score's error (sum of
+    256 products, scaled) counts twice, in the weight and in the row's sum."""
+    kv = k.shape[1]
+    out, tol = np.zeros((kv, ctx)), np.zeros((kv, ctx))
+    q = q[len(q) - m:].astype(np.float64)
+    see = np.arange(ctx)[None] <= ctx - m + np.arange(m)[:, None]
+    for h in range(kv * G):
+        s = q[:, h] @ k[:, h // G].T / 16.0
+        size = (np.abs(q[:, h]) @ np.nan_to_num(np.abs(k[:, h // G])).T / 16.0).max() if m else 0.0
+        s = np.where(see, s, -np.inf)
+        with np.errstate(invalid="ignore"):
+            p = np.exp(s - s.max(-1, keepdims=True))
+        p = np.where(see, p / p.sum(-1, keepdims=True), 0.0)
+        out[h // G] += p.sum(0)
+        tol[h // G] += p.sum(0) * (2 * (D + 16) * F32 * size + 128 * F32)
+    return out, tol + 1e-37
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("heads,kv", [(24, 4), (6, 1), (8, 8), (8, 1), (6, 3)])
+@pytest.mark.parametrize("base,new,obs", [([0, 15, 300, 2100], [1, 1, 1, 1], 1), ([40, 0, 1000], [3, 40, 33], 32),
+                                          ([17, 500], [20, 2], 5), ([5000], [1], 7), ([33, 64], [0, 9], 9)], ids=str)
+def test_weights(device, bits, heads, kv, base, new, obs):
+    say(f"weights {bits} {heads}/{kv} {base} {new} {obs}")
+    rng = np.random.default_rng(heads + obs)
+    lens = [b + n for b, n in zip(base, new)]
+    cache = make(lens, heads=heads, kv=kv, bits=bits)
+    seqs = list(range(len(lens)))
+    data = [rows(rng, n, kv) for n in lens]
+    put(device, cache, seqs, [d[0][:b] for d, b in zip(data, base)], [d[1][:b] for d, b in zip(data, base)])
+    put(device, cache, seqs, [d[0][b:] for d, b in zip(data, base)], [d[1][b:] for d, b in zip(data, base)])
+    q = (rng.standard_normal((max(1, sum(new)), heads, D)) * 1.5).astype(np.float16)
+    width = max(lens) + 3
+    for decay in (0.0, 0.75, 1.0):
+        old = rng.exponential(size=(len(lens), kv, width)).astype(np.float32)
+        old[0, 0, 0] = np.nan if decay == 0 else old[0, 0, 0]
+        w = device.array(old)
+        cache.attn_weights(0, device.array(q), w, width, n_obs=obs, decay=decay)
+        device.synchronize()
+        got, t = w.numpy().astype(np.float64), 0
+        for b, (n, c) in enumerate(zip(new, lens)):
+            want, tol = _weights(q[t:t + n], _values(bits, *data[b])[0], c, min(n, obs), heads // kv)
+            if decay:
+                before = decay * old[b, :, :c].astype(np.float64)
+                want, tol = want + before, tol + 2 * F32 * (want + before)
+            within(got[b, :, :c], want, tol + F32 * np.abs(want))
+            assert np.array_equal(got[b, :, c:], old[b, :, c:].astype(np.float64)), "rows behind the sequence"
+            t += n
+    cache.destroy()
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_weights_of_rows_not_finite(device, bits):
+    """A NaN key gives NaN to every row that the tokens which see it weigh."""
+    say("weights nan")
+    rng = np.random.default_rng(2)
+    k, v = rows(rng, 70, 2)
+    k[40, 0, 3] = np.nan
+    cache = make([70], heads=2, kv=2, bits=bits)
+    put(device, cache, [0], [k], [v])
+    q = rng.standard_normal((70, 2, D)).astype(np.float16)
+    w = device.array(np.zeros((1, 2, 70), np.float32))
+    cache.attn_weights(0, device.array(q), w, 70, n_obs=4)
+    device.synchronize()
+    got = w.numpy()[0]
+    assert np.isnan(got[0]).all()
+    want, tol = _weights(q[:, 1:], _values(bits, k, v)[0][:, 1:], 70, 4, 1)
+    within(got[1:], want, tol + F32 * want)
+    cache.destroy()
+
+
+def test_weights_repeat_to_the_bit(device):
+    say("weights repeat")
+    rng = np.random.default_rng(3)
+    lens = [900, 33, 2000]
+    cache = make(lens)
+    data = [rows(rng, n, 4) for n in lens]
+    put(device, cache, [0, 1, 2], [d[0] for d in data], [d[1] for d in data])
+    q = device.array(rng.standard_normal((sum(lens), 24, D)).astype(np.float16))
+    got = []
+    for _ in range(3):
+        w = device.array(np.ones((3, 4, 2000), np.float32))
+        cache.attn_weights(0, q, w, 2000, n_obs=32)
+        device.synchronize()
+        got.append(w.numpy())
+    assert all(np.array_equal(g.view(np.uint32), got[0].view(np.uint32)) for g in got)
+    cache.destroy()
+
+
+def _stay(w, n, keep, first, recent):
+    if keep >= n:
+        return np.arange(n)
+    w = np.where(np.isnan(w), -np.inf, w[...])[:n].astype(np.float64)
+    inner = np.arange(first, n - recent)
+    inner = inner[np.lexsort((inner, -w[inner]))][:keep - first - recent]
+    return np.sort(np.concatenate([np.arange(first), inner, np.arange(n - recent, n)])).astype(int)
+
+
+KINDS = {
+    "spread": lambda r, n: r.exponential(size=n) ** 3,
+    "ties": lambda r, n: r.integers(0, 4, n) * 0.25,
+    "all_equal": lambda r, n: np.full(n, 0.5),
+    "any_sign": lambda r, n: np.where(r.random(n) < 0.1, r.choice([0.0, -0.0, np.inf, -np.inf, np.nan], n), r.standard_normal(n)),
+    "near": lambda r, n: 1 + r.integers(0, 50, n) * 2.0 ** -23,
+}
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n,keep,first,recent", [(1, 1, 0, 0), (1, 0, 0, 0), (40, 20, 4, 16), (40, 21, 4, 16),
+                                                 (1000, 500, 0, 0), (1000, 999, 3, 0), (2000, 77, 0, 32),
+                                                 (5000, 5000, 4, 16), (33, 100, 4, 16), (33000, 9000, 4, 64)], ids=str)
+def test_which_rows_stay(device, kind, n, keep, first, recent):
+    say(f"which stay {kind} {n} {keep}")
+    rng = np.random.default_rng(n + keep)
+    cache = make([n], heads=1, kv=1, bits=16, step=max(16, n), spare=min(n, keep) // 16 + 1, slots=2)
+    put(device, cache, [0], [np.zeros((n, 1, D), np.float16)], [np.zeros((n, 1, D), np.float16)])
+    width, most = n + 5, min(n, keep) + 3
+    w = np.zeros((1, 1, 1, width), np.float32)
+    w[..., :n] = KINDS[kind](rng, n)
+    w[..., n:] = 1e30  # behind the sequence: never looked at
+    kept = device.array(np.full((1, 1, 1, most), 99, np.int32))
+    out = device.array(np.full(w.shape, 99, np.float32))
+    cache.evict([0], [keep], device.array(w), width, kept, most, first=first, recent=recent, dst_ids=[1],
+                weights_out=out)
+    device.synchronize()
+    want = _stay(w[0, 0, 0], n, keep, first, recent)
+    got = kept.numpy()[0, 0, 0]
+    assert np.array_equal(got[:len(want)], want) and (got[len(want):] == -1).all()
+    back = out.numpy()[0, 0, 0]
+    assert np.array_equal(back[:len(want)].view(np.uint32), w[0, 0, 0][want].view(np.uint32))
+    assert (back[len(want):] == 0).all()
+    assert cache.seq_len(1) == len(want) and cache.seq_len(0) == n
+    cache.destroy()
+
+
+def _filled(device, lens, heads, kv, layers, bits, rng, **kw):
+    cache = make(lens, heads=heads, kv=kv, layers=layers, bits=bits, **kw)
+    data = [[rows(rng, n, kv) for n in lens] for _ in range(layers)]
+    for i in range(layers):
+        put(device, cache, list(range(len(lens))), [d[0] for d in data[i]], [d[1] for d in data[i]], layer=i)
+    return cache, data
+
+
+def _moved(bits, d, places):
+    """Rows d = (k, v) of a sequence, of each head those at places[h]."""
+    got = [np.stack([x[places[h], h] for h in range(x.shape[1])], 1) for x in _values(bits, *d)]
+    return _values(bits, got[0], got[1]) if bits == 8 else got
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("where", ["copy", "in_place", "in_place_tight", "mixed"])
+def test_evict(device, bits, where):
+    say(f"evict {bits} {where}")
+    rng = np.random.default_rng(7)
+    lens, keep, first, recent = [100, 17, 333, 64, 5], [37, 20, 128, 16, 5], 2, 9
+    keep = [k if k >= first + recent or k >= n else first + recent for k, n in zip(keep, lens)]
+    kv, heads, layers, B = 3, 6, 2, len(lens)
+    # tight: room for the largest sequence's new blocks only
+    spare = 8 if where == "in_place_tight" else 30
+    cache, data = _filled(device, lens, heads, kv, layers, bits, rng, spare=spare, slots=2 * B)
+    free = cache.free_block_count()
+    dst = {"copy": [B + b for b in range(B)], "mixed": [0, B + 1, B + 2, 3, 4]}.get(where)
+    w = rng.exponential(size=(layers, B, kv, max(lens))).astype(np.float32)
+    kept = device.empty((layers, B, kv, max(keep)), np.int32)
+    out = device.empty(w.shape, np.float32)
+    before = [held(device, cache, list(range(B)), layer=i) for i in range(layers)]
+    cache.evict(list(range(B)), keep, device.array(w), max(lens), kept, max(keep), first=first, recent=recent,
+                dst_ids=dst, weights_out=out)
+    device.synchronize()
+    to = dst or list(range(B))
+    m = [min(k, n) for k, n in zip(keep, lens)]
+    assert [cache.seq_len(s) for s in to] == m
+    for i in range(layers):
+        got, o = held(device, cache, to, layer=i), 0
+        for b in range(B):
+            places = [_stay(w[i, b, h], lens[b], keep[b], first, recent) for h in range(kv)]
+            assert all(np.array_equal(kept.numpy()[i, b, h][:m[b]], places[h]) for h in range(kv))
+            same = to[b] == b and m[b] == lens[b]  # left as it is
+            want = _values(bits, *data[i][b]) if same else _moved(bits, data[i][b], places)
+            assert same_bits(got[0][o:o + m[b]], want[0]) and same_bits(got[1][o:o + m[b]], want[1]), (i, b)
+            o += m[b]
+        if where == "copy":
+            now = held(device, cache, list(range(B)), layer=i)
+            assert same_bits(now[0], before[i][0]) and same_bits(now[1], before[i][1]), "the sources stay"
+    blocks = lambda ns: sum((n + 15) // 16 for n in ns)  # noqa: E731
+    gone = sum((lens[b] + 15) // 16 for b in range(B) if to[b] == b)
+    assert cache.free_block_count() == free + gone - blocks(m)
+    # the copies again, over themselves: their own blocks come back first
+    if where == "copy":
+        cache.evict(list(range(B)), keep, device.array(w), max(lens), kept, max(keep), first=first, recent=recent,
+                    dst_ids=dst)
+        device.synchronize()
+        assert cache.free_block_count() == free - blocks(m)
+    cache.destroy()
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_evict_then_go_on(device, bits):
+    """A prompt, the weights its last tokens give, eviction in place, then decode
+    steps at their true positions, with the weights followed: every output and
+    every weight against float64 over what the cache holds, and a second eviction."""
+    say(f"evict then go on {bits}")
+    rng = np.random.default_rng(8)
+    H, kv, layers, B = 6, 2, 2, 3
+    lens, keep, first, recent = [200, 90, 47], [64, 50, 40], 4, 16
+    tables = Tables(device, 512)
+    ws = [device.array((1 + 0.02 * rng.standard_normal(D)).astype(np.float16)) for _ in range(2)]
+    cache = make(lens, heads=H, kv=kv, layers=layers, bits=bits, extra=64, spare=16)
+    width = 256
+    w = device.array(np.full((layers, B, kv, width), np.nan, np.float32))  # decay 0 starts them
+    w2 = device.empty((layers, B, kv, width), np.float32)
+    T = sum(lens)
+    cache.begin_step([0, 1, 2], lens)
+    for i in range(layers):
+        q = device.array(rng.standard_normal((T, H, D)).astype(np.float16))
+        k, v = rows(rng, T, kv)
+        cache.append(i, q, device.array(k), device.array(v), *ws, tables.d_cos, tables.d_sin, 512)
+        cache.prefill(i, q, device.empty((T, H, D), np.float16))
+        at = w.ptr + i * B * kv * width * 4
+        cache.attn_weights(i, q, at, width, n_obs=16, decay=0.0)
+        device.synchronize()
+        qn, mine, t = q.numpy(), w.numpy()[i], 0
+        hk, _ = held(device, cache, [0, 1, 2], layer=i)
+        for b, n in enumerate(lens):
+            want, tol = _weights(qn[t:t + n], hk[t:t + n].astype(np.float64), n, 16, H // kv)
+            within(mine[b, :, :n], want, tol + F32 * want)
+            t += n
+    kept = device.empty((layers, B, kv, max(keep)), np.int32)
+    pos = list(lens)
+    for turn in range(2):
+        n_before = [cache.seq_len(b) for b in range(B)]
+        old = w.numpy()
+        before = [held(device, cache, [0, 1, 2], layer=i) for i in range(layers)]
+        cache.evict([0, 1, 2], keep, w, width, kept, max(keep), first=first, recent=recent, weights_out=w2)
+        device.synchronize()
+        for i in range(layers):
+            got, o, p = held(device, cache, [0, 1, 2], layer=i), 0, 0
+            for b in range(B):
+                m = min(keep[b], n_before[b])
+                places = [_stay(old[i, b, h], n_before[b], keep[b], first, recent) for h in range(kv)]
+                rows_ = [np.stack([x[o:o + n_before[b]][places[h], h] for h in range(kv)], 1) for x in before[i]]
+                want = _values(bits, *rows_)
+                assert same_bits(got[0][p:p + m], want[0]) and same_bits(got[1][p:p + m], want[1]), (turn, i, b)
+                o, p = o + n_before[b], p + m
+        w, w2 = w2, w
+        for step in range(18):
+            cache.begin_step([0, 1, 2], [1, 1, 1], rope_pos=pos)
+            for i in range(layers):
+                q = rng.standard_normal((B, H, D)).astype(np.float16)
+                k, v = rows(rng, B, kv)
+                dq, out = device.array(q), device.empty((B, H, D), np.float16)
+                cache.append_decode(i, dq, device.array(k), device.array(v), *ws, tables.d_cos, tables.d_sin, 512, out)
+                at = w.ptr + i * B * kv * width * 4
+                was = w.numpy()[i].astype(np.float64)
+                cache.attn_weights(i, dq, at, width, decay=0.9)
+                device.synchronize()
+                now = w.numpy()[i].astype(np.float64)
+                assert np.array_equal(dq.numpy().view(np.uint16),
+                                      expected_norm(q, ws[0].numpy(), tables, pos).view(np.uint16))
+                if step not in (0, 1, 15, 17):
+                    continue
+                n = [cache.seq_len(b) for b in range(B)]
+                hk, hv = held(device, cache, [0, 1, 2], layer=i)
+                o = 0
+                for b in range(B):
+                    kb, vb = hk[o:o + n[b]].astype(np.float64), hv[o:o + n[b]].astype(np.float64)
+                    qb = dq.numpy()[b:b + 1]
+                    within(out.numpy()[b:b + 1], *orc.attention_bound(qb, kb, vb))
+                    want, tol = _weights(qb, kb, n[b], 1, H // kv)
+                    more = 0.9 * was[b, :, :n[b]]
+                    within(now[b, :, :n[b]], want + more, tol + 4 * F32 * (want + more))
+                    o += n[b]
+            pos = [p + 1 for p in pos]
+    cache.destroy()
+
+
+def test_evict_refuses(device):
+    say("evict refuses")
+    rng = np.random.default_rng(9)
+    cache, _ = _filled(device, [100, 50], 2, 1, 1, 8, rng)  # no spare block
+    w = device.array(np.zeros((1, 2, 1, 100), np.float32))
+    kept = device.empty((1, 2, 1, 40), np.int32)
+    with pytest.raises(KvaError) as e:
+        cache.evict([0, 1], [40, 40], w, 100, kept, 40)
+    assert e.value.code == -4 and cache.seq_len(0) == 100 and cache.free_block_count() == 0
+    before = held(device, cache, [0, 1])
+    cache.evict([0, 1], [100, 50], device.array(np.zeros((1, 2, 1, 100), np.float32)), 100,
+                device.empty((1, 2, 1, 100), np.int32), 100)  # nothing moves: no block needed
+    after = held(device, cache, [0, 1])
+    assert same_bits(before[0], after[0]) and same_bits(before[1], after[1])
+    with pytest.raises(KvaError):
+        cache.evict([0], [40], w, 100, w, 40)  # kept over weights
+    cache.destroy()
