@@ -219,8 +219,9 @@ def _own_cache(s):
         rows = _put(np.concatenate([np.arange(d, d + m) + o for d, m, o in zip(done, n, start)]))
         s.cache.begin_step(s.seqs, n)
         for i in range(p.L):
-            s.cache.append_rows(i, s.k[i, rows].contiguous().data_ptr(), s.v[i, rows].contiguous().data_ptr())
-        torch.cuda.synchronize()
+            k, v = s.k[i, rows], s.v[i, rows]
+            s.cache.append_rows(i, k.data_ptr(), v.data_ptr())
+            torch.cuda.synchronize()  # before k and v go
         done += n
     if p.kind == "evict":
         s.first, s.second = s.seqs, [p.B + b for b in s.seqs]
@@ -235,7 +236,9 @@ def _own_cache(s):
         s.out = [torch.empty_like(s.k_new), torch.empty_like(s.v_new)]
         s.base, s.new = [int(x) for x in p.base], [int(x) for x in p.new]
         return
-    s.cache.append_rows(0, s.k[0, s.at].contiguous().data_ptr(), s.v[0, s.at].contiguous().data_ptr())
+    k, v = s.k[0, s.at], s.v[0, s.at]
+    s.cache.append_rows(0, k.data_ptr(), v.data_ptr())
+    torch.cuda.synchronize()  # before k and v go
     s.out = torch.empty_like(s.q)
 
 
