@@ -66,8 +66,9 @@ enum {
  * the block's largest magnitude, at most 512, and c is x/s rounded to the
  * nearest (ties to even): c*s is an fp16 number, at most s/2 from x while
  * |x| <= 65024.  A sequence's last page, until its sixteenth row arrives, is
- * held in fp16 as it came (32 KB per sequence slot, KV head and layer), so
- * codes depend on a page's rows alone, not on the steps that they came in.
+ * held in fp16 as it came, in one of two open blocks that take turns (32 KB per
+ * sequence slot, KV head and layer), so codes depend on a page's rows alone,
+ * not on the steps that they came in, and a step's append may be repeated.
  * A row of a head in which K or V is not finite reads as NaN keys and zero
  * values, and once its page is full every row of that block has NaN keys:
  * attention that sees such a row gives NaN.  All calls of a step are the same
@@ -75,8 +76,10 @@ enum {
  * KVA_ERR_UNSUPPORTED: kva_layer_pools, kva_row_ptr, tree_bits in
  * kva_step_begin, kva_tree_verify, a kva_rollback that moves rows, and
  * kva_timeline_enable.  kva_seq_set_len goes up only to rows that were
- * written; set back into a full page, that page's rows continue from the
- * values its codes stand for.  kva_seq_set_blocks leaves a last page that is
+ * written; set back into a full page, that page continues from its fp16 rows
+ * where they came one step or more before the page was full and it was the
+ * sequence's open page before the present one, else from the values its codes
+ * stand for.  kva_seq_set_blocks leaves a last page that is
  * not full with the sequence.  Recorded appends take one new token per
  * sequence.                                                                 */
 #define KVA_FLAG_INT8 0x2u

@@ -173,9 +173,23 @@ __global__ __launch_bounds__(64 * kDecodeHeadsPerWg) void decode8_kernel(Decode8
     }
     b0 = __builtin_amdgcn_readfirstlane(b0);
     SeqWindow win;
-    load_window(win, a, b0, lane);
+    int slots = 0;  // lane l: the open block of sequence win.b0 + l
+    auto window = [&](int b) {
+        load_window(win, a, b, lane);
+        slots = b + lane < a.n_seqs ? e.open_slot[b + lane] : 0;
+    };
+    window(b0);
+    struct Place : Cursor {
+        int slot;
+    };
+    auto begin = [&](int b) {
+        Place c;
+        static_cast<Cursor &>(c) = seq_cursor(win, b);
+        c.slot = __builtin_amdgcn_readlane(slots, b - win.b0);
+        return c;
+    };
 
-    auto next = [&](Cursor c) -> Cursor {
+    auto next = [&](Place c) -> Place {
         if (!c.ok) return c;
         if (c.base + c.pg + 1 >= p_end) {
             c.ok = false;
@@ -188,8 +202,8 @@ __global__ __launch_bounds__(64 * kDecodeHeadsPerWg) void decode8_kernel(Decode8
         int b = c.b;
         do {
             ++b;
-            if (b - win.b0 >= 64) load_window(win, a, b, lane);
-            c = seq_cursor(win, b);
+            if (b - win.b0 >= 64) window(b);
+            c = begin(b);
         } while (c.npg == 0);
         return c;
     };
@@ -235,8 +249,8 @@ __global__ __launch_bounds__(64 * kDecodeHeadsPerWg) void decode8_kernel(Decode8
 
     // Cursors cq[0] (folded in now) .. cq[kRing - 1] (issued now), and the
     // page after that, whose id is fetched a block ahead.
-    Cursor cq[kRing];
-    cq[0] = seq_cursor(win, b0);
+    Place cq[kRing];
+    cq[0] = begin(b0);
     cq[0].pg = p_begin - cq[0].base;
     query(b0);
 #pragma unroll
@@ -253,13 +267,13 @@ __global__ __launch_bounds__(64 * kDecodeHeadsPerWg) void decode8_kernel(Decode8
         __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));  // lgkmcnt(0)
         __builtin_amdgcn_sched_barrier(0);
         issue((n + kRing - 1) % kRing, cq[kRing - 1], id);
-        const Cursor after = next(cq[kRing - 1]);
+        const Place after = next(cq[kRing - 1]);
         if (after.ok) id = page_id(after);
         wait_vm<kLoads * (kRing - 1)>();
         __builtin_amdgcn_sched_barrier(0);
-        const Cursor cur = cq[0];
+        const Place cur = cq[0];
         if (is_open(cur))
-            fold_open(st, e.open + (static_cast<size_t>(cur.sid) * hkv + h) * 2 * kPageElems, qb, lane, cur.ctx & 15);
+            fold_open(st, e.open + (static_cast<size_t>(cur.slot) * hkv + h) * 2 * kPageElems, qb, lane, cur.ctx & 15);
         else
             fold_block(st, mine + (n % kRing) * kSlotBytes, qb, lane);
         const bool more = cq[1].ok;

@@ -48,13 +48,14 @@ __device__ __forceinline__ int query_dim(int s, int grp) {
 
 // What a workgroup works on: pages [p0, p1) of sequence b for KV head h.
 struct Span {
-    int b, h, sid, ctx, obs, tok, p0, p1;  // obs: query tokens, from token `tok` of the step
+    int b, h, sid, slot, ctx, obs, tok, p0, p1;  // slot: open block; obs: query tokens, from token `tok` of the step
 };
 __device__ __forceinline__ Span span_of(const WeightArgs &a) {
     Span s;
     s.b = blockIdx.z;
     s.h = blockIdx.y;
     s.sid = ld_uniform(a.seq_ids + s.b);
+    s.slot = a.k8 ? ld_uniform(a.open_slot + s.b) : 0;
     s.ctx = ld_uniform(a.ctx_lens + s.b);
     const int t0 = ld_uniform(a.tok_off + s.b), t1 = ld_uniform(a.tok_off + s.b + 1);
     s.obs = min(t1 - t0, a.n_obs);
@@ -88,7 +89,7 @@ __device__ __forceinline__ void operands(half8_t (&op)[8], float &factor, const 
     factor = k.factor;
     if constexpr (kInt8) {
         if (page == (s.ctx >> 4)) {  // the open page
-            const uint16_t *src = a.open + (static_cast<size_t>(s.sid) * a.num_kv_heads + s.h) * 2 * kPageElems + 16 * lane;
+            const uint16_t *src = a.open + (static_cast<size_t>(s.slot) * a.num_kv_heads + s.h) * 2 * kPageElems + 16 * lane;
 #pragma unroll
             for (int i = 0; i < 8; ++i) op[i] = as_h8(ld16(src + 1024 * (i >> 1) + 8 * (i & 1)));
             factor = kQkScale;
@@ -413,65 +414,49 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(SelectArgs a) {
 // ---- the rows that stay, in pages of their own ----------------------------------
 
 // grid (record, KV head, layer), a half-wave per row of a destination page.
-// The last record of a sequence has its last full page and the rows behind it
-// together: both are read before either is written, so a sequence's open block,
-// whose rows end up in these two at most, may be its own destination's.
+// Nothing that is read is written: destinations are other blocks than the
+// sources', and the last page of an 8-bit cache goes to the sequence's other open
+// block.
 template <bool kInt8>
 __global__ __launch_bounds__(32 * kBlockTokens) void gather_kernel(GatherArgs a) {
     __shared__ CloseLds lds;
     const int hkv = gridDim.y, h = blockIdx.y, layer = blockIdx.z;
     const int row = threadIdx.x >> 5, l32 = threadIdx.x & 31;
     const int32_t *rec = a.recs + static_cast<size_t>(blockIdx.x) * kTouchWords;
-    const int b = ld_uniform(rec), page = ld_uniform(rec + 1), src = ld_uniform(rec + 2), dst = ld_uniform(rec + 3);
-    const int blk0 = ld_uniform(rec + 4), blk1 = ld_uniform(rec + 5), n = ld_uniform(rec + 6), src_open = ld_uniform(rec + 7);
+    const int b = ld_uniform(rec), page = ld_uniform(rec + 1), src = ld_uniform(rec + 2), blk = ld_uniform(rec + 3);
+    const int n = ld_uniform(rec + 4), src_open = ld_uniform(rec + 5), src_slot = ld_uniform(rec + 6);
     const int32_t *kept = a.kept + ((static_cast<size_t>(layer) * a.n_seqs + b) * hkv + h) * a.kept_stride + 16 * page;
     const int32_t *trow = a.table + static_cast<size_t>(src) * a.table_stride;
-    uint16_t *open = kInt8 ? a.open + layer * a.layer_open : nullptr;
-    const uint8_t *k8 = kInt8 ? a.k8 + layer * a.layer_codes : nullptr, *v8 = kInt8 ? a.v8 + layer * a.layer_codes : nullptr;
-    const float *scales = kInt8 ? a.scales + layer * a.layer_scales : nullptr;
-    uint16_t *kp = kInt8 ? nullptr : a.k_pool + layer * a.layer_elems, *vp = kInt8 ? nullptr : a.v_pool + layer * a.layer_elems;
-    auto fetch = [&](int i) -> BlockRow {  // row i of this record's
-        BlockRow x{};
-        if (i >= n) return x;
-        const int j = kept[i], pg = j >> 4;
-        if (kInt8 && pg == src_open)
-            return load_open_row(open + (static_cast<size_t>(src) * hkv + h) * 2 * kPageElems, j & 15, l32);
-        const int id = trow[pg];
-        if constexpr (kInt8) {
-            const size_t at = static_cast<size_t>(id) * hkv + h;
-            return load_code_row(k8 + at * kPageElems, v8 + at * kPageElems, scales + 2 * at, j & 15, l32);
-        } else {
-            const size_t at = ((static_cast<size_t>(id) * kBlockTokens + (j & 15)) * hkv + h) * kHeadDim + 8 * l32;
-            x.k = ld16(kp + at);
-            x.v = ld16(vp + at);
-            return x;
-        }
-    };
-    // A full page (blk0 >= 0) and the rows behind it, or those alone.
-    const bool full = blk0 >= 0;
-    const int more0 = full ? kBlockTokens : 0;
-    BlockRow x{}, y{};
-    if (full) x = fetch(row);
-    if (n > more0) y = fetch(more0 + row);
-    if (n > more0) __syncthreads();  // uniform
-    auto put = [&](int blk, const BlockRow &r) {
-        const size_t at = ((static_cast<size_t>(blk) * kBlockTokens + row) * hkv + h) * kHeadDim + 8 * l32;
-        st16(kp + at, r.k);
-        st16(vp + at, r.v);
-    };
-    if (more0 + row < n) {
-        if constexpr (kInt8)
-            store_open_row(open + (static_cast<size_t>(dst) * hkv + h) * 2 * kPageElems, row, l32, y);
-        else
-            put(blk1, y);
-    }
-    if (!full) return;
+    BlockRow x{};
     if constexpr (kInt8) {
-        const size_t at = static_cast<size_t>(blk0) * hkv + h;
-        close_block(x, a.k8 + layer * a.layer_codes + at * kPageElems, a.v8 + layer * a.layer_codes + at * kPageElems,
-                    a.scales + layer * a.layer_scales + 2 * at, lds);
+        uint8_t *k8 = a.k8 + layer * a.layer_codes, *v8 = a.v8 + layer * a.layer_codes;
+        float *scales = a.scales + layer * a.layer_scales;
+        uint16_t *open = a.open + layer * a.layer_open;
+        if (row < n) {
+            const int j = kept[row], pg = j >> 4;
+            if (pg == src_open) {
+                x = load_open_row(open + (static_cast<size_t>(src_slot) * hkv + h) * 2 * kPageElems, j & 15, l32);
+            } else {
+                const size_t at = static_cast<size_t>(trow[pg]) * hkv + h;
+                x = load_code_row(k8 + at * kPageElems, v8 + at * kPageElems, scales + 2 * at, j & 15, l32);
+            }
+        }
+        if (blk < 0) {  // uniform
+            if (row < n) store_open_row(open + (static_cast<size_t>(-1 - blk) * hkv + h) * 2 * kPageElems, row, l32, x);
+            return;
+        }
+        const size_t at = static_cast<size_t>(blk) * hkv + h;
+        close_block(x, k8 + at * kPageElems, v8 + at * kPageElems, scales + 2 * at, lds);
     } else {
-        put(blk0, x);
+        if (row >= n) return;
+        const int j = kept[row];
+        const uint16_t *kp = a.k_pool + layer * a.layer_elems, *vp = a.v_pool + layer * a.layer_elems;
+        const size_t from = ((static_cast<size_t>(trow[j >> 4]) * kBlockTokens + (j & 15)) * hkv + h) * kHeadDim + 8 * l32;
+        const size_t to = ((static_cast<size_t>(blk) * kBlockTokens + row) * hkv + h) * kHeadDim + 8 * l32;
+        x.k = ld16(kp + from);
+        x.v = ld16(vp + from);
+        st16(a.k_pool + layer * a.layer_elems + to, x.k);
+        st16(a.v_pool + layer * a.layer_elems + to, x.v);
     }
 }
 

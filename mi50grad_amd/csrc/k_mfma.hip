@@ -112,7 +112,6 @@ struct Unit {
     int b, h, tile;       // sequence (index in the step), kv head, query tile
     int ctx, ns, tok, T;  // keys visible, first new slot, first token, new tokens
     const int32_t *trow;  // block-table row
-    int sid;              // cache slot of the sequence
 };
 
 // Units are head-major: unit u is tile r = u % U1 of head u / U1 (U1 =
@@ -136,8 +135,7 @@ __device__ __forceinline__ Unit load_unit(const MultiQueryArgs &a, int u, int b)
     x.ns = ld_uniform(a.new_start + b);
     x.tok = ld_uniform(a.tok_off + b);
     x.T = ld_uniform(a.tok_off + b + 1) - x.tok;
-    x.sid = ld_uniform(a.seq_ids + b);
-    x.trow = a.table + static_cast<size_t>(x.sid) * a.table_stride;
+    x.trow = a.table + static_cast<size_t>(ld_uniform(a.seq_ids + b)) * a.table_stride;
     return x;
 }
 
@@ -306,7 +304,7 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
     const int nt8 = wv >> 1, ih8 = wv & 1, ks8 = wv >> 2, j8 = wv & 3;
     [[maybe_unused]] uint4 rk[2], rv[2];
     [[maybe_unused]] float rsc = 0.0f;  // lane l: scale of page l % kPages, of V where l & kPages
-    [[maybe_unused]] int pg8 = 0, open8 = -1, lim8 = 0, sid8 = 0, h8 = 0;
+    [[maybe_unused]] int pg8 = 0, open8 = -1, lim8 = 0, slot8 = 0, h8 = 0;
     [[maybe_unused]] bool on8 = false;
     [[maybe_unused]] auto ids8 = [&]() {
         const int p0 = (ig - iu.ub) * kPages;
@@ -317,7 +315,7 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
         pg8 = (ig - iu.ub) * kPages;
         open8 = (iu.ctx & 15) ? iu.ctx >> 4 : -1;
         lim8 = iu.ctx & 15;
-        sid8 = iu.sid;
+        slot8 = ld_uniform(a.open_slot + iu.b);
         h8 = iu.h;
         const int full = on8 ? iu.ctx >> 4 : 0;  // full pages of the sequence
         auto codes = [&](const uint8_t *base, int p) {
@@ -342,7 +340,7 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
     };
     [[maybe_unused]] auto put8 = [&](int st) {
         if (!on8) return;  // uniform over the workgroup
-        const uint16_t *open = a.open + (static_cast<size_t>(sid8) * hkv + h8) * 2 * kPageElems;
+        const uint16_t *open = a.open + (static_cast<size_t>(slot8) * hkv + h8) * 2 * kPageElems;
         auto scale_of = [&](int lane_of) {
             return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, rsc), lane_of));
         };

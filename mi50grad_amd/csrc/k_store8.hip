@@ -7,10 +7,10 @@
 // the workgroup takes the rows that came earlier from the sequence's open
 // block and writes the page's codes: from FP16 rows always, so a page's codes do
 // not depend on the steps that its rows came in.  Otherwise the new rows join
-// the open block.  Where a step closes the open page and leaves rows in a later
-// one, one workgroup does both: the open block's old rows have been read when
-// its new ones are written.  Query rows are normalised by further workgroups of
-// the launch.
+// the open block.  A page that is open after another lies in the sequence's other
+// open block, so nothing that a step reads is written by it: its workgroups
+// need no order, and an append that is called again gives the same.  Query rows
+// are normalised by further workgroups of the launch.
 //
 // Bound by latency for a decode step (a touch is one row) and by memory
 // for a prompt.
@@ -44,39 +44,33 @@ __global__ __launch_bounds__(kThreads) void store8_kernel(Store8Args a) {
     const int u = blockIdx.x / hkv, h = blockIdx.x - u * hkv;
     const int32_t *rec = a.touch + static_cast<size_t>(u) * kTouchWords;
     const int seq = ld_uniform(rec), page = ld_uniform(rec + 1), tok0 = ld_uniform(rec + 2);
-    const int r0 = ld_uniform(rec + 3), n = ld_uniform(rec + 4), tok1 = ld_uniform(rec + 5), n1 = ld_uniform(rec + 6);
+    const int r0 = ld_uniform(rec + 3), n = ld_uniform(rec + 4), slot = ld_uniform(rec + 5);
     const bool closes = r0 + n == kBlockTokens;  // uniform over the workgroup
-    uint16_t *open = a.open + (static_cast<size_t>(seq) * hkv + h) * 2 * kPageElems;
-    // Token t's row, as the cache takes it; every half-wave of a wave calls it
-    // (one without a row with t = -1), so the lane exchanges are whole.
-    auto fresh_row = [&](int t) -> BlockRow {
-        BlockRow x{};
-        const size_t at = (static_cast<size_t>(max(t, 0)) * hkv + h) * kHeadDim + 8 * l32;
-        if (t >= 0) {
-            x.k = ld16(ap.k + at);
-            x.v = ld16(ap.v + at);
-        }
-        if (a.norm) {
-            const int pos = t >= 0 ? ap.tok_pos[t] : 0;
-            const NormRopeIn in = norm_rope_in<32>(ap.k_w, ap.cos_tab + static_cast<size_t>(pos) * ap.half_rot,
-                                                   ap.sin_tab + static_cast<size_t>(pos) * ap.half_rot, ap.half_rot, l32);
-            x.k = norm_rope_apply<32>(x.k, in, ap.half_rot, ap.eps, l32);
-            if (t >= 0 && !ap.keep_k) st16(ap.k + at, x.k);
-        }
-        mend_row(x);
-        return x;
-    };
+    uint16_t *open = a.open + (static_cast<size_t>(slot) * hkv + h) * 2 * kPageElems;
     const bool fresh = row >= r0 && row < r0 + n;
-    BlockRow x = fresh_row(fresh ? tok0 + row - r0 : -1);
+    const int t = fresh ? tok0 + row - r0 : 0;
+    const size_t at = (static_cast<size_t>(t) * hkv + h) * kHeadDim + 8 * l32;
+    BlockRow x{};
+    if (fresh) {
+        x.k = ld16(ap.k + at);
+        x.v = ld16(ap.v + at);
+    } else if (closes) {  // row < r0
+        x = load_open_row(open, row, l32);
+    }
+    if (a.norm) {  // by every half-wave, so that its lane exchanges are whole
+        const int pos = fresh ? ap.tok_pos[t] : 0;
+        const NormRopeIn in = norm_rope_in<32>(ap.k_w, ap.cos_tab + static_cast<size_t>(pos) * ap.half_rot,
+                                               ap.sin_tab + static_cast<size_t>(pos) * ap.half_rot, ap.half_rot, l32);
+        const uint4 y = norm_rope_apply<32>(x.k, in, ap.half_rot, ap.eps, l32);
+        if (fresh) {
+            x.k = y;
+            if (!ap.keep_k) st16(ap.k + at, y);
+        }
+    }
+    mend_row(x);  // an earlier row of the open block has been through this
     if (!closes) {
         if (fresh) store_open_row(open, row, l32, x);
         return;
-    }
-    if (!fresh) x = load_open_row(open, row, l32);  // row < r0
-    if (n1 > 0) {
-        const BlockRow y = fresh_row(row < n1 ? tok1 + row : -1);
-        __syncthreads();
-        if (row < n1) store_open_row(open, row, l32, y);
     }
     const int blk = ld_uniform(ap.table + static_cast<size_t>(seq) * ap.table_stride + page);
     const size_t b = static_cast<size_t>(blk) * hkv + h;
@@ -92,7 +86,8 @@ __global__ __launch_bounds__(kThreads) void read_rows_kernel(ReadRowsArgs a) {
     const int u = blockIdx.x / hkv, h = blockIdx.x - u * hkv;
     const int32_t *rec = a.touch + static_cast<size_t>(u) * kTouchWords;
     const int seq = ld_uniform(rec), page = ld_uniform(rec + 1), to = ld_uniform(rec + 2);
-    const int r0 = ld_uniform(rec + 3), n = ld_uniform(rec + 4), is_open = ld_uniform(rec + 5);
+    const int r0 = ld_uniform(rec + 3), n = ld_uniform(rec + 4), slot = ld_uniform(rec + 5);
+    const bool is_open = kInt8 && slot >= 0;
     const bool mine = row >= r0 && row < r0 + n;
     const int blk = is_open ? 0 : ld_uniform(a.table + static_cast<size_t>(seq) * a.table_stride + page);
     BlockRow x{};
@@ -100,7 +95,7 @@ __global__ __launch_bounds__(kThreads) void read_rows_kernel(ReadRowsArgs a) {
         __shared__ __attribute__((aligned(16))) uint8_t codes[2][kPageElems];
         if (is_open) {
             if (mine)
-                x = load_open_row(a.open + (static_cast<size_t>(seq) * hkv + h) * 2 * kPageElems, row, l32);
+                x = load_open_row(a.open + (static_cast<size_t>(slot) * hkv + h) * 2 * kPageElems, row, l32);
         } else {
             const size_t b = static_cast<size_t>(blk) * hkv + h;
             reinterpret_cast<uint2 *>(codes[0])[threadIdx.x] =
@@ -140,11 +135,11 @@ __global__ __launch_bounds__(256) void copy_rows_kernel(AppendArgs a) {
 __global__ __launch_bounds__(kThreads) void reopen_kernel(ReopenArgs a) {
     const int hkv = gridDim.y, h = blockIdx.y, layer = blockIdx.z;
     const int32_t *rec = a.touch + static_cast<size_t>(blockIdx.x) * kTouchWords;
-    const int seq = ld_uniform(rec), page = ld_uniform(rec + 1);
+    const int seq = ld_uniform(rec), page = ld_uniform(rec + 1), slot = ld_uniform(rec + 5);
     const int blk = ld_uniform(a.table + static_cast<size_t>(seq) * a.table_stride + page);
     const size_t b = static_cast<size_t>(blk) * hkv + h;
     const float2 s = *reinterpret_cast<const float2 *>(a.scales + layer * a.layer_scales + 2 * b);
-    uint16_t *open = a.open + layer * a.layer_open + (static_cast<size_t>(seq) * hkv + h) * 2 * kPageElems;
+    uint16_t *open = a.open + layer * a.layer_open + (static_cast<size_t>(slot) * hkv + h) * 2 * kPageElems;
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
         const uint8_t *codes = (kv ? a.v8 : a.k8) + layer * a.layer_codes + b * kPageElems;

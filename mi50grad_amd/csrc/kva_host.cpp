@@ -116,9 +116,15 @@ struct kva_cache {
     std::vector<int32_t> nblk;    // blocks held per sequence
     std::vector<int32_t> len;     // committed length per sequence
     std::vector<uint8_t> freed;   // sequence released by kva_seq_free
-    // 8-bit cache: the page whose rows a sequence's open block holds (-1:
-    // none), and the rows that its pages and open block hold.
-    std::vector<int32_t> open_page, held;
+    // 8-bit cache: a sequence has two open blocks (2 s and 2 s + 1), used in
+    // turn, so that a step that closes one page and opens another reads one and
+    // writes the other.  Which page each holds (-1: none) and how many of its
+    // rows, which was written last, and the rows that the sequence was given.
+    struct OpenBlock {
+        int32_t page = -1, rows = 0;
+    };
+    std::vector<OpenBlock> open_blocks;  // [max_seqs * 2]
+    std::vector<int32_t> open_last, held;
     std::vector<uint8_t> used;    // per block
     std::vector<int32_t> free_list;
     std::vector<int32_t> patches; // pending (seq, idx, block) triples
@@ -139,7 +145,7 @@ struct kva_cache {
     bool st_all_one = false, st_has_bits = false;
     std::vector<int32_t> st_pre;  // pages of the step's earlier sequences, [n_seqs + 1]
     size_t off_seq = 0, off_ctx = 0, off_start = 0, off_tokoff = 0, off_tseq = 0,
-           off_tslot = 0, off_tpos = 0, off_bits = 0, off_pre = 0, off_pids = 0, off_cut = 0, off_touch = 0;
+           off_tslot = 0, off_tpos = 0, off_bits = 0, off_pre = 0, off_pids = 0, off_cut = 0, off_touch = 0, off_slot = 0;
     int32_t st_touch = 0;  // 8-bit cache: pages that the step's rows go to
 
     // Caller's timing events around the dominant kernel of each hot call
@@ -165,7 +171,7 @@ struct kva_graph {
     hipGraphExec_t exec = nullptr;
     int32_t n_seqs = 0, n_tok = 0, table_rows = 0;
     bool all_one = false, has_bits = false;
-    size_t offs[13] = {};
+    size_t offs[14] = {};
 };
 
 namespace {
@@ -315,6 +321,25 @@ int32_t choose_wg(const kva_cache *c, int64_t pages) {
     return static_cast<int32_t>(std::max<int64_t>(1, w));
 }
 
+// The open block that holds the first `rows` rows of sequence s's page (-1: none).
+int open_block_of(const kva_cache *c, int32_t s, int32_t page, int32_t rows) {
+    for (int32_t i = 2 * s; i < 2 * s + 2; ++i)
+        if (c->open_blocks[i].page == page && c->open_blocks[i].rows >= rows) return i;
+    return -1;
+}
+
+// The open block of sequence s's last page as it stands: -1 where the page is
+// full, or its rows are in its codes.
+int last_open_block(const kva_cache *c, int32_t s) {
+    const int32_t rows = c->len[s] % kva::kBlockTokens;
+    return c->int8 && rows ? open_block_of(c, s, c->len[s] / kva::kBlockTokens, rows) : -1;
+}
+
+void forget_open_blocks(kva_cache *c, int32_t s) {
+    c->open_blocks[2 * s] = c->open_blocks[2 * s + 1] = {};
+    c->held[s] = 0;
+}
+
 // An 8-bit cache keeps values, not rows at addresses.
 int refuse_int8(const kva_cache *c, const char *what) {
     if (c->int8) return fail(KVA_ERR_UNSUPPORTED, "%s is not available on an 8-bit cache", what);
@@ -408,12 +433,13 @@ int kva_create(const kva_config *cfg, kva_cache **out) {
     c->nblk.assign(cfg->max_seqs, 0);
     c->len.assign(cfg->max_seqs, 0);
     c->freed.assign(cfg->max_seqs, 0);
-    c->open_page.assign(cfg->max_seqs, -1);
+    c->open_blocks.assign(2 * static_cast<size_t>(cfg->max_seqs), {});
+    c->open_last.assign(cfg->max_seqs, 0);
     c->held.assign(cfg->max_seqs, 0);
     const size_t block_heads = static_cast<size_t>(cfg->max_blocks) * cfg->num_kv_heads;
     c->layer_codes = block_heads * kva::kPageElems;
     c->layer_scales = block_heads * 2;
-    c->layer_open = static_cast<size_t>(cfg->max_seqs) * cfg->num_kv_heads * 2 * kva::kPageElems;
+    c->layer_open = 2 * static_cast<size_t>(cfg->max_seqs) * cfg->num_kv_heads * 2 * kva::kPageElems;
     c->used.assign(cfg->max_blocks, 0);
     c->free_list.resize(cfg->max_blocks);
     for (int32_t i = 0; i < cfg->max_blocks; ++i) c->free_list[i] = cfg->max_blocks - 1 - i;
@@ -433,7 +459,8 @@ int kva_create(const kva_config *cfg, kva_cache **out) {
     if (c->int8)  // a sequence's n new rows lie in at most n / 16 + 2 pages
         c->step_bytes += round_up(sizeof(int32_t) * kva::kTouchWords *
                                       (static_cast<size_t>(cfg->max_step_tokens) / kva::kBlockTokens +
-                                       2 * static_cast<size_t>(cfg->max_seqs)),
+                                       2 * static_cast<size_t>(cfg->max_seqs)) +
+                                      sizeof(int32_t) * static_cast<size_t>(cfg->max_seqs),
                                   256);
     const size_t patch_cap = std::max<size_t>(4096, cfg->max_seqs + cfg->max_step_tokens);
     c->aux_bytes = round_up(std::max(patch_cap * 3 * sizeof(int32_t),
@@ -641,8 +668,7 @@ int kva_seq_free(kva_cache *c, int32_t seq) {
     if (c->freed[seq]) return fail(KVA_ERR_DOUBLE_FREE, "sequence %d already freed", seq);
     release_blocks(c, seq);
     c->len[seq] = 0;
-    c->open_page[seq] = -1;
-    c->held[seq] = 0;
+    forget_open_blocks(c, seq);
     c->freed[seq] = 1;
     c->step_valid = false;
     return KVA_OK;
@@ -802,33 +828,49 @@ int kva_step_begin(kva_cache *c, int32_t n_seqs, const int32_t *seq_ids, const i
     const size_t o_tpos = round_up(o_tslot + sizeof(int32_t) * n_tok, 16);
     const size_t o_bits = round_up(o_tpos + sizeof(int32_t) * n_tok, 16);
     const size_t o_pids = round_up(o_bits + (tree_bits ? sizeof(uint64_t) * n_tok : 0), 16);
-    const size_t o_touch = round_up(o_pids + sizeof(int32_t) * kva::kPlanPages * n_seqs, 16);
-    // 8-bit cache: the pages that the step's rows go to, a record each; and the
-    // sequences whose length was set back into a full page, whose rows become
-    // the open block's again.
-    std::vector<int32_t> touches, reopened;
+    const size_t o_slot = round_up(o_pids + sizeof(int32_t) * kva::kPlanPages * n_seqs, 16);
+    const size_t o_touch = round_up(o_slot + (c->int8 ? sizeof(int32_t) * n_seqs : 0), 16);
+    // 8-bit cache: the pages that the step's rows go to, a record each; each
+    // sequence's open block behind the step; and the sequences whose length was
+    // set back into a page that no open block holds, which takes its values then.
+    std::vector<int32_t> touches, reopened, slots;
     if (c->int8) {
         int32_t tok = 0;
         for (int32_t b = 0; b < n_seqs; ++b) {
             const int32_t s = seq_ids[b], start = c->len[s], end = start + n_new[b];
-            if (start % kva::kBlockTokens && c->open_page[s] != start / kva::kBlockTokens)
-                reopened.insert(reopened.end(), {s, start / kva::kBlockTokens, 0, 0, 0, 0, 0, 0});
-            c->open_page[s] = end % kva::kBlockTokens ? end / kva::kBlockTokens : -1;
+            const int32_t from = start / kva::kBlockTokens, to = end / kva::kBlockTokens;
+            const int32_t rows = start % kva::kBlockTokens, behind = end % kva::kBlockTokens;
+            // The block of the page that the step starts in, if rows are there.
+            int32_t old = rows ? open_block_of(c, s, from, rows) : -1;
+            if (rows && old < 0) {
+                old = 2 * s + 1 - c->open_last[s];
+                reopened.insert(reopened.end(), {s, from, 0, 0, 0, old, 0, 0});
+            }
+            if (old >= 0) {
+                c->open_blocks[old] = {from, rows};
+                c->open_last[s] = old & 1;
+            }
+            // Pages from this one on are written anew: what else was held of them is not theirs.
+            kva_cache::OpenBlock &other = c->open_blocks[2 * s + 1 - c->open_last[s]];
+            if (other.page >= from) other = {};
+            if (old < 0 && c->open_blocks[2 * s + c->open_last[s]].page >= from)
+                c->open_blocks[2 * s + c->open_last[s]] = {};
+            int32_t now = old;
+            if (behind && (old < 0 || to != from)) {
+                c->open_last[s] ^= 1;
+                now = 2 * s + c->open_last[s];
+            }
+            if (behind) c->open_blocks[now] = {to, behind};
+            slots.push_back(std::max(now, 0));
             c->held[s] = end;
-            // The open page, closed by this step, and the rows that are then open
-            // are one record: the open block holds both, one after the other.
-            const int32_t behind = end % kva::kBlockTokens;
-            const bool both = start % kva::kBlockTokens && behind && end / kva::kBlockTokens != start / kva::kBlockTokens;
-            const int32_t last = both ? end - behind : end;
-            for (int32_t at = start; at < last;) {
-                const int32_t r0 = at % kva::kBlockTokens, n = std::min(last - at, kva::kBlockTokens - r0);
-                const int32_t tok1 = tok + last - at;  // the first of the rows behind
-                touches.insert(touches.end(), {s, at / kva::kBlockTokens, tok, r0, n, r0 && both ? tok1 : 0,
-                                               r0 && both ? behind : 0, 0});
+            for (int32_t at = start; at < end;) {
+                const int32_t page = at / kva::kBlockTokens, r0 = at % kva::kBlockTokens;
+                const int32_t n = std::min(end - at, kva::kBlockTokens - r0);
+                const int32_t slot = r0 ? old : page == to ? now : 0;
+                touches.insert(touches.end(), {s, page, tok, r0, n, slot, 0, 0});
                 at += n;
                 tok += n;
             }
-            tok += end - last;
         }
     }
     const size_t o_cut = o_touch + touches.size() * sizeof(int32_t);
@@ -917,6 +959,7 @@ int kva_step_begin(kva_cache *c, int32_t n_seqs, const int32_t *seq_ids, const i
     }
     p_mqpre[units] = static_cast<int32_t>(blocks);
     if (tree_bits) std::memcpy(h + o_bits, tree_bits, sizeof(uint64_t) * n_tok);
+    if (!slots.empty()) std::memcpy(h + o_slot, slots.data(), slots.size() * sizeof(int32_t));
     if (!touches.empty()) std::memcpy(h + o_touch, touches.data(), touches.size() * sizeof(int32_t));
     // The units the multi-query launch will cut across workgroups (the same
     // shares: kva::mq_wg_count workgroups over the unit positions), one
@@ -984,6 +1027,7 @@ int kva_step_begin(kva_cache *c, int32_t n_seqs, const int32_t *seq_ids, const i
     } else {
         c->patches.clear();
     }
+    c->off_slot = o_slot;
     c->off_touch = o_touch;
     c->st_touch = static_cast<int32_t>(touches.size() / kva::kTouchWords);
     c->off_seq = o_seq;
@@ -1488,6 +1532,7 @@ static int decode_impl(kva_cache *c, int32_t layer, const void *q, const void *g
         kva::Decode8Args d{};
         d.d = a;
         set_layer8(c, layer, d);
+        d.open_slot = at<int32_t>(c->d_step, c->off_slot);
         KVA_HIP(kva::launch_decode8(d, static_cast<hipStream_t>(stream)));
         return KVA_OK;
     }
@@ -1571,12 +1616,12 @@ int kva_read_rows(kva_cache *c, int32_t layer, int32_t n_seqs, const int32_t *se
             return fail(KVA_ERR_INVALID_ARG, "sequence %d: rows [%d, %d + %d) outside its %d", s, first[b], first[b],
                         count[b], c->len[s]);
         if (rows + count[b] > INT32_MAX) return fail(KVA_ERR_INVALID_ARG, "more than %d rows", INT32_MAX);
-        const int32_t end = first[b] + count[b];
+        const int32_t end = first[b] + count[b], open = last_open_block(c, s);
         for (int32_t at = first[b]; at < end;) {
             const int32_t page = at / kva::kBlockTokens, r0 = at % kva::kBlockTokens;
             const int32_t n = std::min(end - at, kva::kBlockTokens - r0);
-            const int32_t open = c->int8 && c->open_page[s] == page;
-            touches.insert(touches.end(), {s, page, static_cast<int32_t>(rows), r0, n, open, 0, 0});
+            const int32_t slot = page == c->len[s] / kva::kBlockTokens ? open : -1;
+            touches.insert(touches.end(), {s, page, static_cast<int32_t>(rows), r0, n, slot, 0, 0});
             at += n;
             rows += n;
         }
@@ -1649,10 +1694,12 @@ int kva_attn_weights(kva_cache *c, int32_t layer, const void *q, int32_t n_obs, 
     a.tok_off = at<int32_t>(c->d_step, c->off_tokoff);
     a.table = c->d_table;
     a.table_stride = c->cfg.max_blocks_per_seq;
-    if (c->int8)
+    if (c->int8) {
         set_layer8(c, layer, a);
-    else
+        a.open_slot = at<int32_t>(c->d_step, c->off_slot);
+    } else {
         a.k_pool = c->d_k + c->layer_elems * layer;
+    }
     a.n_seqs = c->st_n_seqs;
     a.num_heads = c->cfg.num_heads;
     a.num_kv_heads = c->cfg.num_kv_heads;
@@ -1806,20 +1853,22 @@ int kva_evict(kva_cache *c, int32_t n_seqs, const int32_t *src_ids, const int32_
             c->used[id] = 1;
         }
         const int32_t full = n / kva::kBlockTokens, behind = n % kva::kBlockTokens;
-        const int32_t src_open = c->int8 ? c->open_page[src] : -1;
-        for (int32_t p = 0; p < full; ++p) {
-            const bool last = p + 1 == full && behind;
-            recs.insert(recs.end(), {b, p, src, dst, ids[p], last ? ids[p + 1] : -1,
-                                     kva::kBlockTokens + (last ? behind : 0), src_open});
-        }
-        if (full == 0 && behind) recs.insert(recs.end(), {b, 0, src, dst, -1, ids[0], behind, src_open});
+        const int32_t src_slot = last_open_block(c, src);
+        const int32_t src_open = src_slot >= 0 ? c->len[src] / kva::kBlockTokens : -1;
+        for (int32_t p = 0; p < full; ++p)
+            recs.insert(recs.end(), {b, p, src, ids[p], kva::kBlockTokens, src_open, src_slot, 0});
+        const int32_t dst_slot = 2 * dst + (dst == src && src_slot >= 0 ? 1 - (src_slot & 1) : 0);
+        if (behind)
+            recs.insert(recs.end(), {b, full, src, c->int8 ? -1 - dst_slot : ids[full], behind, src_open, src_slot, 0});
         if (dst == src)
             replaced.emplace_back(src, std::move(ids));
         else
             adopt(dst, ids);
         c->len[dst] = n;
+        forget_open_blocks(c, dst);
         c->held[dst] = n;
-        c->open_page[dst] = behind ? full : -1;
+        if (behind) c->open_blocks[dst_slot] = {full, behind};
+        c->open_last[dst] = dst_slot & 1;
     }
     if ((rc = run_group())) return rc;
     return flush_patches(c, s);
@@ -1939,6 +1988,7 @@ static int multi_query(kva_cache *c, int32_t layer, const void *q, void *out, kv
     a.out = static_cast<uint16_t *>(out);
     if (c->int8) {
         set_layer8(c, layer, a);
+        a.open_slot = at<int32_t>(c->d_step, c->off_slot);
     } else {
         a.k_pool = c->d_k + c->layer_elems * layer;
         a.v_pool = c->d_v + c->layer_elems * layer;
@@ -2159,9 +2209,9 @@ int kva_graph_capture_end(kva_cache *c, kva_stream_t stream, kva_graph **out) {
     g->table_rows = c->cap_table_rows;
     g->all_one = c->st_all_one;
     g->has_bits = c->st_has_bits;
-    const size_t offs[13] = {c->off_seq,  c->off_ctx,  c->off_start, c->off_tokoff, c->off_tseq,
-                             c->off_tslot, c->off_tpos, c->off_bits, c->off_pre,    c->off_upre,
-                             c->off_mqpre, c->off_pids, c->off_touch};
+    const size_t offs[14] = {c->off_seq,   c->off_ctx,  c->off_start, c->off_tokoff, c->off_tseq,
+                             c->off_tslot, c->off_tpos, c->off_bits,  c->off_pre,    c->off_upre,
+                             c->off_mqpre, c->off_pids, c->off_slot,  c->off_touch};
     std::memcpy(g->offs, offs, sizeof(offs));
     *out = g;
     return KVA_OK;
@@ -2172,9 +2222,9 @@ int kva_graph_launch(kva_graph *g, kva_stream_t stream) {
     kva_cache *c = g->cache;
     if (c->capturing) return fail(KVA_ERR_STATE, "a graph is being recorded");
     if (!c->step_valid) return fail(KVA_ERR_STATE, "no step begun (kva_step_begin)");
-    const size_t offs[13] = {c->off_seq,  c->off_ctx,  c->off_start, c->off_tokoff, c->off_tseq,
-                             c->off_tslot, c->off_tpos, c->off_bits, c->off_pre,    c->off_upre,
-                             c->off_mqpre, c->off_pids, c->off_touch};
+    const size_t offs[14] = {c->off_seq,   c->off_ctx,  c->off_start, c->off_tokoff, c->off_tseq,
+                             c->off_tslot, c->off_tpos, c->off_bits,  c->off_pre,    c->off_upre,
+                             c->off_mqpre, c->off_pids, c->off_slot,  c->off_touch};
     if (c->st_n_seqs != g->n_seqs || c->st_n_tok != g->n_tok || c->st_all_one != g->all_one ||
         c->st_has_bits != g->has_bits || std::memcmp(offs, g->offs, sizeof(offs)) != 0)
         return fail(KVA_ERR_STATE, "the current step (%d sequences, %d tokens) is not the recorded shape (%d, %d)",

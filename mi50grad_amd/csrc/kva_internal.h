@@ -20,9 +20,9 @@ constexpr int kCombineChunk = 16; // decode partials a combine wave requests tog
 constexpr size_t kPageElems = kBlockTokens * kHeadDim;  // values of a block: a KV head's share of a page, K or V
 // A touch: the rows of one page that a step writes or a read wants.  int32
 // words: sequence, page of it, first row's place among the step's tokens (or
-// the output's rows), first row within the page, rows; then for a read 1 if the
-// page is the sequence's open block, for a write that closes the open page the
-// step's first row of the page that is open then, and its rows (0: none).
+// the output's rows), first row within the page, rows, open block (of a write:
+// the one that the page's earlier rows are in, or its rows stay in; of a read:
+// the one that holds the page, -1: none); two spare.
 constexpr int kTouchWords = 8;
 
 // Fused QK-RMSNorm + RoPE + K/V append over all new tokens of a step.
@@ -313,6 +313,7 @@ struct MultiQueryArgs {
     const uint8_t *k8, *v8;
     const float *scales;
     const uint16_t *open;
+    const int32_t *open_slot;  // device [n_seqs]
 };
 // Keys per multi-query block.  64 for a step of eight-wave prefill tiles
 // (half the barriers, page lookups and softmax reductions per key, two LDS
@@ -372,7 +373,7 @@ struct Store8Args {
     int32_t norm;
     uint8_t *k8, *v8;         // this layer's codes [blocks][Hkv][kPageElems]
     float *scales;            // [blocks][Hkv][2]: K's, V's
-    uint16_t *open;           // open blocks [max_seqs][Hkv][2][kPageElems]
+    uint16_t *open;           // open blocks [max_seqs * 2][Hkv][2: K, V][kPageElems]
 };
 hipError_t launch_store8(const Store8Args &a, hipStream_t s);
 // append_rows on an FP16 cache: ap.k, ap.v to their slots as they are.
@@ -384,6 +385,7 @@ struct Decode8Args {
     const uint8_t *k8, *v8;   // as in Store8Args
     const float *scales;
     const uint16_t *open;
+    const int32_t *open_slot; // device [n_seqs]: each sequence's open block after the step
 };
 hipError_t launch_decode8(const Decode8Args &a, hipStream_t s);
 // Rows as FP16, from an FP16 cache (k8 null) or an 8-bit one.
@@ -402,7 +404,7 @@ struct ReadRowsArgs {
 hipError_t launch_read_rows(const ReadRowsArgs &a, hipStream_t s);
 // Open blocks from their pages' codes, in every layer (bases of layer 0).
 struct ReopenArgs {
-    const int32_t *touch;     // device [n][kTouchWords]: sequence, page
+    const int32_t *touch;     // device [n][kTouchWords]: sequence, page, .., open block
     const int32_t *table;
     int32_t table_stride;
     const uint8_t *k8, *v8;
@@ -428,6 +430,7 @@ struct WeightArgs {
     const uint8_t *v8;
     const float *scales;
     const uint16_t *open;
+    const int32_t *open_slot; // device [n_seqs] (8-bit cache)
     int32_t n_seqs, num_heads, num_kv_heads;
     int32_t n_obs;
     int32_t splits;           // workgroups that share a sequence's pages
@@ -455,9 +458,9 @@ hipError_t launch_select(const SelectArgs &a, int32_t n_seqs, int32_t n_layers, 
 
 struct GatherArgs {
     // Device [n][kTouchWords]: sequence's index in the call, destination page,
-    // source sequence, destination sequence, block of the page (-1: none full),
-    // block of the rows behind it (FP16 cache), rows of both, the source's open
-    // page (-1: none).
+    // source sequence, destination block (of an 8-bit cache's last page, not
+    // full: -1 - its open block), rows, the source's open page (-1: none) and
+    // open block.
     const int32_t *recs;
     const int32_t *kept;
     int64_t kept_stride;

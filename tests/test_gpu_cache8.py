@@ -69,6 +69,49 @@ def test_rows_that_close_the_open_page_and_open_another(device):
     cache.destroy()
 
 
+def test_append_again_in_a_step_gives_the_same(device):
+    """Each append of a step may be called more than once: pages that close take
+    their earlier rows as they were before the step."""
+    say("append again")
+    rng = np.random.default_rng(15)
+    kv, lens, new = 3, [5, 20, 47, 16], [30, 29, 1, 9]
+    cache = make([o + n for o, n in zip(lens, new)], heads=kv, kv=kv)
+    data = [rows(rng, o + n, kv) for o, n in zip(lens, new)]
+    seqs = list(range(4))
+    put(device, cache, seqs, [d[0][:o] for d, o in zip(data, lens)], [d[1][:o] for d, o in zip(data, lens)])
+    cache.begin_step(seqs, new)
+    k, v = [device.array(np.concatenate([d[i][o:] for d, o in zip(data, lens)])) for i in range(2)]
+    want = [orc.int8_rows(*d) for d in data]
+    for _ in range(3):
+        cache.append_rows(0, k, v)
+        got = held(device, cache, seqs)
+        assert same_bits(got[0], np.concatenate([w[0] for w in want]))
+        assert same_bits(got[1], np.concatenate([w[1] for w in want]))
+    cache.destroy()
+
+
+def test_set_back_past_the_page_before(device):
+    """Back into the page that was open before the present one: its FP16 rows
+    are still there, up to those that came with the row that filled it."""
+    say("set back past a page")
+    rng = np.random.default_rng(16)
+    for back, exact in ((19, True), (16, True), (20, True), (21, False), (31, False), (9, False)):
+        k, v = rows(rng, 40, 2)
+        cache = make([60], heads=2, kv=2)
+        for lo, hi in ((0, 20), (20, 40)):
+            put(device, cache, [0], [k[lo:hi]], [v[lo:hi]])
+        cache.set_len(0, back)
+        k1, v1 = rows(rng, 2, 2)
+        full = [a.astype(np.float16) for a in orc.int8_rows(k, v)]
+        p = back // 16 * 16
+        before = (k[:back], v[:back]) if exact else [np.concatenate([x[:p], f[p:back]]) for x, f in zip((k, v), full)]
+        put(device, cache, [0], [k1], [v1])
+        got = held(device, cache, [0])
+        want = orc.int8_rows(np.concatenate([before[0], k1]), np.concatenate([before[1], v1]))
+        assert same_bits(got[0], want[0]) and same_bits(got[1], want[1]), back
+        cache.destroy()
+
+
 @pytest.mark.parametrize("what", ["zeros", "tiny", "huge", "halfway", "borders", "one_large"])
 def test_rows_of_hard_values(device, what):
     """Magnitudes at the ends of the scales, values half-way between two codes,
