@@ -69,6 +69,8 @@ enum {
  * held in fp16 as it came, in one of two open blocks that take turns (32 KB per
  * sequence slot, KV head and layer), so codes depend on a page's rows alone,
  * not on the steps that they came in, and a step's append may be repeated.
+ * Attention is over these values, in fp32 but for the probabilities, which
+ * are fp16; gated, its output is rounded once, after the gate.
  * A row of a head in which K or V is not finite reads as NaN keys and zero
  * values, and once its page is full every row of that block has NaN keys:
  * attention that sees such a row gives NaN.  All calls of a step are the same

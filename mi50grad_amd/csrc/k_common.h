@@ -284,9 +284,23 @@ __device__ __forceinline__ uint2 gate4(uint2 o, uint2 gw) {
     return make_uint2(y[0], y[1]);
 }
 
+// The gate on four outputs that are not rounded yet (8-bit caches): their only
+// rounding is the last one.
+__device__ __forceinline__ uint2 gate4(float o0, float o1, float o2, float o3, uint2 gw) {
+    const half2_t hi = {static_cast<_Float16>(kGateClamp), static_cast<_Float16>(kGateClamp)};
+    const half2_t a = __builtin_elementwise_maximum(
+        __builtin_elementwise_minimum(__builtin_bit_cast(half2_t, gw.x), hi), -hi);
+    const half2_t b = __builtin_elementwise_maximum(
+        __builtin_elementwise_minimum(__builtin_bit_cast(half2_t, gw.y), hi), -hi);
+    return pack_out4(o0 * sigmoid(static_cast<float>(a.x)), o1 * sigmoid(static_cast<float>(a.y)),
+                     o2 * sigmoid(static_cast<float>(b.x)), o3 * sigmoid(static_cast<float>(b.y)));
+}
+
 // Four attention output dims as fp16, through the gate at g4 (8-byte
-// aligned) unless it is null.
-__device__ __forceinline__ uint2 out_fp16x4(float o0, float o1, float o2, float o3, const uint16_t *g4) {
+// aligned) unless it is null; once: rounded after the gate only.
+__device__ __forceinline__ uint2 out_fp16x4(float o0, float o1, float o2, float o3, const uint16_t *g4,
+                                            bool once = false) {
+    if (g4 && once) return gate4(o0, o1, o2, o3, ld8(g4));
     const uint2 o = pack_out4(o0, o1, o2, o3);
     return g4 ? gate4(o, ld8(g4)) : o;
 }

@@ -233,7 +233,7 @@ __global__ __launch_bounds__(64 * kDecodeHeadsPerWg) void decode8_kernel(Decode8
             for (int t = 0; t < 16; ++t)
                 *reinterpret_cast<uint2 *>(o + 16 * t) =
                     out_fp16x4(st.acc[t][0] * inv, st.acc[t][1] * inv, st.acc[t][2] * inv, st.acc[t][3] * inv,
-                               g ? g + 16 * t : nullptr);
+                               g ? g + 16 * t : nullptr, true);
         } else {
             const int slot = 2 * w + (c.b == b0 ? 0 : 1);
             const size_t u = (static_cast<size_t>(slot) * hkv + h) * G + col;

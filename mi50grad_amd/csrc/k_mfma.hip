@@ -677,16 +677,21 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
 #pragma unroll
                             for (int hh = 0; hh < 2; ++hh) gw[k][hh] = ld16g(a.gate + grow[hh] + 64 * (c + k));
                     }
+                    if (Q8 && a.gate) {  // one rounding, after the gate: the gate comes to the accumulators
+#pragma unroll
+                        for (int hh = 0; hh < 2; ++hh)
+                            *reinterpret_cast<uint4 *>(strip + kStripRow * (8 * hh + r8) + 16 * c8) = gw[c % kGateAhead][hh];
+                    }
 #pragma unroll
                     for (int d = 0; d < 4; ++d) {
                         const float4_t o = acc[t][4 * c + d] * inv;
-                        *reinterpret_cast<uint2 *>(strip + kStripRow * col + 32 * d + 8 * grp) =
-                            pack_out4(o[0], o[1], o[2], o[3]);
+                        uint2 *at = reinterpret_cast<uint2 *>(strip + kStripRow * col + 32 * d + 8 * grp);
+                        *at = Q8 && a.gate ? gate4(o[0], o[1], o[2], o[3], *at) : pack_out4(o[0], o[1], o[2], o[3]);
                     }
 #pragma unroll
                     for (int hh = 0; hh < 2; ++hh) {
                         uint4 y = *reinterpret_cast<const uint4 *>(strip + kStripRow * (8 * hh + r8) + 16 * c8);
-                        if (a.gate) {
+                        if (!Q8 && a.gate) {
                             const uint2 lo = gate4(make_uint2(y.x, y.y), make_uint2(gw[c % kGateAhead][hh].x, gw[c % kGateAhead][hh].y));
                             const uint2 hi = gate4(make_uint2(y.z, y.w), make_uint2(gw[c % kGateAhead][hh].z, gw[c % kGateAhead][hh].w));
                             y = make_uint4(lo.x, lo.y, hi.x, hi.y);
@@ -788,7 +793,7 @@ __global__ __launch_bounds__(64 * kMqCombineRows) void mq_combine_kernel(MultiQu
     }
     const float inv = 1.0f / lt;
     uint2 y = pack_out4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-    if (a.gate) y = gate4(y, gw);
+    if (a.gate) y = a.k8 ? gate4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv, gw) : gate4(y, gw);
     *reinterpret_cast<uint2 *>(a.out + (tq * a.num_heads + hq) * kHeadDim + 4 * lane) = y;
 }
 

@@ -1481,6 +1481,7 @@ static int decode_impl(kva_cache *c, int32_t layer, const void *q, const void *g
     kva::DecodeArgs a{};
     a.gate = static_cast<const uint16_t *>(gate);
     a.gate_stride = gate_stride;
+    a.gate_once = c->int8;
     a.q = static_cast<const uint16_t *>(q);
     if (!c->int8) {
         a.k_pool = c->d_k + c->layer_elems * layer;

@@ -204,6 +204,7 @@ struct DecodeArgs {
     // gate row of sequence b, query head hq at gate + b*gate_stride + hq*256.
     const uint16_t *gate;
     int64_t gate_stride;
+    int32_t gate_once;        // 1: out = fp16(attn * sigmoid(gate)) (8-bit caches)
     // Per-workgroup timeline (null = off): record kTimelineWords words per
     // wave, [n_wg][grid rows][8 waves], see kva_timeline_read.
     uint64_t *timeline;

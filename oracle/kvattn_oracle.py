@@ -509,6 +509,5 @@ def attention_bound(q, k, v, seen=None, gate=None):
         tol[:, h] = (half + 2 * delta + 64 * f32) * (p @ np.abs(vh) + np.abs(out[:, h]))
     if gate is not None:
         g = 1.0 / (1.0 + np.exp(-np.asarray(gate, np.float64)))
-        tol = tol * g + half * np.abs(out) * g  # the ungated output is rounded first
-        out = out * g
+        out, tol = out * g, tol * g + 4 * f32 * np.abs(out) * g
     return out, tol + half * np.abs(out) + np.finfo(np.float16).smallest_subnormal
