@@ -75,22 +75,26 @@ __device__ __forceinline__ half4_t fold_scores(State &st, const float4_t &x) {
     return as_h4(make_uint2(p0, p1));
 }
 
-// A full block from LDS.
+// A full block from LDS.  Every read is requested before any is used.
 __device__ __forceinline__ void fold_block(State &st, const uint8_t *slot, const uint4 (&qb)[8], int lane) {
+    uint4 k[4], v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) k[i] = *reinterpret_cast<const uint4 *>(slot + 1024 * i + 16 * lane);
     const float2 sc = *reinterpret_cast<const float2 *>(slot + 2 * kPageElems);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4 *>(slot + kPageElems + 1024 * i + 16 * lane);
+    __builtin_amdgcn_sched_barrier(0);
     float4_t s[2] = {float4_t{0.f, 0.f, 0.f, 0.f}, float4_t{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint4 w = *reinterpret_cast<const uint4 *>(slot + 1024 * i + 16 * lane);
-        s[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(codes8(w.x, w.y)), as_h8(qb[2 * i]), s[0], 0, 0, 0);
-        s[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(codes8(w.z, w.w)), as_h8(qb[2 * i + 1]), s[1], 0, 0, 0);
+        s[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(codes8(k[i].x, k[i].y)), as_h8(qb[2 * i]), s[0], 0, 0, 0);
+        s[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(codes8(k[i].z, k[i].w)), as_h8(qb[2 * i + 1]), s[1], 0, 0, 0);
     }
     const half4_t p = fold_scores(st, (s[0] + s[1]) * (sc.x * kQkScale));
     const uint32_t vs = scale_h2(sc.y);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const uint4 w = *reinterpret_cast<const uint4 *>(slot + kPageElems + 1024 * j + 16 * lane);
-        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+        const uint32_t ws[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
 #pragma unroll
         for (int t = 0; t < 4; ++t)
             st.acc[4 * j + t] = __builtin_amdgcn_mfma_f32_16x16x16f16(as_h4(values4(ws[t], vs)), p, st.acc[4 * j + t], 0, 0, 0);
@@ -146,7 +150,9 @@ __device__ __forceinline__ void issue_block(uint32_t slot, const uint8_t *k, con
     touch_line(rs, slot + 2 * kPageElems, 4 * (lane & 1), 0);
 }
 
-__global__ __launch_bounds__(64 * kDecodeHeadsPerWg) void decode8_kernel(Decode8Args e) {
+// Held to 256 registers: with 512 the compiler keeps the accumulators in the
+// other half and moves all 64 over at every block.
+__global__ __launch_bounds__(64 * kDecodeHeadsPerWg, 2) void decode8_kernel(Decode8Args e) {
     const DecodeArgs &a = e.d;
     extern __shared__ __attribute__((aligned(16))) uint8_t ring[];  // [waves][kRing][kSlotBytes]
     const int w = blockIdx.x;
@@ -172,70 +178,114 @@ __global__ __launch_bounds__(64 * kDecodeHeadsPerWg) void decode8_kernel(Decode8
         if (before != ~0ull) break;
     }
     b0 = __builtin_amdgcn_readfirstlane(b0);
-    SeqWindow win;
-    int slots = 0;  // lane l: the open block of sequence win.b0 + l
-    auto window = [&](int b) {
-        load_window(win, a, b, lane);
-        slots = b + lane < a.n_seqs ? e.open_slot[b + lane] : 0;
+    // A sequence's pages in the share: [p0, p1) of its npg, the full ones before
+    // `full`; only its last page can be open.  (Every field is wave-uniform.)
+    struct Segment {
+        int b, p0, p1, npg, ctx, full;
+        const int32_t *row;
     };
-    window(b0);
-    struct Place : Cursor {
-        int slot;
+    auto segment = [&](int b) -> Segment {
+        Segment g;
+        g.b = b;
+        g.ctx = ld_uniform(a.ctx_lens + b);
+        const int base = ld_uniform(a.pre_seq + b);
+        g.row = a.table + static_cast<size_t>(ld_uniform(a.seq_ids + b)) * a.table_stride;
+        g.npg = (g.ctx + kBlockTokens - 1) / kBlockTokens;
+        g.p0 = max(0, p_begin - base);
+        g.p1 = min(g.npg, p_end - base);
+        g.full = min(g.p1, g.ctx / kBlockTokens);
+        return g;
     };
-    auto begin = [&](int b) {
-        Place c;
-        static_cast<Cursor &>(c) = seq_cursor(win, b);
-        c.slot = __builtin_amdgcn_readlane(slots, b - win.b0);
-        return c;
-    };
-
-    auto next = [&](Place c) -> Place {
-        if (!c.ok) return c;
-        if (c.base + c.pg + 1 >= p_end) {
-            c.ok = false;
-            return c;
+    // The issue side, kRing - 1 full pages ahead of the products across
+    // sequences: page ip of segment ig next, whose id is `id`; past the share the
+    // same loads go through empty resources, so the load counter advances alike.
+    const int b_last = [&] {  // the sequence of the share's last page
+        int b = b0;
+        while (ld_uniform(a.pre_seq + b + 1) < p_end) ++b;
+        return b;
+    }();
+    Segment ig = segment(b0);
+    int ip = ig.p0, id = 0;
+    bool on = true;
+    auto settle = [&]() {  // to the next full page of the share, if there is one
+        while (ip >= ig.full) {
+            if (ig.b >= b_last) {
+                on = false;
+                return;
+            }
+            ig = segment(ig.b + 1);
+            ip = ig.p0;
         }
-        if (c.pg + 1 < c.npg) {
-            ++c.pg;
-            return c;
-        }
-        int b = c.b;
-        do {
-            ++b;
-            if (b - win.b0 >= 64) window(b);
-            c = begin(b);
-        } while (c.npg == 0);
-        return c;
     };
-    auto page_id = [&](const Cursor &c) -> int {
-        return ld_uniform(a.table + static_cast<size_t>(c.sid) * a.table_stride + c.pg);
+    auto fetch = [&]() {
+        if (on) id = ld_uniform(ig.row + ip);
     };
-    auto is_open = [](const Cursor &c) { return c.pg == (c.ctx >> 4); };  // rows ctx & 15 > 0 of it
-    auto issue = [&](int slot, const Cursor &c, int id) {
+    auto issue = [&](int slot) {
         const size_t blk = static_cast<size_t>(id) * hkv + h;
-        issue_block(lds_addr(mine + slot * kSlotBytes), e.k8 + blk * kPageElems, e.v8 + blk * kPageElems,
-                    e.scales + 2 * blk, c.ok && !is_open(c), lane);
+        issue_block(__builtin_amdgcn_readfirstlane(lds_addr(mine + slot * kSlotBytes)), e.k8 + blk * kPageElems, e.v8 + blk * kPageElems,
+                    e.scales + 2 * blk, on, lane);
+        if (on) {
+            ++ip;
+            settle();
+        }
     };
-
-    uint4 qb[8];
-    auto query = [&](int b) { load_query(qb, a.q + (static_cast<size_t>(b) * nh + h * G) * kHeadDim, G, lane); };
-    State st;
-    reset(st);
-    auto finish = [&](const Cursor &c) {
-        const float lt = group4_sum(st.l);  // the four lane groups hold disjoint rows
-        if (col >= G) return;
-        if (c.base >= p_begin && c.base + c.npg <= p_end) {
-            const float inv = 1.0f / lt;
-            uint16_t *o = a.out + (static_cast<size_t>(c.b) * nh + h * G + col) * kHeadDim + 4 * grp;
-            const uint16_t *g =
-                a.gate ? a.gate + static_cast<int64_t>(c.b) * a.gate_stride + (h * G + col) * kHeadDim + 4 * grp : nullptr;
+    settle();
 #pragma unroll
-            for (int t = 0; t < 16; ++t)
+    for (int i = 0; i + 1 < kRing; ++i) {
+        fetch();
+        issue(i);
+    }
+    fetch();
+
+    int n = 0;  // blocks folded in: the next is in slot n % kRing
+    for (int b = b0; b <= b_last; ++b) {
+        const Segment g = segment(b);
+        if (g.p0 >= g.p1) continue;
+        uint4 qb[8];
+        load_query(qb, a.q + (static_cast<size_t>(b) * nh + h * G) * kHeadDim, G, lane);
+        // Taken in here: left to the compiler, the wait would sit in front of every
+        // block's products and, not seeing the loads to LDS, drain the ring there.
+#pragma unroll
+        for (int k = 0; k < 8; ++k) asm volatile("" : "+v"(qb[k].x), "+v"(qb[k].y), "+v"(qb[k].z), "+v"(qb[k].w));
+        State st;
+        reset(st);
+#pragma unroll 1
+        for (int p = g.p0; p < g.full; ++p, ++n) {
+            // The last reads of the slot that is issued over have returned, and
+            // the page id is there.
+            __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));  // lgkmcnt(0)
+            __builtin_amdgcn_sched_barrier(0);
+            issue((n + kRing - 1) % kRing);
+            wait_vm<kLoads * (kRing - 1)>();
+            __builtin_amdgcn_sched_barrier(0);
+            fold_block(st, mine + (n % kRing) * kSlotBytes, qb, lane);
+            // Behind the block's LDS reads: a scalar load in flight makes each of
+            // their waits a wait for all.
+            __builtin_amdgcn_sched_barrier(0);
+            fetch();
+        }
+        if (g.full < g.p1)
+            fold_open(st, e.open + (static_cast<size_t>(ld_uniform(e.open_slot + b)) * hkv + h) * 2 * kPageElems, qb, lane,
+                      g.ctx & 15);
+        const float lt = group4_sum(st.l);  // the four lane groups hold disjoint rows
+        if (g.p0 == 0 && g.p1 == g.npg && col < G) {
+            const float inv = 1.0f / lt;
+            uint16_t *o = a.out + (static_cast<size_t>(b) * nh + h * G + col) * kHeadDim + 4 * grp;
+            const uint16_t *gate =
+                a.gate ? a.gate + static_cast<int64_t>(b) * a.gate_stride + (h * G + col) * kHeadDim + 4 * grp : nullptr;
+            uint2 gw[16];
+            if (gate) {
+#pragma unroll
+                for (int t = 0; t < 16; ++t) gw[t] = ld8(gate + 16 * t);
+            }
+#pragma unroll
+            for (int t = 0; t < 16; ++t) {
+                const float4_t y = st.acc[t] * inv;
                 *reinterpret_cast<uint2 *>(o + 16 * t) =
-                    out_fp16x4(st.acc[t][0] * inv, st.acc[t][1] * inv, st.acc[t][2] * inv, st.acc[t][3] * inv,
-                               g ? g + 16 * t : nullptr, true);
-        } else {
-            const int slot = 2 * w + (c.b == b0 ? 0 : 1);
+                    gate ? gate4(y[0], y[1], y[2], y[3], gw[t]) : pack_out4(y[0], y[1], y[2], y[3]);
+            }
+        } else if (col < G) {
+            const int slot = 2 * w + (b == b0 ? 0 : 1);
             const size_t u = (static_cast<size_t>(slot) * hkv + h) * G + col;
 #pragma unroll
             for (int t = 0; t < 16; ++t)
@@ -245,48 +295,6 @@ __global__ __launch_bounds__(64 * kDecodeHeadsPerWg) void decode8_kernel(Decode8
                 a.ws_ml[u * 2 + 1] = lt;
             }
         }
-    };
-
-    // Cursors cq[0] (folded in now) .. cq[kRing - 1] (issued now), and the
-    // page after that, whose id is fetched a block ahead.
-    Place cq[kRing];
-    cq[0] = begin(b0);
-    cq[0].pg = p_begin - cq[0].base;
-    query(b0);
-#pragma unroll
-    for (int i = 1; i < kRing; ++i) cq[i] = next(cq[i - 1]);
-    int id = page_id(cq[0]);
-#pragma unroll
-    for (int i = 0; i + 1 < kRing; ++i) {
-        issue(i, cq[i], id);
-        if (cq[i + 1].ok) id = page_id(cq[i + 1]);
-    }
-    int n = 0;
-    while (true) {
-        // Slot n - 1's last reads have returned: it is issued over.
-        __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));  // lgkmcnt(0)
-        __builtin_amdgcn_sched_barrier(0);
-        issue((n + kRing - 1) % kRing, cq[kRing - 1], id);
-        const Place after = next(cq[kRing - 1]);
-        if (after.ok) id = page_id(after);
-        wait_vm<kLoads * (kRing - 1)>();
-        __builtin_amdgcn_sched_barrier(0);
-        const Place cur = cq[0];
-        if (is_open(cur))
-            fold_open(st, e.open + (static_cast<size_t>(cur.slot) * hkv + h) * 2 * kPageElems, qb, lane, cur.ctx & 15);
-        else
-            fold_block(st, mine + (n % kRing) * kSlotBytes, qb, lane);
-        const bool more = cq[1].ok;
-        if (!more || cq[1].b != cur.b) {
-            finish(cur);
-            if (!more) break;
-            query(cq[1].b);
-            reset(st);
-        }
-#pragma unroll
-        for (int i = 0; i + 1 < kRing; ++i) cq[i] = cq[i + 1];
-        cq[kRing - 1] = after;
-        ++n;
     }
     // Loads past the share write LDS too: none may land after it is handed on.
     __builtin_amdgcn_s_waitcnt(0);
