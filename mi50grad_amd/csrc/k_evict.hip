@@ -297,8 +297,8 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(SelectArgs a) {
     const int u = blockIdx.x, layer = blockIdx.y;
     const int b = u / a.num_kv_heads;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int n = ld_uniform(a.seqs + 2 * b), keep = ld_uniform(a.seqs + 2 * b + 1);
-    const size_t at = static_cast<size_t>(layer) * gridDim.x + u;
+    const int n = a.rows[b], keep = a.keep[b];
+    const size_t at = (static_cast<size_t>(layer) * a.n_seqs + a.b0) * a.num_kv_heads + u;
     const float *w = a.weights + at * a.w_stride;
     int32_t *kept = a.kept + at * a.kept_stride;
     float *w_out = a.weights_out ? a.weights_out + at * a.w_stride : nullptr;
@@ -485,9 +485,9 @@ hipError_t launch_weights(const WeightArgs &a, hipStream_t s) {
     return a.k8 ? launch_weights_kind<true>(a, s) : launch_weights_kind<false>(a, s);
 }
 
-hipError_t launch_select(const SelectArgs &a, int32_t n_seqs, int32_t n_layers, int32_t most, hipStream_t s) {
-    if (n_seqs <= 0) return hipSuccess;
-    const dim3 grid(n_seqs * a.num_kv_heads, n_layers), block(kSelectThreads);
+hipError_t launch_select(const SelectArgs &a, int32_t n, int32_t n_layers, int32_t most, hipStream_t s) {
+    if (n <= 0) return hipSuccess;
+    const dim3 grid(n * a.num_kv_heads, n_layers), block(kSelectThreads);
     if (most <= kSelectLds) {
         const size_t lds = static_cast<size_t>(most) * sizeof(uint32_t);
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(select_kernel<true>),

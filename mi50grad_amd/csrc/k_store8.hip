@@ -77,17 +77,24 @@ __global__ __launch_bounds__(kThreads) void store8_kernel(Store8Args a) {
     close_block(x, a.k8 + b * kPageElems, a.v8 + b * kPageElems, a.scales + 2 * b, lds);
 }
 
-// Rows of both kinds of cache as FP16 [row][Hkv][256], packed in the order of
-// the touches; a touch and a KV head per workgroup.
+// Rows of both kinds of cache as FP16 [row][Hkv][256]; a page of a range and a
+// KV head per workgroup.
 template <bool kInt8>
 __global__ __launch_bounds__(kThreads) void read_rows_kernel(ReadRowsArgs a) {
     const int hkv = a.num_kv_heads;
     const int row = threadIdx.x >> 5, l32 = threadIdx.x & 31;
     const int u = blockIdx.x / hkv, h = blockIdx.x - u * hkv;
-    const int32_t *rec = a.touch + static_cast<size_t>(u) * kTouchWords;
-    const int seq = ld_uniform(rec), page = ld_uniform(rec + 1), to = ld_uniform(rec + 2);
-    const int r0 = ld_uniform(rec + 3), n = ld_uniform(rec + 4), slot = ld_uniform(rec + 5);
-    const bool is_open = kInt8 && slot >= 0;
+    // The range: the last whose pages begin at or before this one (each has some).
+    static_assert(kReadSeqs == 64, "a range per lane");
+    const int lane = threadIdx.x & 63;
+    const uint64_t before = __ballot(lane < a.n_ranges && a.range[lane].touch0 <= u);
+    const ReadRange &g = a.range[__builtin_amdgcn_readfirstlane(63 - __clzll(before))];
+    const int seq = g.seq, slot = g.slot;
+    const int page = (g.first >> 4) + u - g.touch0;
+    const int from = max(g.first, 16 * page), r0 = from & 15;
+    const int n = min(g.first + g.count, 16 * page + 16) - from;
+    const int to = g.to + from - g.first;
+    const bool is_open = kInt8 && slot >= 0 && page == g.open_page;
     const bool mine = row >= r0 && row < r0 + n;
     const int blk = is_open ? 0 : ld_uniform(a.table + static_cast<size_t>(seq) * a.table_stride + page);
     BlockRow x{};

@@ -1608,7 +1608,6 @@ int kva_read_rows(kva_cache *c, int32_t layer, int32_t n_seqs, const int32_t *se
     if (rc) return rc;
     if (n_seqs < 0) return fail(KVA_ERR_INVALID_ARG, "n_seqs %d < 0", n_seqs);
     if (n_seqs > 0 && (!seq_ids || !first || !count)) return fail(KVA_ERR_INVALID_ARG, "NULL index array");
-    std::vector<int32_t> touches;
     int64_t rows = 0;
     for (int32_t b = 0; b < n_seqs; ++b) {
         const int32_t s = seq_ids[b];
@@ -1616,17 +1615,9 @@ int kva_read_rows(kva_cache *c, int32_t layer, int32_t n_seqs, const int32_t *se
         if (first[b] < 0 || count[b] < 0 || static_cast<int64_t>(first[b]) + count[b] > c->len[s])
             return fail(KVA_ERR_INVALID_ARG, "sequence %d: rows [%d, %d + %d) outside its %d", s, first[b], first[b],
                         count[b], c->len[s]);
-        if (rows + count[b] > INT32_MAX) return fail(KVA_ERR_INVALID_ARG, "more than %d rows", INT32_MAX);
-        const int32_t end = first[b] + count[b], open = last_open_block(c, s);
-        for (int32_t at = first[b]; at < end;) {
-            const int32_t page = at / kva::kBlockTokens, r0 = at % kva::kBlockTokens;
-            const int32_t n = std::min(end - at, kva::kBlockTokens - r0);
-            const int32_t slot = page == c->len[s] / kva::kBlockTokens ? open : -1;
-            touches.insert(touches.end(), {s, page, static_cast<int32_t>(rows), r0, n, slot, 0, 0});
-            at += n;
-            rows += n;
-        }
+        rows += count[b];
     }
+    if (rows > INT32_MAX) return fail(KVA_ERR_INVALID_ARG, "more than %d rows", INT32_MAX);
     if (rows > 0) {
         if (!k_out || !v_out) return fail(KVA_ERR_INVALID_ARG, "NULL tensor pointer");
         if (!aligned16(k_out) || !aligned16(v_out))
@@ -1648,11 +1639,21 @@ int kva_read_rows(kva_cache *c, int32_t layer, int32_t n_seqs, const int32_t *se
     }
     a.k_out = static_cast<uint16_t *>(k_out);
     a.v_out = static_cast<uint16_t *>(v_out);
-    return upload_touches(c, touches, s, [&](const int32_t *recs, int32_t n) {
-        a.touch = recs;
-        a.n_touch = n;
-        return kva::launch_read_rows(a, s);
-    });
+    int32_t to = 0;
+    for (int32_t b = 0; b < n_seqs; ++b) {
+        const int32_t q = seq_ids[b];
+        if (count[b] > 0) {
+            a.range[a.n_ranges++] = {q,  first[b],  count[b], last_open_block(c, q), c->len[q] / kva::kBlockTokens,
+                                     to, a.n_touch};
+            a.n_touch += (first[b] + count[b] - 1) / kva::kBlockTokens - first[b] / kva::kBlockTokens + 1;
+            to += count[b];
+        }
+        if (a.n_ranges == kva::kReadSeqs || (b + 1 == n_seqs && a.n_ranges > 0)) {
+            KVA_HIP(kva::launch_read_rows(a, s));
+            a.n_ranges = a.n_touch = 0;
+        }
+    }
+    return KVA_OK;
 }
 
 int kva_attn_weights(kva_cache *c, int32_t layer, const void *q, int32_t n_obs, float decay, float *weights,
@@ -1778,27 +1779,26 @@ int kva_evict(kva_cache *c, int32_t n_seqs, const int32_t *src_ids, const int32_
     int rc = flush_patches(c, s);
     if (rc) return rc;
     c->step_valid = false;
-    {
-        kva::SelectArgs a{};
-        a.weights = weights;
-        a.weights_out = weights_out;
-        a.w_stride = w_stride;
-        a.kept = kept;
-        a.kept_stride = kept_stride;
-        a.num_kv_heads = c->cfg.num_kv_heads;
-        a.first = first;
-        a.recent = recent;
-        uint8_t *h;
-        int idx;
-        if ((rc = acquire_stage(c, &h, &idx))) return rc;
-        for (int32_t b = 0; b < n_seqs; ++b) {
-            at<int32_t>(h, 0)[2 * b] = c->len[src_ids[b]];
-            at<int32_t>(h, 0)[2 * b + 1] = n_keep[b];
+    kva::SelectArgs sel{};
+    sel.weights = weights;
+    sel.weights_out = weights_out;
+    sel.w_stride = w_stride;
+    sel.kept = kept;
+    sel.kept_stride = kept_stride;
+    sel.num_kv_heads = c->cfg.num_kv_heads;
+    sel.n_seqs = n_seqs;
+    sel.first = first;
+    sel.recent = recent;
+    for (int32_t b0 = 0; b0 < n_seqs; b0 += kva::kSelectSeqs) {
+        sel.b0 = b0;
+        const int32_t n = std::min(kva::kSelectSeqs, n_seqs - b0);
+        int32_t most_rows = 0;
+        for (int32_t i = 0; i < n; ++i) {
+            sel.rows[i] = c->len[src_ids[b0 + i]];
+            sel.keep[i] = n_keep[b0 + i];
+            most_rows = std::max(most_rows, sel.rows[i]);
         }
-        KVA_HIP(hipMemcpyAsync(c->d_aux, h, 2 * sizeof(int32_t) * n_seqs, hipMemcpyHostToDevice, s));
-        if ((rc = release_stage(c, idx, s))) return rc;
-        a.seqs = reinterpret_cast<const int32_t *>(c->d_aux);
-        KVA_HIP(kva::launch_select(a, n_seqs, c->cfg.n_layers, longest, s));
+        KVA_HIP(kva::launch_select(sel, n, c->cfg.n_layers, most_rows, s));
     }
     kva::GatherArgs g{};
     g.kept = kept;
@@ -1827,17 +1827,40 @@ int kva_evict(kva_cache *c, int32_t n_seqs, const int32_t *src_ids, const int32_
         c->freed[seq] = 0;
     };
     auto run_group = [&]() -> int {
-        const int rc = upload_touches(c, recs, s, [&](const int32_t *r, int32_t n) {
-            g.recs = r;
-            return kva::launch_gather(g, n, c->cfg.num_kv_heads, c->cfg.n_layers, s);
-        });
-        recs.clear();
         for (auto &[seq, ids] : replaced) {
             release_blocks(c, seq);
             adopt(seq, ids);
         }
         replaced.clear();
-        return rc;
+        // The records and the new tables in one copy where they fit it; the
+        // tables are changed behind the launch that reads the old ones.
+        const size_t rec_bytes = recs.size() * sizeof(int32_t), patch_bytes = c->patches.size() * sizeof(int32_t);
+        const int32_t n_recs = static_cast<int32_t>(recs.size() / kva::kTouchWords);
+        if (rec_bytes + patch_bytes <= c->aux_bytes) {
+            if (patch_bytes == 0) return KVA_OK;
+            uint8_t *h;
+            int idx;
+            int rc = acquire_stage(c, &h, &idx);
+            if (rc) return rc;
+            std::memcpy(h, recs.data(), rec_bytes);
+            std::memcpy(h + rec_bytes, c->patches.data(), patch_bytes);
+            KVA_HIP(hipMemcpyAsync(c->d_aux, h, rec_bytes + patch_bytes, hipMemcpyHostToDevice, s));
+            if ((rc = release_stage(c, idx, s))) return rc;
+            g.recs = reinterpret_cast<const int32_t *>(c->d_aux);
+            KVA_HIP(kva::launch_gather(g, n_recs, c->cfg.num_kv_heads, c->cfg.n_layers, s));
+            KVA_HIP(kva::launch_table_patch(c->d_table, c->cfg.max_blocks_per_seq,
+                                            reinterpret_cast<const int32_t *>(c->d_aux + rec_bytes),
+                                            static_cast<int32_t>(c->patches.size() / 3), s));
+            recs.clear();
+            c->patches.clear();
+            return KVA_OK;
+        }
+        int rc = upload_touches(c, recs, s, [&](const int32_t *r, int32_t n) {
+            g.recs = r;
+            return kva::launch_gather(g, n, c->cfg.num_kv_heads, c->cfg.n_layers, s);
+        });
+        recs.clear();
+        return rc ? rc : flush_patches(c, s);
     };
     for (int32_t b = 0; b < n_seqs; ++b) {
         const int32_t src = src_ids[b], dst = dst_ids ? dst_ids[b] : src, n = n_keep[b];
@@ -1871,8 +1894,7 @@ int kva_evict(kva_cache *c, int32_t n_seqs, const int32_t *src_ids, const int32_
         if (behind) c->open_blocks[dst_slot] = {full, behind};
         c->open_last[dst] = dst_slot & 1;
     }
-    if ((rc = run_group())) return rc;
-    return flush_patches(c, s);
+    return run_group();
 }
 
 int kva_project_append(kva_cache *c, int32_t layer, const void *x, int32_t hidden, const void *w_q_fused,

@@ -18,11 +18,10 @@ constexpr int kCombineRecs = 64;  // sequences whose combine facts travel in the
 constexpr int kPlanPages = 64;    // page ids per sequence in the step plan (one per lane)
 constexpr int kCombineChunk = 16; // decode partials a combine wave requests together
 constexpr size_t kPageElems = kBlockTokens * kHeadDim;  // values of a block: a KV head's share of a page, K or V
-// A touch: the rows of one page that a step writes or a read wants.  int32
-// words: sequence, page of it, first row's place among the step's tokens (or
-// the output's rows), first row within the page, rows, open block (of a write:
-// the one that the page's earlier rows are in, or its rows stay in; of a read:
-// the one that holds the page, -1: none); two spare.
+// A touch: the rows of one page that a step writes.  int32 words: sequence, page
+// of it, first row's place among the step's tokens, first row within the page,
+// rows, the open block that the page's earlier rows are in or its rows stay in;
+// two spare.
 constexpr int kTouchWords = 8;
 
 // Fused QK-RMSNorm + RoPE + K/V append over all new tokens of a step.
@@ -389,10 +388,21 @@ struct Decode8Args {
     const int32_t *open_slot; // device [n_seqs]: each sequence's open block after the step
 };
 hipError_t launch_decode8(const Decode8Args &a, hipStream_t s);
-// Rows as FP16, from an FP16 cache (k8 null) or an 8-bit one.
+// Rows as FP16, from an FP16 cache (k8 null) or an 8-bit one.  What is read
+// travels in the arguments: a copy to the device in front of each read would
+// cost more than a small read itself.
+constexpr int kReadSeqs = 64;  // ranges of a launch, at most
+struct ReadRange {
+    int32_t seq, first, count;  // rows [first, first + count), count > 0
+    int32_t slot;               // the open block that holds its last page (-1: none)
+    int32_t open_page;          // and that page
+    int32_t to;                 // its first row's place among the output's
+    int32_t touch0;             // pages of earlier ranges
+};
 struct ReadRowsArgs {
-    const int32_t *touch;
-    int32_t n_touch;
+    ReadRange range[kReadSeqs];
+    int32_t n_ranges;
+    int32_t n_touch;            // pages of all ranges
     int32_t num_kv_heads;
     const int32_t *table;
     int32_t table_stride;
@@ -444,8 +454,10 @@ struct WeightArgs {
 hipError_t launch_weights(const WeightArgs &a, hipStream_t s);
 
 constexpr int kSelectLds = 32768;    // rows whose keys select_kernel holds in LDS, at most
+constexpr int kSelectSeqs = 64;      // sequences of a launch, at most (their sizes travel in its arguments)
 struct SelectArgs {
-    const int32_t *seqs;      // device [n_seqs][2]: rows, rows that stay
+    int32_t rows[kSelectSeqs], keep[kSelectSeqs];  // of sequence b0 + i: rows, rows that stay
+    int32_t b0, n_seqs;       // of the call
     const float *weights;     // [layers][n_seqs][Hkv][w_stride]
     float *weights_out;       // nullable
     int64_t w_stride;
@@ -454,8 +466,8 @@ struct SelectArgs {
     int32_t num_kv_heads;
     int32_t first, recent;
 };
-// most: rows of the longest sequence.
-hipError_t launch_select(const SelectArgs &a, int32_t n_seqs, int32_t n_layers, int32_t most, hipStream_t s);
+// n: sequences of the launch; most: rows of the longest.
+hipError_t launch_select(const SelectArgs &a, int32_t n, int32_t n_layers, int32_t most, hipStream_t s);
 
 struct GatherArgs {
     // Device [n][kTouchWords]: sequence's index in the call, destination page,
