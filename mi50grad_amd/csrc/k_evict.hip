@@ -4,14 +4,23 @@
 //
 // Weights.  For a sequence's last m = min(new tokens, n_obs) tokens and the G
 // query heads of a KV head: w[row] = decay * w[row] + sum over (token, head) of
-// softmax(q K^T / 16)[row], each token seeing rows up to its own.  Two passes
-// over K: the first leaves every query row's max and sum, the second the
-// probabilities, summed.  Query rows are (token, head) pairs, 16 to a tile, the
-// operand B of 16x16x32 products, in LDS for the whole workgroup; a wave takes a
-// page as A and multiplies it with every tile.  In the C layout a lane holds
-// one query row (column l % 16) and four keys (4 (l / 16) .. + 3), so the max and
-// sum of the first pass stay in the lane until the end, and the second pass
-// sums its tiles in the lane before the sixteen lanes of a row once per page.
+// softmax(q K^T / 16)[row], each token seeing rows up to its own.  Query rows are
+// (token, head) pairs, 16 to a tile, the operand B of 16x16x32 products, in LDS
+// for the whole workgroup; a wave takes two pages as A and multiplies them with
+// every tile, so an operand read from LDS serves two products.  In the C layout
+// a lane holds one query row (column l % 16) and four keys of each page (4 (l /
+// 16) .. + 3).  A first pass over K leaves every query row's max and sum, which
+// stay in the lane until the end; then
+//   - up to 16 query rows (a decode step), it has left the scores too (a
+//     query row's are 4 bytes to a key's 256 or 512), and the probabilities are
+//     made and summed from them (score_kernel);
+//   - more rows, the scores would outweigh the keys, and a second pass over K
+//     sums the probabilities, in the lane over its tiles, before the sixteen
+//     lanes of a row once per page (sum_kernel).
+// A workgroup takes a chunk of a sequence's pages, the same number for every
+// sequence, so a ragged batch is shared out by its pages.
+#include <type_traits>
+
 #include "k_common.h"
 #include "k_page8.h"
 #include "kva_internal.h"
@@ -20,7 +29,6 @@ namespace kva {
 namespace {
 
 constexpr float kQkScale = 1.4426950408889634f / 16.0f;
-constexpr int kWeightWaves = 4;
 
 __device__ __forceinline__ half8_t as_h8(uint4 v) { return __builtin_bit_cast(half8_t, v); }
 
@@ -46,23 +54,48 @@ __device__ __forceinline__ int query_dim(int s, int grp) {
     return kInt8 ? 64 * (s >> 1) + 16 * grp + 8 * (s & 1) : 64 * grp + 8 * s;
 }
 
-// What a workgroup works on: pages [p0, p1) of sequence b for KV head h.
+// What a workgroup works on: pages [p0, p1) of sequence b for KV head h; obs:
+// query tokens, from token `tok` of the step; slot: the open block; page0: pages
+// of earlier sequences; the sequence's chunks are [c0, c1).
 struct Span {
-    int b, h, sid, slot, ctx, obs, tok, p0, p1;  // slot: open block; obs: query tokens, from token `tok` of the step
+    int b, h, sid, slot, ctx, obs, tok, p0, p1, page0, c0, c1;
 };
 __device__ __forceinline__ Span span_of(const WeightArgs &a) {
     Span s;
-    s.b = blockIdx.z;
+    const int lane = threadIdx.x & 63, x = blockIdx.x;
+    // The sequence whose chunks hold chunk x: 64 sequences at a time.
+    int base = 0, b = 0;
+    for (int g = 0; g < a.n_seqs; g += 64) {
+        const int i = g + lane;
+        int n = i < a.n_seqs ? (a.pre_seq[i + 1] - a.pre_seq[i] + a.chunk - 1) / a.chunk : 0;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(n, o);
+            n += lane >= o ? y : 0;
+        }
+        const uint64_t before = __ballot(base + n <= x);  // sequences that end at or before it: a prefix
+        if (before != ~0ull) {
+            const int k = __popcll(before);
+            s.c0 = base + (k ? __builtin_amdgcn_readlane(n, k - 1) : 0);
+            s.c1 = base + __builtin_amdgcn_readlane(n, k);
+            b = g + k;
+            break;
+        }
+        base += __builtin_amdgcn_readlane(n, 63);
+    }
+    s.b = __builtin_amdgcn_readfirstlane(b);
+    s.c0 = __builtin_amdgcn_readfirstlane(s.c0);
+    s.c1 = __builtin_amdgcn_readfirstlane(s.c1);
     s.h = blockIdx.y;
     s.sid = ld_uniform(a.seq_ids + s.b);
     s.slot = a.k8 ? ld_uniform(a.open_slot + s.b) : 0;
     s.ctx = ld_uniform(a.ctx_lens + s.b);
+    s.page0 = ld_uniform(a.pre_seq + s.b);
     const int t0 = ld_uniform(a.tok_off + s.b), t1 = ld_uniform(a.tok_off + s.b + 1);
     s.obs = min(t1 - t0, a.n_obs);
     s.tok = t1 - s.obs;
-    const int n = (s.ctx + kBlockTokens - 1) / kBlockTokens;
-    s.p0 = floor_muldiv(blockIdx.x, n, gridDim.x);
-    s.p1 = floor_muldiv(blockIdx.x + 1, n, gridDim.x);
+    s.p0 = (x - s.c0) * a.chunk;
+    s.p1 = min(s.p0 + a.chunk, (s.ctx + kBlockTokens - 1) / kBlockTokens);
     return s;
 }
 
@@ -107,99 +140,161 @@ __device__ __forceinline__ void operands(half8_t (&op)[8], float &factor, const 
 }
 
 // The span's query rows to LDS as B operands: [tile][k-step][lane] of 16 bytes,
-// zeros past the last row.
-template <bool kInt8>
-__device__ __forceinline__ void load_queries(uint4 *qs, const WeightArgs &a, const Span &s, int tiles) {
+// zeros past the last row.  Requested together: a workgroup starts with them.
+template <bool kInt8, int NT, int WAVES>
+__device__ __forceinline__ void load_queries(uint4 *qs, const WeightArgs &a, const Span &s) {
+    constexpr int kEach = NT * 512 / (64 * WAVES);
     const int G = a.num_heads / a.num_kv_heads;
-    for (int i = threadIdx.x; i < tiles * 512; i += blockDim.x) {
+    uint4 x[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const int i = threadIdx.x + 64 * WAVES * e;
         const int lane = i & 63, step = (i >> 6) & 7, row = 16 * (i >> 9) + (lane & 15);
         const int iq = row / G;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (iq < s.obs)
-            x = ld16(a.q + (static_cast<size_t>(s.tok + iq) * a.num_heads + s.h * G + row - iq * G) * kHeadDim +
-                     query_dim<kInt8>(step, lane >> 4));
-        qs[i] = x;
+        x[e] = iq < s.obs ? ld16(a.q + (static_cast<size_t>(s.tok + iq) * a.num_heads + s.h * G + row - iq * G) * kHeadDim +
+                                 query_dim<kInt8>(step, lane >> 4))
+                          : make_uint4(0, 0, 0, 0);
     }
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) qs[threadIdx.x + 64 * WAVES * e] = x[e];
 }
 
-// Walks the span's pages, this wave's in turn: scores(t, x) gets tile t's in
-// log2 units, -inf where the row does not see the key; done(page) ends a page.
-template <bool kInt8, int NT, class Scores, class Done>
-__device__ __forceinline__ void walk(const WeightArgs &a, const Span &s, const uint4 *qs, int tiles, Scores scores,
-                                     Done done) {
+// The page ids of a walk, 64 to a vector load, one per lane: as scalar loads
+// they would make every wait for LDS a wait for them.  Places only go up.
+struct PageIds {
+    const int32_t *row;
+    int base, ids;
+    __device__ __forceinline__ void load(int from, int last, int lane) {
+        base = from;
+        ids = row[min(from + lane, last)];
+    }
+    __device__ __forceinline__ int at(int page, int last, int lane) {
+        if (page - base >= 64) load(page, last, lane);  // wave-uniform
+        return __builtin_amdgcn_readlane(ids, page - base);
+    }
+};
+
+// Pages that a wave takes at a time: two share the operands read from LDS; with
+// one tile of query rows there is little to share, and more waves fit.
+constexpr int pages_for(int tiles) { return tiles == 1 ? 1 : 2; }
+
+// Walks the span's pages, PG at a time, this wave's in turn: scores(t, x) gets
+// tile t's of them in log2 units, -inf where the row does not see the key (or
+// there is no such page); done(page) ends them.
+template <bool kInt8, int NT, int WAVES, class Scores, class Done>
+__device__ __forceinline__ void walk(const WeightArgs &a, const Span &s, const uint4 *qs, Scores scores, Done done) {
+    constexpr int PG = pages_for(NT);
     const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int G = a.num_heads / a.num_kv_heads;
-    const int32_t *row = a.table + static_cast<size_t>(s.sid) * a.table_stride;
     const int last = s.p1 - 1;
-    int p = s.p0 + wave;
+    int p = s.p0 + PG * wave;
     if (p > last) return;
-    // The last key that this lane's query row of each tile sees.
-    int see[NT];
+    PageIds ids{a.table + static_cast<size_t>(s.sid) * a.table_stride, 0, 0};
+    ids.load(p, last, lane);
+    Keys<kInt8> cur[PG], nxt[PG];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int iq = (16 * t + col) / G;
-        see[t] = iq < s.obs ? s.ctx - s.obs + iq : -1;
-    }
-    Keys<kInt8> cur, nxt;
-    load_keys(cur, a, s, p, ld_uniform(row + p), lane);
-    int id = ld_uniform(row + min(p + kWeightWaves, last));
-    for (; p <= last; p += kWeightWaves) {
-        load_keys(nxt, a, s, min(p + kWeightWaves, last), id, lane);
-        id = ld_uniform(row + min(p + 2 * kWeightWaves, last));
-        half8_t op[8];
-        float factor;
-        operands<kInt8>(op, factor, cur, a, s, p, lane);
-        const bool whole = 16 * p + 15 <= s.ctx - s.obs;  // every query row sees every key
+    for (int j = 0; j < PG; ++j) load_keys(cur[j], a, s, min(p + j, last), ids.at(min(p + j, last), last, lane), lane);
+    for (; p <= last; p += PG * WAVES) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            if (t >= tiles) continue;  // uniform
-            float4_t x = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                x = __builtin_amdgcn_mfma_f32_16x16x32_f16(op[k], as_h8(qs[(t * 8 + k) * 64 + lane]), x, 0, 0, 0);
-            x *= factor;
-            if (!whole || 16 * t + 15 >= s.obs * G) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = 16 * p + 4 * grp + i <= see[t] ? x[i] : -INFINITY;
-            }
-            scores(t, x);
+        for (int j = 0; j < PG; ++j) {
+            const int q = min(p + PG * WAVES + j, last);
+            load_keys(nxt[j], a, s, q, ids.at(q, last, lane), lane);
         }
+        __builtin_amdgcn_sched_barrier(0);
+        half8_t op[PG][8];
+        float factor[PG];
+#pragma unroll
+        for (int j = 0; j < PG; ++j) operands<kInt8>(op[j], factor[j], cur[j], a, s, min(p + j, last), lane);
+        auto tiles = [&](auto masked) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float4_t x[PG];
+#pragma unroll
+                for (int j = 0; j < PG; ++j) x[j] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const half8_t b = as_h8(qs[(t * 8 + k) * 64 + lane]);
+#pragma unroll
+                    for (int j = 0; j < PG; ++j) x[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(op[j][k], b, x[j], 0, 0, 0);
+                }
+#pragma unroll
+                for (int j = 0; j < PG; ++j) {
+                    x[j] *= factor[j];
+                    if constexpr (masked) {
+                        // The last key that the lane's query row sees (none: no such row).
+                        const int iq = (16 * t + col) / G;
+                        const int see = iq < s.obs && p + j <= last ? s.ctx - s.obs + iq : -1;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) x[j][i] = 16 * (p + j) + 4 * grp + i <= see ? x[j][i] : -INFINITY;
+                    }
+                }
+                scores(t, x);
+                // Two tiles' reads and products overlap; more would only cost registers.
+                if (t & 1) __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        // Every query row sees every key of the pages (rows that there are not
+        // have zeros for q; nothing of them is written, or they weigh nothing).
+        if (p + PG - 1 <= last && 16 * (p + PG) - 1 <= s.ctx - s.obs)
+            tiles(std::false_type{});
+        else
+            tiles(std::true_type{});
         done(p);
-        cur = nxt;
+#pragma unroll
+        for (int j = 0; j < PG; ++j) cur[j] = nxt[j];
     }
 }
 
-// (m, l) of every query row over the span's pages: part[b][h][split][row].
-template <bool kInt8, int NT>
-__global__ __launch_bounds__(64 * kWeightWaves) void stats_kernel(WeightArgs a) {
+__device__ __forceinline__ float exp_sum(const float4_t &x, float mu) {
+    return (__builtin_amdgcn_exp2f(x[0] - mu) + __builtin_amdgcn_exp2f(x[1] - mu)) +
+           (__builtin_amdgcn_exp2f(x[2] - mu) + __builtin_amdgcn_exp2f(x[3] - mu));
+}
+__device__ __forceinline__ float max4(const float4_t &x) { return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])); }
+
+// (m, l) of every query row over the chunk: part[chunk][h][row].  kScores: and
+// the scores, scores[page of the step][h][row][16 keys] (one tile).
+template <bool kInt8, int NT, int WAVES, bool kScores>
+__global__ __launch_bounds__(64 * WAVES) void stats_kernel(WeightArgs a) {
+    static_assert(!kScores || NT == 1, "one tile of scores");
     __shared__ uint4 qs[NT * 512];
-    __shared__ float2 wave_ml[kWeightWaves][NT * 16];
+    __shared__ float2 wave_ml[WAVES][NT * 16];
     const Span s = span_of(a);
     if (s.obs == 0) return;
-    const int rows = s.obs * (a.num_heads / a.num_kv_heads), tiles = (rows + 15) / 16;
-    load_queries<kInt8>(qs, a, s, tiles);
+    const int rows = s.obs * (a.num_heads / a.num_kv_heads);
+    load_queries<kInt8, NT, WAVES>(qs, a, s);
     __syncthreads();
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float m[NT], l[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         m[t] = -INFINITY;
         l[t] = 0.0f;
     }
-    walk<kInt8, NT>(
-        a, s, qs, tiles,
-        [&](int t, const float4_t &x) {
-            const float mn = fmaxf(m[t], fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+    constexpr int PG = pages_for(NT);
+    float4_t kept = float4_t{0.f, 0.f, 0.f, 0.f};
+    walk<kInt8, NT, WAVES>(
+        a, s, qs,
+        [&](int t, const float4_t (&x)[PG]) {
+            float mn = m[t], sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < PG; ++j) mn = fmaxf(mn, max4(x[j]));
             const float mu = mn == -INFINITY ? 0.0f : mn;
-            l[t] = l[t] * __builtin_amdgcn_exp2f(m[t] - mu) + (__builtin_amdgcn_exp2f(x[0] - mu) + __builtin_amdgcn_exp2f(x[1] - mu)) +
-                   (__builtin_amdgcn_exp2f(x[2] - mu) + __builtin_amdgcn_exp2f(x[3] - mu));
+#pragma unroll
+            for (int j = 0; j < PG; ++j) sum += exp_sum(x[j], mu);
+            l[t] = l[t] * __builtin_amdgcn_exp2f(m[t] - mu) + sum;
             m[t] = mn;
+            if constexpr (kScores) kept = x[0];
         },
-        [](int) {});
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        [&](int page) {
+            if constexpr (kScores) {
+                const int col = lane & 15, grp = lane >> 4;
+                const size_t at = (static_cast<size_t>(s.page0 + page) * a.num_kv_heads + s.h) * a.part_rows;
+                if (col < rows) *reinterpret_cast<float4_t *>(a.scores + (at + col) * kBlockTokens + 4 * grp) = kept;
+            }
+        });
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        if (t >= tiles) continue;
         const float mx = group4_max(m[t]);
         const float mu = mx == -INFINITY ? 0.0f : mx;
         const float lt = group4_sum(l[t] * __builtin_amdgcn_exp2f(m[t] - mu));
@@ -209,66 +304,125 @@ __global__ __launch_bounds__(64 * kWeightWaves) void stats_kernel(WeightArgs a) 
     for (int r = threadIdx.x; r < rows; r += blockDim.x) {
         float mx = -INFINITY, lt = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWeightWaves; ++w) mx = fmaxf(mx, wave_ml[w][r].x);
+        for (int w = 0; w < WAVES; ++w) mx = fmaxf(mx, wave_ml[w][r].x);
         const float mu = mx == -INFINITY ? 0.0f : mx;
 #pragma unroll
-        for (int w = 0; w < kWeightWaves; ++w) lt += wave_ml[w][r].y * __builtin_amdgcn_exp2f(wave_ml[w][r].x - mu);
-        a.part[((static_cast<size_t>(s.b) * a.num_kv_heads + s.h) * gridDim.x + blockIdx.x) * a.part_rows + r] =
-            make_float2(mx, lt);
+        for (int w = 0; w < WAVES; ++w) lt += wave_ml[w][r].y * __builtin_amdgcn_exp2f(wave_ml[w][r].x - mu);
+        a.part[(static_cast<size_t>(blockIdx.x) * a.num_kv_heads + s.h) * a.part_rows + r] = make_float2(mx, lt);
     }
 }
 
-// The probabilities of the span's rows, summed over the query rows, onto the
-// decayed weights.
-template <bool kInt8, int NT>
-__global__ __launch_bounds__(64 * kWeightWaves) void sum_kernel(WeightArgs a) {
+// A query row's max and 1 / sum over the sequence's chunks, by 16 lanes of a
+// DPP row: row r of rows rows by the lanes that hold r, every lane gets them.
+// Rows that there are not weigh nothing.  `first` is the lane's first partial,
+// requested before (a workgroup starts with these).
+__device__ __forceinline__ float2 first_part(const WeightArgs &a, const Span &s, int r, int rows, int l16) {
+    if (r >= rows || l16 >= s.c1 - s.c0) return make_float2(-INFINITY, 0.0f);
+    return a.part[(static_cast<size_t>(s.c0 + l16) * a.num_kv_heads + s.h) * a.part_rows + r];
+}
+__device__ __forceinline__ float2 row_stat(const WeightArgs &a, const Span &s, float2 first, int r, int rows, int l16) {
+    float mx = first.x, lt = first.y;
+    if (r < rows)
+        for (int i = s.c0 + l16 + 16; i < s.c1; i += 16) {
+            const float2 p = a.part[(static_cast<size_t>(i) * a.num_kv_heads + s.h) * a.part_rows + r];
+            const float mn = fmaxf(mx, p.x);
+            const float mu = mn == -INFINITY ? 0.0f : mn;
+            lt = lt * __builtin_amdgcn_exp2f(mx - mu) + p.y * __builtin_amdgcn_exp2f(p.x - mu);
+            mx = mn;
+        }
+    float all = mx;
+#pragma unroll
+    for (int o = 8; o >= 1; o >>= 1) all = fmaxf(all, __shfl_xor(all, o));
+    const float mu = all == -INFINITY ? 0.0f : all;
+    lt = row16_sum(lt * __builtin_amdgcn_exp2f(mx - mu));
+    return r < rows ? make_float2(mu, 1.0f / lt) : make_float2(0.0f, 0.0f);
+}
+
+__device__ __forceinline__ void put_weight(const WeightArgs &a, const Span &s, int key, float x) {
+    float *w = a.weights + (static_cast<size_t>(s.b) * a.num_kv_heads + s.h) * a.w_stride + key;
+    *w = a.decay == 0.0f ? x : fmaf(a.decay, *w, x);
+}
+
+// The probabilities of the chunk's rows, summed over the query rows, onto the
+// decayed weights: from K.
+template <bool kInt8, int NT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void sum_kernel(WeightArgs a) {
     __shared__ uint4 qs[NT * 512];
     __shared__ float2 stat[NT * 16];
     const Span s = span_of(a);
-    const int rows = s.obs * (a.num_heads / a.num_kv_heads), tiles = (rows + 15) / 16;
-    load_queries<kInt8>(qs, a, s, tiles);
-    for (int r = threadIdx.x; r < NT * 16; r += blockDim.x) {
-        float mx = -INFINITY, lt = 0.0f;
-        if (r < rows) {
-            const float2 *part = a.part + (static_cast<size_t>(s.b) * a.num_kv_heads + s.h) * gridDim.x * a.part_rows + r;
-            for (int i = 0; i < static_cast<int>(gridDim.x); ++i) mx = fmaxf(mx, part[static_cast<size_t>(i) * a.part_rows].x);
-            const float mu = mx == -INFINITY ? 0.0f : mx;
-            for (int i = 0; i < static_cast<int>(gridDim.x); ++i) {
-                const float2 p = part[static_cast<size_t>(i) * a.part_rows];
-                lt += p.y * __builtin_amdgcn_exp2f(p.x - mu);
-            }
-        }
-        stat[r] = make_float2(mx, 1.0f / lt);
+    const int rows = s.obs * (a.num_heads / a.num_kv_heads);
+    if (s.obs == 0) {  // decayed only
+        for (int key = 16 * s.p0 + threadIdx.x; key < min(16 * s.p1, s.ctx); key += blockDim.x) put_weight(a, s, key, 0.0f);
+        return;
+    }
+    constexpr int kEach = NT * 256 / (64 * WAVES);
+    float2 first[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) first[e] = first_part(a, s, 4 * WAVES * e + (threadIdx.x >> 4), rows, threadIdx.x & 15);
+    load_queries<kInt8, NT, WAVES>(qs, a, s);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const int r = 4 * WAVES * e + (threadIdx.x >> 4);
+        const float2 x = row_stat(a, s, first[e], r, rows, threadIdx.x & 15);
+        if ((threadIdx.x & 15) == 0) stat[r] = x;
     }
     __syncthreads();
     const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
-    float m[NT], inv[NT];
+    constexpr int PG = pages_for(NT);
+    float4_t sum[PG] = {};
+    walk<kInt8, NT, WAVES>(
+        a, s, qs,
+        [&](int t, const float4_t (&x)[PG]) {
+            const float2 st = stat[16 * t + col];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const float2 x = stat[16 * t + col];
-        m[t] = x.x == -INFINITY ? 0.0f : x.x;
-        inv[t] = x.y;
-    }
-    float *w = a.weights + (static_cast<size_t>(s.b) * a.num_kv_heads + s.h) * a.w_stride;
-    float4_t sum = float4_t{0.f, 0.f, 0.f, 0.f};
-    walk<kInt8, NT>(
-        a, s, qs, tiles,
-        [&](int t, const float4_t &x) {
+            for (int j = 0; j < PG; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                sum[i] += x[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[i] - m[t]) * inv[t];
+                for (int i = 0; i < 4; ++i)
+                    // A row that does not see the key adds nothing, whatever its sum is.
+                    sum[j][i] += x[j][i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[j][i] - st.x) * st.y;
         },
         [&](int page) {
-            float mine = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float all = row16_sum(sum[i]);
-                mine = col == i ? all : mine;
+            for (int j = 0; j < PG; ++j) {
+                float mine = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float all = row16_sum(sum[j][i]);
+                    mine = col == i ? all : mine;
+                }
+                sum[j] = float4_t{0.f, 0.f, 0.f, 0.f};
+                const int key = 16 * (page + j) + 4 * grp + col;
+                if (col < 4 && page + j < s.p1 && key < s.ctx) put_weight(a, s, key, mine);
             }
-            sum = float4_t{0.f, 0.f, 0.f, 0.f};
-            const int key = 16 * page + 4 * grp + col;
-            if (col < 4 && key < s.ctx) w[key] = a.decay == 0.0f ? mine : fmaf(a.decay, w[key], mine);
         });
+}
+
+// The same from the scores that stats_kernel left: a thread per key.
+__global__ __launch_bounds__(256) void score_kernel(WeightArgs a) {
+    __shared__ float2 stat[16];
+    const Span s = span_of(a);
+    const int rows = s.obs * (a.num_heads / a.num_kv_heads);
+    constexpr int kAhead = 8;  // scores requested together
+    const int r0 = threadIdx.x >> 4, l16 = threadIdx.x & 15;
+    const float2 mine = row_stat(a, s, first_part(a, s, r0, rows, l16), r0, rows, l16);
+    if (l16 == 0) stat[r0] = mine;
+    __syncthreads();
+    const int end = min(16 * s.p1, s.ctx);
+    for (int key = 16 * s.p0 + threadIdx.x; key < end; key += blockDim.x) {
+        const float *x = a.scores +
+                         (static_cast<size_t>(s.page0 + (key >> 4)) * a.num_kv_heads + s.h) * a.part_rows * kBlockTokens +
+                         (key & 15);
+        float sum = 0.0f;
+        for (int r = 0; r < rows; r += kAhead) {
+            float v[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) v[i] = r + i < rows ? x[(r + i) * kBlockTokens] : -INFINITY;
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+                sum += v[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(v[i] - stat[r + i].x) * stat[r + i].y;
+        }
+        put_weight(a, s, key, sum);
+    }
 }
 
 // ---- which rows stay ---------------------------------------------------------
@@ -460,22 +614,32 @@ __global__ __launch_bounds__(32 * kBlockTokens) void gather_kernel(GatherArgs a)
     }
 }
 
-template <bool kInt8, int NT>
+template <bool kInt8, int NT, int WAVES>
 hipError_t launch_weights_tiles(const WeightArgs &a, hipStream_t s) {
-    const dim3 grid(a.splits, a.num_kv_heads, a.n_seqs), block(64 * kWeightWaves);
-    hipLaunchKernelGGL((stats_kernel<kInt8, NT>), grid, block, 0, s, a);
-    hipLaunchKernelGGL((sum_kernel<kInt8, NT>), grid, block, 0, s, a);
+    const dim3 grid(a.n_chunks, a.num_kv_heads), block(64 * WAVES);
+    if constexpr (NT == 1) {
+        if (a.scores) {
+            hipLaunchKernelGGL((stats_kernel<kInt8, 1, WAVES, true>), grid, block, 0, s, a);
+            hipLaunchKernelGGL(score_kernel, grid, dim3(256), 0, s, a);
+            return hipGetLastError();
+        }
+    }
+    hipLaunchKernelGGL((stats_kernel<kInt8, NT, WAVES, false>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((sum_kernel<kInt8, NT, WAVES>), grid, block, 0, s, a);
     return hipGetLastError();
 }
 
 template <bool kInt8>
 hipError_t launch_weights_kind(const WeightArgs &a, hipStream_t s) {
-    const int tiles = (a.n_obs * (a.num_heads / a.num_kv_heads) + 15) / 16;
-    if (tiles <= 1) return launch_weights_tiles<kInt8, 1>(a, s);
-    if (tiles <= 4) return launch_weights_tiles<kInt8, 4>(a, s);
-    if (tiles <= 8) return launch_weights_tiles<kInt8, 8>(a, s);
-    if (tiles <= 16) return launch_weights_tiles<kInt8, 16>(a, s);
-    return hipErrorInvalidValue;
+    switch (weight_tiles(a.part_rows)) {
+        case 1: return launch_weights_tiles<kInt8, 1, 4>(a, s);
+        case 2: return launch_weights_tiles<kInt8, 2, 4>(a, s);
+        case 4: return launch_weights_tiles<kInt8, 4, 4>(a, s);
+        case 8: return launch_weights_tiles<kInt8, 8, 8>(a, s);
+        case 12: return launch_weights_tiles<kInt8, 12, 8>(a, s);
+        case 16: return launch_weights_tiles<kInt8, 16, 8>(a, s);
+        default: return hipErrorInvalidValue;
+    }
 }
 
 }  // namespace

@@ -1677,18 +1677,30 @@ int kva_attn_weights(kva_cache *c, int32_t layer, const void *q, int32_t n_obs, 
     kva::WeightArgs a{};
     a.n_obs = std::min(n_obs, std::max(1, c->st_max_new));
     a.part_rows = a.n_obs * group;
-    // Workgroups of four waves: as many as the chip holds of them, by the LDS
-    // that their query rows take, some more where a batch is ragged, and four
-    // pages each at least.
-    const int32_t tiles = (a.part_rows + 15) / 16;
-    const int64_t target = static_cast<int64_t>(c->n_cu) * (tiles <= 1 ? 8 : tiles <= 4 ? 4 : tiles <= 8 ? 2 : 1);
-    const int64_t units = static_cast<int64_t>(c->st_n_seqs) * c->cfg.num_kv_heads;
-    const int64_t pages = (c->st_max_ctx + kva::kBlockTokens - 1) / kva::kBlockTokens;
-    const int64_t fit = static_cast<int64_t>(c->mq_floats) / (2 * units * a.part_rows);
-    if (fit < 1)
+    // Chunks of pages: as many as the chip holds workgroups at once, a page
+    // per wave at least.  A sequence's last chunk may be short, so a chunk size
+    // that gives one round by the sum of pages is raised until the chunks do.
+    const int32_t tiles = kva::weight_tiles(a.part_rows);
+    const int64_t hkv = c->cfg.num_kv_heads;
+    const int64_t target = std::max<int64_t>(1, c->n_cu * kva::weight_wgs_per_cu(tiles) / hkv);
+    auto chunks_of = [&](int64_t chunk) {
+        int64_t n = 0;
+        for (int32_t b = 0; b < c->st_n_seqs; ++b) n += (c->st_pre[b + 1] - c->st_pre[b] + chunk - 1) / chunk;
+        return n;
+    };
+    const int64_t pages = c->st_total_pages;
+    int64_t chunk = std::max<int64_t>(4, (pages + target - 1) / target);
+    while (chunks_of(chunk) > target && chunk < pages) chunk += std::max<int64_t>(1, chunk / 16);
+    const int64_t n_chunks = chunks_of(chunk);
+    const int64_t part_floats = 2 * n_chunks * hkv * a.part_rows;
+    if (part_floats > static_cast<int64_t>(c->mq_floats))
         return fail(KVA_ERR_CAPACITY, "%d sequences of %d query rows exceed the workspace", c->st_n_seqs, a.part_rows);
-    a.splits = static_cast<int32_t>(std::max<int64_t>(
-        1, std::min<int64_t>({(target + units - 1) / units, (pages + 3) / 4, fit, int64_t{256}})));
+    // The scores behind the partials (16-byte aligned), where one tile's fit.
+    const int64_t scores_at = (part_floats + 3) / 4 * 4;
+    const bool scores =
+        tiles == 1 && scores_at + pages * hkv * a.part_rows * kva::kBlockTokens <= static_cast<int64_t>(c->mq_floats);
+    a.chunk = static_cast<int32_t>(chunk);
+    a.n_chunks = static_cast<int32_t>(n_chunks);
     if ((rc = require_device(c))) return rc;
     a.q = static_cast<const uint16_t *>(q);
     a.seq_ids = at<int32_t>(c->d_step, c->off_seq);
@@ -1705,7 +1717,9 @@ int kva_attn_weights(kva_cache *c, int32_t layer, const void *q, int32_t n_obs, 
     a.n_seqs = c->st_n_seqs;
     a.num_heads = c->cfg.num_heads;
     a.num_kv_heads = c->cfg.num_kv_heads;
+    a.pre_seq = at<int32_t>(c->d_step, c->off_pre);
     a.part = reinterpret_cast<float2 *>(c->d_mq_acc);
+    a.scores = scores ? c->d_mq_acc + scores_at : nullptr;
     a.decay = decay;
     a.weights = weights;
     a.w_stride = w_stride;

@@ -428,12 +428,19 @@ hipError_t launch_reopen(const ReopenArgs &a, int32_t n, int32_t num_kv_heads, i
 // ---- eviction (k_evict.hip) ----
 
 constexpr int kMaxObserved = 32;     // query tokens per sequence that kva_attn_weights looks at, at most
-constexpr int kMaxWeightRows = 256;  // query rows (tokens x heads of a group), at most: 16 tiles
+// Tiles of 16 query rows (tokens x heads of a group) that a kernel is built for.
+constexpr int weight_tiles(int rows) {
+    const int t = (rows + 15) / 16;
+    return t <= 2 ? t : t <= 4 ? 4 : t <= 8 ? 8 : t <= 12 ? 12 : 16;
+}
+// Workgroups of it that a CU holds: by LDS (8 KB a tile) and registers.
+constexpr int weight_wgs_per_cu(int tiles) { return tiles <= 1 ? 4 : tiles <= 2 ? 3 : tiles <= 4 ? 2 : 1; }
 struct WeightArgs {
     const uint16_t *q;        // [T][H][256]
     const int32_t *seq_ids;   // device, as in MultiQueryArgs
     const int32_t *ctx_lens;
     const int32_t *tok_off;
+    const int32_t *pre_seq;   // device [n_seqs + 1]: pages of earlier sequences
     const int32_t *table;
     int32_t table_stride;
     const uint16_t *k_pool;   // FP16 cache
@@ -444,9 +451,11 @@ struct WeightArgs {
     const int32_t *open_slot; // device [n_seqs] (8-bit cache)
     int32_t n_seqs, num_heads, num_kv_heads;
     int32_t n_obs;
-    int32_t splits;           // workgroups that share a sequence's pages
+    int32_t chunk;            // pages of a workgroup
+    int32_t n_chunks;         // of all sequences
     int32_t part_rows;        // query rows at most
-    float2 *part;             // [n_seqs][Hkv][splits][part_rows]: max (log2 units), sum
+    float2 *part;             // [n_chunks][Hkv][part_rows]: max (log2 units), sum
+    float *scores;            // [pages][Hkv][part_rows][16], or null: K is read again
     float decay;
     float *weights;           // [n_seqs][Hkv][w_stride]
     int64_t w_stride;
