@@ -150,6 +150,137 @@ __device__ __forceinline__ void issue_block(uint32_t slot, const uint8_t *k, con
     touch_line(rs, slot + 2 * kPageElems, 4 * (lane & 1), 0);
 }
 
+// The step's sequences as the walk reads them.
+struct StepRefs {
+    const int32_t *pre_seq, *ctx_lens, *seq_ids, *open_slot, *table;
+    int32_t table_stride, n_seqs;
+};
+
+// A sequence's pages in a share: [p0, p1) of its npg, those before `full` not
+// open.
+struct Segment {
+    int b, p0, p1, npg, ctx, full, base, slot;
+    const int32_t *row;
+};
+
+// A share [p_begin, p_end) of the step's pages, its sequences b0 .. b_last.  What
+// is known of 64 sequences lies in the lanes of four registers, loaded
+// together, so a walk of few sequences waits for memory once for all of it.
+struct Share {
+    StepRefs r;
+    int p_begin, p_end, b0, b_last;
+    int win;                   // the lanes' first sequence
+    int ctx, pre, sid, slot;   // lane l: of sequence win + l
+
+    __device__ __forceinline__ void window(int b, int lane) {
+        win = b;
+        const int i = min(b + lane, r.n_seqs - 1);
+        ctx = r.ctx_lens[i];
+        pre = r.pre_seq[i];
+        sid = r.seq_ids[i];
+        slot = r.open_slot[i];
+        // Taken in here, so that no later use waits for loads in flight.
+        asm volatile("" : "+v"(ctx), "+v"(pre), "+v"(sid), "+v"(slot));
+    }
+    // False: the share is empty.
+    __device__ __forceinline__ bool begin(const StepRefs &refs, int w, int P, int W, int lane) {
+        r = refs;
+        p_begin = wg_start(w, P, W);
+        p_end = wg_start(w + 1, P, W);
+        if (p_begin >= p_end) return false;
+        // The last sequence that begins at or before the share, and the last
+        // before its end: 64 at a time (empty ones share their beginning with the next).
+        b0 = 0;
+        for (int g = 0; g < r.n_seqs; g += 64) {
+            window(g, lane);
+            const uint64_t there = r.n_seqs - g >= 64 ? ~0ull : (1ull << (r.n_seqs - g)) - 1;
+            const int n = __popcll(__ballot(pre <= p_begin) & there);
+            if (n > 0) b0 = g + n - 1;
+            if (n < 64) break;
+        }
+        if (b0 < win) window(b0, lane);
+        b_last = b0 = __builtin_amdgcn_readfirstlane(b0);
+        const uint64_t there = r.n_seqs - win >= 64 ? ~0ull : (1ull << (r.n_seqs - win)) - 1;
+        b_last = __builtin_amdgcn_readfirstlane(win + __popcll(__ballot(pre < p_end) & there) - 1);
+        while (b_last + 1 < r.n_seqs && b_last == win + 63 && ld_uniform(r.pre_seq + b_last + 1) < p_end) {
+            window(b_last + 1, lane);
+            const uint64_t more = r.n_seqs - win >= 64 ? ~0ull : (1ull << (r.n_seqs - win)) - 1;
+            b_last = __builtin_amdgcn_readfirstlane(win + __popcll(__ballot(pre < p_end) & more) - 1);
+        }
+        if (b0 < win) window(b0, lane);
+        return true;
+    }
+    __device__ __forceinline__ Segment at(int b) const {
+        Segment g;
+        g.b = b;
+        int s;
+        if (b - win < 64) {
+            g.ctx = __builtin_amdgcn_readlane(ctx, b - win);
+            g.base = __builtin_amdgcn_readlane(pre, b - win);
+            g.slot = __builtin_amdgcn_readlane(slot, b - win);
+            s = __builtin_amdgcn_readlane(sid, b - win);
+        } else {
+            g.ctx = ld_uniform(r.ctx_lens + b);
+            g.base = ld_uniform(r.pre_seq + b);
+            g.slot = ld_uniform(r.open_slot + b);
+            s = ld_uniform(r.seq_ids + b);
+        }
+        g.row = r.table + static_cast<size_t>(s) * r.table_stride;
+        g.npg = (g.ctx + kBlockTokens - 1) / kBlockTokens;
+        g.p0 = max(0, p_begin - g.base);
+        g.p1 = min(g.npg, p_end - g.base);
+        g.full = min(g.p1, g.ctx / kBlockTokens);
+        return g;
+    }
+};
+
+// The issue side of the walk: the share's full pages in order, across
+// sequences.  `id` is the next one's, fetched a page ahead by a scalar load,
+// the first 64 by one vector load together.
+struct PageFeed {
+    Segment g;
+    int ip, id, first, n_first;  // n_first pages from `first` of the first sequence are in ids
+    int ids;
+    bool on;
+
+    __device__ __forceinline__ void settle(const Share &sh) {  // to the next page, if there is one
+        while (ip >= g.full) {
+            if (g.b >= sh.b_last) {
+                on = false;
+                return;
+            }
+            g = sh.at(g.b + 1);
+            ip = g.p0;
+            n_first = 0;
+        }
+    }
+    // Requests the first ids; take() before fetch().
+    __device__ __forceinline__ void begin(const Share &sh, int lane) {
+        g = sh.at(sh.b0);
+        ip = g.p0;
+        on = true;
+        id = 0;
+        n_first = 64;
+        settle(sh);
+        n_first = on ? 64 : 0;
+        first = ip;
+        ids = on ? g.row[min(ip + lane, g.npg - 1)] : 0;
+    }
+    __device__ __forceinline__ void take() { asm volatile("" : "+v"(ids)); }
+    __device__ __forceinline__ void fetch() {
+        if (!on) return;
+        if (ip - first < n_first)
+            id = __builtin_amdgcn_readlane(ids, ip - first);
+        else
+            id = ld_uniform(g.row + ip);
+    }
+    __device__ __forceinline__ void next(const Share &sh) {
+        if (!on) return;
+        ++ip;
+        settle(sh);
+    }
+};
+
 // Held to 256 registers: with 512 the compiler keeps the accumulators in the
 // other half and moves all 64 over at every block.
 __global__ __launch_bounds__(64 * kDecodeHeadsPerWg, 2) void decode8_kernel(Decode8Args e) {
@@ -159,9 +290,6 @@ __global__ __launch_bounds__(64 * kDecodeHeadsPerWg, 2) void decode8_kernel(Deco
     int P, W;
     stream_k_shape(a, P, W);
     if (w >= W) return;
-    const int p_begin = wg_start(w, P, W);
-    const int p_end = wg_start(w + 1, P, W);
-    if (p_begin >= p_end) return;
     const int hkv = a.num_kv_heads, nh = a.num_heads, G = nh / hkv;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = __builtin_amdgcn_readfirstlane(blockIdx.y * (blockDim.x >> 6) + wave);
@@ -169,84 +297,48 @@ __global__ __launch_bounds__(64 * kDecodeHeadsPerWg, 2) void decode8_kernel(Deco
     const int col = lane & 15, grp = lane >> 4;
     uint8_t *mine = ring + static_cast<size_t>(wave) * kRing * kSlotBytes;
 
-    // The first sequence of the share: the last with pages before it <= p_begin.
-    int b0 = 0;
-    for (int c0 = 0; c0 < a.n_seqs; c0 += 64) {
-        const int i = c0 + lane;
-        const uint64_t before = __ballot((i < a.n_seqs ? a.pre_seq[i + 1] : INT32_MAX) <= p_begin);
-        b0 += __popcll(before);
-        if (before != ~0ull) break;
-    }
-    b0 = __builtin_amdgcn_readfirstlane(b0);
-    // A sequence's pages in the share: [p0, p1) of its npg, the full ones before
-    // `full`; only its last page can be open.  (Every field is wave-uniform.)
-    struct Segment {
-        int b, p0, p1, npg, ctx, full;
-        const int32_t *row;
-    };
-    auto segment = [&](int b) -> Segment {
-        Segment g;
-        g.b = b;
-        g.ctx = ld_uniform(a.ctx_lens + b);
-        const int base = ld_uniform(a.pre_seq + b);
-        g.row = a.table + static_cast<size_t>(ld_uniform(a.seq_ids + b)) * a.table_stride;
-        g.npg = (g.ctx + kBlockTokens - 1) / kBlockTokens;
-        g.p0 = max(0, p_begin - base);
-        g.p1 = min(g.npg, p_end - base);
-        g.full = min(g.p1, g.ctx / kBlockTokens);
-        return g;
-    };
-    // The issue side, kRing - 1 full pages ahead of the products across
-    // sequences: page ip of segment ig next, whose id is `id`; past the share the
-    // same loads go through empty resources, so the load counter advances alike.
-    const int b_last = [&] {  // the sequence of the share's last page
-        int b = b0;
-        while (ld_uniform(a.pre_seq + b + 1) < p_end) ++b;
-        return b;
-    }();
-    Segment ig = segment(b0);
-    int ip = ig.p0, id = 0;
-    bool on = true;
-    auto settle = [&]() {  // to the next full page of the share, if there is one
-        while (ip >= ig.full) {
-            if (ig.b >= b_last) {
-                on = false;
-                return;
-            }
-            ig = segment(ig.b + 1);
-            ip = ig.p0;
-        }
-    };
-    auto fetch = [&]() {
-        if (on) id = ld_uniform(ig.row + ip);
-    };
-    auto issue = [&](int slot) {
-        const size_t blk = static_cast<size_t>(id) * hkv + h;
-        issue_block(__builtin_amdgcn_readfirstlane(lds_addr(mine + slot * kSlotBytes)), e.k8 + blk * kPageElems, e.v8 + blk * kPageElems,
-                    e.scales + 2 * blk, on, lane);
-        if (on) {
-            ++ip;
-            settle();
-        }
-    };
-    settle();
-#pragma unroll
-    for (int i = 0; i + 1 < kRing; ++i) {
-        fetch();
-        issue(i);
-    }
-    fetch();
-
-    int n = 0;  // blocks folded in: the next is in slot n % kRing
-    for (int b = b0; b <= b_last; ++b) {
-        const Segment g = segment(b);
-        if (g.p0 >= g.p1) continue;
-        uint4 qb[8];
-        load_query(qb, a.q + (static_cast<size_t>(b) * nh + h * G) * kHeadDim, G, lane);
-        // Taken in here: left to the compiler, the wait would sit in front of every
-        // block's products and, not seeing the loads to LDS, drain the ring there.
+    // A workgroup starts with three waits for memory: the sequences' facts, the
+    // first page ids with the first query rows, the first blocks.
+    Share share;
+    if (!share.begin({a.pre_seq, a.ctx_lens, a.seq_ids, e.open_slot, a.table, a.table_stride, a.n_seqs}, w, P, W, lane)) return;
+    const int b0 = share.b0;
+    uint4 qb[8];
+    auto query = [&](int b) { load_query(qb, a.q + (static_cast<size_t>(b) * nh + h * G) * kHeadDim, G, lane); };
+    // Taken in before the blocks' loads go out (a sequence's first wait): left to
+    // the compiler, the wait would sit in front of every block's products and, not
+    // seeing the loads to LDS, drain the ring there.
+    auto take_query = [&]() {
 #pragma unroll
         for (int k = 0; k < 8; ++k) asm volatile("" : "+v"(qb[k].x), "+v"(qb[k].y), "+v"(qb[k].z), "+v"(qb[k].w));
+    };
+    // kRing - 1 blocks ahead of the products; past the share the same loads go
+    // through empty resources, so the load counter advances alike.
+    PageFeed feed;
+    feed.begin(share, lane);
+    query(b0);
+    feed.take();
+    take_query();
+    auto issue = [&](int slot) {
+        const size_t blk = static_cast<size_t>(feed.id) * hkv + h;
+        issue_block(__builtin_amdgcn_readfirstlane(lds_addr(mine + slot * kSlotBytes)), e.k8 + blk * kPageElems,
+                    e.v8 + blk * kPageElems, e.scales + 2 * blk, feed.on, lane);
+        feed.next(share);
+    };
+#pragma unroll
+    for (int i = 0; i + 1 < kRing; ++i) {
+        feed.fetch();
+        issue(i);
+    }
+    feed.fetch();
+
+    int n = 0;  // blocks folded in: the next is in slot n % kRing
+    for (int b = b0; b <= share.b_last; ++b) {
+        const Segment g = share.at(b);
+        if (g.p0 >= g.p1) continue;
+        if (b > b0) {
+            query(b);
+            take_query();
+        }
         State st;
         reset(st);
 #pragma unroll 1
@@ -262,10 +354,10 @@ __global__ __launch_bounds__(64 * kDecodeHeadsPerWg, 2) void decode8_kernel(Deco
             // Behind the block's LDS reads: a scalar load in flight makes each of
             // their waits a wait for all.
             __builtin_amdgcn_sched_barrier(0);
-            fetch();
+            feed.fetch();
         }
         if (g.full < g.p1)
-            fold_open(st, e.open + (static_cast<size_t>(ld_uniform(e.open_slot + b)) * hkv + h) * 2 * kPageElems, qb, lane,
+            fold_open(st, e.open + (static_cast<size_t>(g.slot) * hkv + h) * 2 * kPageElems, qb, lane,
                       g.ctx & 15);
         const float lt = group4_sum(st.l);  // the four lane groups hold disjoint rows
         if (g.p0 == 0 && g.p1 == g.npg && col < G) {
@@ -305,8 +397,7 @@ __global__ __launch_bounds__(64 * kDecodeHeadsPerWg, 2) void decode8_kernel(Deco
 hipError_t launch_decode8(const Decode8Args &a, hipStream_t s) {
     const DecodeArgs &d = a.d;
     if (d.n_seqs <= 0) return hipSuccess;
-    int hpw = d.num_kv_heads <= kDecodeHeadsPerWg ? d.num_kv_heads : kDecodeHeadsPerWg;
-    while (d.num_kv_heads % hpw) --hpw;
+    const int hpw = heads_per_wg(d.num_kv_heads);
     const size_t lds = static_cast<size_t>(hpw) * kRing * kSlotBytes;
     hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(decode8_kernel),
                                        hipFuncAttributeMaxDynamicSharedMemorySize,

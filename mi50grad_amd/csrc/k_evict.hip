@@ -11,9 +11,9 @@
 // a lane holds one query row (column l % 16) and four keys of each page (4 (l /
 // 16) .. + 3).  A first pass over K leaves every query row's max and sum, which
 // stay in the lane until the end; then
-//   - up to 16 query rows (a decode step), it has left the scores too (a
-//     query row's are 4 bytes to a key's 256 or 512), and the probabilities are
-//     made and summed from them (score_kernel);
+//   - up to 16 query rows (a decode step), it leaves the scores too (a query
+//     row's are 4 bytes to a key's 256 or 512), and the probabilities are made and
+//     summed from them (scores_kernel, score_kernel, below);
 //   - more rows, the scores would outweigh the keys, and a second pass over K
 //     sums the probabilities, in the lane over its tiles, before the sixteen
 //     lanes of a row once per page (sum_kernel).
@@ -117,21 +117,12 @@ __device__ __forceinline__ void load_keys(Keys<kInt8> &k, const WeightArgs &a, c
     }
 }
 template <bool kInt8>
-__device__ __forceinline__ void operands(half8_t (&op)[8], float &factor, const Keys<kInt8> &k, const WeightArgs &a,
-                                         const Span &s, int page, int lane) {
-    factor = k.factor;
+__device__ __forceinline__ void operands(half8_t (&op)[8], const Keys<kInt8> &k) {
     if constexpr (kInt8) {
-        if (page == (s.ctx >> 4)) {  // the open page
-            const uint16_t *src = a.open + (static_cast<size_t>(s.slot) * a.num_kv_heads + s.h) * 2 * kPageElems + 16 * lane;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) op[i] = as_h8(ld16(src + 1024 * (i >> 1) + 8 * (i & 1)));
-            factor = kQkScale;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                op[2 * i] = as_h8(codes8(k.raw[i].x, k.raw[i].y));
-                op[2 * i + 1] = as_h8(codes8(k.raw[i].z, k.raw[i].w));
-            }
+        for (int i = 0; i < 4; ++i) {
+            op[2 * i] = as_h8(codes8(k.raw[i].x, k.raw[i].y));
+            op[2 * i + 1] = as_h8(codes8(k.raw[i].z, k.raw[i].w));
         }
     } else {
 #pragma unroll
@@ -167,6 +158,9 @@ struct PageIds {
     __device__ __forceinline__ void load(int from, int last, int lane) {
         base = from;
         ids = row[min(from + lane, last)];
+        // Taken in here: a load that one path leaves pending would make every
+        // later use wait for all loads in flight.
+        asm volatile("" : "+v"(ids));
     }
     __device__ __forceinline__ int at(int page, int last, int lane) {
         if (page - base >= 64) load(page, last, lane);  // wave-uniform
@@ -175,80 +169,118 @@ struct PageIds {
 };
 
 // Pages that a wave takes at a time: two share the operands read from LDS; with
-// one tile of query rows there is little to share, and more waves fit.
+// one tile of query rows there is little to share, more waves fit, and what
+// counts is how many pages are on their way (kAhead steps' worth).
 constexpr int pages_for(int tiles) { return tiles == 1 ? 1 : 2; }
+constexpr int steps_ahead(int tiles, bool int8) { return tiles > 1 ? 1 : int8 ? 3 : 2; }
 
-// Walks the span's pages, PG at a time, this wave's in turn: scores(t, x) gets
-// tile t's of them in log2 units, -inf where the row does not see the key (or
-// there is no such page); done(page) ends them.
+// Walks the span's pages, PG at a time, this wave's in turn: scores(t, x, f)
+// gets tile t's products with them, f times which are log2 units, with -inf (and f
+// = 1) where the row does not see the key or there is no such page; done(page)
+// ends them.
 template <bool kInt8, int NT, int WAVES, class Scores, class Done>
 __device__ __forceinline__ void walk(const WeightArgs &a, const Span &s, const uint4 *qs, Scores scores, Done done) {
-    constexpr int PG = pages_for(NT);
+    constexpr int PG = pages_for(NT), kAhead = steps_ahead(NT, kInt8);
     const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int G = a.num_heads / a.num_kv_heads;
-    const int last = s.p1 - 1;
+    // The open page of an 8-bit cache is FP16 rows and goes by itself, after the others.
+    const int end = kInt8 ? min(s.p1, s.ctx / kBlockTokens) : s.p1;
+    const int last = end - 1;
     int p = s.p0 + PG * wave;
+    half8_t op[PG][8];
+    float factor[PG];
+    // Every tile of query rows against the pages in op, of which `there` are: masked, or every
+    // query row sees every key (rows that there are not have zeros for q; nothing
+    // of them is written, or they weigh nothing).
+    auto tiles = [&](int page, int there, auto masked) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            float4_t x[PG];
+            float f[PG];
+#pragma unroll
+            for (int j = 0; j < PG; ++j) x[j] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const half8_t b = as_h8(qs[(t * 8 + k) * 64 + lane]);
+#pragma unroll
+                for (int j = 0; j < PG; ++j) x[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(op[j][k], b, x[j], 0, 0, 0);
+            }
+#pragma unroll
+            for (int j = 0; j < PG; ++j) {
+                f[j] = factor[j];
+                if constexpr (masked) {
+                    // The last key that the lane's query row sees (none: no such row).
+                    const int iq = (16 * t + col) / G;
+                    const int see = iq < s.obs && j < there ? s.ctx - s.obs + iq : -1;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        x[j][i] = 16 * (page + j) + 4 * grp + i <= see ? x[j][i] * factor[j] : -INFINITY;
+                    f[j] = 1.0f;
+                }
+            }
+            scores(t, x, f);
+            // Two tiles' reads and products overlap; more would only cost registers.
+            if (t & 1) __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    if (kInt8 && end < s.p1 && wave == WAVES - 1) {
+        const uint16_t *src = a.open + (static_cast<size_t>(s.slot) * a.num_kv_heads + s.h) * 2 * kPageElems + 16 * lane;
+#pragma unroll
+        for (int j = 0; j < PG; ++j) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) op[j][i] = as_h8(ld16(src + 1024 * (i >> 1) + 8 * (i & 1)));
+            factor[j] = kQkScale;
+        }
+        tiles(end, 1, std::true_type{});
+        done(end);
+    }
     if (p > last) return;
     PageIds ids{a.table + static_cast<size_t>(s.sid) * a.table_stride, 0, 0};
     ids.load(p, last, lane);
-    Keys<kInt8> cur[PG], nxt[PG];
-#pragma unroll
-    for (int j = 0; j < PG; ++j) load_keys(cur[j], a, s, min(p + j, last), ids.at(min(p + j, last), last, lane), lane);
-    for (; p <= last; p += PG * WAVES) {
+    Keys<kInt8> ring[kAhead + 1][PG];
+    auto request = [&](Keys<kInt8> (&k)[PG], int page) {
 #pragma unroll
         for (int j = 0; j < PG; ++j) {
-            const int q = min(p + PG * WAVES + j, last);
-            load_keys(nxt[j], a, s, q, ids.at(q, last, lane), lane);
+            const int q = min(page + j, last);
+            load_keys(k[j], a, s, q, ids.at(q, last, lane), lane);
         }
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) request(ring[i], p + i * PG * WAVES);
+    // One step: the pages in `cur`, with those kAhead steps on requested first.
+    auto step = [&](const Keys<kInt8> (&cur)[PG], Keys<kInt8> (&nxt)[PG]) -> bool {
+        request(nxt, p + kAhead * PG * WAVES);
         __builtin_amdgcn_sched_barrier(0);
-        half8_t op[PG][8];
-        float factor[PG];
 #pragma unroll
-        for (int j = 0; j < PG; ++j) operands<kInt8>(op[j], factor[j], cur[j], a, s, min(p + j, last), lane);
-        auto tiles = [&](auto masked) {
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                float4_t x[PG];
-#pragma unroll
-                for (int j = 0; j < PG; ++j) x[j] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const half8_t b = as_h8(qs[(t * 8 + k) * 64 + lane]);
-#pragma unroll
-                    for (int j = 0; j < PG; ++j) x[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(op[j][k], b, x[j], 0, 0, 0);
-                }
-#pragma unroll
-                for (int j = 0; j < PG; ++j) {
-                    x[j] *= factor[j];
-                    if constexpr (masked) {
-                        // The last key that the lane's query row sees (none: no such row).
-                        const int iq = (16 * t + col) / G;
-                        const int see = iq < s.obs && p + j <= last ? s.ctx - s.obs + iq : -1;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) x[j][i] = 16 * (p + j) + 4 * grp + i <= see ? x[j][i] : -INFINITY;
-                    }
-                }
-                scores(t, x);
-                // Two tiles' reads and products overlap; more would only cost registers.
-                if (t & 1) __builtin_amdgcn_sched_barrier(0);
-            }
-        };
-        // Every query row sees every key of the pages (rows that there are not
-        // have zeros for q; nothing of them is written, or they weigh nothing).
+        for (int j = 0; j < PG; ++j) {
+            operands<kInt8>(op[j], cur[j]);
+            factor[j] = cur[j].factor;
+        }
         if (p + PG - 1 <= last && 16 * (p + PG) - 1 <= s.ctx - s.obs)
-            tiles(std::false_type{});
+            tiles(p, PG, std::false_type{});
         else
-            tiles(std::true_type{});
+            tiles(p, last - p + 1, std::true_type{});
         done(p);
-#pragma unroll
-        for (int j = 0; j < PG; ++j) cur[j] = nxt[j];
+        p += PG * WAVES;
+        return p <= last;
+    };
+    if constexpr (kAhead == 1) {
+        while (step(ring[0], ring[1]) && step(ring[1], ring[0])) {
+        }
+    } else if constexpr (kAhead == 2) {
+        while (step(ring[0], ring[2]) && step(ring[1], ring[0]) && step(ring[2], ring[1])) {
+        }
+    } else {
+        static_assert(kAhead == 3, "a ring of two to four");
+        while (step(ring[0], ring[3]) && step(ring[1], ring[0]) && step(ring[2], ring[1]) && step(ring[3], ring[2])) {
+        }
     }
 }
 
-__device__ __forceinline__ float exp_sum(const float4_t &x, float mu) {
-    return (__builtin_amdgcn_exp2f(x[0] - mu) + __builtin_amdgcn_exp2f(x[1] - mu)) +
-           (__builtin_amdgcn_exp2f(x[2] - mu) + __builtin_amdgcn_exp2f(x[3] - mu));
+__device__ __forceinline__ float exp_sum(const float4_t &x, float f, float mu) {
+    return (__builtin_amdgcn_exp2f(fmaf(x[0], f, -mu)) + __builtin_amdgcn_exp2f(fmaf(x[1], f, -mu))) +
+           (__builtin_amdgcn_exp2f(fmaf(x[2], f, -mu)) + __builtin_amdgcn_exp2f(fmaf(x[3], f, -mu)));
 }
 __device__ __forceinline__ float max4(const float4_t &x) { return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])); }
 
@@ -275,16 +307,16 @@ __global__ __launch_bounds__(64 * WAVES) void stats_kernel(WeightArgs a) {
     float4_t kept = float4_t{0.f, 0.f, 0.f, 0.f};
     walk<kInt8, NT, WAVES>(
         a, s, qs,
-        [&](int t, const float4_t (&x)[PG]) {
+        [&](int t, const float4_t (&x)[PG], const float (&f)[PG]) {
             float mn = m[t], sum = 0.0f;
 #pragma unroll
-            for (int j = 0; j < PG; ++j) mn = fmaxf(mn, max4(x[j]));
+            for (int j = 0; j < PG; ++j) mn = fmaxf(mn, max4(x[j]) * f[j]);  // f >= 0 keeps the order
             const float mu = mn == -INFINITY ? 0.0f : mn;
 #pragma unroll
-            for (int j = 0; j < PG; ++j) sum += exp_sum(x[j], mu);
+            for (int j = 0; j < PG; ++j) sum += exp_sum(x[j], f[j], mu);
             l[t] = l[t] * __builtin_amdgcn_exp2f(m[t] - mu) + sum;
             m[t] = mn;
-            if constexpr (kScores) kept = x[0];
+            if constexpr (kScores) kept = x[0] * f[0];
         },
         [&](int page) {
             if constexpr (kScores) {
@@ -320,6 +352,14 @@ __device__ __forceinline__ float2 first_part(const WeightArgs &a, const Span &s,
     if (r >= rows || l16 >= s.c1 - s.c0) return make_float2(-INFINITY, 0.0f);
     return a.part[(static_cast<size_t>(s.c0 + l16) * a.num_kv_heads + s.h) * a.part_rows + r];
 }
+// (max, 1 / sum) of the (max, sum) of a DPP row's 16 lanes.
+__device__ __forceinline__ float2 row_merge(float mx, float lt) {
+    float all = mx;
+#pragma unroll
+    for (int o = 8; o >= 1; o >>= 1) all = fmaxf(all, __shfl_xor(all, o));
+    const float mu = all == -INFINITY ? 0.0f : all;
+    return make_float2(mu, 1.0f / row16_sum(lt * __builtin_amdgcn_exp2f(mx - mu)));
+}
 __device__ __forceinline__ float2 row_stat(const WeightArgs &a, const Span &s, float2 first, int r, int rows, int l16) {
     float mx = first.x, lt = first.y;
     if (r < rows)
@@ -330,12 +370,8 @@ __device__ __forceinline__ float2 row_stat(const WeightArgs &a, const Span &s, f
             lt = lt * __builtin_amdgcn_exp2f(mx - mu) + p.y * __builtin_amdgcn_exp2f(p.x - mu);
             mx = mn;
         }
-    float all = mx;
-#pragma unroll
-    for (int o = 8; o >= 1; o >>= 1) all = fmaxf(all, __shfl_xor(all, o));
-    const float mu = all == -INFINITY ? 0.0f : all;
-    lt = row16_sum(lt * __builtin_amdgcn_exp2f(mx - mu));
-    return r < rows ? make_float2(mu, 1.0f / lt) : make_float2(0.0f, 0.0f);
+    const float2 all = row_merge(mx, lt);
+    return r < rows ? all : make_float2(0.0f, 0.0f);
 }
 
 __device__ __forceinline__ void put_weight(const WeightArgs &a, const Span &s, int key, float x) {
@@ -369,17 +405,22 @@ __global__ __launch_bounds__(64 * WAVES) void sum_kernel(WeightArgs a) {
     __syncthreads();
     const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
     constexpr int PG = pages_for(NT);
+    const int end = kInt8 ? min(s.p1, s.ctx / kBlockTokens) : s.p1;  // full pages
     float4_t sum[PG] = {};
     walk<kInt8, NT, WAVES>(
         a, s, qs,
-        [&](int t, const float4_t (&x)[PG]) {
+        [&](int t, const float4_t (&x)[PG], const float (&f)[PG]) {
             const float2 st = stat[16 * t + col];
 #pragma unroll
             for (int j = 0; j < PG; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    // A row that does not see the key adds nothing, whatever its sum is.
-                    sum[j][i] += x[j][i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[j][i] - st.x) * st.y;
+                for (int i = 0; i < 4; ++i) {
+                    const float p = __builtin_amdgcn_exp2f(fmaf(x[j][i], f[j], -st.x));
+                    // A row that does not see the key (-inf: p = 0) adds nothing,
+                    // whatever its sum is (NaN, where it saw such a key).
+                    const float y = fmaf(p, st.y, sum[j][i]);
+                    sum[j][i] = x[j][i] == -INFINITY ? sum[j][i] : y;
+                }
         },
         [&](int page) {
 #pragma unroll
@@ -392,7 +433,7 @@ __global__ __launch_bounds__(64 * WAVES) void sum_kernel(WeightArgs a) {
                 }
                 sum[j] = float4_t{0.f, 0.f, 0.f, 0.f};
                 const int key = 16 * (page + j) + 4 * grp + col;
-                if (col < 4 && page + j < s.p1 && key < s.ctx) put_weight(a, s, key, mine);
+                if (col < 4 && (j == 0 || page + j < end) && key < s.ctx) put_weight(a, s, key, mine);
             }
         });
 }
@@ -419,7 +460,7 @@ __global__ __launch_bounds__(256) void score_kernel(WeightArgs a) {
             for (int i = 0; i < kAhead; ++i) v[i] = r + i < rows ? x[(r + i) * kBlockTokens] : -INFINITY;
 #pragma unroll
             for (int i = 0; i < kAhead; ++i)
-                sum += v[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(v[i] - stat[r + i].x) * stat[r + i].y;
+                if (r + i < rows && v[i] != -INFINITY) sum += __builtin_amdgcn_exp2f(v[i] - stat[r + i].x) * stat[r + i].y;
         }
         put_weight(a, s, key, sum);
     }

@@ -334,6 +334,13 @@ constexpr int mq_keys_for(int waves, bool tree_plan) { return (waves == 8 && !tr
 // 165, 161, 161 and 164, 8 on up to 3000 52.8, 52.4, 51.4, 51.9 and 52.0.  Of
 // sixteen such shapes four is within 2 % of the best on each.
 constexpr int kMqUnitCost = 4;
+// KV heads (one wave each) of a workgroup of the page walks: the largest divisor
+// of all that is at most kDecodeHeadsPerWg.
+constexpr int heads_per_wg(int num_kv_heads) {
+    int h = num_kv_heads <= kDecodeHeadsPerWg ? num_kv_heads : kDecodeHeadsPerWg;
+    while (num_kv_heads % h) --h;
+    return h;
+}
 constexpr int kMqMaxGroup = 8;    // largest GQA group of the multi-query kernel
 constexpr int kMqCutWords = 8;    // int32 words of a cut-unit record (6 used)
 // Workgroups of a multi-query launch over `blocks` positions: one per CU (the
@@ -434,7 +441,7 @@ constexpr int weight_tiles(int rows) {
     return t <= 2 ? t : t <= 4 ? 4 : t <= 8 ? 8 : t <= 12 ? 12 : 16;
 }
 // Workgroups of it that a CU holds: by LDS (8 KB a tile) and registers.
-constexpr int weight_wgs_per_cu(int tiles) { return tiles <= 1 ? 4 : tiles <= 2 ? 3 : tiles <= 4 ? 2 : 1; }
+constexpr int weight_wgs_per_cu(int tiles) { return tiles <= 1 ? 3 : tiles <= 2 ? 3 : tiles <= 4 ? 2 : 1; }
 struct WeightArgs {
     const uint16_t *q;        // [T][H][256]
     const int32_t *seq_ids;   // device, as in MultiQueryArgs
