@@ -48,7 +48,8 @@
 // group g) is matched by the V^T reads, so the sum is over the right pairs.
 //
 // Over the 8-bit cache (Q8; causal steps) the same, but a block comes in
-// through registers: its codes (half the bytes, k_page8.h) are converted once
+// through registers (two row tiles per wave: LDS): its codes (half the bytes,
+// k_page8.h) are converted once
 // per workgroup, each wave its share, and put into LDS as operands, K as integers
 // (the blocks' scales go to the scores), V as values.  Two stages: while block i
 // is multiplied, block i+1's conversion has been written and block i+2's codes
@@ -238,8 +239,15 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
     constexpr int kKT = kFold / 16;  // 16-key tiles of a fold (QK)
     constexpr int kKS = kFold / 32;  // 32-key steps of a fold (PV)
     __shared__ __attribute__((aligned(16))) uint8_t ring[kRing][2 * kTileBytes];
-    __shared__ __attribute__((aligned(16))) uint8_t strips[WAVES][16 * kStripRow];  // the epilogue's, per wave
-    __shared__ float factor[2][Q8 ? KEYS / 16 : 1];  // Q8: what a stage's scores are multiplied by, per page
+    // Q8: the codes of the block that is converted next wait in registers, or,
+    // where two row tiles leave none (16 registers of codes in flight spilled:
+    // 2048 tokens after 16384 took 1243 us, 848 without; one tile 1010), in LDS.  (One tile per
+    // wave: 4 x 512 tokens take 130 us with registers, 134 with LDS.)
+    constexpr bool kRaw = Q8 && NT > 1;
+    // The epilogue's strips, a part per wave; kRaw: those codes (and the strips lie
+    // in the stage that was just multiplied: beside both, two stages would not fit).
+    constexpr int kStripBytes = 16 * kStripRow, kRawBytes = KEYS / WAVES * kHeadDim * 2;
+    __shared__ __attribute__((aligned(16))) uint8_t strips[WAVES][kRaw ? kRawBytes : kStripBytes];
     const int w = mq_share_of(blockIdx.x, a.n_wg);  // this workgroup's share (and partial slots)
     const int W = a.n_wg;
     const int NB = a.total_blocks;
@@ -295,15 +303,21 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
         }
     };
     // Q8: ids8 requests the page ids of the next block (lane l: page l % pages
-    // of a block), load8 its codes and scales into registers (and moves on to the
+    // of a block), load8 its codes and scales (and moves on to the
     // block after it), put8 converts what load8 brought and writes it to a stage.
     // Wave wv takes chunk groups 2 (wv % 2), + 1 of K page wv / 2 and tile group
-    // wv % 4 of V pages 2 (wv / 4), + 1.  Pages past the sequence are zeros, the
-    // open page is FP16 rows, of which the stale ones are masked (K) or zeroed (V).
+    // wv % 4 of V pages 2 (wv / 4), + 1, which no other wave touches.  Pages past
+    // the sequence are zeros, the open page is FP16 rows, of which the stale ones
+    // are masked (K) or zeroed (V).
     constexpr int kPages = KEYS / 16;
     const int nt8 = wv >> 1, ih8 = wv & 1, ks8 = wv >> 2, j8 = wv & 3;
+    [[maybe_unused]] const uint8_t *raw = strips[wv];
     [[maybe_unused]] uint4 rk[2], rv[2];
+    [[maybe_unused]] const uint32_t raw_at = __builtin_amdgcn_readfirstlane(lds_addr(raw));
     [[maybe_unused]] float rsc = 0.0f;  // lane l: scale of page l % kPages, of V where l & kPages
+    // What the scores of the page are multiplied by, of the stage that is
+    // multiplied and of the one that is written (lane l < kPages).
+    [[maybe_unused]] float fac = 0.0f, fac_put = 0.0f;
     [[maybe_unused]] int pg8 = 0, open8 = -1, lim8 = 0, slot8 = 0, h8 = 0;
     [[maybe_unused]] bool on8 = false;
     [[maybe_unused]] auto ids8 = [&]() {
@@ -322,15 +336,19 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
             const int id = __builtin_amdgcn_readlane(vpage, p);
             return ro_rsrc(base + (static_cast<size_t>(id) * hkv + iu.h) * kPageElems, pg8 + p < full ? kPageElems : 0u);
         };
-        auto load = [&](__amdgpu_buffer_rsrc_t r, int ofs) {
-            const auto x = __builtin_amdgcn_raw_buffer_load_b128(r, 16 * lane, ofs, 0);
-            return make_uint4(x[0], x[1], x[2], x[3]);
-        };
         const auto k = codes(a.k8, nt8), v0 = codes(a.v8, 2 * ks8), v1 = codes(a.v8, 2 * ks8 + 1);
-        rk[0] = load(k, 2048 * ih8);
-        rk[1] = load(k, 2048 * ih8 + 1024);
-        rv[0] = load(v0, 1024 * j8);
-        rv[1] = load(v1, 1024 * j8);
+        auto load = [&](uint4 &to, int piece, __amdgpu_buffer_rsrc_t r, int ofs) {
+            if constexpr (kRaw) {
+                load_to_lds_at(r, raw_at + 1024 * piece, 16 * lane, ofs);
+            } else {
+                const auto x = __builtin_amdgcn_raw_buffer_load_b128(r, 16 * lane, ofs, 0);
+                to = make_uint4(x[0], x[1], x[2], x[3]);
+            }
+        };
+        load(rk[0], 0, k, 2048 * ih8);
+        load(rk[1], 1, k, 2048 * ih8 + 1024);
+        load(rv[0], 2, v0, 1024 * j8);
+        load(rv[1], 3, v1, 1024 * j8);
         const float sc = a.scales[(static_cast<size_t>(vpage) * hkv + iu.h) * 2 + ((lane & kPages) ? 1 : 0)];
         rsc = pg8 + (lane & (kPages - 1)) < full ? sc : 0.0f;
         if (on8 && ++ig < q1 && ig >= iu.ue) {
@@ -339,7 +357,16 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
         }
     };
     [[maybe_unused]] auto put8 = [&](int st) {
+        fac = fac_put;
         if (!on8) return;  // uniform over the workgroup
+        if constexpr (kRaw) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                rk[e] = *reinterpret_cast<const uint4 *>(raw + 1024 * e + 16 * lane);
+                rv[e] = *reinterpret_cast<const uint4 *>(raw + 2048 + 1024 * e + 16 * lane);
+            }
+        }
+        fac_put = (pg8 + lane == open8 ? 1.0f : rsc) * (kLog2e / 16.0f);
         const uint16_t *open = a.open + (static_cast<size_t>(slot8) * hkv + h8) * 2 * kPageElems;
         auto scale_of = [&](int lane_of) {
             return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, rsc), lane_of));
@@ -360,7 +387,6 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
             *reinterpret_cast<uint4 *>(kd + 2048 * e) = lo;
             *reinterpret_cast<uint4 *>(kd + 2048 * e + 1024) = hi;
         }
-        if (ih8 == 0 && lane == 0) factor[st][nt8] = (k_open ? 1.0f : scale_of(nt8)) * (kLog2e / 16.0f);
         uint8_t *vd = ring[st] + kTileBytes + ((ks8 * 16 + 4 * j8) * 64 + lane) * 16;
         uint2 part[2][4];
 #pragma unroll
@@ -390,7 +416,9 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
         ids8();
         load8();
         ids8();
+        if constexpr (kRaw) wait_vm<0>();
         put8(0);
+        if constexpr (kRaw) wait_vm_lds<63>();  // the codes are read before others land there
         load8();
         ids8();
     } else {
@@ -462,10 +490,16 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
 
         for (; g < seg_end; ++g) {
             if constexpr (Q8) {
-                wait_vm_lds<63>();  // this wave's part of the stage is written (LDS only)
+                // This wave's part of the stage is written, and (kRaw) the codes that
+                // it requested a block ago are there.
+                wait_vm_lds<kRaw ? 0 : 63>();
                 __builtin_amdgcn_s_barrier();
                 __builtin_amdgcn_sched_barrier(0);
                 put8((n_done + 1) & 1);
+                if constexpr (kRaw) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    wait_vm_lds<63>();  // they are read before others land there
+                }
                 load8();
                 ids8();
                 __builtin_amdgcn_sched_barrier(0);
@@ -517,7 +551,8 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
                 if constexpr (Q8) {
 #pragma unroll
                     for (int nt = 0; nt < kKT; ++nt) {
-                        const float f = factor[n_done % kRing][fold * kKT + nt];
+                        const float f =
+                            __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, fac), fold * kKT + nt));
 #pragma unroll
                         for (int t = 0; t < NT; ++t) s[t][nt] *= f;
                     }
@@ -641,6 +676,13 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
             ++n_done;
         }
 
+        // kRaw: the strips come where other waves may still read operands; the
+        // stage is written again behind the next block's barrier.
+        uint8_t *strip = strips[wv];
+        if constexpr (kRaw) {
+            strip = ring[(n_done + 1) & 1] + wv * kStripBytes;
+            if (whole) __builtin_amdgcn_s_barrier();
+        }
         // The four lane groups hold disjoint keys of each row.
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -668,7 +710,6 @@ __global__ __launch_bounds__(64 * WAVES) void mq_kernel(MultiQueryArgs a) {
                 }
                 constexpr int kGateAhead = NT == 1 ? 4 : 1;  // strips of gate requested together
                 uint4 gw[kGateAhead][2];
-                uint8_t *strip = strips[wv];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     if (a.gate && c % kGateAhead == 0) {
@@ -799,7 +840,7 @@ __global__ __launch_bounds__(64 * kMqCombineRows) void mq_combine_kernel(MultiQu
 
 template <int NT, int WAVES>
 hipError_t launch_mq(const MultiQueryArgs &a, hipStream_t s) {
-    if (a.k8 && (NT > 1 || a.tree || a.keys != 8 * WAVES)) return hipErrorInvalidValue;
+    if (a.k8 && (a.tree || a.keys != 8 * WAVES)) return hipErrorInvalidValue;
     // 64-key blocks only for eight-wave causal tiles (mq_keys_for).
     const bool k64 = a.keys == 64 && WAVES == 8 && !a.tree;
     if (a.keys != 32 && !k64) return hipErrorInvalidValue;
@@ -808,8 +849,7 @@ hipError_t launch_mq(const MultiQueryArgs &a, hipStream_t s) {
         if (e != hipSuccess) return e;
     }
     if (a.k8) {
-        if constexpr (NT == 1)
-            hipLaunchKernelGGL((mq_kernel<NT, WAVES, false, 8 * WAVES, true>), dim3(a.n_wg), dim3(64 * WAVES), 0, s, a);
+        hipLaunchKernelGGL((mq_kernel<NT, WAVES, false, 8 * WAVES, true>), dim3(a.n_wg), dim3(64 * WAVES), 0, s, a);
     } else if constexpr (NT > 1) {  // long prefill steps only
         hipLaunchKernelGGL((mq_kernel<NT, WAVES, false, 64>), dim3(a.n_wg), dim3(64 * WAVES), 0, s, a);
     } else if (a.tree) {

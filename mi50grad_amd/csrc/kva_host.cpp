@@ -380,7 +380,6 @@ int upload_touches(kva_cache *c, const std::vector<int32_t> &touches, hipStream_
 // Whether any step of this cache can be long enough for two row tiles per
 // wave: every tile of the longest step at the longest sequence.
 bool may_take_two_tiles(const kva_cache *c) {
-    if (c->int8) return false;
     const int32_t q = kva::mq_tile_tokens(c->group, 8, 1);
     const int64_t tiles = (static_cast<int64_t>(c->cfg.max_step_tokens) / q + c->cfg.max_seqs) * c->cfg.num_kv_heads;
     const int64_t blocks = static_cast<int64_t>(c->cfg.max_blocks_per_seq) * kva::kBlockTokens / 64 + 1;

@@ -289,6 +289,42 @@ def test_prefill(device, heads, kv, base, new):
     cache.destroy()
 
 
+# Steps long enough for two row tiles per wave (48 blocks of 64 keys for each of
+# 256 workgroups), as in test_gpu_long_prefill.py; rows of whole tiles, of their
+# ends and of a sequence without a past are looked at.
+@pytest.mark.parametrize("heads,kv,base,new", [(24, 4, [16400, 16390, 7], [131, 85, 3]),
+                                               (16, 2, [24600, 0], [257, 33])])
+def test_prefill_of_two_row_tiles(device, heads, kv, base, new):
+    say(f"prefill8 two tiles {heads}/{kv} {base} {new}")
+    rng = np.random.default_rng(heads + sum(new))
+    lens = [b + n for b, n in zip(base, new)]
+    cache = make(lens, heads=heads, kv=kv, step=sum(base))
+    data = [rows(rng, n, kv) for n in lens]
+    seqs = list(range(len(lens)))
+    put(device, cache, seqs, [d[0][:b] for d, b in zip(data, base)], [d[1][:b] for d, b in zip(data, base)])
+    put(device, cache, seqs, [d[0][b:] for d, b in zip(data, base)], [d[1][b:] for d, b in zip(data, base)])
+    tokens = 256 // (heads // kv)
+    assert cache.query_tile() == (2, tokens)
+    T = sum(new)
+    q = rng.standard_normal((T, heads, D)).astype(np.float16)
+    gate = rng.standard_normal((T, heads, D)).astype(np.float16)
+    out, gated = device.empty(q.shape, np.float16), device.empty(q.shape, np.float16)
+    cache.prefill(0, device.array(q), out)
+    cache.prefill(0, device.array(q), gated, gate=device.array(gate))
+    device.synchronize()
+    t = 0
+    for b, n in zip(range(len(lens)), new):
+        k, v = orc.int8_rows(*data[b])
+        for i in sorted({0, 1, tokens // 2, tokens - 1, tokens, n - 2, n - 1}):
+            if 0 <= i < n:
+                at = slice(t + i, t + i + 1)
+                seen = np.arange(lens[b])[None] <= base[b] + i
+                within(out.numpy()[at], *orc.attention_bound(q[at], k, v, seen))
+                within(gated.numpy()[at], *orc.attention_bound(q[at], k, v, seen, gate[at]))
+        t += n
+    cache.destroy()
+
+
 def test_what_is_not_finite_reaches_only_who_sees_it(device):
     say("not finite in attention")
     rng = np.random.default_rng(9)
