@@ -476,6 +476,11 @@ __device__ __forceinline__ uint32_t order_key(float w) {
     const uint32_t u = __builtin_bit_cast(uint32_t, w == w ? w + 0.0f : -INFINITY);
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
+// Whether the weight is its key's value, bit for bit.
+__device__ __forceinline__ bool key_tells(uint32_t key) { return key != ~0xff800000u && key != 0x80000000u; }
+__device__ __forceinline__ float key_value(uint32_t key) {
+    return __builtin_bit_cast(float, (key & 0x80000000u) ? key & 0x7fffffffu : ~key);
+}
 
 // A workgroup per (sequence and KV head, layer).  The key of the last row that
 // stays is found by its digits (12, 10 and 10 bits, the first with sign, exponent
@@ -483,6 +488,9 @@ __device__ __forceinline__ uint32_t order_key(float w) {
 // over many counters); then the rows above it, and as many of its equals from
 // the lowest place on as there is room for, are written in order.  kLds: the
 // keys are held in LDS (up to kSelectLds rows), else read again for each step.
+// The weights are few (64 KB of 16384 rows); the time goes by in waits, so they
+// are requested eight to a thread, and those that stay are written from their
+// keys (16384 rows, 2048 of them kept: 28 us; one at a time and read again 32).
 template <bool kLds>
 __global__ __launch_bounds__(kSelectThreads) void select_kernel(SelectArgs a) {
     extern __shared__ uint32_t keys[];
@@ -505,7 +513,15 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(SelectArgs a) {
         return order_key(w[j]);
     };
     if constexpr (kLds) {
-        for (int j = lo + tid; j < hi; j += kSelectThreads) keys[j] = order_key(w[j]);
+        constexpr int kEach = 8;
+        for (int j0 = tid; j0 < n; j0 += kEach * kSelectThreads) {
+            float x[kEach];
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) x[i] = w[min(j0 + i * kSelectThreads, n - 1)];
+#pragma unroll
+            for (int i = 0; i < kEach; ++i)
+                if (j0 + i * kSelectThreads < n) keys[j0 + i * kSelectThreads] = order_key(x[i]);
+        }
     }
     // Digits of the least key that stays; `want` counts down to its equals.
     uint32_t prefix = 0;
@@ -595,7 +611,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(SelectArgs a) {
         if (stay) {
             const int i = out + __popcll(set & below);
             kept[i] = j;
-            if (w_out) w_out[i] = w[j];
+            if (w_out) w_out[i] = kLds && key_tells(keys[j]) ? key_value(keys[j]) : w[j];
         }
         out += __popcll(set);
         ties += __popcll(tie_set);

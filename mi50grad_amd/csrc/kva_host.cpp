@@ -1849,7 +1849,7 @@ int kva_evict(kva_cache *c, int32_t n_seqs, const int32_t *src_ids, const int32_
         // tables are changed behind the launch that reads the old ones.
         const size_t rec_bytes = recs.size() * sizeof(int32_t), patch_bytes = c->patches.size() * sizeof(int32_t);
         const int32_t n_recs = static_cast<int32_t>(recs.size() / kva::kTouchWords);
-        if (rec_bytes + patch_bytes <= c->aux_bytes) {
+        if (round_up(rec_bytes + patch_bytes, 16) <= c->aux_bytes) {
             if (patch_bytes == 0) return KVA_OK;
             uint8_t *h;
             int idx;
@@ -1857,7 +1857,9 @@ int kva_evict(kva_cache *c, int32_t n_seqs, const int32_t *src_ids, const int32_
             if (rc) return rc;
             std::memcpy(h, recs.data(), rec_bytes);
             std::memcpy(h + rec_bytes, c->patches.data(), patch_bytes);
-            KVA_HIP(hipMemcpyAsync(c->d_aux, h, rec_bytes + patch_bytes, hipMemcpyHostToDevice, s));
+            // By a kernel: with a copy engine's the selection, the copy and the
+            // gather each wait for the other's queue (22 us between the kernels).
+            KVA_HIP(kva::launch_copy(c->d_aux, h, round_up(rec_bytes + patch_bytes, 16), s));
             if ((rc = release_stage(c, idx, s))) return rc;
             g.recs = reinterpret_cast<const int32_t *>(c->d_aux);
             KVA_HIP(kva::launch_gather(g, n_recs, c->cfg.num_kv_heads, c->cfg.n_layers, s));
