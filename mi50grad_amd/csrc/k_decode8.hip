@@ -4,7 +4,12 @@
 // stands for (k_page8.h), as decode over the FP16 cache, with half its bytes.
 // Stream-K over pages as there (k_walk.h): workgroup w walks the w-th share of
 // the pages of all sequences, one wave per KV head; a sequence that the share
-// holds whole is written out, a cut one leaves partials for the merge.
+// holds whole is written out, a cut one leaves partials for the merge.  Short
+// steps take a workgroup per sequence and KV head instead (whole8_kernel).
+//
+// What bounds it is HBM: 48 sequences of about 32000 rows (2.05 GB) take 355 us,
+// 5.8 TB/s; 32 of about 8000 (285 MB) 63 us, some 14 us of it the start (three
+// waits for memory in turn), the tail and the merge.
 //
 // A block is 8 KB in operand order, so a wave brings it in as eight 1 KB loads
 // that write LDS directly (and one of its scales), through a ring of its own:
@@ -269,7 +274,7 @@ struct PageFeed {
     __device__ __forceinline__ void take() { asm volatile("" : "+v"(ids)); }
     __device__ __forceinline__ void fetch() {
         if (!on) return;
-        if (ip - first < n_first)
+        if (n_first && ip - first < n_first)
             id = __builtin_amdgcn_readlane(ids, ip - first);
         else
             id = ld_uniform(g.row + ip);
@@ -392,11 +397,120 @@ __global__ __launch_bounds__(64 * kDecodeHeadsPerWg, 2) void decode8_kernel(Deco
     __builtin_amdgcn_s_waitcnt(0);
 }
 
+// ---- short steps: a workgroup per sequence and KV head ----
+//
+// Its waves take the sequence's pages in turn and merge in LDS: no partials, no
+// second launch, and at the start one wait for memory fewer (the step plan holds
+// the ids of the first pages).  The wave that has the fewest pages takes the open
+// block, before its others, while those are on their way.
+constexpr int kShortWaves = 8, kShortRing = 2;
+constexpr int kShortLds = kShortWaves * kShortRing * kSlotBytes;
+static_assert(kShortWaves * 8 * kHeadDim * 4 <= kShortLds, "eight heads' accumulators of every wave take the ring's place");
+
+__global__ __launch_bounds__(64 * kShortWaves) void whole8_kernel(Decode8Args e) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t ring[];  // [waves][kShortRing][kSlotBytes]
+    __shared__ float2 ml[kShortWaves][16];
+    const DecodeArgs &a = e.d;
+    const int hkv = a.num_kv_heads, nh = a.num_heads, G = nh / hkv;
+    const int b = blockIdx.x / hkv, h = blockIdx.x - b * hkv;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+    uint8_t *mine = ring + static_cast<size_t>(wave) * kShortRing * kSlotBytes;
+
+    // The wave's i-th page is wave + kShortWaves i; lane l: the id of page i0 + l of
+    // its own, the first ones from the plan.
+    constexpr int kPlanned = kPlanPages / kShortWaves;
+    int ids = lane < kPlanned ? a.plan_pages[b * kPlanPages + wave + kShortWaves * lane] : 0, i0 = 0;
+    uint4 qb[8];
+    load_query(qb, a.q + (static_cast<size_t>(b) * nh + h * G) * kHeadDim, G, lane);
+    const int ctx = ld_uniform(a.ctx_lens + b), slot_open = ld_uniform(e.open_slot + b);
+    const int32_t *row = a.table + static_cast<size_t>(ld_uniform(a.seq_ids + b)) * a.table_stride;
+    asm volatile("" : "+v"(ids));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) asm volatile("" : "+v"(qb[k].x), "+v"(qb[k].y), "+v"(qb[k].z), "+v"(qb[k].w));
+    const int full = ctx / kBlockTokens;  // pages that are not open
+    const int n = full > wave ? (full - wave + kShortWaves - 1) / kShortWaves : 0;  // this wave's
+    auto table_ids = [&](int from, int skip) {
+        if (lane >= skip) ids = row[min(wave + kShortWaves * (from + lane), full - 1)];
+        asm volatile("" : "+v"(ids));
+    };
+    if (n > kPlanned) table_ids(0, kPlanned);
+    auto issue = [&](int i) {
+        if (i - i0 == 64 && i < n) {
+            i0 = i;
+            table_ids(i, 0);
+        }
+        const size_t blk = static_cast<size_t>(__builtin_amdgcn_readlane(ids, min(i - i0, 63))) * hkv + h;
+        issue_block(__builtin_amdgcn_readfirstlane(lds_addr(mine + i % kShortRing * kSlotBytes)), e.k8 + blk * kPageElems,
+                    e.v8 + blk * kPageElems, e.scales + 2 * blk, i < n, lane);
+    };
+#pragma unroll
+    for (int i = 0; i + 1 < kShortRing; ++i) issue(i);
+    State st;
+    reset(st);
+    if ((ctx & 15) && wave == full % kShortWaves)
+        fold_open(st, e.open + (static_cast<size_t>(slot_open) * hkv + h) * 2 * kPageElems, qb, lane, ctx & 15);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+        __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));  // lgkmcnt(0): the slot's last reads have returned
+        __builtin_amdgcn_sched_barrier(0);
+        issue(i + kShortRing - 1);
+        wait_vm<kLoads * (kShortRing - 1)>();
+        __builtin_amdgcn_sched_barrier(0);
+        fold_block(st, mine + i % kShortRing * kSlotBytes, qb, lane);
+    }
+    const float lt = group4_sum(st.l);
+    // No load may land in the ring any more, nor may a wave still read it.
+    wait_vm_lds<0>();
+    __syncthreads();
+    float *acc = reinterpret_cast<float *>(ring);  // [wave][G][256]
+    if (col < G) {
+        float *to = acc + (wave * G + col) * kHeadDim + 4 * grp;
+#pragma unroll
+        for (int t = 0; t < 16; ++t) *reinterpret_cast<float4_t *>(to + 16 * t) = st.acc[t];
+        if (grp == 0) ml[wave][col] = make_float2(st.m, lt);
+    }
+    __syncthreads();
+    // Four dims to a thread.
+    for (int i = threadIdx.x; i < G * (kHeadDim / 4); i += 64 * kShortWaves) {
+        const int g = i / (kHeadDim / 4), d = 4 * (i % (kHeadDim / 4)), hq = h * G + g;
+        const uint2 gw =
+            a.gate ? ld8(a.gate + static_cast<int64_t>(b) * a.gate_stride + hq * kHeadDim + d) : make_uint2(0, 0);
+        float big = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kShortWaves; ++w) big = fmaxf(big, ml[w][g].x);
+        // A head whose every score is NaN stays at -inf, its sum NaN.
+        const float mu = big == -INFINITY ? 0.0f : big;
+        float l = 0.0f;
+        float4_t o = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kShortWaves; ++w) {
+            const float2 x = ml[w][g];
+            // At -inf: a wave without pages (zeros), or NaN sums that stay.
+            const float c = x.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(x.x - mu);
+            l += c * x.y;
+            o += c * *reinterpret_cast<const float4_t *>(acc + (w * G + g) * kHeadDim + d);
+        }
+        o *= 1.0f / l;
+        *reinterpret_cast<uint2 *>(a.out + (static_cast<size_t>(b) * nh + hq) * kHeadDim + d) =
+            a.gate ? gate4(o[0], o[1], o[2], o[3], gw) : pack_out4(o[0], o[1], o[2], o[3]);
+    }
+}
+
 }  // namespace
 
 hipError_t launch_decode8(const Decode8Args &a, hipStream_t s) {
     const DecodeArgs &d = a.d;
     if (d.n_seqs <= 0) return hipSuccess;
+    if (d.whole) {
+        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(whole8_kernel),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, kShortLds);
+        if (e != hipSuccess) return e;
+        if (d.ev_before && (e = hipEventRecord(d.ev_before, s)) != hipSuccess) return e;
+        hipLaunchKernelGGL(whole8_kernel, dim3(d.n_seqs * d.num_kv_heads), dim3(64 * kShortWaves), kShortLds, s, a);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+        return d.ev_after ? hipEventRecord(d.ev_after, s) : hipSuccess;
+    }
     const int hpw = heads_per_wg(d.num_kv_heads);
     const size_t lds = static_cast<size_t>(hpw) * kRing * kSlotBytes;
     hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(decode8_kernel),

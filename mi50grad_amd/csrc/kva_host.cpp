@@ -57,6 +57,14 @@ constexpr int kMinPagesPerWg = 1;   // a short sequence still spreads over sever
 // many rows runs the whole-sequence form: one workgroup per sequence and kv
 // head, no partials and no combine launch.
 constexpr int kWholeMaxTokens = 1024;
+// Over an 8-bit cache the same up to half of that, and up to all of it where
+// its workgroups fill a quarter of the CUs (it takes 9.5 to 9.9 us for 1 to 16
+// sequences of 512 rows with four KV heads, stream-K 9.9 to 13.7; of 1024 rows
+// 14.2 to 14.7 against 10.5, 13.0, 13.6 and 16.2 for 1, 4, 8 and 16 of them, 24.4
+// against 30.0 for 64).
+constexpr int64_t whole8_max_tokens(int64_t units, int32_t n_cu) {
+    return 4 * units >= n_cu ? kWholeMaxTokens : kWholeMaxTokens / 2;
+}
 // The CU count a host-only cache validates against (MI355X).
 constexpr int kHostOnlyCus = 256;
 
@@ -1429,12 +1437,12 @@ static void set_stream_k(kva_cache *c, kva::DecodeArgs &a, int64_t pages, int32_
 }
 
 // Switch a decode launch to the whole-sequence form when the split is
-// automatic and no sequence is longer than kWholeMaxTokens rows: returns the
+// automatic and no sequence is longer than `most` rows: returns the
 // workgroups per (sequence, kv head), each serving group / n of its query
 // heads, n as large as fits one workgroup per CU (0: stream-K instead).
 static int32_t use_whole(kva_cache *c, int32_t split_user, int64_t max_ctx, int32_t n_seqs, int32_t num_heads,
-                         int32_t num_kv_heads, int32_t n_cu) {
-    const bool whole = split_user == 0 && max_ctx <= kWholeMaxTokens;
+                         int32_t num_kv_heads, int32_t n_cu, int64_t most = kWholeMaxTokens) {
+    const bool whole = split_user == 0 && max_ctx <= most;
     if (c) c->last_whole = whole;
     if (!whole) return 0;
     const int32_t g = num_heads / num_kv_heads;
@@ -1497,8 +1505,13 @@ static int decode_impl(kva_cache *c, int32_t layer, const void *q, const void *g
     a.num_kv_heads = c->cfg.num_kv_heads;
     set_stream_k(c, a, c->st_total_pages, c->cfg.num_heads);
     c->last_whole = false;
-    if (!c->int8 && (a.whole = use_whole(c, c->split_user, c->st_max_ctx, c->st_n_seqs, c->cfg.num_heads,
-                                         c->cfg.num_kv_heads, c->n_cu))) {
+    // Over an 8-bit cache a workgroup serves all query heads of its KV head: their
+    // products are columns of one.
+    const int32_t hkv = c->cfg.num_kv_heads;
+    a.whole = c->int8 ? use_whole(c, c->split_user, c->st_max_ctx, c->st_n_seqs, hkv, hkv, c->n_cu,
+                                  whole8_max_tokens(static_cast<int64_t>(c->st_n_seqs) * hkv, c->n_cu))
+                      : use_whole(c, c->split_user, c->st_max_ctx, c->st_n_seqs, c->cfg.num_heads, hkv, c->n_cu);
+    if (a.whole) {
         // Every launch of this form reads the lengths from the step plan: a
         // recorded one stays correct when they grow.
     } else if (c->capturing) {
@@ -1521,7 +1534,7 @@ static int decode_impl(kva_cache *c, int32_t layer, const void *q, const void *g
     if (app) {
         kva::AppendArgs ap = *app;
         ap.keep_k = 1;
-        if (a.whole) {
+        if (a.whole && !c->int8) {
             a.fused = 1;
             a.app = ap;
         } else {

@@ -240,7 +240,7 @@ def _attend(cache_rows, q, base, gate=None):
 
 
 @pytest.mark.parametrize("heads,kv", [(24, 4), (6, 1), (8, 8), (8, 1), (6, 3), (10, 5), (40, 10)])
-@pytest.mark.parametrize("lens", [[1], [16], [5, 17, 33, 300, 2, 1100], [4000]], ids=str)
+@pytest.mark.parametrize("lens", [[1], [16], [5, 17, 33, 300, 2, 1100], [4000], [300, 1, 129, 1024, 16, 1023]], ids=str)
 def test_decode(device, heads, kv, lens):
     say(f"decode8 {heads}/{kv} {lens}")
     rng = np.random.default_rng(heads + kv)
@@ -258,6 +258,30 @@ def test_decode(device, heads, kv, lens):
     for b, n in enumerate(lens):
         within(out.numpy()[b:b + 1], *_attend(data[b], q[b:b + 1], n - 1))
         within(gated.numpy()[b:b + 1], *_attend(data[b], q[b:b + 1], n - 1, gate[b:b + 1, :heads]))
+    cache.destroy()
+
+
+# Shares of many pages that begin inside a sequence and go on over others, by
+# whole pages and by their last rows: 0 is a workgroup per CU, 2048 shares of
+# more pages than a wave has lanes.
+@pytest.mark.parametrize("split", [0, 112, 2048])
+@pytest.mark.parametrize("heads,kv", [(24, 4), (8, 1)])
+def test_decode_of_long_shares(device, heads, kv, split):
+    say(f"decode8 long shares {heads}/{kv} {split}")
+    rng = np.random.default_rng(heads + split)
+    lens = [3001, 9000, 16, 5007, 1, 4444, 2032]
+    cache = make(lens, heads=heads, kv=kv, step=sum(lens))
+    cache.set_decode_split(split)
+    data = [rows(rng, n, kv) for n in lens]
+    seqs = list(range(len(lens)))
+    put(device, cache, seqs, [d[0][:-1] for d in data], [d[1][:-1] for d in data])
+    put(device, cache, seqs, [d[0][-1:] for d in data], [d[1][-1:] for d in data])
+    q = rng.standard_normal((len(lens), heads, D)).astype(np.float16)
+    out = device.empty(q.shape, np.float16)
+    cache.decode(0, device.array(q), out)
+    device.synchronize()
+    for b, n in enumerate(lens):
+        within(out.numpy()[b:b + 1], *_attend(data[b], q[b:b + 1], n - 1))
     cache.destroy()
 
 
@@ -460,6 +484,51 @@ def test_recorded_step(device):
     graph.destroy()
     for c in caches:
         c.destroy()
+    s.destroy()
+
+
+def test_recorded_short_step_of_sequences_grown(device):
+    """A decode recorded in its form for short sequences, replayed when they
+    have grown past what the step plan holds the pages of and past 512 pages."""
+    from mi50grad_amd.device import Stream
+
+    say("recorded short step 8")
+    rng = np.random.default_rng(14)
+    H, kv, seqs = 12, 2, [0, 1, 2]
+    parts = [[1, 1000, 17], [1100, 0, 15], [0, 8200, 16]]
+    data = [rows(rng, sum(n) + len(parts), kv) for n in zip(*parts)]
+    cache = make([len(d[0]) for d in data], heads=H, kv=kv, step=9000)
+    s = Stream()
+    at = [0, 0, 0]
+
+    def grow(n):
+        ks = [d[0][a:a + m] for d, a, m in zip(data, at, n)]
+        vs = [d[1][a:a + m] for d, a, m in zip(data, at, n)]
+        put(device, cache, seqs, ks, vs, stream=s.handle)
+        s.synchronize()
+        for b, m in enumerate(n):
+            at[b] += m
+
+    dq, out = device.empty((3, H, D), np.float16), device.empty((3, H, D), np.float16)
+    graph = None
+    for n in parts:
+        if any(n):
+            grow(n)
+        grow([1, 1, 1])
+        q = rng.standard_normal((3, H, D)).astype(np.float16)
+        dq.copy_from(q)
+        device.synchronize()
+        if graph is None:
+            graph = cache.record_step(s.handle)
+            cache.decode(0, dq, out, stream=s.handle)
+            graph.end()
+        graph.launch()
+        s.synchronize()
+        got = out.numpy()
+        for b in seqs:
+            within(got[b:b + 1], *_attend([x[:at[b]] for x in data[b]], q[b:b + 1], at[b] - 1))
+    graph.destroy()
+    cache.destroy()
     s.destroy()
 
 
