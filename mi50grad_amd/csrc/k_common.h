@@ -296,11 +296,18 @@ __device__ __forceinline__ uint2 gate4(float o0, float o1, float o2, float o3, u
                      o2 * sigmoid(static_cast<float>(b.x)), o3 * sigmoid(static_cast<float>(b.y)));
 }
 
+// o * inv through the gate, rounded once.  The products are this branch's own:
+// shared with one that rounds them to fp16, they would there be rounded to fp32
+// first and not, as a product alone is, in one step with the conversion
+// (v_fma_mixlo_f16), and a merge's bits would depend on its kernel.
+__device__ __forceinline__ uint2 gate4_once(const float4_t &o, float inv, uint2 gw) {
+    asm volatile("" : "+v"(inv));
+    return gate4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv, gw);
+}
+
 // Four attention output dims as fp16, through the gate at g4 (8-byte
-// aligned) unless it is null; once: rounded after the gate only.
-__device__ __forceinline__ uint2 out_fp16x4(float o0, float o1, float o2, float o3, const uint16_t *g4,
-                                            bool once = false) {
-    if (g4 && once) return gate4(o0, o1, o2, o3, ld8(g4));
+// aligned) unless it is null.
+__device__ __forceinline__ uint2 out_fp16x4(float o0, float o1, float o2, float o3, const uint16_t *g4) {
     const uint2 o = pack_out4(o0, o1, o2, o3);
     return g4 ? gate4(o, ld8(g4)) : o;
 }

@@ -645,7 +645,7 @@ __global__ __launch_bounds__(64 * G) void combine_kernel(DecodeArgs a) {
     const float4_t at = merge_few<G>(a, p, h, g, 4 * lane, lane, lt);
     const float inv = 1.0f / lt;
     uint2 y = pack_out4(at[0] * inv, at[1] * inv, at[2] * inv, at[3] * inv);
-    if (gp) y = a.gate_once ? gate4(at[0] * inv, at[1] * inv, at[2] * inv, at[3] * inv, gw) : gate4(y, gw);
+    if (gp) y = a.gate_once ? gate4_once(at, inv, gw) : gate4(y, gw);
     *reinterpret_cast<uint2 *>(a.out + (static_cast<size_t>(b) * a.num_heads + h * G + g) * kHeadDim + 4 * lane) = y;
 }
 
@@ -734,7 +734,7 @@ __global__ __launch_bounds__(64 * NW) void combine_wide_kernel(DecodeArgs a) {
         const uint16_t *gp =
             a.gate ? a.gate + static_cast<int64_t>(b) * a.gate_stride + (h * G + g) * kHeadDim + d0 : nullptr;
         *reinterpret_cast<uint2 *>(a.out + (static_cast<size_t>(b) * a.num_heads + h * G + g) * kHeadDim + d0) =
-            out_fp16x4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv, gp, a.gate_once);
+            gp && a.gate_once ? gate4_once(o, inv, ld8(gp)) : out_fp16x4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv, gp);
     };
     if (p.n <= kCombineChunk) {
         if (wave != 0) return;
@@ -844,8 +844,9 @@ __global__ __launch_bounds__(256) void combine_head_kernel(DecodeArgs a) {
         l = m[0].lt;
     }
     const float inv = 1.0f / l;
+    const uint16_t *gp = gate_of(a, b, h * G + g, lane);
     *reinterpret_cast<uint2 *>(a.out + (static_cast<size_t>(b) * a.num_heads + h * G + g) * kHeadDim + 4 * lane) =
-        out_fp16x4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv, gate_of(a, b, h * G + g, lane), a.gate_once);
+        gp && a.gate_once ? gate4_once(o, inv, ld8(gp)) : out_fp16x4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv, gp);
 }
 
 // Query heads a workgroup from which whole_kernel walks pages: where the

@@ -834,7 +834,7 @@ __global__ __launch_bounds__(64 * kMqCombineRows) void mq_combine_kernel(MultiQu
     }
     const float inv = 1.0f / lt;
     uint2 y = pack_out4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-    if (a.gate) y = a.k8 ? gate4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv, gw) : gate4(y, gw);
+    if (a.gate) y = a.k8 ? gate4_once(o, inv, gw) : gate4(y, gw);
     *reinterpret_cast<uint2 *>(a.out + (tq * a.num_heads + hq) * kHeadDim + 4 * lane) = y;
 }
 
