@@ -399,7 +399,8 @@ int kva_evict(kva_cache *cache, int32_t n_seqs, const int32_t *src_ids, const in
 
 /* Split-K tuning for kva_decode: tokens per split (multiple of 16); 0 =
  * automatic.  Automatic runs a step whose longest sequence is at most 1024
- * rows in the whole-sequence form (each sequence walked whole by workgroups
+ * rows (over an 8-bit cache 512, or 1024 where n_seqs * num_kv_heads is at
+ * least a quarter of the CUs) in the whole-sequence form (each sequence walked whole by workgroups
  * that split its kv heads' query-head groups among them, no partials, no
  * combine launch; kva_get_decode_split then reports split 0 and the
  * workgroup count) and longer steps stream-K over all CUs.  A nonzero split

@@ -702,7 +702,7 @@ hipError_t launch_weights_kind(const WeightArgs &a, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_weights(const WeightArgs &a, hipStream_t s) {
-    if (a.n_seqs <= 0) return hipSuccess;
+    if (a.n_chunks <= 0) return hipSuccess;  // no sequence has rows
     return a.k8 ? launch_weights_kind<true>(a, s) : launch_weights_kind<false>(a, s);
 }
 

@@ -19,6 +19,7 @@
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <string>
 #include <vector>
 
@@ -409,6 +410,9 @@ int capture_note(kva_cache *c, int rc) {
     return rc;
 }
 
+// What a C entry answers when the host's memory runs out inside it.
+int no_memory(const char *what) { return fail(KVA_ERR_CAPACITY, "%s: out of host memory", what); }
+
 // A call that cannot be recorded: its launch shape or its host work depends
 // on the step (or it is the step change itself).
 int refuse_while_capturing(const kva_cache *c, const char *what) {
@@ -423,12 +427,9 @@ extern "C" {
 const char *kva_last_error_string(void) { return g_err.c_str(); }
 const char *kva_version(void) { return "kvattn 0.1 gfx950"; }
 
-int kva_create(const kva_config *cfg, kva_cache **out) {
-    if (!out) return fail(KVA_ERR_INVALID_ARG, "out is NULL");
-    *out = nullptr;
-    int rc = check_cfg(cfg);
-    if (rc) return rc;
-    kva_cache *c = new kva_cache();
+// *made: the cache as far as it has come.
+static int create_cache(const kva_config *cfg, kva_cache **made) {
+    kva_cache *c = *made = new kva_cache();
     c->cfg = *cfg;
     c->int8 = (cfg->flags & KVA_FLAG_INT8) != 0;
     c->host_only = (cfg->flags & KVA_FLAG_HOST_ONLY) != 0;
@@ -489,10 +490,6 @@ int kva_create(const kva_config *cfg, kva_cache **out) {
     c->mq_two_tiles = may_take_two_tiles(c);
     c->mq_floats = static_cast<size_t>(2) * c->mq_max_wg * (c->mq_two_tiles ? 256 : 128) * kva::kHeadDim;
     if (!c->host_only) {
-        auto cleanup = [&](int code) {
-            kva_destroy(c);
-            return code;
-        };
         hipError_t e;
         // Zeroed pools: rows never written read as finite zeros.
         auto filled = [&](auto **p, size_t n, int byte) {
@@ -502,37 +499,37 @@ int kva_create(const kva_config *cfg, kva_cache **out) {
         const size_t layers = cfg->n_layers;
         if (c->int8) {
             if ((e = filled(&c->d_k8, c->layer_codes * layers, 128)) != hipSuccess)
-                return cleanup(hip_fail(e, "hipMalloc(K codes)"));
+                return hip_fail(e, "hipMalloc(K codes)");
             if ((e = filled(&c->d_v8, c->layer_codes * layers, 128)) != hipSuccess)
-                return cleanup(hip_fail(e, "hipMalloc(V codes)"));
+                return hip_fail(e, "hipMalloc(V codes)");
             if ((e = filled(&c->d_scales, c->layer_scales * layers, 0)) != hipSuccess)
-                return cleanup(hip_fail(e, "hipMalloc(scales)"));
+                return hip_fail(e, "hipMalloc(scales)");
             if ((e = filled(&c->d_open, c->layer_open * layers, 0)) != hipSuccess)
-                return cleanup(hip_fail(e, "hipMalloc(open blocks)"));
+                return hip_fail(e, "hipMalloc(open blocks)");
             const size_t step_rows = static_cast<size_t>(cfg->max_step_tokens) * c->row_elems;
             if ((e = hipMalloc(&c->d_stage, 2 * step_rows * sizeof(uint16_t))) != hipSuccess)
-                return cleanup(hip_fail(e, "hipMalloc(projected rows)"));
+                return hip_fail(e, "hipMalloc(projected rows)");
             std::vector<int32_t> count(cfg->max_step_tokens);
             for (int32_t i = 0; i < cfg->max_step_tokens; ++i) count[i] = i;
             if ((e = hipMalloc(&c->d_count, count.size() * sizeof(int32_t))) != hipSuccess ||
                 (e = hipMemcpy(c->d_count, count.data(), count.size() * sizeof(int32_t), hipMemcpyHostToDevice)) !=
                     hipSuccess)
-                return cleanup(hip_fail(e, "hipMalloc(row numbers)"));
+                return hip_fail(e, "hipMalloc(row numbers)");
         } else {
             if ((e = filled(&c->d_k, c->layer_elems * layers, 0)) != hipSuccess)
-                return cleanup(hip_fail(e, "hipMalloc(K pool)"));
+                return hip_fail(e, "hipMalloc(K pool)");
             if ((e = filled(&c->d_v, c->layer_elems * layers, 0)) != hipSuccess)
-                return cleanup(hip_fail(e, "hipMalloc(V pool)"));
+                return hip_fail(e, "hipMalloc(V pool)");
         }
         const size_t tbytes = c->table.size() * sizeof(int32_t);
-        if ((e = hipMalloc(&c->d_table, tbytes)) != hipSuccess) return cleanup(hip_fail(e, "hipMalloc(table)"));
-        if ((e = hipMemset(c->d_table, 0, tbytes)) != hipSuccess) return cleanup(hip_fail(e, "hipMemset(table)"));
-        if ((e = hipMalloc(&c->d_step, c->step_bytes)) != hipSuccess) return cleanup(hip_fail(e, "hipMalloc(step)"));
-        if ((e = hipMalloc(&c->d_aux, c->aux_bytes)) != hipSuccess) return cleanup(hip_fail(e, "hipMalloc(aux)"));
+        if ((e = hipMalloc(&c->d_table, tbytes)) != hipSuccess) return hip_fail(e, "hipMalloc(table)");
+        if ((e = hipMemset(c->d_table, 0, tbytes)) != hipSuccess) return hip_fail(e, "hipMemset(table)");
+        if ((e = hipMalloc(&c->d_step, c->step_bytes)) != hipSuccess) return hip_fail(e, "hipMalloc(step)");
+        if ((e = hipMalloc(&c->d_aux, c->aux_bytes)) != hipSuccess) return hip_fail(e, "hipMalloc(aux)");
         int dev = 0, ncu = 0;
-        if ((e = hipGetDevice(&dev)) != hipSuccess) return cleanup(hip_fail(e, "hipGetDevice"));
+        if ((e = hipGetDevice(&dev)) != hipSuccess) return hip_fail(e, "hipGetDevice");
         if ((e = hipDeviceGetAttribute(&ncu, hipDeviceAttributeMultiprocessorCount, dev)) != hipSuccess)
-            return cleanup(hip_fail(e, "hipDeviceGetAttribute(CU count)"));
+            return hip_fail(e, "hipDeviceGetAttribute(CU count)");
         c->n_cu = std::max(1, ncu);
         // Partial slots: two per decode workgroup, each [heads][256] floats;
         // up to four workgroups per CU can be requested.
@@ -540,28 +537,46 @@ int kva_create(const kva_config *cfg, kva_cache **out) {
         c->ws_rows = static_cast<size_t>(2) * c->max_wg * c->cfg.num_heads;
         const size_t units = c->ws_rows;
         if ((e = hipMalloc(&c->d_ws_acc, units * kva::kHeadDim * sizeof(float))) != hipSuccess)
-            return cleanup(hip_fail(e, "hipMalloc(workspace)"));
+            return hip_fail(e, "hipMalloc(workspace)");
         if ((e = hipMalloc(&c->d_ws_ml, units * 2 * sizeof(float))) != hipSuccess)
-            return cleanup(hip_fail(e, "hipMalloc(workspace ml)"));
+            return hip_fail(e, "hipMalloc(workspace ml)");
         // Multi-query partial slots: two per workgroup, one workgroup per CU.
         c->mq_max_wg = c->n_cu;
         c->mq_two_tiles = may_take_two_tiles(c);
         const size_t mq_rows = static_cast<size_t>(2) * c->mq_max_wg * (c->mq_two_tiles ? 256 : 128);
         c->mq_floats = mq_rows * kva::kHeadDim;
         if ((e = hipMalloc(&c->d_mq_acc, c->mq_floats * sizeof(float))) != hipSuccess)
-            return cleanup(hip_fail(e, "hipMalloc(multi-query workspace)"));
+            return hip_fail(e, "hipMalloc(multi-query workspace)");
         if ((e = hipMalloc(&c->d_mq_ml, mq_rows * 2 * sizeof(float))) != hipSuccess)
-            return cleanup(hip_fail(e, "hipMalloc(multi-query workspace ml)"));
+            return hip_fail(e, "hipMalloc(multi-query workspace ml)");
         if ((e = hipMalloc(&c->d_proj, c->part_floats * sizeof(float))) != hipSuccess)
-            return cleanup(hip_fail(e, "hipMalloc(projection workspace)"));
+            return hip_fail(e, "hipMalloc(projection workspace)");
         for (int i = 0; i < kStageSlots; ++i) {
             if ((e = hipHostMalloc(reinterpret_cast<void **>(&c->h_stage[i]), c->stage_bytes,
                                    hipHostMallocDefault)) != hipSuccess)
-                return cleanup(hip_fail(e, "hipHostMalloc(staging)"));
+                return hip_fail(e, "hipHostMalloc(staging)");
             if ((e = hipEventCreateWithFlags(&c->ev[i], hipEventDisableTiming)) != hipSuccess)
-                return cleanup(hip_fail(e, "hipEventCreate"));
+                return hip_fail(e, "hipEventCreate");
         }
-        if ((e = hipDeviceSynchronize()) != hipSuccess) return cleanup(hip_fail(e, "hipDeviceSynchronize"));
+        if ((e = hipDeviceSynchronize()) != hipSuccess) return hip_fail(e, "hipDeviceSynchronize");
+    }
+    return KVA_OK;
+}
+
+int kva_create(const kva_config *cfg, kva_cache **out) {
+    if (!out) return fail(KVA_ERR_INVALID_ARG, "out is NULL");
+    *out = nullptr;
+    int rc = check_cfg(cfg);
+    if (rc) return rc;
+    kva_cache *c = nullptr;
+    try {
+        rc = create_cache(cfg, &c);
+    } catch (const std::exception &) {
+        rc = no_memory("kva_create");
+    }
+    if (rc) {
+        if (c) (void)kva_destroy(c);
+        return rc;
     }
     *out = c;
     return KVA_OK;
@@ -748,7 +763,7 @@ int kva_sync_tables(kva_cache *c, kva_stream_t stream) {
 }
 
 int kva_step_begin(kva_cache *c, int32_t n_seqs, const int32_t *seq_ids, const int32_t *n_new,
-                   const int32_t *rope_pos, const uint64_t *tree_bits, kva_stream_t stream) {
+                   const int32_t *rope_pos, const uint64_t *tree_bits, kva_stream_t stream) try {
     if (!c) return fail(KVA_ERR_INVALID_ARG, "cache is NULL");
     if (int rc = refuse_while_capturing(c, "kva_step_begin")) return rc;
     c->step_valid = false;
@@ -797,6 +812,15 @@ int kva_step_begin(kva_cache *c, int32_t n_seqs, const int32_t *seq_ids, const i
             }
         }
     }
+    // All that the commit below appends to, so that none of it stops half way.
+    std::vector<int32_t> touches, reopened, slots;
+    if (c->int8) {
+        touches.reserve((static_cast<size_t>(n_tok) / kva::kBlockTokens + 2 * static_cast<size_t>(n_seqs)) *
+                        kva::kTouchWords);
+        reopened.reserve(static_cast<size_t>(n_seqs) * kva::kTouchWords);
+        slots.reserve(n_seqs);
+    }
+    c->patches.reserve(c->patches.size() + 3 * static_cast<size_t>(extra_blocks));
     // Commit: reserve, assign slots, advance lengths.
     for (int32_t b = 0; b < n_seqs; ++b) {
         const int32_t s = seq_ids[b];
@@ -840,7 +864,6 @@ int kva_step_begin(kva_cache *c, int32_t n_seqs, const int32_t *seq_ids, const i
     // 8-bit cache: the pages that the step's rows go to, a record each; each
     // sequence's open block behind the step; and the sequences whose length was
     // set back into a page that no open block holds, which takes its values then.
-    std::vector<int32_t> touches, reopened, slots;
     if (c->int8) {
         int32_t tok = 0;
         for (int32_t b = 0; b < n_seqs; ++b) {
@@ -1069,6 +1092,8 @@ int kva_step_begin(kva_cache *c, int32_t n_seqs, const int32_t *seq_ids, const i
     c->st_has_bits = tree_bits != nullptr;
     c->step_valid = true;
     return KVA_OK;
+} catch (const std::exception &) {
+    return no_memory("kva_step_begin");
 }
 
 // Where the step's rows go, for an append's launch.
@@ -1741,7 +1766,7 @@ int kva_attn_weights(kva_cache *c, int32_t layer, const void *q, int32_t n_obs, 
 
 int kva_evict(kva_cache *c, int32_t n_seqs, const int32_t *src_ids, const int32_t *dst_ids, const int32_t *keep,
               int32_t first, int32_t recent, const float *weights, float *weights_out, int64_t w_stride,
-              int32_t *kept, int64_t kept_stride, kva_stream_t stream) {
+              int32_t *kept, int64_t kept_stride, kva_stream_t stream) try {
     if (!c) return fail(KVA_ERR_INVALID_ARG, "cache is NULL");
     if (int rc = refuse_while_capturing(c, "kva_evict")) return rc;
     if (n_seqs < 0 || n_seqs > c->cfg.max_seqs) return fail(KVA_ERR_INVALID_ARG, "bad n_seqs %d", n_seqs);
@@ -1801,9 +1826,22 @@ int kva_evict(kva_cache *c, int32_t n_seqs, const int32_t *src_ids, const int32_
         overlaps(kept, 2 * heads * kept_stride, weights_out, 2 * heads * w_stride))
         return fail(KVA_ERR_INVALID_ARG, "weights, weights_out and kept must not overlap");
     if (int rc = require_device(c)) return rc;
+    // All that the work below appends to, so that none of it stops half way.
+    size_t pages = 0;
+    for (int32_t b = 0; b < n_seqs; ++b) pages += (static_cast<size_t>(n_keep[b]) + kva::kBlockTokens - 1) / kva::kBlockTokens;
+    struct Replaced {  // a source and its new blocks, ids[first .. first + count)
+        int32_t seq;
+        size_t first, count;
+    };
+    std::vector<int32_t> ids, recs;
+    std::vector<Replaced> replaced;
+    ids.reserve(pages);
+    recs.reserve(pages * kva::kTouchWords);
+    replaced.reserve(n_seqs);
     hipStream_t s = static_cast<hipStream_t>(stream);
     int rc = flush_patches(c, s);
     if (rc) return rc;
+    c->patches.reserve(3 * pages);
     c->step_valid = false;
     kva::SelectArgs sel{};
     sel.weights = weights;
@@ -1841,21 +1879,19 @@ int kva_evict(kva_cache *c, int32_t n_seqs, const int32_t *src_ids, const int32_
     g.layer_open = c->layer_open;
     // Sequences in groups: a group's rows are copied in one launch, then its
     // sources give up the blocks that they are replaced from.
-    std::vector<int32_t> recs;
-    std::vector<std::pair<int32_t, std::vector<int32_t>>> replaced;  // sequence, its new blocks
-    auto adopt = [&](int32_t seq, const std::vector<int32_t> &ids) {
+    auto adopt = [&](int32_t seq, size_t first, size_t count) {
         const size_t base = static_cast<size_t>(seq) * c->cfg.max_blocks_per_seq;
-        for (size_t i = 0; i < ids.size(); ++i) {
-            c->table[base + i] = ids[i];
-            c->patches.insert(c->patches.end(), {seq, static_cast<int32_t>(i), ids[i]});
+        for (size_t i = 0; i < count; ++i) {
+            c->table[base + i] = ids[first + i];
+            c->patches.insert(c->patches.end(), {seq, static_cast<int32_t>(i), ids[first + i]});
         }
-        c->nblk[seq] = static_cast<int32_t>(ids.size());
+        c->nblk[seq] = static_cast<int32_t>(count);
         c->freed[seq] = 0;
     };
     auto run_group = [&]() -> int {
-        for (auto &[seq, ids] : replaced) {
-            release_blocks(c, seq);
-            adopt(seq, ids);
+        for (const Replaced &r : replaced) {
+            release_blocks(c, r.seq);
+            adopt(r.seq, r.first, r.count);
         }
         replaced.clear();
         // The records and the new tables in one copy where they fit it; the
@@ -1898,24 +1934,24 @@ int kva_evict(kva_cache *c, int32_t n_seqs, const int32_t *src_ids, const int32_
             continue;
         const int32_t need = (n + kva::kBlockTokens - 1) / kva::kBlockTokens;
         if (static_cast<size_t>(need) > c->free_list.size() && (rc = run_group())) return rc;
-        std::vector<int32_t> ids(need);
-        for (int32_t &id : ids) {
-            id = c->free_list.back();
+        const size_t at0 = ids.size();
+        for (int32_t i = 0; i < need; ++i) {
+            ids.push_back(c->free_list.back());
             c->free_list.pop_back();
-            c->used[id] = 1;
+            c->used[ids.back()] = 1;
         }
         const int32_t full = n / kva::kBlockTokens, behind = n % kva::kBlockTokens;
         const int32_t src_slot = last_open_block(c, src);
         const int32_t src_open = src_slot >= 0 ? c->len[src] / kva::kBlockTokens : -1;
         for (int32_t p = 0; p < full; ++p)
-            recs.insert(recs.end(), {b, p, src, ids[p], kva::kBlockTokens, src_open, src_slot, 0});
+            recs.insert(recs.end(), {b, p, src, ids[at0 + p], kva::kBlockTokens, src_open, src_slot, 0});
         const int32_t dst_slot = 2 * dst + (dst == src && src_slot >= 0 ? 1 - (src_slot & 1) : 0);
         if (behind)
-            recs.insert(recs.end(), {b, full, src, c->int8 ? -1 - dst_slot : ids[full], behind, src_open, src_slot, 0});
+            recs.insert(recs.end(), {b, full, src, c->int8 ? -1 - dst_slot : ids[at0 + full], behind, src_open, src_slot, 0});
         if (dst == src)
-            replaced.emplace_back(src, std::move(ids));
+            replaced.push_back({src, at0, static_cast<size_t>(need)});
         else
-            adopt(dst, ids);
+            adopt(dst, at0, need);
         c->len[dst] = n;
         forget_open_blocks(c, dst);
         c->held[dst] = n;
@@ -1923,6 +1959,8 @@ int kva_evict(kva_cache *c, int32_t n_seqs, const int32_t *src_ids, const int32_
         c->open_last[dst] = dst_slot & 1;
     }
     return run_group();
+} catch (const std::exception &) {
+    return no_memory("kva_evict");
 }
 
 int kva_project_append(kva_cache *c, int32_t layer, const void *x, int32_t hidden, const void *w_q_fused,

@@ -183,3 +183,10 @@ def test_evict_refuses():
     tight.begin_step([0, 1], [40, 40])
     refused(-4, tight.evict, [0], [20], **ok)
     refused(NO_DEVICE, tight.evict, [0, 1], [40, 40], 16, 40, big, 40)
+
+
+def test_out_of_host_memory_is_an_error():
+    """Tables of 4 PiB: the call answers, it does not end the process."""
+    with pytest.raises(KvaError) as e:
+        make(max_seqs=2**30, max_blocks_per_seq=2**20)
+    assert "out of host memory" in str(e.value)

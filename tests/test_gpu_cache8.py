@@ -532,6 +532,41 @@ def test_recorded_short_step_of_sequences_grown(device):
     s.destroy()
 
 
+def test_pages_past_32_bits(device):
+    """Blocks whose codes lie more than 4 GiB into their pools."""
+    from mi50grad_amd.kv_cache import PagedKVCache
+
+    say("pages past 32 bits")
+    rng = np.random.default_rng(15)
+    H, kv, lens, blocks = 24, 4, [300, 1000], 270000  # 4.4 GB of K codes
+    cache = PagedKVCache(n_layers=1, max_seqs=2, max_blocks=blocks, max_blocks_per_seq=64, max_step_tokens=1300,
+                         num_heads=H, num_kv_heads=kv, kv_bits=8)
+    assert blocks * 16 * kv * D > 2**32
+    for b, at in enumerate((blocks - 19, blocks - 19 - 63)):
+        cache.set_blocks(b, range(at, at + (lens[b] + 15) // 16))
+    data = [rows(rng, n, kv) for n in lens]
+    q = rng.standard_normal((9, H, D)).astype(np.float16)
+    out, w = device.empty(q.shape, np.float16), device.empty((2, kv, 1000), np.float32)
+    put(device, cache, [0, 1], [d[0][:-5] for d in data], [d[1][:-5] for d in data])
+    put(device, cache, [0, 1], [d[0][-5:-1] for d in data], [d[1][-5:-1] for d in data])
+    cache.prefill(0, device.array(q[:8]), out)
+    device.synchronize()
+    for b, n in enumerate(lens):
+        at = slice(4 * b, 4 * b + 4)
+        within(out.numpy()[at], *_attend([x[:-1] for x in data[b]], q[at], n - 5))
+    put(device, cache, [0, 1], [d[0][-1:] for d in data], [d[1][-1:] for d in data])
+    cache.decode(0, device.array(q[:2]), out)
+    cache.attn_weights(0, device.array(q[:2]), w, 1000, decay=0.0)
+    device.synchronize()
+    got = held(device, cache, [0, 1])
+    want = [np.concatenate(x) for x in zip(*(orc.int8_rows(*d) for d in data))]
+    assert same_bits(got[0], want[0]) and same_bits(got[1], want[1])
+    for b, n in enumerate(lens):
+        within(out.numpy()[b:b + 1], *_attend(data[b], q[b:b + 1], n - 1))
+        assert np.abs(w.numpy()[b, :, :n].sum(-1) - H // kv).max() < 1e-3  # each head's weights sum to one
+    cache.destroy()
+
+
 def test_half_the_difference_of_a_step(device):
     """Against the FP16 rows themselves a value is off by half a step at most,
     and a step is at most 1/8 wider than 1/127 of the block's largest."""

@@ -89,6 +89,155 @@ def test_weights_of_rows_not_finite(device, bits):
     cache.destroy()
 
 
+@pytest.mark.parametrize("bits", [8, 16])
+def test_weights_without_rows(device, bits):
+    """Sequences without rows, and without new ones, beside others and alone."""
+    say(f"weights without rows {bits}")
+    rng = np.random.default_rng(5)
+    k, v = rows(rng, 40, 2)
+    cache = make([40, 16, 16], heads=4, kv=2, bits=bits)
+    q = device.array(rng.standard_normal((40, 4, D)).astype(np.float16))
+    old = rng.exponential(size=(3, 2, 48)).astype(np.float32)
+    w = device.array(old)
+    cache.begin_step([1, 2], [0, 0])
+    cache.attn_weights(0, q, w, 48, decay=0.5)
+    device.synchronize()
+    assert np.array_equal(w.numpy(), old)
+    cache.begin_step([1, 0, 2], [0, 40, 0])
+    cache.append_rows(0, device.array(k), device.array(v))
+    cache.attn_weights(0, q, w, 48, n_obs=3, decay=0.5)
+    device.synchronize()
+    got = w.numpy()
+    assert np.array_equal(got[[0, 2]], old[[0, 2]]) and np.array_equal(got[1, :, 40:], old[1, :, 40:])
+    want, tol = _weights(q.numpy()[:40], _values(bits, k, v)[0], 40, 3, 2)
+    want = want + 0.5 * old[1, :, :40].astype(np.float64)
+    within(got[1, :, :40], want, tol + 3 * F32 * want)
+    cache.destroy()
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_weights_whose_scores_do_not_fit(device, bits):
+    """One tile of query rows over so many pages that K is read twice: the same
+    8192 rows over and over, so each of their weights is the same in every turn."""
+    say(f"weights of many pages {bits}")
+    rng = np.random.default_rng(6)
+    kv, each, turns, obs = 8, 8192, 34, 16
+    n = each * turns + obs
+    cache = make([n], heads=kv, kv=kv, bits=bits, step=each)
+    k, v = rows(rng, each, kv)
+    last = rows(rng, obs, kv)
+    dk, dv = device.array(k), device.array(v)
+    for _ in range(turns):
+        cache.begin_step([0], [each])
+        cache.append_rows(0, dk, dv)
+    put(device, cache, [0], [last[0]], [last[1]])
+    q = rng.standard_normal((obs, kv, D)).astype(np.float16)
+    w = device.array(np.zeros((1, kv, n), np.float32))
+    cache.attn_weights(0, device.array(q), w, n, n_obs=obs, decay=0.0)
+    device.synchronize()
+    got = w.numpy()[0].astype(np.float64)
+    kd, kl = _values(bits, k, v)[0], _values(bits, *last)[0]
+    see = np.arange(obs)[None] <= np.arange(obs)[:, None]
+    for h in range(kv):
+        x = q[:, h].astype(np.float64)
+        s, sl = x @ kd[:, h].T / 16.0, np.where(see, x @ kl[:, h].T / 16.0, -np.inf)
+        m = np.maximum(s.max(-1), sl.max(-1))[:, None]
+        p, pl = np.exp(s - m), np.exp(sl - m)
+        total = turns * p.sum(-1, keepdims=True) + pl.sum(-1, keepdims=True)
+        want = np.concatenate([np.tile((p / total).sum(0), turns), (pl / total).sum(0)])
+        size = (np.abs(x) @ np.abs(kd[:, h]).T / 16.0).max()
+        # as in _weights; a lane's running sum takes n / 1024 terms at most here
+        within(got[h], want, want * (2 * (D + 16) * F32 * size + 512 * F32) + 1e-37)
+    cache.destroy()
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_more_sequences_than_lanes(device, bits):
+    """150 sequences, some without rows: weights, eviction in place and as copies
+    (their sizes go to the kernels 64 at a time), reading and decode."""
+    say(f"150 sequences {bits}")
+    rng = np.random.default_rng(10)
+    B, H, kv, keep, first, recent = 150, 4, 2, 24, 2, 8
+    lens = [int(x) for x in rng.integers(1, 70, B)]
+    for b in (0, 63, 64, 149):
+        lens[b] = 16 * (b % 3 + 1)
+    cache = make(lens, heads=H, kv=kv, bits=bits, spare=400, slots=2 * B, extra=16)
+    data = [rows(rng, n + 1, kv) for n in lens]
+    seqs = [int(x) for x in rng.permutation(B)]
+    put(device, cache, list(range(B)), [d[0][:-1] for d in data], [d[1][:-1] for d in data])
+    put(device, cache, seqs, [data[s][0][-1:] for s in seqs], [data[s][1][-1:] for s in seqs])
+    q = rng.standard_normal((B, H, D)).astype(np.float16)
+    out, w = device.empty(q.shape, np.float16), device.array(np.zeros((1, B, kv, 80), np.float32))
+    cache.decode(0, device.array(q), out)
+    cache.attn_weights(0, device.array(q), w, 80, decay=0.0)
+    device.synchronize()
+    vals = [_values(bits, *d) for d in data]
+    got = w.numpy()
+    for i, s in enumerate(seqs):
+        want, tol = _weights(q[i:i + 1], vals[s][0], lens[s] + 1, 1, H // kv)
+        within(got[0, i, :, :lens[s] + 1], want, tol + F32 * want)
+        within(out.numpy()[i:i + 1], *orc.attention_bound(q[i:i + 1], *vals[s]))
+    dst = [s if i % 2 else B + i for i, s in enumerate(seqs)]
+    kept = device.empty((1, B, kv, keep), np.int32)
+    cache.evict(seqs, [keep] * B, w, 80, kept, keep, first=first, recent=recent, dst_ids=dst)
+    have, o = held(device, cache, dst), 0
+    for i, s in enumerate(seqs):
+        n = lens[s] + 1
+        m = min(n, keep)
+        places = [_stay(got[0, i, h], n, keep, first, recent) for h in range(kv)]
+        assert all(np.array_equal(kept.numpy()[0, i, h][:m], places[h]) for h in range(kv)), i
+        want = vals[s] if dst[i] == s and m == n else _moved(bits, data[s], places)
+        assert same_bits(have[0][o:o + m], want[0]) and same_bits(have[1][o:o + m], want[1]), i
+        o += m
+    cache.destroy()
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_two_caches_on_two_streams(device, bits):
+    """The same work on two caches at once, each on a stream of its own, gives
+    what it gives alone."""
+    from mi50grad_amd.device import Stream
+
+    say(f"two caches {bits}")
+    rng = np.random.default_rng(11)
+    H, kv, lens, keep = 12, 2, [700, 129, 2000], [256, 100, 512]
+    data = [rows(rng, n, kv) for n in lens]
+    q = device.array(rng.standard_normal((3, H, D)).astype(np.float16))
+    hold = [device.array(np.concatenate([d[j][:-1] for d in data])) for j in (0, 1)]
+    tail = [device.array(np.concatenate([d[j][-1:] for d in data])) for j in (0, 1)]
+
+    def work(cache, stream, out, w, kept):
+        cache.begin_step([0, 1, 2], [n - 1 for n in lens], stream=stream)
+        cache.append_rows(0, *hold, stream=stream)
+        cache.begin_step([0, 1, 2], [1] * 3, stream=stream)
+        cache.append_rows(0, *tail, stream=stream)
+        for _ in range(4):
+            cache.decode(0, q, out, stream=stream)
+            cache.attn_weights(0, q, w, 2048, decay=0.5, stream=stream)
+        cache.evict([0, 1, 2], keep, w, 2048, kept, 512, first=4, recent=16, stream=stream)
+
+    streams = [Stream(), Stream()]
+    caches = [make(lens, heads=H, kv=kv, bits=bits, spare=60) for _ in range(3)]
+    outs = [[device.empty((3, H, D), np.float16), device.array(np.ones((1, 3, kv, 2048), np.float32)),
+             device.array(np.full((1, 3, kv, 512), 7, np.int32))] for _ in range(3)]
+    device.synchronize()
+    work(caches[2], None, *outs[2])
+    device.synchronize()
+    for c, s, o in zip(caches, streams, outs):
+        work(c, s.handle, *o)
+    for s in streams:
+        s.synchronize()
+    want = held(device, caches[2], [0, 1, 2])
+    for c, o in zip(caches[:2], outs):
+        assert all(np.array_equal(x.numpy(), y.numpy()) for x, y in zip(o, outs[2]))
+        got = held(device, c, [0, 1, 2])
+        assert same_bits(got[0], want[0]) and same_bits(got[1], want[1])
+    for c in caches:
+        c.destroy()
+    for s in streams:
+        s.destroy()
+
+
 def test_weights_repeat_to_the_bit(device):
     say("weights repeat")
     rng = np.random.default_rng(3)
