@@ -22,7 +22,7 @@
 //
 // A decode step is bound by HBM and by its start (dependent loads: the plan, the
 // page ids, the first keys): 32 sequences of about 8000 rows in 8 bits, 141 MB of
-// K, take 43 us in stats_kernel, three steps of keys on their way, and 9 in
+// K, take 43 us in stats_kernel, three steps of keys on their way, and 8 in
 // score_kernel; a walk of equal shares through LDS, as the 8-bit decode's, 45.
 // Many rows are bound by the vector unit and LDS: four sequences of about 13000
 // rows with 192 query rows, FP16, 46 us and 42 (the products alone would take 8).
@@ -449,27 +449,33 @@ __global__ __launch_bounds__(64 * WAVES) void sum_kernel(WeightArgs a) {
 __global__ __launch_bounds__(256) void score_kernel(WeightArgs a) {
     __shared__ float2 stat[16];
     const Span s = span_of(a);
-    const int rows = s.obs * (a.num_heads / a.num_kv_heads);
-    constexpr int kAhead = 8;  // scores requested together
+    const int rows = s.obs * (a.num_heads / a.num_kv_heads);  // at most 16
     const int r0 = threadIdx.x >> 4, l16 = threadIdx.x & 15;
-    const float2 mine = row_stat(a, s, first_part(a, s, r0, rows, l16), r0, rows, l16);
-    if (l16 == 0) stat[r0] = mine;
-    __syncthreads();
     const int end = min(16 * s.p1, s.ctx);
-    for (int key = 16 * s.p0 + threadIdx.x; key < end; key += blockDim.x) {
+    float *w = a.weights + (static_cast<size_t>(s.b) * a.num_kv_heads + s.h) * a.w_stride;
+    float v[16], old = 0.0f;
+    auto request = [&](int key) {
+        if (a.decay != 0.0f) old = w[key];
         const float *x = a.scores +
                          (static_cast<size_t>(s.page0 + (key >> 4)) * a.num_kv_heads + s.h) * a.part_rows * kBlockTokens +
                          (key & 15);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) v[r] = r < rows ? x[r * kBlockTokens] : -INFINITY;
+    };
+    int key = 16 * s.p0 + threadIdx.x;
+    const float2 first = first_part(a, s, r0, rows, l16);
+    if (key < end) request(key);
+    const float2 mine = row_stat(a, s, first, r0, rows, l16);
+    if (l16 == 0) stat[r0] = mine;
+    __syncthreads();
+    while (key < end) {
         float sum = 0.0f;
-        for (int r = 0; r < rows; r += kAhead) {
-            float v[kAhead];
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) v[i] = r + i < rows ? x[(r + i) * kBlockTokens] : -INFINITY;
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i)
-                if (r + i < rows && v[i] != -INFINITY) sum += __builtin_amdgcn_exp2f(v[i] - stat[r + i].x) * stat[r + i].y;
-        }
-        put_weight(a, s, key, sum);
+        for (int r = 0; r < 16; ++r)
+            if (v[r] != -INFINITY) sum += __builtin_amdgcn_exp2f(v[r] - stat[r].x) * stat[r].y;
+        w[key] = fmaf(a.decay, old, sum);
+        key += blockDim.x;
+        if (key < end) request(key);
     }
 }
 
