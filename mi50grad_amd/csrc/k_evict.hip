@@ -22,7 +22,7 @@
 //
 // A decode step is bound by HBM and by its start (dependent loads: the plan, the
 // page ids, the first keys): 32 sequences of about 8000 rows in 8 bits, 141 MB of
-// K, take 43 us in stats_kernel, three steps of keys on their way, and 8 in
+// K, take 43 us in stats_kernel and 8 in
 // score_kernel; a walk of equal shares through LDS, as the 8-bit decode's, 45.
 // Many rows are bound by the vector unit and LDS: four sequences of about 13000
 // rows with 192 query rows, FP16, 46 us and 42 (the products alone would take 8).
@@ -49,17 +49,15 @@ __device__ __forceinline__ float row16_sum(float x) {
 }
 
 // A page's keys as this lane's part of A: row l % 16, and the dims that the
-// lane's B holds at each k-step (FP16: 64 (l / 16) + 8 s .. + 7; 8-bit cache:
-// 64 (s / 2) + 16 (l / 16) + 8 (s % 2) .. + 7).  raw: what memory holds of them.
+// lane's B holds at each k-step: 64 (s / 2) + 16 (l / 16) + 8 (s % 2) .. + 7, the
+// order of an 8-bit page; of an FP16 row, two steps take a 128-byte line.
+// raw: what memory holds of them.
 template <bool kInt8>
 struct Keys {
     uint4 raw[kInt8 ? 4 : 8];
     float factor;  // of the scores, log2(e) / 16 included
 };
-template <bool kInt8>
-__device__ __forceinline__ int query_dim(int s, int grp) {
-    return kInt8 ? 64 * (s >> 1) + 16 * grp + 8 * (s & 1) : 64 * grp + 8 * s;
-}
+__device__ __forceinline__ int query_dim(int s, int grp) { return 64 * (s >> 1) + 16 * grp + 8 * (s & 1); }
 
 // What a workgroup works on: pages [p0, p1) of sequence b for KV head h; obs:
 // query tokens, from token `tok` of the step; slot: the open block; page0: pages
@@ -117,9 +115,9 @@ __device__ __forceinline__ void load_keys(Keys<kInt8> &k, const WeightArgs &a, c
         k.factor = a.scales[2 * b] * kQkScale;
     } else {
         const uint16_t *src =
-            a.k_pool + ((static_cast<size_t>(id) * kBlockTokens + (lane & 15)) * hkv + s.h) * kHeadDim + 64 * (lane >> 4);
+            a.k_pool + ((static_cast<size_t>(id) * kBlockTokens + (lane & 15)) * hkv + s.h) * kHeadDim + 16 * (lane >> 4);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) k.raw[i] = ld16(src + 8 * i);
+        for (int i = 0; i < 8; ++i) k.raw[i] = ld16(src + query_dim(i, 0));
         k.factor = kQkScale;
     }
 }
@@ -139,7 +137,7 @@ __device__ __forceinline__ void operands(half8_t (&op)[8], const Keys<kInt8> &k)
 
 // The span's query rows to LDS as B operands: [tile][k-step][lane] of 16 bytes,
 // zeros past the last row.  Requested together: a workgroup starts with them.
-template <bool kInt8, int NT, int WAVES>
+template <int NT, int WAVES>
 __device__ __forceinline__ void load_queries(uint4 *qs, const WeightArgs &a, const Span &s) {
     constexpr int kEach = NT * 512 / (64 * WAVES);
     const int G = a.num_heads / a.num_kv_heads;
@@ -150,7 +148,7 @@ __device__ __forceinline__ void load_queries(uint4 *qs, const WeightArgs &a, con
         const int lane = i & 63, step = (i >> 6) & 7, row = 16 * (i >> 9) + (lane & 15);
         const int iq = row / G;
         x[e] = iq < s.obs ? ld16(a.q + (static_cast<size_t>(s.tok + iq) * a.num_heads + s.h * G + row - iq * G) * kHeadDim +
-                                 query_dim<kInt8>(step, lane >> 4))
+                                 query_dim(step, lane >> 4))
                           : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
@@ -176,10 +174,8 @@ struct PageIds {
 };
 
 // Pages that a wave takes at a time: two share the operands read from LDS; with
-// one tile of query rows there is little to share, more waves fit, and what
-// counts is how many pages are on their way (kAhead steps' worth).
+// one tile of query rows there is little to share, and more waves fit.
 constexpr int pages_for(int tiles) { return tiles == 1 ? 1 : 2; }
-constexpr int steps_ahead(int tiles, bool int8) { return tiles > 1 ? 1 : int8 ? 3 : 2; }
 
 // Walks the span's pages, PG at a time, this wave's in turn: scores(t, x, f)
 // gets tile t's products with them, f times which are log2 units, with -inf (and f
@@ -187,7 +183,7 @@ constexpr int steps_ahead(int tiles, bool int8) { return tiles > 1 ? 1 : int8 ? 
 // ends them.
 template <bool kInt8, int NT, int WAVES, class Scores, class Done>
 __device__ __forceinline__ void walk(const WeightArgs &a, const Span &s, const uint4 *qs, Scores scores, Done done) {
-    constexpr int PG = pages_for(NT), kAhead = steps_ahead(NT, kInt8);
+    constexpr int PG = pages_for(NT);
     const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int G = a.num_heads / a.num_kv_heads;
@@ -218,7 +214,11 @@ __device__ __forceinline__ void walk(const WeightArgs &a, const Span &s, const u
                 f[j] = factor[j];
                 if constexpr (masked) {
                     // The last key that the lane's query row sees (none: no such row).
-                    const int iq = (16 * t + col) / G;
+                    // Divided by here: FP16's keys leave no registers for a quotient per
+                    // tile from step to step.
+                    int g = G;
+                    if constexpr (!kInt8) asm volatile("" : "+s"(g));
+                    const int iq = (16 * t + col) / g;
                     const int see = iq < s.obs && j < there ? s.ctx - s.obs + iq : -1;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
@@ -245,7 +245,7 @@ __device__ __forceinline__ void walk(const WeightArgs &a, const Span &s, const u
     if (p > last) return;
     PageIds ids{a.table + static_cast<size_t>(s.sid) * a.table_stride, 0, 0};
     ids.load(p, last, lane);
-    Keys<kInt8> ring[kAhead + 1][PG];
+    Keys<kInt8> keys[2][PG];
     auto request = [&](Keys<kInt8> (&k)[PG], int page) {
 #pragma unroll
         for (int j = 0; j < PG; ++j) {
@@ -253,11 +253,12 @@ __device__ __forceinline__ void walk(const WeightArgs &a, const Span &s, const u
             load_keys(k[j], a, s, q, ids.at(q, last, lane), lane);
         }
     };
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) request(ring[i], p + i * PG * WAVES);
-    // One step: the pages in `cur`, with those kAhead steps on requested first.
+    request(keys[0], p);
+    // One step: the pages in `cur`, with the next step's requested first.  (More
+    // steps on their way take longer: 32 sequences of 1000 rows, 8-bit and FP16,
+    // 14.1 and 19.9 us with one, 14.4 with three and 21.8 with two; of 8000 the same.)
     auto step = [&](const Keys<kInt8> (&cur)[PG], Keys<kInt8> (&nxt)[PG]) -> bool {
-        request(nxt, p + kAhead * PG * WAVES);
+        request(nxt, p + PG * WAVES);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < PG; ++j) {
@@ -272,16 +273,7 @@ __device__ __forceinline__ void walk(const WeightArgs &a, const Span &s, const u
         p += PG * WAVES;
         return p <= last;
     };
-    if constexpr (kAhead == 1) {
-        while (step(ring[0], ring[1]) && step(ring[1], ring[0])) {
-        }
-    } else if constexpr (kAhead == 2) {
-        while (step(ring[0], ring[2]) && step(ring[1], ring[0]) && step(ring[2], ring[1])) {
-        }
-    } else {
-        static_assert(kAhead == 3, "a ring of two to four");
-        while (step(ring[0], ring[3]) && step(ring[1], ring[0]) && step(ring[2], ring[1]) && step(ring[3], ring[2])) {
-        }
+    while (step(keys[0], keys[1]) && step(keys[1], keys[0])) {
     }
 }
 
@@ -301,7 +293,7 @@ __global__ __launch_bounds__(64 * WAVES) void stats_kernel(WeightArgs a) {
     const Span s = span_of(a);
     if (s.obs == 0) return;
     const int rows = s.obs * (a.num_heads / a.num_kv_heads);
-    load_queries<kInt8, NT, WAVES>(qs, a, s);
+    load_queries<NT, WAVES>(qs, a, s);
     __syncthreads();
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float m[NT], l[NT];
@@ -402,7 +394,7 @@ __global__ __launch_bounds__(64 * WAVES) void sum_kernel(WeightArgs a) {
     float2 first[kEach];
 #pragma unroll
     for (int e = 0; e < kEach; ++e) first[e] = first_part(a, s, 4 * WAVES * e + (threadIdx.x >> 4), rows, threadIdx.x & 15);
-    load_queries<kInt8, NT, WAVES>(qs, a, s);
+    load_queries<NT, WAVES>(qs, a, s);
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
         const int r = 4 * WAVES * e + (threadIdx.x >> 4);
