@@ -25,7 +25,7 @@
 // K, take 43 us in stats_kernel and 8 in
 // score_kernel; a walk of equal shares through LDS, as the 8-bit decode's, 45.
 // Many rows are bound by the vector unit and LDS: four sequences of about 13000
-// rows with 192 query rows, FP16, 46 us and 42 (the products alone would take 8).
+// rows with 192 query rows, FP16, 43 us and 41 (the products alone would take 8).
 #include <type_traits>
 
 #include "k_common.h"
