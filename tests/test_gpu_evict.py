@@ -177,6 +177,12 @@ def test_more_sequences_than_lanes(device, bits):
         want, tol = _weights(q[i:i + 1], vals[s][0], lens[s] + 1, 1, H // kv)
         within(got[0, i, :, :lens[s] + 1], want, tol + F32 * want)
         within(out.numpy()[i:i + 1], *orc.attention_bound(q[i:i + 1], *vals[s]))
+    for split in (32, 2048, 16384):  # shares of two pages, of some forty sequences, of all
+        cache.set_decode_split(split)
+        cache.decode(0, device.array(q), out)
+        device.synchronize()
+        for i, s in enumerate(seqs):
+            within(out.numpy()[i:i + 1], *orc.attention_bound(q[i:i + 1], *vals[s]))
     dst = [s if i % 2 else B + i for i, s in enumerate(seqs)]
     kept = device.empty((1, B, kv, keep), np.int32)
     cache.evict(seqs, [keep] * B, w, 80, kept, keep, first=first, recent=recent, dst_ids=dst)
