@@ -48,7 +48,8 @@ enum {
     KVA_ERR_UNSUPPORTED = -2,   /* shape outside what the kernels implement */
     KVA_ERR_NO_DEVICE = -3,     /* device call on a host-only cache         */
     KVA_ERR_OUT_OF_BLOCKS = -4, /* block pool exhausted                     */
-    KVA_ERR_CAPACITY = -5,      /* length beyond max_blocks_per_seq * 16    */
+    KVA_ERR_CAPACITY = -5,      /* length beyond max_blocks_per_seq * 16, a
+                                   workspace too small, out of host memory  */
     KVA_ERR_BAD_SEQ = -6,       /* sequence id out of range / not active    */
     KVA_ERR_BAD_BLOCK = -7,     /* block id out of range or already in use  */
     KVA_ERR_STATE = -8,         /* call order (no step begun, wrong mode)   */
