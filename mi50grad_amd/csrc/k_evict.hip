@@ -177,10 +177,11 @@ struct PageIds {
 // one tile of query rows there is little to share, and more waves fit.
 constexpr int pages_for(int tiles) { return tiles == 1 ? 1 : 2; }
 
-// Walks the span's pages, PG at a time, this wave's in turn: scores(t, x, f)
+// Walks the span's pages, PG at a time, this wave's in turn: scores(t, x, f, seen)
 // gets tile t's products with them, f times which are log2 units, with -inf (and f
-// = 1) where the row does not see the key or there is no such page; done(page)
-// ends them.
+// = 1) where the row does not see the key or there is no such page; seen(j, i)
+// tells those from a score that is -inf (an infinite key or query) for key i of
+// page j; done(page) ends them.
 template <bool kInt8, int NT, int WAVES, class Scores, class Done>
 __device__ __forceinline__ void walk(const WeightArgs &a, const Span &s, const uint4 *qs, Scores scores, Done done) {
     constexpr int PG = pages_for(NT);
@@ -201,6 +202,7 @@ __device__ __forceinline__ void walk(const WeightArgs &a, const Span &s, const u
         for (int t = 0; t < NT; ++t) {
             float4_t x[PG];
             float f[PG];
+            [[maybe_unused]] int see[PG];
 #pragma unroll
             for (int j = 0; j < PG; ++j) x[j] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -219,14 +221,17 @@ __device__ __forceinline__ void walk(const WeightArgs &a, const Span &s, const u
                     int g = G;
                     if constexpr (!kInt8) asm volatile("" : "+s"(g));
                     const int iq = (16 * t + col) / g;
-                    const int see = iq < s.obs && j < there ? s.ctx - s.obs + iq : -1;
+                    see[j] = iq < s.obs && j < there ? s.ctx - s.obs + iq : -1;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        x[j][i] = 16 * (page + j) + 4 * grp + i <= see ? x[j][i] * factor[j] : -INFINITY;
+                        x[j][i] = 16 * (page + j) + 4 * grp + i <= see[j] ? x[j][i] * factor[j] : -INFINITY;
                     f[j] = 1.0f;
                 }
             }
-            scores(t, x, f);
+            scores(t, x, f, [&](int j, int i) {
+                if constexpr (masked) return 16 * (page + j) + 4 * grp + i <= see[j];
+                return true;
+            });
             // Two tiles' reads and products overlap; more would only cost registers.
             if (t & 1) __builtin_amdgcn_sched_barrier(0);
         }
@@ -306,7 +311,7 @@ __global__ __launch_bounds__(64 * WAVES) void stats_kernel(WeightArgs a) {
     float4_t kept = float4_t{0.f, 0.f, 0.f, 0.f};
     walk<kInt8, NT, WAVES>(
         a, s, qs,
-        [&](int t, const float4_t (&x)[PG], const float (&f)[PG]) {
+        [&](int t, const float4_t (&x)[PG], const float (&f)[PG], auto) {
             float mn = m[t], sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < PG; ++j) mn = fmaxf(mn, max4(x[j]) * f[j]);  // f >= 0 keeps the order
@@ -408,17 +413,18 @@ __global__ __launch_bounds__(64 * WAVES) void sum_kernel(WeightArgs a) {
     float4_t sum[PG] = {};
     walk<kInt8, NT, WAVES>(
         a, s, qs,
-        [&](int t, const float4_t (&x)[PG], const float (&f)[PG]) {
+        [&](int t, const float4_t (&x)[PG], const float (&f)[PG], auto seen) {
             const float2 st = stat[16 * t + col];
 #pragma unroll
             for (int j = 0; j < PG; ++j)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float p = __builtin_amdgcn_exp2f(fmaf(x[j][i], f[j], -st.x));
-                    // A row that does not see the key (-inf: p = 0) adds nothing,
-                    // whatever its sum is (NaN, where it saw such a key).
+                    // A row that does not see the key (p = 0) adds nothing, whatever
+                    // its sum is; one that does adds NaN where its sum is NaN or zero
+                    // (none but scores of -inf), also at p = 0.
                     const float y = fmaf(p, st.y, sum[j][i]);
-                    sum[j][i] = x[j][i] == -INFINITY ? sum[j][i] : y;
+                    sum[j][i] = seen(j, i) ? y : sum[j][i];
                 }
         },
         [&](int page) {
@@ -440,8 +446,10 @@ __global__ __launch_bounds__(64 * WAVES) void sum_kernel(WeightArgs a) {
 // The same from the scores that stats_kernel left: a thread per key.
 __global__ __launch_bounds__(256) void score_kernel(WeightArgs a) {
     __shared__ float2 stat[16];
+    __shared__ int last[16];  // the last key that the row sees
     const Span s = span_of(a);
-    const int rows = s.obs * (a.num_heads / a.num_kv_heads);  // at most 16
+    const int G = a.num_heads / a.num_kv_heads;
+    const int rows = s.obs * G;  // at most 16
     const int r0 = threadIdx.x >> 4, l16 = threadIdx.x & 15;
     const int end = min(16 * s.p1, s.ctx);
     float *w = a.weights + (static_cast<size_t>(s.b) * a.num_kv_heads + s.h) * a.w_stride;
@@ -458,13 +466,16 @@ __global__ __launch_bounds__(256) void score_kernel(WeightArgs a) {
     const float2 first = first_part(a, s, r0, rows, l16);
     if (key < end) request(key);
     const float2 mine = row_stat(a, s, first, r0, rows, l16);
-    if (l16 == 0) stat[r0] = mine;
+    if (l16 == 0) {
+        stat[r0] = mine;
+        last[r0] = r0 < rows ? s.ctx - s.obs + r0 / G : -1;
+    }
     __syncthreads();
     while (key < end) {
         float sum = 0.0f;
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-            if (v[r] != -INFINITY) sum += __builtin_amdgcn_exp2f(v[r] - stat[r].x) * stat[r].y;
+            if (key <= last[r]) sum += __builtin_amdgcn_exp2f(v[r] - stat[r].x) * stat[r].y;
         w[key] = fmaf(a.decay, old, sum);
         key += blockDim.x;
         if (key < end) request(key);

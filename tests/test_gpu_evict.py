@@ -89,6 +89,59 @@ def test_weights_of_rows_not_finite(device, bits):
     cache.destroy()
 
 
+def _not_finite(q, k, ctx, m, G):
+    """_weights with scores that are not finite: q [n, H, D], k [ctx, kv, D] in
+    float64.  The tolerance's score size is that of the finite ones."""
+    kv = k.shape[1]
+    out, tol = np.zeros((kv, ctx)), np.zeros((kv, ctx))
+    q = q[len(q) - m:].astype(np.float64)
+    see = np.arange(ctx)[None] <= ctx - m + np.arange(m)[:, None]
+    finite = lambda x: np.where(np.isfinite(x), np.abs(x), 0.0)  # noqa: E731
+    with np.errstate(invalid="ignore"):
+        for h in range(kv * G):
+            s = np.where(see, q[:, h] @ k[:, h // G].T / 16.0, -np.inf)
+            size = (finite(q[:, h]) @ finite(k[:, h // G]).T / 16.0).max()
+            p = np.exp(s - s.max(-1, keepdims=True))
+            p = np.where(see, p / p.sum(-1, keepdims=True), 0.0)
+            out[h // G] += p.sum(0)
+            tol[h // G] += np.nan_to_num(p).sum(0) * (2 * (D + 16) * F32 * size + 128 * F32)
+    return out, tol + 1e-37
+
+
+@pytest.mark.parametrize("obs", [1, 3, 5, 32])
+@pytest.mark.parametrize("heads,kv", [(24, 4), (6, 2)])
+@pytest.mark.parametrize("what", ["lowest and highest", "query", "all lowest"])
+def test_weights_of_infinite_scores(device, what, heads, kv, obs):
+    """A score of -inf is a score: where its row's sum is NaN (a score of +inf
+    elsewhere, or none but -inf), so is its weight.  Rows that a token does not
+    see get nothing of it."""
+    say(f"infinite scores: {what} {heads}/{kv} {obs}")
+    rng = np.random.default_rng(obs + heads)
+    for bits in (16, 8) if what == "query" else (16,):
+        n = 333
+        k, v = rows(rng, n, kv)
+        q = rng.standard_normal((obs, heads, D)).astype(np.float16)
+        if what == "query":  # a token's every score: infinite, of both signs
+            q[0, ::2, 7] = np.inf
+        elif what == "all lowest":
+            q[0, :, 7] = np.abs(q[0, :, 7]) + np.float16(0.5)
+            q[1:, :, 7] = -np.abs(q[1:, :, 7]) - np.float16(0.5)
+            k[:, 0, 7] = -np.inf
+        else:  # a score of -inf for every query row of a head, and one of +inf that only the last token sees
+            q[:, :, 7] = np.abs(q[:, :, 7]) + np.float16(0.5)
+            k[100, 0, 7] = -np.inf
+            k[n - 1, 0, 7] = np.inf
+        cache = make([n], heads=heads, kv=kv, bits=bits)
+        put(device, cache, [0], [k[:n - obs]], [v[:n - obs]])
+        put(device, cache, [0], [k[n - obs:]], [v[n - obs:]])
+        w = device.array(np.full((1, kv, n), 3.0, np.float32))
+        cache.attn_weights(0, device.array(q), w, n, n_obs=obs, decay=0.0)
+        device.synchronize()
+        want, tol = _not_finite(q, _values(bits, k, v)[0], n, obs, heads // kv)
+        within(w.numpy()[0], want, tol + F32 * np.abs(want))
+        cache.destroy()
+
+
 @pytest.mark.parametrize("bits", [8, 16])
 def test_weights_without_rows(device, bits):
     """Sequences without rows, and without new ones, beside others and alone."""
