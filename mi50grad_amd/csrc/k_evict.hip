@@ -179,9 +179,9 @@ constexpr int pages_for(int tiles) { return tiles == 1 ? 1 : 2; }
 
 // Walks the span's pages, PG at a time, this wave's in turn: scores(t, x, f, seen)
 // gets tile t's products with them, f times which are log2 units, with -inf (and f
-// = 1) where the row does not see the key or there is no such page; seen(j, i)
-// tells those from a score that is -inf (an infinite key or query) for key i of
-// page j; done(page) ends them.
+// = 1) where the row does not see the key or there is no such page; seen(j, i):
+// whether the row sees key i of page j, which tells those from a score that is
+// -inf (an infinite key or query); done(page) ends them.
 template <bool kInt8, int NT, int WAVES, class Scores, class Done>
 __device__ __forceinline__ void walk(const WeightArgs &a, const Span &s, const uint4 *qs, Scores scores, Done done) {
     constexpr int PG = pages_for(NT);
@@ -195,8 +195,8 @@ __device__ __forceinline__ void walk(const WeightArgs &a, const Span &s, const u
     half8_t op[PG][8];
     float factor[PG];
     // Every tile of query rows against the pages in op, of which `there` are: masked, or every
-    // query row sees every key (rows that there are not have zeros for q; nothing
-    // of them is written, or they weigh nothing).
+    // query row sees every key (rows that there are not have zeros for q, so scores
+    // of 0, or of NaN with an infinite key; nothing of them is written or summed).
     auto tiles = [&](int page, int there, auto masked) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -230,7 +230,7 @@ __device__ __forceinline__ void walk(const WeightArgs &a, const Span &s, const u
             }
             scores(t, x, f, [&](int j, int i) {
                 if constexpr (masked) return 16 * (page + j) + 4 * grp + i <= see[j];
-                return true;
+                return 16 * t + col < s.obs * G;
             });
             // Two tiles' reads and products overlap; more would only cost registers.
             if (t & 1) __builtin_amdgcn_sched_barrier(0);

@@ -142,6 +142,30 @@ def test_weights_of_infinite_scores(device, what, heads, kv, obs):
         cache.destroy()
 
 
+@pytest.mark.parametrize("obs", [1, 3, 5, 32])
+@pytest.mark.parametrize("heads,kv", [(24, 4), (6, 2), (6, 1)])
+def test_weights_of_a_key_that_no_token_weighs(device, heads, kv, obs):
+    """A key with scores of -inf only weighs nothing, also where the token and
+    head pairs do not fill the tiles of 16 that they are multiplied in."""
+    say(f"a key of -inf {heads}/{kv} {obs}")
+    rng = np.random.default_rng(obs + heads)
+    n = 333
+    k, v = rows(rng, n, kv)
+    q = rng.standard_normal((obs, heads, D)).astype(np.float16)
+    q[:, :, 7] = np.abs(q[:, :, 7]) + np.float16(0.5)
+    k[[100, 301], :, 7] = -np.inf
+    cache = make([n], heads=heads, kv=kv, bits=16)
+    put(device, cache, [0], [k[:n - obs]], [v[:n - obs]])
+    put(device, cache, [0], [k[n - obs:]], [v[n - obs:]])
+    w = device.array(np.full((1, kv, n), 3.0, np.float32))
+    cache.attn_weights(0, device.array(q), w, n, n_obs=obs, decay=0.0)
+    device.synchronize()
+    want, tol = _not_finite(q, k.astype(np.float64), n, obs, heads // kv)
+    assert (want[:, [100, 301]] == 0).all()
+    within(w.numpy()[0], want, tol + F32 * want)
+    cache.destroy()
+
+
 @pytest.mark.parametrize("bits", [8, 16])
 def test_weights_without_rows(device, bits):
     """Sequences without rows, and without new ones, beside others and alone."""
