@@ -375,6 +375,11 @@ int kva_rollback(kva_cache *cache, int32_t n_seqs, const int32_t *seq_ids,
  * a fixed order.  Not for a step with tree_bits, not while a graph is recorded. */
 int kva_attn_weights(kva_cache *cache, int32_t layer, const void *q, int32_t n_obs, float decay,
                      float *weights, int64_t w_stride, kva_stream_t stream);
+/* The launch of the last kva_attn_weights on this cache that passed its checks
+ * (on a host-only cache the one it would have made): the most pages of one
+ * sequence that a workgroup takes, and the chunks of all sequences, a
+ * workgroup each per KV head.                                               */
+int kva_get_weights_plan(const kva_cache *cache, int32_t *chunk_pages, int32_t *n_chunks);
 /* Keep keep[b] rows of each sequence src_ids[b], in every layer and KV head
  * apart: the first `first`, the latest `recent`, and of the others those of
  * largest weight (equal ones from the lowest slot on; NaN counts as -inf), in

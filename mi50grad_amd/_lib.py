@@ -76,6 +76,7 @@ SIGNATURES = {
     "kva_append_rows": [_P, _I, _P, _P, _P],
     "kva_read_rows": [_P, _I, _I, _PI, _PI, _PI, _P, _P, _P],
     "kva_attn_weights": [_P, _I, _P, _I, c_float, _P, c_int64, _P],
+    "kva_get_weights_plan": [_P, _PI, _PI],
     "kva_evict": [_P, _I, _PI, _PI, _PI, _I, _I, _P, _P, c_int64, _P, c_int64, _P],
     "kva_project_append": [_P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P],
     "kva_out_project": [_P, _P, _I, _I, _P, _I, _P, _P, _P],

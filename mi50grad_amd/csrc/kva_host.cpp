@@ -71,6 +71,12 @@ constexpr int kHostOnlyCus = 256;
 
 }  // namespace
 
+// What a workgroup of kva_attn_weights takes: pages of one sequence (its last
+// chunk may be shorter), and the chunks of all sequences.
+struct WeightChunks {
+    int32_t pages = 0, n = 0;
+};
+
 struct kva_cache {
     kva_config cfg{};
     bool host_only = false;
@@ -164,6 +170,7 @@ struct kva_cache {
     int32_t split_user = 0;  // decode tokens per workgroup (0 = automatic)
     int32_t last_split = 0, last_nwg = 0;
     bool last_whole = false;  // the last decode ran the whole-sequence form
+    WeightChunks last_weights;  // of the last kva_attn_weights
 
     // Graph recording (kva_graph_capture_begin .. _end) on `cap_stream`.
     bool capturing = false;
@@ -328,6 +335,44 @@ int32_t choose_wg(const kva_cache *c, int64_t pages) {
     w = std::min<int64_t>(w, (pages + kMinPagesPerWg - 1) / kMinPagesPerWg);
     w = std::min<int64_t>(w, c->max_wg);
     return static_cast<int32_t>(std::max<int64_t>(1, w));
+}
+
+// Chunks for kva_attn_weights of a step whose sequence b has the pages from
+// pre[b] to pre[b + 1], when `slots` chunks run at once and `most` fit the
+// workspace.  A call takes about its rounds times its longest chunk and what a
+// workgroup starts with (12 to 13 us, as long as 24 pages), so the chunk size is
+// the one of those tried for which this is least, from an equal share of the
+// rounds that the sequences alone make, four pages at least.  With slots for few
+// more than the sequences, one round would leave the longest nearly whole: 2048
+// pages beside 190 sequences of 10 (192 slots) take 24 us in two rounds and 179
+// in one.  More rounds than needed are starts for nothing: four sequences of 560
+// to 1000 pages, 192 query rows (64 slots), take 73 us in one round and 121 in
+// two, 65 of 47 pages 118 in chunks of 47 and 137 in chunks of 24.
+WeightChunks weight_chunks(const std::vector<int32_t> &pre, int32_t n_seqs, int32_t slots, int64_t most) {
+    constexpr int64_t kStart = 24;
+    int32_t longest = 0;
+    int64_t alone = 0;  // sequences with pages
+    for (int32_t b = 0; b < n_seqs; ++b) {
+        longest = std::max(longest, pre[b + 1] - pre[b]);
+        alone += pre[b + 1] > pre[b];
+    }
+    const int64_t rounds = std::max<int64_t>(1, (alone + slots - 1) / slots);
+    int32_t pages = std::max<int32_t>(4, static_cast<int32_t>((pre[n_seqs] + rounds * slots - 1) / (rounds * slots)));
+    WeightChunks best;
+    int64_t least = INT64_MAX;
+    // Every size takes `rounds` at least.
+    while (least == INT64_MAX || rounds * (pages + kStart) < least) {
+        int64_t n = 0;
+        for (int32_t b = 0; b < n_seqs; ++b) n += (pre[b + 1] - pre[b] + pages - 1) / pages;
+        const int64_t cost = (n + slots - 1) / slots * (std::min(pages, longest) + kStart);
+        if ((n <= most || pages >= longest) && cost < least) {
+            least = cost;
+            best = {pages, static_cast<int32_t>(n)};
+        }
+        if (pages >= longest) break;
+        pages = std::min(longest, pages + std::max(1, pages / 16));
+    }
+    return best;
 }
 
 // The open block that holds the first `rows` rows of sequence s's page (-1: none).
@@ -1714,30 +1759,22 @@ int kva_attn_weights(kva_cache *c, int32_t layer, const void *q, int32_t n_obs, 
     kva::WeightArgs a{};
     a.n_obs = std::min(n_obs, std::max(1, c->st_max_new));
     a.part_rows = a.n_obs * group;
-    // Chunks of pages: as many as the chip holds workgroups at once, a page
-    // per wave at least.  A sequence's last chunk may be short, so a chunk size
-    // that gives one round by the sum of pages is raised until the chunks do.
     const int32_t tiles = kva::weight_tiles(a.part_rows);
     const int64_t hkv = c->cfg.num_kv_heads;
-    const int64_t target = std::max<int64_t>(1, c->n_cu * kva::weight_wgs_per_cu(tiles) / hkv);
-    auto chunks_of = [&](int64_t chunk) {
-        int64_t n = 0;
-        for (int32_t b = 0; b < c->st_n_seqs; ++b) n += (c->st_pre[b + 1] - c->st_pre[b] + chunk - 1) / chunk;
-        return n;
-    };
-    const int64_t pages = c->st_total_pages;
-    int64_t chunk = std::max<int64_t>(4, (pages + target - 1) / target);
-    while (chunks_of(chunk) > target && chunk < pages) chunk += std::max<int64_t>(1, chunk / 16);
-    const int64_t n_chunks = chunks_of(chunk);
-    const int64_t part_floats = 2 * n_chunks * hkv * a.part_rows;
+    const int32_t target = std::max<int32_t>(1, static_cast<int32_t>(c->n_cu * kva::weight_wgs_per_cu(tiles) / hkv));
+    const int64_t pages = c->st_total_pages, chunk_floats = 2 * hkv * a.part_rows;
+    const WeightChunks plan =
+        weight_chunks(c->st_pre, c->st_n_seqs, target, static_cast<int64_t>(c->mq_floats) / chunk_floats);
+    const int64_t part_floats = plan.n * chunk_floats;
     if (part_floats > static_cast<int64_t>(c->mq_floats))
         return fail(KVA_ERR_CAPACITY, "%d sequences of %d query rows exceed the workspace", c->st_n_seqs, a.part_rows);
     // The scores behind the partials (16-byte aligned), where one tile's fit.
     const int64_t scores_at = (part_floats + 3) / 4 * 4;
     const bool scores =
         tiles == 1 && scores_at + pages * hkv * a.part_rows * kva::kBlockTokens <= static_cast<int64_t>(c->mq_floats);
-    a.chunk = static_cast<int32_t>(chunk);
-    a.n_chunks = static_cast<int32_t>(n_chunks);
+    a.chunk = plan.pages;
+    a.n_chunks = plan.n;
+    c->last_weights = plan;
     if ((rc = require_device(c))) return rc;
     a.q = static_cast<const uint16_t *>(q);
     a.seq_ids = at<int32_t>(c->d_step, c->off_seq);
@@ -1761,6 +1798,13 @@ int kva_attn_weights(kva_cache *c, int32_t layer, const void *q, int32_t n_obs, 
     a.weights = weights;
     a.w_stride = w_stride;
     KVA_HIP(kva::launch_weights(a, static_cast<hipStream_t>(stream)));
+    return KVA_OK;
+}
+
+int kva_get_weights_plan(const kva_cache *c, int32_t *chunk_pages, int32_t *n_chunks) {
+    if (!c || !chunk_pages || !n_chunks) return fail(KVA_ERR_INVALID_ARG, "NULL argument");
+    *chunk_pages = c->last_weights.pages;
+    *n_chunks = c->last_weights.n;
     return KVA_OK;
 }
 

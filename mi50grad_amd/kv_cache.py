@@ -175,6 +175,13 @@ class PagedKVCache:
         the query heads of KV head h: weights [n_seqs, Hkv, w_stride] fp32."""
         _lib.call("kva_attn_weights", self.handle, layer, _ptr(q), n_obs, decay, _ptr(weights), w_stride, stream)
 
+    def weights_plan(self) -> tuple[int, int]:
+        """Pages of a chunk and chunks of all sequences in the last
+        attn_weights (kva_get_weights_plan)."""
+        pages, n = ctypes.c_int32(), ctypes.c_int32()
+        _lib.call("kva_get_weights_plan", self.handle, ctypes.byref(pages), ctypes.byref(n))
+        return pages.value, n.value
+
     def evict(self, seq_ids: Sequence[int], keep: Sequence[int], weights, w_stride: int, kept, kept_stride: int,
               first: int = 0, recent: int = 0, dst_ids: Sequence[int] | None = None, weights_out=None,
               stream=None) -> None:

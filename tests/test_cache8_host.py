@@ -153,6 +153,33 @@ def test_attn_weights_refuses(bits):
         refused(STATE, c.attn_weights, *ok)
 
 
+def long_ones(pages, heads, kv, obs):
+    """Sequences of `pages` full pages less the obs rows of the next step."""
+    c = make(n_layers=1, max_seqs=len(pages), max_blocks=sum(pages), max_blocks_per_seq=max(pages),
+             max_step_tokens=16 * sum(pages), num_heads=heads, num_kv_heads=kv)
+    c.begin_step(list(range(len(pages))), [16 * p - obs for p in pages])
+    return c
+
+
+@pytest.mark.parametrize("heads,kv,obs,slots", [(24, 4, 1, 192), (24, 4, 32, 64), (8, 8, 1, 96), (8, 8, 32, 96),
+                                                (8, 1, 32, 256)])
+@pytest.mark.parametrize("long,short", [(1000, 32), (2048, 10), (2000, 2), (47, 47)])
+def test_weights_share_out_a_long_sequence(heads, kv, obs, slots, long, short):
+    """A long sequence beside short ones, fewer, as many and more than there are
+    workgroups at once: no chunk is longer than about two even shares of the
+    rounds that the sequences make, and a workgroup's start (24 pages)."""
+    for n_short in (1, slots // 2, slots - 2, slots - 1, slots, 2 * slots, 3 * slots):
+        pages = [short] * n_short + [long]
+        c = long_ones(pages, heads, kv, obs)
+        c.begin_step(list(range(len(pages))), [obs] * len(pages))
+        refused(NO_DEVICE, c.attn_weights, 0, 16, 16, 16 * long, n_obs=obs)
+        chunk, n = c.weights_plan()
+        assert n == sum(-(-p // chunk) for p in pages)
+        rounds = -(-len(pages) // slots)
+        share = -(-sum(pages) // (rounds * slots))
+        assert min(chunk, long) <= 2 * max(share, 4) + 24, (n_short, chunk)
+
+
 def test_evict_refuses():
     c = make()
     c.begin_step([0, 1], [40, 20])

@@ -276,6 +276,40 @@ def test_more_sequences_than_lanes(device, bits):
 
 
 @pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("n_short", [62, 70, 150])
+def test_weights_of_a_long_sequence_among_short_ones(device, n_short, bits):
+    """About as many sequences as workgroups run at once (64 of 192 query rows
+    each per KV head) and more, one of them long: in several chunks, and right."""
+    say(f"one long sequence, {n_short} short, {bits}")
+    rng = np.random.default_rng(n_short + bits)
+    H, kv, obs = 24, 4, 32
+    lens = [int(x) for x in rng.integers(1, 60, n_short)]
+    lens.insert(n_short // 2, 2500)
+    new = [min(n, obs) for n in lens]
+    cache = make(lens, heads=H, kv=kv, bits=bits)
+    seqs = list(range(len(lens)))
+    data = [rows(rng, n, kv) for n in lens]
+    put(device, cache, seqs, [d[0][:len(d[0]) - n] for d, n in zip(data, new)],
+        [d[1][:len(d[1]) - n] for d, n in zip(data, new)])
+    put(device, cache, seqs, [d[0][len(d[0]) - n:] for d, n in zip(data, new)],
+        [d[1][len(d[1]) - n:] for d, n in zip(data, new)])
+    q = rng.standard_normal((sum(new), H, D)).astype(np.float16)
+    old = rng.exponential(size=(len(lens), kv, 2500)).astype(np.float32)
+    w = device.array(old)
+    cache.attn_weights(0, device.array(q), w, 2500, n_obs=obs, decay=0.5)
+    device.synchronize()
+    assert cache.weights_plan()[0] < 40, "pages of the long sequence's 157 in one chunk"
+    got, t = w.numpy().astype(np.float64), 0
+    for b, (n, c) in enumerate(zip(new, lens)):
+        want, tol = _weights(q[t:t + n], _values(bits, *data[b])[0], c, n, H // kv)
+        before = 0.5 * old[b, :, :c].astype(np.float64)
+        within(got[b, :, :c], want + before, tol + F32 * (2 * (want + before) + want))
+        assert np.array_equal(got[b, :, c:], old[b, :, c:].astype(np.float64))
+        t += n
+    cache.destroy()
+
+
+@pytest.mark.parametrize("bits", [8, 16])
 def test_two_caches_on_two_streams(device, bits):
     """The same work on two caches at once, each on a stream of its own, gives
     what it gives alone."""
