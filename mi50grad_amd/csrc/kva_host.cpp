@@ -489,6 +489,7 @@ static int create_cache(const kva_config *cfg, kva_cache **made) {
     c->open_blocks.assign(2 * static_cast<size_t>(cfg->max_seqs), {});
     c->open_last.assign(cfg->max_seqs, 0);
     c->held.assign(cfg->max_seqs, 0);
+    c->st_pre.reserve(static_cast<size_t>(cfg->max_seqs) + 1);
     const size_t block_heads = static_cast<size_t>(cfg->max_blocks) * cfg->num_kv_heads;
     c->layer_codes = block_heads * kva::kPageElems;
     c->layer_scales = block_heads * 2;
@@ -857,22 +858,6 @@ int kva_step_begin(kva_cache *c, int32_t n_seqs, const int32_t *seq_ids, const i
             }
         }
     }
-    // All that the commit below appends to, so that none of it stops half way.
-    std::vector<int32_t> touches, reopened, slots;
-    if (c->int8) {
-        touches.reserve((static_cast<size_t>(n_tok) / kva::kBlockTokens + 2 * static_cast<size_t>(n_seqs)) *
-                        kva::kTouchWords);
-        reopened.reserve(static_cast<size_t>(n_seqs) * kva::kTouchWords);
-        slots.reserve(n_seqs);
-    }
-    c->patches.reserve(c->patches.size() + 3 * static_cast<size_t>(extra_blocks));
-    // Commit: reserve, assign slots, advance lengths.
-    for (int32_t b = 0; b < n_seqs; ++b) {
-        const int32_t s = seq_ids[b];
-        const int64_t end = static_cast<int64_t>(c->len[s]) + n_new[b];
-        int rc = grow_seq(c, s, static_cast<int32_t>((end + kva::kBlockTokens - 1) / kva::kBlockTokens));
-        if (rc) return rc;
-    }
     const size_t o_seq = 0;
     const size_t o_ctx = o_seq + sizeof(int32_t) * n_seqs;
     const size_t o_start = o_ctx + sizeof(int32_t) * n_seqs;
@@ -906,6 +891,26 @@ int kva_step_begin(kva_cache *c, int32_t n_seqs, const int32_t *seq_ids, const i
     const size_t o_pids = round_up(o_bits + (tree_bits ? sizeof(uint64_t) * n_tok : 0), 16);
     const size_t o_slot = round_up(o_pids + sizeof(int32_t) * kva::kPlanPages * n_seqs, 16);
     const size_t o_touch = round_up(o_slot + (c->int8 ? sizeof(int32_t) * n_seqs : 0), 16);
+    // All host memory that the commit below takes, so that none of it stops half way.
+    const size_t most_touches =
+        c->int8 ? static_cast<size_t>(n_tok) / kva::kBlockTokens + 2 * static_cast<size_t>(n_seqs) : 0;
+    std::vector<int32_t> touches, reopened, slots;
+    if (c->int8) {
+        touches.reserve(most_touches * kva::kTouchWords);
+        reopened.reserve(static_cast<size_t>(n_seqs) * kva::kTouchWords);
+        slots.reserve(n_seqs);
+    }
+    std::vector<uint8_t> local;  // the plan of a host-only cache
+    if (c->host_only)
+        local.resize(o_touch + sizeof(int32_t) * (most_touches * kva::kTouchWords + n_units * kva::kMqCutWords) + 16);
+    c->patches.reserve(c->patches.size() + 3 * static_cast<size_t>(extra_blocks));
+    // Commit: reserve, assign slots, advance lengths.
+    for (int32_t b = 0; b < n_seqs; ++b) {
+        const int32_t s = seq_ids[b];
+        const int64_t end = static_cast<int64_t>(c->len[s]) + n_new[b];
+        int rc = grow_seq(c, s, static_cast<int32_t>((end + kva::kBlockTokens - 1) / kva::kBlockTokens));
+        if (rc) return rc;
+    }
     // 8-bit cache: the pages that the step's rows go to, a record each; each
     // sequence's open block behind the step; and the sequences whose length was
     // set back into a page that no open block holds, which takes its values then.
@@ -951,15 +956,9 @@ int kva_step_begin(kva_cache *c, int32_t n_seqs, const int32_t *seq_ids, const i
     const size_t o_cut = o_touch + touches.size() * sizeof(int32_t);
     // The cut-unit records (below) take at most one per unit; only those
     // written are uploaded.
-    const size_t total_max = o_cut + sizeof(int32_t) * kva::kMqCutWords * n_units;
-
-    std::vector<uint8_t> local;
-    uint8_t *h = nullptr;
+    uint8_t *h = local.data();
     int idx = -1;
-    if (c->host_only) {
-        local.resize(total_max + 16);
-        h = local.data();
-    } else {
+    if (!c->host_only) {
         int rc = acquire_stage(c, &h, &idx);
         if (rc) return rc;
     }
