@@ -20,20 +20,21 @@
 #include <cstdio>
 #include <cstring>
 #include <exception>
-#include <string>
+#include <new>
 #include <vector>
 
 namespace {
 
-thread_local std::string g_err;
+// Not a std::string: an error is told when memory has run out, too.
+thread_local char g_err[512];
 
 int fail(int code, const char *fmt, ...) {
-    char buf[512];
+    char buf[sizeof(g_err)];  // an argument may be g_err itself
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(buf, sizeof(buf), fmt, ap);
     va_end(ap);
-    g_err = buf;
+    std::memcpy(g_err, buf, sizeof(buf));
     return code;
 }
 
@@ -223,6 +224,12 @@ int check_seq(const kva_cache *c, int32_t seq) {
     return KVA_OK;
 }
 
+// Room for `n` more elements, so that appending them cannot fail half way.
+template <class T>
+void room_for(std::vector<T> &v, size_t n) {
+    if (v.capacity() - v.size() < n) v.reserve(std::max(2 * v.capacity(), v.size() + n));
+}
+
 // Take free blocks until `seq` holds `need` blocks.
 int grow_seq(kva_cache *c, int32_t seq, int32_t need) {
     if (need > c->cfg.max_blocks_per_seq)
@@ -233,6 +240,7 @@ int grow_seq(kva_cache *c, int32_t seq, int32_t need) {
     if (static_cast<size_t>(need - have) > c->free_list.size())
         return fail(KVA_ERR_OUT_OF_BLOCKS, "pool exhausted: sequence %d needs %d more blocks, %zu free",
                     seq, need - have, c->free_list.size());
+    room_for(c->patches, 3 * static_cast<size_t>(need - have));
     for (int32_t i = have; i < need; ++i) {
         const int32_t blk = c->free_list.back();
         c->free_list.pop_back();
@@ -469,7 +477,7 @@ int refuse_while_capturing(const kva_cache *c, const char *what) {
 
 extern "C" {
 
-const char *kva_last_error_string(void) { return g_err.c_str(); }
+const char *kva_last_error_string(void) { return g_err; }
 const char *kva_version(void) { return "kvattn 0.1 gfx950"; }
 
 // *made: the cache as far as it has come.
@@ -680,7 +688,7 @@ int kva_layer_pools(const kva_cache *c, int32_t layer, void **k_pool, void **v_p
     return KVA_OK;
 }
 
-int kva_seq_reserve(kva_cache *c, int32_t seq, int32_t n_tokens) {
+int kva_seq_reserve(kva_cache *c, int32_t seq, int32_t n_tokens) try {
     if (!c) return fail(KVA_ERR_INVALID_ARG, "cache is NULL");
     int rc = check_seq(c, seq);
     if (rc) return rc;
@@ -690,9 +698,11 @@ int kva_seq_reserve(kva_cache *c, int32_t seq, int32_t n_tokens) {
         return fail(KVA_ERR_CAPACITY, "sequence %d: %d tokens exceed capacity %d", seq, n_tokens,
                     c->cfg.max_blocks_per_seq * kva::kBlockTokens);
     return grow_seq(c, seq, static_cast<int32_t>(need));
+} catch (const std::exception &) {
+    return no_memory("kva_seq_reserve");
 }
 
-int kva_seq_set_blocks(kva_cache *c, int32_t seq, const int32_t *ids, int32_t n) {
+int kva_seq_set_blocks(kva_cache *c, int32_t seq, const int32_t *ids, int32_t n) try {
     if (!c) return fail(KVA_ERR_INVALID_ARG, "cache is NULL");
     int rc = check_seq(c, seq);
     if (rc) return rc;
@@ -713,6 +723,7 @@ int kva_seq_set_blocks(kva_cache *c, int32_t seq, const int32_t *ids, int32_t n)
         seen[b] = 1;
         if (c->used[b] && !mine[b]) return fail(KVA_ERR_BAD_BLOCK, "block id %d is in use", b);
     }
+    room_for(c->patches, 3 * static_cast<size_t>(n));
     release_blocks(c, seq);
     // Remove the new blocks from the free list.
     c->free_list.erase(std::remove_if(c->free_list.begin(), c->free_list.end(),
@@ -727,6 +738,8 @@ int kva_seq_set_blocks(kva_cache *c, int32_t seq, const int32_t *ids, int32_t n)
     c->freed[seq] = 0;
     c->step_valid = false;  // the step plan holds the old block ids
     return KVA_OK;
+} catch (const std::exception &) {
+    return no_memory("kva_seq_set_blocks");
 }
 
 int kva_seq_free(kva_cache *c, int32_t seq) {
@@ -903,7 +916,7 @@ int kva_step_begin(kva_cache *c, int32_t n_seqs, const int32_t *seq_ids, const i
     std::vector<uint8_t> local;  // the plan of a host-only cache
     if (c->host_only)
         local.resize(o_touch + sizeof(int32_t) * (most_touches * kva::kTouchWords + n_units * kva::kMqCutWords) + 16);
-    c->patches.reserve(c->patches.size() + 3 * static_cast<size_t>(extra_blocks));
+    room_for(c->patches, 3 * static_cast<size_t>(extra_blocks));
     // Commit: reserve, assign slots, advance lengths.
     for (int32_t b = 0; b < n_seqs; ++b) {
         const int32_t s = seq_ids[b];
@@ -2214,7 +2227,7 @@ int kva_append_prefill_gated(kva_cache *c, int32_t layer, void *q, const void *k
 }
 
 int kva_rollback(kva_cache *c, int32_t n_seqs, const int32_t *seq_ids, const int32_t *base_len,
-                 const int32_t *keep_off, const int32_t *keep_rows, kva_stream_t stream) {
+                 const int32_t *keep_off, const int32_t *keep_rows, kva_stream_t stream) try {
     if (!c) return fail(KVA_ERR_INVALID_ARG, "cache is NULL");
     if (int rc = refuse_while_capturing(c, "kva_rollback")) return rc;
     if (n_seqs < 0 || n_seqs > c->cfg.max_seqs) return fail(KVA_ERR_INVALID_ARG, "bad n_seqs %d", n_seqs);
@@ -2258,6 +2271,8 @@ int kva_rollback(kva_cache *c, int32_t n_seqs, const int32_t *seq_ids, const int
                     n_moves_all, c->aux_bytes);
     if (n_moves_all > 0)
         if (int rc = refuse_int8(c, "a rollback that moves rows")) return rc;
+    moves.reserve(3 * n_moves_all);
+    move_off.reserve(n_groups_all + 1);
     for (int32_t b = 0; b < n_seqs; ++b) {
         const int32_t s = seq_ids[b];
         const int32_t n = keep_off[b + 1] - keep_off[b];
@@ -2298,6 +2313,8 @@ int kva_rollback(kva_cache *c, int32_t n_seqs, const int32_t *seq_ids, const int
     a.num_kv_heads = c->cfg.num_kv_heads;
     KVA_HIP(kva::launch_rollback(a, st));
     return KVA_OK;
+} catch (const std::exception &) {
+    return no_memory("kva_rollback");
 }
 
 int kva_graph_capture_begin(kva_cache *c, kva_stream_t stream) {
@@ -2329,13 +2346,18 @@ int kva_graph_capture_end(kva_cache *c, kva_stream_t stream, kva_graph **out) {
         (void)hipGraphDestroy(graph);
         return fail(KVA_ERR_STATE, "a call failed while the graph was being recorded; nothing was kept");
     }
-    hipGraphExec_t exec = nullptr;
-    e = hipGraphInstantiate(&exec, graph, nullptr, nullptr, 0);
+    auto *g = new (std::nothrow) kva_graph;
+    if (!g) {
+        (void)hipGraphDestroy(graph);
+        return no_memory("kva_graph_capture_end");
+    }
+    e = hipGraphInstantiate(&g->exec, graph, nullptr, nullptr, 0);
     (void)hipGraphDestroy(graph);
-    if (e != hipSuccess) return hip_fail(e, "hipGraphInstantiate");
-    auto *g = new kva_graph;
+    if (e != hipSuccess) {
+        delete g;
+        return hip_fail(e, "hipGraphInstantiate");
+    }
     g->cache = c;
-    g->exec = exec;
     g->n_seqs = c->st_n_seqs;
     g->n_tok = c->st_n_tok;
     g->table_rows = c->cap_table_rows;

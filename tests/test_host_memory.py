@@ -15,10 +15,15 @@ pytestmark = pytest.mark.skipif(LIB_PATH.name == "libkvattn_san.so", reason="the
 ALLOCATOR = """
 #include <cstdlib>
 #include <new>
-static long left = -1;
-extern "C" void fail_at(long n) { left = n; }
+static long left = -1;  // allocations that succeed before one (forever: all) fails; -1: none does
+static bool forever = false;
+extern "C" void fail_at(long n, bool all) { left = n, forever = all; }
 void *operator new(std::size_t n) {
-    if (left >= 0 && left-- == 0) throw std::bad_alloc();
+    if (left == 0) {
+        if (!forever) left = -1;
+        throw std::bad_alloc();
+    }
+    if (left > 0) --left;
     if (void *p = std::malloc(n ? n : 1)) return p;
     throw std::bad_alloc();
 }
@@ -29,7 +34,7 @@ void operator delete(void *p, std::size_t) noexcept { std::free(p); }
 SCRIPT = """
 import ctypes, sys
 alloc = ctypes.CDLL(sys.argv[1], ctypes.RTLD_GLOBAL)
-alloc.fail_at.argtypes = [ctypes.c_long]
+alloc.fail_at.argtypes = [ctypes.c_long, ctypes.c_bool]
 from mi50grad_amd._lib import KvaError
 from mi50grad_amd.kv_cache import PagedKVCache
 
@@ -46,26 +51,26 @@ def state(c):
     return [(c.seq_len(s), c.blocks(s)) for s in range(40)], c.free_block_count()
 
 def failing(bits, call):
-    \"\"\"`call` with its first, second, ... allocation refused: an error that leaves
-    the cache as it was, and the call works afterwards.\"\"\"
+    \"\"\"`call` with its first, second, ... allocation refused, it alone or all from
+    there on: an error that leaves the cache as it was, and the call works afterwards.\"\"\"
     whole = make(bits)
     call(whole)
     n = 0
     while True:
         c = make(bits)
         before = state(c)
-        alloc.fail_at(n)
+        alloc.fail_at(n // 2, n % 2 == 1)
         try:
             call(c)
         except KvaError as e:
-            alloc.fail_at(-1)
+            alloc.fail_at(-1, False)
             assert e.code == -5 and "out of host memory" in str(e), e
-            assert state(c) == before, f"allocation {n}"
+            assert state(c) == before, f"allocation {n // 2}"
             call(c)
         else:
-            alloc.fail_at(-1)
+            alloc.fail_at(-1, False)
             print(n, flush=True)
-            assert n > 0, "no allocation was refused"
+            assert n > 1, "no allocation was refused"
             return
         assert state(c) == state(whole)
         c.destroy()
@@ -76,6 +81,9 @@ def failing(bits, call):
 CALLS = {
     "begin_step": "lambda c: c.begin_step(list(range(30)), [5 * b for b in range(30)])",
     "begin_step of tokens": "lambda c: c.begin_step(list(range(40)), [1] * 40)",
+    "reserve": "lambda c: c.reserve(5, 640)",
+    "set_blocks": "lambda c: c.set_blocks(0, list(range(300, 340)))",
+    "rollback": "lambda c: c.rollback([0, 1], [20, 30], {8: [[0, 1], [0]], 16: [[0, 2, 5], [3, 4]]}[c.kv_bits])",
 }
 
 
