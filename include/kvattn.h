@@ -83,8 +83,9 @@ enum {
  * where they came one step or more before the page was full and it was the
  * sequence's open page before the present one, else from the values its codes
  * stand for.  kva_seq_set_blocks leaves a last page that is
- * not full with the sequence.  Recorded appends take one new token per
- * sequence.                                                                 */
+ * not full with the sequence; every other page has the rows of the block that
+ * it is given, and rows behind the length in a page whose block changes count
+ * as not written.  Recorded appends take one new token per sequence.        */
 #define KVA_FLAG_INT8 0x2u
 
 /*

@@ -724,6 +724,22 @@ int kva_seq_set_blocks(kva_cache *c, int32_t seq, const int32_t *ids, int32_t n)
         if (c->used[b] && !mine[b]) return fail(KVA_ERR_BAD_BLOCK, "block id %d is in use", b);
     }
     room_for(c->patches, 3 * static_cast<size_t>(n));
+    if (c->int8) {
+        // A page that gets another block has that one's rows: FP16 rows held of it
+        // are not its own, but for the last page's, which are in no block, and
+        // rows behind the length were not written.
+        auto changes = [&](int32_t page) {
+            return page >= std::min(n, c->nblk[seq]) || c->table[base + page] != ids[page];
+        };
+        const int32_t last = c->len[seq] / kva::kBlockTokens;
+        for (int32_t i = 2 * seq; i < 2 * seq + 2; ++i) {
+            kva_cache::OpenBlock &open = c->open_blocks[i];
+            const bool stays = open.page == last && c->len[seq] % kva::kBlockTokens;
+            if (open.page >= 0 && !stays && changes(open.page)) open = {};
+        }
+        for (int32_t page = last; page * kva::kBlockTokens < c->held[seq]; ++page)
+            if (changes(page)) c->held[seq] = std::max(c->len[seq], page * kva::kBlockTokens);
+    }
     release_blocks(c, seq);
     // Remove the new blocks from the free list.
     c->free_list.erase(std::remove_if(c->free_list.begin(), c->free_list.end(),

@@ -104,6 +104,26 @@ def test_length_goes_up_only_to_rows_written():
     refused(STATE, c.set_len, 0, 1)
 
 
+def test_rows_go_with_their_blocks():
+    """Rows behind the length whose page gets another block, or none, were not
+    written any more."""
+    c = make()
+    c.set_blocks(0, [5, 6, 7])
+    c.begin_step([0], [40])
+    c.set_len(0, 10)
+    c.set_blocks(0, [5, 6, 8])
+    refused(STATE, c.set_len, 0, 33)
+    c.set_len(0, 32)
+    c.set_len(0, 10)
+    c.set_blocks(0, [5])
+    c.reserve(0, 100)
+    refused(STATE, c.set_len, 0, 17)
+    c.set_len(0, 16)
+    c.set_len(0, 10)
+    c.set_blocks(0, [9, 6])
+    refused(STATE, c.set_len, 0, 11)
+
+
 @pytest.mark.parametrize("bits", [8, 16])
 def test_append_rows_and_read_rows_refuse(bits):
     c = make(kv_bits=bits)

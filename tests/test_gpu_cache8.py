@@ -441,6 +441,31 @@ def test_length_set_back(device, layers):
     cache.destroy()
 
 
+def test_blocks_that_change_places(device):
+    """A full page reads as the block that it was given, also where the length
+    goes back into it and rows follow; the last page stays with the sequence."""
+    say("blocks change places")
+    rng = np.random.default_rng(16)
+    kv = 2
+    k, v = rows(rng, 42, kv)
+    cache = make([40], heads=2, kv=kv, extra=8)
+    for a, b in ((0, 20), (20, 40)):  # page 1 is open once
+        put(device, cache, [0], [k[a:b]], [v[a:b]])
+    page = [orc.int8_rows(k[16 * p:16 * p + 16], v[16 * p:16 * p + 16]) for p in range(2)]
+    b0, b1, b2 = cache.blocks(0)
+    cache.set_blocks(0, [b1, b0, b2])
+    swapped = [np.concatenate([page[1][i], page[0][i], x[32:40].astype(np.float64)]) for i, x in enumerate((k, v))]
+    for n in (40, 18):
+        cache.set_len(0, n)
+        got = held(device, cache, [0])
+        assert all(same_bits(g, w[:n]) for g, w in zip(got, swapped)), n
+    put(device, cache, [0], [k[40:]], [v[40:]])
+    got = held(device, cache, [0])
+    for g, w, x in zip(got, swapped, (k, v)):
+        assert same_bits(g[:18], w[:18]) and same_bits(g[18:], x[40:])
+    cache.destroy()
+
+
 def test_recorded_step(device):
     """A replayed step gives the eager bits while lengths grow over page ends,
     with eager work between the replays."""
