@@ -947,6 +947,10 @@ int kva_step_begin(kva_cache *c, int32_t n_seqs, const int32_t *seq_ids, const i
         int32_t tok = 0;
         for (int32_t b = 0; b < n_seqs; ++b) {
             const int32_t s = seq_ids[b], start = c->len[s], end = start + n_new[b];
+            if (n_new[b] == 0) {  // nothing is written or attended to: what is held stays
+                slots.push_back(0);
+                continue;
+            }
             const int32_t from = start / kva::kBlockTokens, to = end / kva::kBlockTokens;
             const int32_t rows = start % kva::kBlockTokens, behind = end % kva::kBlockTokens;
             // The block of the page that the step starts in, if rows are there.

@@ -124,6 +124,15 @@ def test_rows_go_with_their_blocks():
     refused(STATE, c.set_len, 0, 11)
 
 
+def test_a_step_without_rows_leaves_the_sequence():
+    c = make()
+    c.begin_step([0], [40])
+    c.set_len(0, 20)
+    c.begin_step([0, 1], [0, 3])
+    c.set_len(0, 40)
+    assert c.seq_len(0) == 40
+
+
 @pytest.mark.parametrize("bits", [8, 16])
 def test_append_rows_and_read_rows_refuse(bits):
     c = make(kv_bits=bits)

@@ -466,6 +466,28 @@ def test_blocks_that_change_places(device):
     cache.destroy()
 
 
+def test_a_step_without_rows_leaves_the_sequence(device):
+    """Listed with no new rows, a sequence that was set back keeps what lies
+    behind its length, the open page's FP16 rows among it."""
+    say("a step without rows")
+    rng = np.random.default_rng(17)
+    kv = 2
+    k, v = rows(rng, 41, kv)
+    cache = make([40, 10], heads=2, kv=kv, extra=8)
+    for a, b in ((0, 20), (20, 40)):
+        put(device, cache, [0], [k[a:b]], [v[a:b]])
+    for back in (18, 9, 16, 0):  # pages held in FP16, in codes, none
+        cache.set_len(0, back)
+        put(device, cache, [0, 1], [k[:0], k[:2]], [v[:0], v[:2]])
+        cache.set_len(0, 40)
+        got, want = held(device, cache, [0]), orc.int8_rows(k[:40], v[:40])
+        assert same_bits(got[0], want[0]) and same_bits(got[1], want[1]), back
+    put(device, cache, [0], [k[40:]], [v[40:]])
+    got, want = held(device, cache, [0]), orc.int8_rows(k, v)
+    assert same_bits(got[0], want[0]) and same_bits(got[1], want[1])
+    cache.destroy()
+
+
 def test_recorded_step(device):
     """A replayed step gives the eager bits while lengths grow over page ends,
     with eager work between the replays."""
