@@ -387,9 +387,13 @@ int kva_get_weights_plan(const kva_cache *cache, int32_t *chunk_pages, int32_t *
  * their order.  A sequence of at most keep[b] rows keeps all of them.  The
  * rows become slots 0..keep-1 of dst_ids[b], in blocks of its own, and its
  * length; what it held goes.  dst_ids NULL, or the source itself: the source is
- * replaced (its blocks are released, in groups where the pool is short: the
- * largest of the sequences has to find its new blocks free; one that keeps all
- * its rows is left as it is); another sequence is a copy, the source stays.  Keys keep the positions that they were rotated
+ * replaced (one that keeps all its rows is left as it is); another sequence is a
+ * copy, the source stays.  A replaced source's blocks are released once its rows
+ * are copied, so a pool needs some free blocks to evict from: the sequences are
+ * taken by the blocks that they need, the fewest first, and each has to find
+ * its own among the free ones and those that earlier ones gave up (a copy's
+ * destination gives up its blocks before); else KVA_ERR_OUT_OF_BLOCKS and
+ * nothing changes.  Keys keep the positions that they were rotated
  * to, so the steps that follow pass rope_pos.  On an 8-bit cache the values held
  * are rounded once more, to their new page's scale.
  * weights: device fp32 [n_layers][n_seqs][num_kv_heads][w_stride]; kept:

@@ -1871,18 +1871,37 @@ int kva_evict(kva_cache *c, int32_t n_seqs, const int32_t *src_ids, const int32_
         longest = std::max(longest, len);
         most = std::max(most, n_keep[b]);
     }
-    int64_t free_blocks = static_cast<int64_t>(c->free_list.size()), held_back = 0;
+    // Blocks that the rows of sequence b which stay take.
+    auto need_of = [&](int32_t b) { return (static_cast<int64_t>(n_keep[b]) + kva::kBlockTokens - 1) / kva::kBlockTokens; };
+    // In an order that asks the least of the pool: copies for which their
+    // destination's own blocks do, sequences that are replaced (they give up as
+    // many as they take, or more) by the blocks that they need, other copies.
+    std::vector<int32_t> order;
+    order.reserve(n_seqs);
     for (int32_t b = 0; b < n_seqs; ++b) {
         const int32_t s = src_ids[b], d = dst_ids ? dst_ids[b] : s;
         if (int rc = check_seq(c, d)) return rc;
         if (d != s) {
             if (role[d]) return fail(KVA_ERR_INVALID_ARG, "sequence %d is listed twice or is another's source", d);
             role[d] = 2;
-            free_blocks += c->nblk[d];
         } else if (n_keep[b] == c->len[s]) {
             continue;  // nothing moves
         }
-        const int64_t need = (static_cast<int64_t>(n_keep[b]) + kva::kBlockTokens - 1) / kva::kBlockTokens;
+        order.push_back(b);
+    }
+    auto turn = [&](int32_t b) {
+        const int32_t s = src_ids[b], d = dst_ids ? dst_ids[b] : s;
+        return d == s ? need_of(b) : need_of(b) <= c->nblk[d] ? int64_t{-1} : INT64_MAX;
+    };
+    std::sort(order.begin(), order.end(), [&](int32_t x, int32_t y) {
+        const int64_t tx = turn(x), ty = turn(y);
+        return tx != ty ? tx < ty : x < y;
+    });
+    int64_t free_blocks = static_cast<int64_t>(c->free_list.size()), held_back = 0;
+    for (const int32_t b : order) {
+        const int32_t s = src_ids[b], d = dst_ids ? dst_ids[b] : s;
+        if (d != s) free_blocks += c->nblk[d];
+        const int64_t need = need_of(b);
         if (need > free_blocks) {  // the sequences before this one give up theirs first
             free_blocks += held_back;
             held_back = 0;
@@ -1904,7 +1923,7 @@ int kva_evict(kva_cache *c, int32_t n_seqs, const int32_t *src_ids, const int32_
     if (int rc = require_device(c)) return rc;
     // All that the work below appends to, so that none of it stops half way.
     size_t pages = 0;
-    for (int32_t b = 0; b < n_seqs; ++b) pages += (static_cast<size_t>(n_keep[b]) + kva::kBlockTokens - 1) / kva::kBlockTokens;
+    for (const int32_t b : order) pages += need_of(b);
     struct Replaced {  // a source and its new blocks, ids[first .. first + count)
         int32_t seq;
         size_t first, count;
@@ -2002,13 +2021,10 @@ int kva_evict(kva_cache *c, int32_t n_seqs, const int32_t *src_ids, const int32_
         recs.clear();
         return rc ? rc : flush_patches(c, s);
     };
-    for (int32_t b = 0; b < n_seqs; ++b) {
+    for (const int32_t b : order) {
         const int32_t src = src_ids[b], dst = dst_ids ? dst_ids[b] : src, n = n_keep[b];
-        if (dst != src)
-            release_blocks(c, dst);
-        else if (n == c->len[src])
-            continue;
-        const int32_t need = (n + kva::kBlockTokens - 1) / kva::kBlockTokens;
+        if (dst != src) release_blocks(c, dst);
+        const int32_t need = static_cast<int32_t>(need_of(b));
         if (static_cast<size_t>(need) > c->free_list.size() && (rc = run_group())) return rc;
         const size_t at0 = ids.size();
         for (int32_t i = 0; i < need; ++i) {

@@ -189,7 +189,8 @@ class PagedKVCache:
         first `first`, the latest `recent` and those of largest weight
         (kva_evict).  weights, weights_out [n_layers, n_seqs, Hkv, w_stride]
         fp32; kept [n_layers, n_seqs, Hkv, kept_stride] int32.  dst_ids: the
-        sequences that get them (by default the sources themselves).  Later
+        sequences that get them (by default the sources themselves: the pool
+        needs ceil(keep / 16) free blocks for the smallest of them).  Later
         steps pass rope_pos: slots are no positions any more."""
         if len(keep) != len(seq_ids) or (dst_ids is not None and len(dst_ids) != len(seq_ids)):
             raise ValueError("seq_ids, dst_ids and keep differ in length")

@@ -241,6 +241,24 @@ def test_evict_refuses():
     refused(NO_DEVICE, tight.evict, [0, 1], [40, 40], 16, 40, big, 40)
 
 
+def test_evict_does_not_depend_on_the_order_listed():
+    """A sequence that finds its blocks free gives up more of them than it takes."""
+    big = 1 << 20
+    args = dict(weights=16, w_stride=64, kept=big, kept_stride=40)
+    for seqs, keep in (([0, 1], [40, 20]), ([1, 0], [20, 40])):
+        c = make(max_blocks=10, max_step_tokens=128)
+        c.begin_step([0, 1], [64, 64])  # two blocks are free
+        refused(NO_DEVICE, c.evict, seqs, keep, **args)
+        refused(-4, c.evict, seqs, [40, 40], **args)
+    for seqs, keep, dst in (([0, 1], [20, 10], [0, 2]), ([1, 0], [10, 20], [2, 0])):
+        c = make(max_blocks=12, max_step_tokens=192)
+        c.begin_step([0, 1, 2], [64, 64, 48])  # one is free, and the copy takes two fewer than sequence 2 holds
+        refused(NO_DEVICE, c.evict, seqs, keep, dst_ids=dst, **args)
+        refused(-4, c.evict, [0], [20], **args)
+        c.begin_step([1], [1])  # none is free
+        refused(-4, c.evict, seqs, [k + 16 for k in keep], dst_ids=dst, **args)
+
+
 @pytest.mark.skipif(LIB_PATH.name == "libkvattn_san.so", reason="the sanitizer ends the process at such an allocation")
 def test_out_of_host_memory_is_an_error():
     """Tables of 4 PiB: the call answers, it does not end the process."""

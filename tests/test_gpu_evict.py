@@ -481,6 +481,35 @@ def test_evict(device, bits, where):
 
 
 @pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("turn", [1, -1])
+def test_evict_from_a_full_pool_in_any_order(device, bits, turn):
+    """Two free blocks: sequences that need four, three and two of them, and a copy
+    over a sequence that holds more than it gets, listed in either order."""
+    say(f"evict from a full pool {bits} {turn}")
+    rng = np.random.default_rng(18)
+    lens, kv, heads, layers = [120, 100, 90, 50, 64], 2, 4, 2
+    cache, data = _filled(device, lens, heads, kv, layers, bits, rng, spare=2)
+    assert cache.free_block_count() == 2
+    jobs = [(0, 0, 60), (1, 1, 40), (2, 2, 25), (3, 4, 20)][::turn]
+    src, dst, keep = (list(x) for x in zip(*jobs))
+    width, first, recent = max(lens), 3, 8
+    w = rng.exponential(size=(layers, len(jobs), kv, width)).astype(np.float32)
+    kept = device.empty((layers, len(jobs), kv, max(keep)), np.int32)
+    cache.evict(src, keep, device.array(w), width, kept, max(keep), first=first, recent=recent, dst_ids=dst)
+    device.synchronize()
+    for i in range(layers):
+        got, o = held(device, cache, dst, layer=i), 0
+        for j, (s, _, m) in enumerate(jobs):
+            places = [_stay(w[i, j, h], lens[s], m, first, recent) for h in range(kv)]
+            want = _moved(bits, data[i][s], places)
+            assert same_bits(got[0][o:o + m], want[0]) and same_bits(got[1][o:o + m], want[1]), (i, s)
+            o += m
+        stayed, want = held(device, cache, [3], layer=i), _values(bits, *data[i][3])
+        assert same_bits(stayed[0], want[0]) and same_bits(stayed[1], want[1]), "a copy's source stays"
+    cache.destroy()
+
+
+@pytest.mark.parametrize("bits", [8, 16])
 def test_evict_then_go_on(device, bits):
     """A prompt, the weights its last tokens give, eviction in place, then decode
     steps at their true positions, with the weights followed: every output and
