@@ -606,8 +606,10 @@ static int create_cache(const kva_config *cfg, kva_cache **made) {
         if ((e = hipMalloc(&c->d_proj, c->part_floats * sizeof(float))) != hipSuccess)
             return hip_fail(e, "hipMalloc(projection workspace)");
         for (int i = 0; i < kStageSlots; ++i) {
+            // Coherent by request, not by the environment's default: kva_evict's
+            // records are read from it by a kernel, and the slots are used again.
             if ((e = hipHostMalloc(reinterpret_cast<void **>(&c->h_stage[i]), c->stage_bytes,
-                                   hipHostMallocDefault)) != hipSuccess)
+                                   hipHostMallocCoherent)) != hipSuccess)
                 return hip_fail(e, "hipHostMalloc(staging)");
             if ((e = hipEventCreateWithFlags(&c->ev[i], hipEventDisableTiming)) != hipSuccess)
                 return hip_fail(e, "hipEventCreate");
