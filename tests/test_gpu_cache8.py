@@ -349,6 +349,66 @@ def test_prefill_of_two_row_tiles(device, heads, kv, base, new):
     cache.destroy()
 
 
+@pytest.mark.parametrize("heads,kv,base,new", [(24, 4, [0, 37, 300], [70, 9, 140]), (8, 8, [100, 7], [9, 5]),
+                                               (8, 1, [31, 0], [1, 33]), (24, 4, [16400], [181])], ids=str)
+@pytest.mark.parametrize("gated", [False, True])
+def test_append_prefill(device, heads, kv, base, new, gated):
+    """The one call against append and prefill, to the bit: output, query rows
+    and what the cache holds; k is only read.  RoPE positions other than the slots."""
+    say(f"append_prefill8 {heads}/{kv} {base} {new} {gated}")
+    rng = np.random.default_rng(heads + sum(new))
+    lens = [b + n for b, n in zip(base, new)]
+    seqs, T = list(range(len(lens))), sum(new)
+    tables = Tables(device, 32768)
+    ws = [device.array((1 + 0.02 * rng.standard_normal(D)).astype(np.float16)) for _ in range(2)]
+    before = [rows(rng, b, kv) for b in base]
+    q = rng.standard_normal((T, heads, D)).astype(np.float16)
+    k, v = rows(rng, T, kv)
+    gate = device.array(rng.standard_normal((T, heads, D)).astype(np.float16)) if gated else None
+    pos = [700 + p for b, n in zip(base, new) for p in range(b, b + n)]
+    got = []
+    for one in (False, True):
+        cache = make(lens, heads=heads, kv=kv, step=max(8192, sum(base)))
+        put(device, cache, seqs, [d[0] for d in before], [d[1] for d in before])
+        cache.begin_step(seqs, new, rope_pos=pos)
+        dq, dk, out = device.array(q), device.array(k), device.empty(q.shape, np.float16)
+        args = (dq, dk, device.array(v), *ws, tables.d_cos, tables.d_sin, tables.rows)
+        if one:
+            cache.append_prefill(0, *args, out, gate=gate)
+        else:
+            cache.append(0, *args)
+            cache.prefill(0, dq, out, gate=gate)
+        device.synchronize()
+        got.append([x.view(np.uint16) for x in (out.numpy(), dq.numpy(), *held(device, cache, seqs))])
+        if one:
+            assert np.array_equal(dk.numpy().view(np.uint16), k.view(np.uint16)), "k is only read"
+        cache.destroy()
+    assert all(np.array_equal(a, b) for a, b in zip(*got))
+
+
+def test_infinite_query(device):
+    """A query head with an infinite value has scores of +inf, or none but -inf:
+    its output is NaN, in every form of the decode and in a prefill, and no other's."""
+    say("infinite query 8")
+    rng = np.random.default_rng(19)
+    H, kv = 12, 2
+    for lens in ([5, 300, 16], [5, 1100, 4000], [20000, 31, 700]):
+        cache = make(lens, heads=H, kv=kv, extra=3, step=32768)
+        data = [rows(rng, n + 3, kv) for n in lens]
+        put(device, cache, [0, 1, 2], [d[0][:-3] for d in data], [d[1][:-3] for d in data])
+        for at, m in ((0, 1), (1, 2)):
+            put(device, cache, [0, 1, 2], *([d[j][len(d[j]) - 3 + at:][:m] for d in data] for j in (0, 1)))
+            q = rng.standard_normal((3 * m, H, D)).astype(np.float16)
+            q[0, 1, 7], q[m, 9, 200], q[2 * m, 4, 0] = np.inf, -np.inf, np.inf
+            out = device.empty(q.shape, np.float16)
+            (cache.decode if m == 1 else cache.prefill)(0, device.array(q), out)
+            device.synchronize()
+            want = np.zeros(q.shape, bool)
+            want[0, 1] = want[m, 9] = want[2 * m, 4] = True
+            assert np.array_equal(np.isnan(out.numpy()), want), (lens, m)
+        cache.destroy()
+
+
 def test_what_is_not_finite_reaches_only_who_sees_it(device):
     say("not finite in attention")
     rng = np.random.default_rng(9)
