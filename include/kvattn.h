@@ -71,7 +71,8 @@ enum {
  * sequence slot, KV head and layer), so codes depend on a page's rows alone,
  * not on the steps that they came in, and a step's append may be repeated.
  * Attention is over these values, in fp32 but for the probabilities, which
- * are fp16; gated, its output is rounded once, after the gate.
+ * are fp16 (one below 2^-25 of the largest may count as 0); gated, its output
+ * is rounded once, after the gate.
  * A row of a head in which K or V is not finite reads as NaN keys and zero
  * values, and once its page is full every row of that block has NaN keys:
  * attention that sees such a row gives NaN.  All calls of a step are the same
@@ -109,9 +110,13 @@ typedef struct kva_config {
     uint32_t flags;             /* KVA_FLAG_*                               */
 } kva_config;
 
-/* Byte layout of the pools, for callers that address rows themselves. */
+/* Byte layout of the pools, for callers that address rows themselves.  Of an
+ * 8-bit cache these are bytes of codes, no strides (a row's codes do not lie
+ * together), and not all that it holds: the scales are 8 bytes per block and KV
+ * head, the open blocks 32 KB per sequence slot and KV head, both per layer.   */
 typedef struct kva_layout {
-    uint64_t row_bytes;   /* one token, all KV heads: kv_heads*head_dim*2   */
+    uint64_t row_bytes;   /* one token, all KV heads: kv_heads*head_dim*2
+                             (8 bits: kv_heads*head_dim)                    */
     uint64_t block_bytes; /* block_tokens * row_bytes                       */
     uint64_t layer_bytes; /* max_blocks * block_bytes (per K or V pool)     */
     int32_t block_tokens;

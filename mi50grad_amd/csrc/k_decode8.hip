@@ -7,9 +7,13 @@
 // holds whole is written out, a cut one leaves partials for the merge.  Short
 // steps take a workgroup per sequence and KV head instead (whole8_kernel).
 //
-// What bounds it is HBM: 48 sequences of about 32000 rows (2.05 GB) take 355 us,
-// 5.8 TB/s; 32 of about 8000 (285 MB) 63 us, some 14 us of it the start (three
-// waits for memory in turn), the tail and the merge.
+// What bounds it is HBM: 48 sequences of 4096 to 32768 rows (20800 in the mean,
+// 2.05 GB) take 355 us, 5.8 TB/s; 32 of 1024 to 8192 (4300 in the mean, 285 MB)
+// 63 us, some 14 us of it the start (three waits for memory in turn), the tail
+// and the merge.  That is with four KV heads; a workgroup has a wave per KV head,
+// four at most, and its ring leaves room for one of four waves to a CU.  The 32
+// sequences with eight KV heads (two rounds of workgroups) take 115 us where their
+// bytes take 96, with two 44 (24), with one, a wave to a CU, 39 (12).
 //
 // A block is 8 KB in operand order, so a wave brings it in as eight 1 KB loads
 // that write LDS directly (and one of its scales), through a ring of its own:
@@ -59,7 +63,9 @@ __device__ __forceinline__ void reset(State &st) {
 }
 
 // Scores x (log2 units, masked ones -inf) of this lane's four rows to
-// probabilities as the B operand.
+// probabilities as the B operand.  They are rounded to FP16, which the products
+// take: with sums in FP32 over the rounded ones an output is off by 2.9e-4
+// (root mean square, relative), 2.1e-4 of it its own rounding to FP16.
 __device__ __forceinline__ half4_t fold_scores(State &st, const float4_t &x) {
     constexpr uint32_t kOnes = 0x3c003c00u;  // FP16 pair (1, 1)
     const float mx = group4_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));

@@ -21,11 +21,12 @@
 // sequence, so a ragged batch is shared out by its pages.
 //
 // A decode step is bound by HBM and by its start (dependent loads: the plan, the
-// page ids, the first keys): 32 sequences of about 8000 rows in 8 bits, 141 MB of
-// K, take 43 us in stats_kernel and 8 in
-// score_kernel; a walk of equal shares through LDS, as the 8-bit decode's, 45.
-// Many rows are bound by the vector unit and LDS: four sequences of about 13000
-// rows with 192 query rows, FP16, 43 us and 41 (the products alone would take 8).
+// page ids, the first keys): 32 sequences of 1024 to 8192 rows (5200 in the mean) in
+// 8 bits, 171 MB of K, take 42 us in stats_kernel and 8 in score_kernel; a walk of
+// equal shares through LDS, as the 8-bit decode's, took 45 in place of the 42.
+// Many rows are bound by the vector unit and LDS: four sequences of 9000 to 16000
+// rows (13300 in the mean) with 192 query rows, FP16, 40 us and 39 (the products
+// alone would take 8).
 #include <type_traits>
 
 #include "k_common.h"
@@ -642,7 +643,10 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(SelectArgs a) {
 
 // grid (record, KV head, layer), a half-wave per row of a destination page.  Bound
 // by memory: 200 MB of FP16 rows read here and there and written in order 79 us,
-// 5.1 TB/s.
+// 5.1 TB/s.  The same rows of an 8-bit cache, half the bytes, take 119 us: a row's
+// codes lie among those of its block's other rows (K's in pieces of 16 bytes, V's
+// one by one), so 100 MB of them fetch two to four times that, in loads of 8
+// bytes and of one.
 // Nothing that is read is written: destinations are other blocks than the
 // sources', and the last page of an 8-bit cache goes to the sequence's other open
 // block.

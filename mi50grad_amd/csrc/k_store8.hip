@@ -12,9 +12,11 @@
 // need no order, and an append that is called again gives the same.  Query rows
 // are normalised by further workgroups of the launch.
 //
-// Bound by latency for a decode step (a touch is one row: 5.5 us for 32 sequences)
-// and by memory for a prompt (7000 tokens, 43 MB read and written, 17 us; read
-// back 10).
+// Bound by latency: a decode step's touch is one row (5.5 us for 32 sequences); a
+// prompt's workgroups each wait in turn for their rows, three barriers and their
+// stores, 1.7 rounds of them for 7000 tokens (43 MB read and written, 17 us where
+// a copy takes 9).  LDS is busy for 5 of the 17, over half of that in bank
+// conflicts of V's codes, which go there one byte at a time.  Read back 10 us.
 #include "k_common.h"
 #include "k_normrope.h"
 #include "k_page8.h"
