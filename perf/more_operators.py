@@ -237,9 +237,11 @@ class _State:
 
 
 class _Memory:
-    """Device memory that torch may see without a copy."""
+    """Device memory that torch may see without a copy; a tensor made of it
+    keeps it, and it its owner."""
 
-    def __init__(self, ptr, shape, kind):
+    def __init__(self, owner, ptr, shape, kind):
+        self.owner = owner
         self.__cuda_array_interface__ = {"data": (ptr, False), "shape": shape, "typestr": kind, "version": 3}
 
 
@@ -308,7 +310,7 @@ def _own_prepare(s):
         s.cache.set_len(b, int(p.base[b]))
     s.cache.begin_step(range(len(p.new)), p.new, rope_pos=p.pos)
     s.q, s.gate = new(n, heads, D), new(n, heads, D)
-    s.k, s.v = (torch.as_tensor(_Memory(x, (p.pages * PAGE, kv, D), "<f2"), device="cuda")
+    s.k, s.v = (torch.as_tensor(_Memory(s.cache, x, (p.pages * PAGE, kv, D), "<f2"), device="cuda")
                 for x in s.cache.layer_pools(0))
 
 
