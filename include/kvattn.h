@@ -413,6 +413,68 @@ int kva_evict(kva_cache *cache, int32_t n_seqs, const int32_t *src_ids, const in
               float *weights_out, int64_t w_stride, int32_t *kept, int64_t kept_stride,
               kva_stream_t stream);
 
+/* ---- microscaled rows and products --------------------------------------- */
+/* A microscaled row is a row of blocks of 32 elements, each block with a scale
+ * byte b, its scale 2^(b-127) (255: the block is NaN).  An element has 8 bits
+ * (1 sign, 4 exponent bits of bias 7, 3 mantissa bits: up to 448) or 4 (1, 2 of
+ * bias 1, 1: 0, 0.5, 1, 1.5, 2, 3, 4, 6); rows are codes [rows][cols*bits/8],
+ * the even one of two 4-bit elements in a byte's low half, and scales
+ * [rows][cols/32].  Rows that these calls make have the smallest scale, from
+ * 2^-126 on, whose largest element covers the block's largest magnitude, and
+ * elements x/scale rounded to the nearest, ties to even; a block in which a
+ * value is not finite is NaN.  Rows from elsewhere in this format are taken as
+ * they are.  All of it but the products needs no cache and may be recorded
+ * into a graph.  Pointers are 16-byte aligned and, where nothing else is said,
+ * outputs overlap no operand (KVA_ERR_INVALID_ARG).  bits is 8 or 4
+ * (KVA_ERR_UNSUPPORTED).  The reference holds 4-bit weights for its other
+ * layers as integers with an fp16 scale per group (its GPTQ form); its
+ * attention projections are fp16.                                           */
+/* x [rows][cols] fp16, x_stride values between rows (a multiple of 8, at least
+ * cols), as microscaled rows.  cols a multiple of 32.                       */
+int kva_mx_quantize(const void *x, int64_t x_stride, int32_t rows, int32_t cols, int32_t bits,
+                    void *codes, void *scales, kva_stream_t stream);
+/* The values of microscaled rows, y [rows][cols] fp16: rounded to it, so exact
+ * but below 2^-24 (largest magnitudes above 65504 become infinite).         */
+int kva_mx_dequantize(const void *codes, const void *scales, int32_t rows, int32_t cols, int32_t bits,
+                      void *y, kva_stream_t stream);
+/* 4-bit weight rows in the order that the products read, made once per weight:
+ * kva_mx_packed_bytes bytes at `packed` (rows in tiles of 32, zeros behind the
+ * last).  cols a multiple of 512.                                           */
+int kva_mx_packed_bytes(int32_t rows, int32_t cols, size_t *bytes);
+int kva_mx_pack_weights(const void *codes, const void *scales, int32_t rows, int32_t cols, void *packed,
+                        kva_stream_t stream);
+/* The norm before a layer's projections, with the residual's addition: s =
+ * fp16(hidden + delta) to sum_out, and x = s / sqrt(mean(s^2) + eps) * w to
+ * out, in fp32 and rounded once: fp16 rows (bits 16, scales NULL) or
+ * microscaled ones.  hidden, delta, sum_out [n_tok][cols] fp16, w [cols] fp16
+ * (the 1+w stored norm weight).  delta and sum_out NULL: the norm of hidden.
+ * sum_out may be hidden or delta.  cols a multiple of 32, at most 32768.  The
+ * engine's own _launch_rmsnorm before _decode_full_attention, one launch for
+ * all rows (engine.py:3043-3139 launches it per token).                     */
+int kva_add_rmsnorm(const void *hidden, const void *delta, const void *w, int32_t n_tok, int32_t cols,
+                    float eps, int32_t bits, void *out, void *scales, void *sum_out, kva_stream_t stream);
+/* kva_project_append by 4-bit weights: the packed rows [Q; Q_gate] and [K; V]
+ * of w_q_fused and w_kv_fused there.  x is microscaled rows of `bits`, codes
+ * and x_scales (kva_add_rmsnorm's); with x_scales NULL fp16 rows [T][hidden],
+ * which the call takes to `bits` as kva_mx_quantize does.  A projected value
+ * is the fp32 sum of the elements' products, times both blocks' scales,
+ * rounded to fp16; the rest, and every output, as there.  No output overlaps
+ * an operand.  fp16 rows go through the cache's projection workspace.        */
+int kva_mx_project_append(kva_cache *cache, int32_t layer, const void *x, const void *x_scales,
+                          int32_t bits, int32_t hidden, const void *w_q_packed, const void *w_kv_packed,
+                          const void *q_norm_w, const void *k_norm_w, const void *cos_tab,
+                          const void *sin_tab, int32_t table_rows, void *q_out, void *q_gate_out,
+                          void *kv_out, kva_stream_t stream);
+/* kva_out_project by 4-bit weights: out[t] = fp16(attn[t] . W_o^T +
+ * residual[t]).  attn is fp16 rows [n_tok][q_dim], taken to `bits` on the way
+ * (attn_scales NULL), or microscaled rows.  residual NULL, apart from out, or
+ * out itself.  q_dim a multiple of 512, n_out of 16; a token's fp32 sums and
+ * its row have to fit the cache's projection workspace
+ * (KVA_ERR_INVALID_ARG).                                                    */
+int kva_mx_out_project(kva_cache *cache, const void *attn, const void *attn_scales, int32_t bits,
+                       int32_t n_tok, int32_t q_dim, const void *w_o_packed, int32_t n_out,
+                       const void *residual, void *out, kva_stream_t stream);
+
 /* Split-K tuning for kva_decode: tokens per split (multiple of 16); 0 =
  * automatic.  Automatic runs a step whose longest sequence is at most 1024
  * rows (over an 8-bit cache 512, or 1024 where n_seqs * num_kv_heads is at

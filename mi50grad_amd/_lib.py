@@ -80,6 +80,13 @@ SIGNATURES = {
     "kva_evict": [_P, _I, _PI, _PI, _PI, _I, _I, _P, _P, c_int64, _P, c_int64, _P],
     "kva_project_append": [_P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P],
     "kva_out_project": [_P, _P, _I, _I, _P, _I, _P, _P, _P],
+    "kva_mx_quantize": [_P, c_int64, _I, _I, _I, _P, _P, _P],
+    "kva_mx_dequantize": [_P, _P, _I, _I, _I, _P, _P],
+    "kva_mx_packed_bytes": [_I, _I, POINTER(c_size_t)],
+    "kva_mx_pack_weights": [_P, _P, _I, _I, _P, _P],
+    "kva_add_rmsnorm": [_P, _P, _P, _I, _I, c_float, _I, _P, _P, _P, _P],
+    "kva_mx_project_append": [_P, _I, _P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P],
+    "kva_mx_out_project": [_P, _P, _P, _I, _I, _I, _P, _I, _P, _P, _P],
     "kva_decode": [_P, _I, _P, _P, _P],
     "kva_decode_gated": [_P, _I, _P, _P, c_int64, _P, _P],
     "kva_append_decode": [_P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P],

@@ -345,10 +345,7 @@ bool plan_product(const ProjectArgs &a, bool heads, int n_cu, size_t part_floats
     return true;
 }
 
-hipError_t launch_project(ProjectArgs a, const ProductPlan &plan, hipStream_t s) {
-    if (a.n_tok <= 0) return hipSuccess;
-    const hipError_t e = launch_product(a, true, plan, s);
-    if (e != hipSuccess || !plan.partial) return e;
+hipError_t launch_project_finish(const ProjectArgs &a, hipStream_t s) {
     const int blocks_per_tok = (2 * a.num_heads + 2 * a.num_kv_heads + 7) / 8;
     const dim3 grid(static_cast<unsigned>(a.n_tok) * blocks_per_tok), block(256);
     if (a.splits <= 2) hipLaunchKernelGGL(proj_finish_kernel<2>, grid, block, 0, s, a);
@@ -357,17 +354,26 @@ hipError_t launch_project(ProjectArgs a, const ProductPlan &plan, hipStream_t s)
     return hipGetLastError();
 }
 
-hipError_t launch_out_project(ProjectArgs a, const ProductPlan &plan, hipStream_t s) {
+hipError_t launch_project(ProjectArgs a, const ProductPlan &plan, hipStream_t s) {
     if (a.n_tok <= 0) return hipSuccess;
-    if (a.n_b != 0 || a.n_a % 16 != 0) return hipErrorInvalidValue;
-    const hipError_t e = launch_product(a, false, plan, s);
-    if (e != hipSuccess || !plan.partial) return e;
+    const hipError_t e = launch_product(a, true, plan, s);
+    return e != hipSuccess || !plan.partial ? e : launch_project_finish(a, s);
+}
+
+hipError_t launch_out_finish(const ProjectArgs &a, hipStream_t s) {
     const int64_t threads = static_cast<int64_t>(a.n_tok) * (a.n_a / 8);
     const dim3 grid(static_cast<unsigned>((threads + 255) / 256)), block(256);
     if (a.splits <= 2) hipLaunchKernelGGL(oproj_finish_kernel<2>, grid, block, 0, s, a);
     else if (a.splits <= 4) hipLaunchKernelGGL(oproj_finish_kernel<4>, grid, block, 0, s, a);
     else hipLaunchKernelGGL(oproj_finish_kernel<kGemmMaxSplits>, grid, block, 0, s, a);
     return hipGetLastError();
+}
+
+hipError_t launch_out_project(ProjectArgs a, const ProductPlan &plan, hipStream_t s) {
+    if (a.n_tok <= 0) return hipSuccess;
+    if (a.n_b != 0 || a.n_a % 16 != 0) return hipErrorInvalidValue;
+    const hipError_t e = launch_product(a, false, plan, s);
+    return e != hipSuccess || !plan.partial ? e : launch_out_finish(a, s);
 }
 
 }  // namespace kva

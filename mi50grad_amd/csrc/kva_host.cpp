@@ -1305,6 +1305,90 @@ static int32_t tokens_per_launch(const kva_cache *c, const kva::ProjectArgs &a) 
     return static_cast<int32_t>(std::min<size_t>(fit, kva::kBigProjMaxTokens));
 }
 
+// The checks of a projection that its operands' form does not touch: hidden,
+// the RoPE tables, the step's positions.
+static int check_project(const kva_cache *c, int32_t hidden, const void *cos_tab, const void *sin_tab,
+                         int32_t table_rows) {
+    if (hidden <= 0 || hidden % kva::kProjHiddenQuantum != 0)
+        return fail(KVA_ERR_INVALID_ARG, "hidden %d must be a positive multiple of %d", hidden,
+                    kva::kProjHiddenQuantum);
+    if (static_cast<int64_t>(kva::kProjTokens) * hidden * 2 > INT32_MAX)
+        return fail(KVA_ERR_INVALID_ARG, "hidden %d too large", hidden);
+    if (c->cfg.rotary_dim > 0 &&
+        ((reinterpret_cast<uintptr_t>(cos_tab) | reinterpret_cast<uintptr_t>(sin_tab)) & 7u))
+        return fail(KVA_ERR_MISALIGNED, "cos/sin tables must be 8-byte aligned");
+    if (c->st_max_pos >= table_rows)
+        return fail(KVA_ERR_INVALID_ARG, "RoPE position %d beyond the %d table rows", c->st_max_pos,
+                    table_rows);
+    return KVA_OK;
+}
+
+// A projection's launch arguments but for its operands, plan and tokens.
+static kva::ProjectArgs project_args(const kva_cache *c, int32_t hidden, const void *q_norm_w, const void *k_norm_w,
+                                     const void *cos_tab, const void *sin_tab) {
+    kva::ProjectArgs a{};
+    a.n_a = 2 * c->cfg.num_heads * kva::kHeadDim;
+    a.n_b = 2 * c->cfg.num_kv_heads * kva::kHeadDim;
+    a.hidden = hidden;
+    a.part = c->d_proj;
+    a.q_w = static_cast<const uint16_t *>(q_norm_w);
+    a.k_w = static_cast<const uint16_t *>(k_norm_w);
+    a.cos_tab = static_cast<const uint16_t *>(cos_tab);
+    a.sin_tab = static_cast<const uint16_t *>(sin_tab);
+    a.table = c->d_table;
+    a.table_stride = c->cfg.max_blocks_per_seq;
+    a.num_heads = c->cfg.num_heads;
+    a.num_kv_heads = c->cfg.num_kv_heads;
+    a.half_rot = c->cfg.rotary_dim / 2;
+    a.eps = c->cfg.eps;
+    a.ev_before = c->kev_before;
+    a.ev_after = c->kev_after;
+    return a;
+}
+
+// The step's tokens through a projection, a.n_tok (the plan made for them) at a
+// time, and its rows into the cache.  launch(a, t0) takes a.n_tok tokens from
+// t0 on, planning anew where they are fewer.
+extern "C++" {
+template <class Launch>
+static int run_project(kva_cache *c, int32_t layer, kva::ProjectArgs &a, void *q_out, void *q_gate_out, void *kv_out,
+                       hipStream_t s, Launch launch) {
+    const size_t q_row = static_cast<size_t>(c->cfg.num_heads) * kva::kHeadDim,
+                 kv_row = 2 * static_cast<size_t>(c->cfg.num_kv_heads) * kva::kHeadDim;
+    // Onto an 8-bit cache the projection leaves its rows in token order (token t
+    // in slot t of a sequence whose i-th page is block i) and an append of rows
+    // takes them from there.
+    uint16_t *staged_v = c->int8 ? c->d_stage + static_cast<size_t>(c->cfg.max_step_tokens) * c->row_elems : nullptr;
+    a.k_pool = c->int8 ? c->d_stage : c->d_k + c->layer_elems * layer;
+    a.v_pool = c->int8 ? staged_v : c->d_v + c->layer_elems * layer;
+    if (c->int8) {
+        a.table = c->d_count;
+        a.table_stride = 0;
+    }
+    const int32_t per = a.n_tok;
+    for (int32_t t0 = 0; t0 < c->st_n_tok; t0 += per) {
+        a.q_out = static_cast<uint16_t *>(q_out) + t0 * q_row;
+        a.gate_out = q_gate_out ? static_cast<uint16_t *>(q_gate_out) + t0 * q_row : nullptr;
+        a.kv_out = kv_out ? static_cast<uint16_t *>(kv_out) + t0 * kv_row : nullptr;
+        a.tok_seq = at<int32_t>(c->d_step, c->off_tseq) + t0;
+        a.tok_slot = (c->int8 ? c->d_count : at<int32_t>(c->d_step, c->off_tslot)) + t0;
+        a.tok_pos = at<int32_t>(c->d_step, c->off_tpos) + t0;
+        a.n_tok = std::min(per, c->st_n_tok - t0);
+        KVA_HIP(launch(a, t0));
+    }
+    if (c->int8) {
+        kva::AppendArgs rows{};
+        rows.k = c->d_stage;
+        rows.v = staged_v;
+        rows.keep_k = 1;
+        set_append_plan(c, layer, rows);
+        KVA_HIP(launch_rows(c, layer, rows, false, s));
+    }
+    c->last_proj_path = c->st_n_tok > kva::kProjTokens ? KVA_PROJECT_PREFILL_GEMM : KVA_PROJECT_KERNELS;
+    return KVA_OK;
+}
+}  // extern "C++"
+
 static int project_impl(kva_cache *c, int32_t layer, const void *x, int32_t hidden, const void *w_q_fused,
                         const void *w_kv_fused, const void *q_norm_w, const void *k_norm_w, const void *cos_tab,
                         const void *sin_tab, int32_t table_rows, void *q_out, void *q_gate_out, void *kv_out,
@@ -1319,37 +1403,11 @@ static int project_impl(kva_cache *c, int32_t layer, const void *x, int32_t hidd
     if (!aligned16(x) || !aligned16(w_q_fused) || !aligned16(w_kv_fused) || !aligned16(q_norm_w) ||
         !aligned16(k_norm_w) || !aligned16(q_out) || !aligned16(q_gate_out) || !aligned16(kv_out))
         return fail(KVA_ERR_MISALIGNED, "x, weights, norm weights and outputs must be 16-byte aligned");
-    if (hidden <= 0 || hidden % kva::kProjHiddenQuantum != 0)
-        return fail(KVA_ERR_INVALID_ARG, "hidden %d must be a positive multiple of %d", hidden,
-                    kva::kProjHiddenQuantum);
-    if (static_cast<int64_t>(kva::kProjTokens) * hidden * 2 > INT32_MAX)
-        return fail(KVA_ERR_INVALID_ARG, "hidden %d too large", hidden);
-    const int half_rot = c->cfg.rotary_dim / 2;
-    if (half_rot > 0 && ((reinterpret_cast<uintptr_t>(cos_tab) | reinterpret_cast<uintptr_t>(sin_tab)) & 7u))
-        return fail(KVA_ERR_MISALIGNED, "cos/sin tables must be 8-byte aligned");
-    if (c->st_max_pos >= table_rows)
-        return fail(KVA_ERR_INVALID_ARG, "RoPE position %d beyond the %d table rows", c->st_max_pos,
-                    table_rows);
-    kva::ProjectArgs a{};
+    if ((rc = check_project(c, hidden, cos_tab, sin_tab, table_rows))) return rc;
+    kva::ProjectArgs a = project_args(c, hidden, q_norm_w, k_norm_w, cos_tab, sin_tab);
     a.w_a = static_cast<const uint16_t *>(w_q_fused);
     a.w_b = static_cast<const uint16_t *>(w_kv_fused);
-    a.n_a = 2 * c->cfg.num_heads * kva::kHeadDim;
-    a.n_b = 2 * c->cfg.num_kv_heads * kva::kHeadDim;
-    a.hidden = hidden;
     a.splits = project_splits(c, hidden, a.n_a + a.n_b);
-    a.part = c->d_proj;
-    a.q_w = static_cast<const uint16_t *>(q_norm_w);
-    a.k_w = static_cast<const uint16_t *>(k_norm_w);
-    a.cos_tab = static_cast<const uint16_t *>(cos_tab);
-    a.sin_tab = static_cast<const uint16_t *>(sin_tab);
-    a.table = c->d_table;
-    a.table_stride = c->cfg.max_blocks_per_seq;
-    a.num_heads = c->cfg.num_heads;
-    a.num_kv_heads = c->cfg.num_kv_heads;
-    a.half_rot = half_rot;
-    a.eps = c->cfg.eps;
-    a.ev_before = c->kev_before;
-    a.ev_after = c->kev_after;
     const size_t T = c->st_n_tok, q_row = static_cast<size_t>(c->cfg.num_heads) * kva::kHeadDim,
                  kv_row = 2 * static_cast<size_t>(c->cfg.num_kv_heads) * kva::kHeadDim, h = hidden;
     auto over_operand = [&](const void *out, size_t n) {
@@ -1357,47 +1415,357 @@ static int project_impl(kva_cache *c, int32_t layer, const void *x, int32_t hidd
                overlaps(out, n, w_kv_fused, a.n_b * h);
     };
     a.hold = over_operand(q_out, T * q_row) || over_operand(q_gate_out, T * q_row) || over_operand(kv_out, T * kv_row);
-    const int32_t per = tokens_per_launch(c, a);
-    a.n_tok = std::min(per, c->st_n_tok);
+    a.n_tok = std::min(tokens_per_launch(c, a), c->st_n_tok);
     kva::ProductPlan plan{};
     bool planned = kva::plan_product(a, true, c->n_cu, c->part_floats, plan);
+    int32_t planned_for = a.n_tok;
     c->last_product = plan;
     if ((rc = check_rows8_capture(c))) return rc;
     if ((rc = require_device(c))) return rc;
-    // Onto an 8-bit cache the projection leaves its rows in token order (token t
-    // in slot t of a sequence whose i-th page is block i) and an append of rows
-    // takes them from there.
-    uint16_t *staged_v = c->int8 ? c->d_stage + static_cast<size_t>(c->cfg.max_step_tokens) * c->row_elems : nullptr;
-    a.k_pool = c->int8 ? c->d_stage : c->d_k + c->layer_elems * layer;
-    a.v_pool = c->int8 ? staged_v : c->d_v + c->layer_elems * layer;
-    if (c->int8) {
-        a.table = c->d_count;
-        a.table_stride = 0;
-    }
-    for (int32_t t0 = 0; t0 < c->st_n_tok; t0 += per) {
-        a.x = static_cast<const uint16_t *>(x) + t0 * h;
-        a.q_out = static_cast<uint16_t *>(q_out) + t0 * q_row;
-        a.gate_out = q_gate_out ? static_cast<uint16_t *>(q_gate_out) + t0 * q_row : nullptr;
-        a.kv_out = kv_out ? static_cast<uint16_t *>(kv_out) + t0 * kv_row : nullptr;
-        a.tok_seq = at<int32_t>(c->d_step, c->off_tseq) + t0;
-        a.tok_slot = (c->int8 ? c->d_count : at<int32_t>(c->d_step, c->off_tslot)) + t0;
-        a.tok_pos = at<int32_t>(c->d_step, c->off_tpos) + t0;
-        if (const int32_t n = std::min(per, c->st_n_tok - t0); n != a.n_tok) {
-            a.n_tok = n;
-            planned = kva::plan_product(a, true, c->n_cu, c->part_floats, plan);
+    const auto s = static_cast<hipStream_t>(stream);
+    return run_project(c, layer, a, q_out, q_gate_out, kv_out, s, [&](kva::ProjectArgs &b, int32_t t0) {
+        b.x = static_cast<const uint16_t *>(x) + t0 * h;
+        if (b.n_tok != planned_for) {
+            planned_for = b.n_tok;
+            planned = kva::plan_product(b, true, c->n_cu, c->part_floats, plan);
         }
-        KVA_HIP(planned ? kva::launch_project(a, plan, static_cast<hipStream_t>(stream)) : hipErrorInvalidValue);
-    }
-    if (c->int8) {
-        kva::AppendArgs rows{};
-        rows.k = c->d_stage;
-        rows.v = staged_v;
-        rows.keep_k = 1;
-        set_append_plan(c, layer, rows);
-        KVA_HIP(launch_rows(c, layer, rows, false, static_cast<hipStream_t>(stream)));
-    }
-    c->last_proj_path = c->st_n_tok > kva::kProjTokens ? KVA_PROJECT_PREFILL_GEMM : KVA_PROJECT_KERNELS;
+        return planned ? kva::launch_project(b, plan, s) : hipErrorInvalidValue;
+    });
+}
+
+// ---- microscaled rows and products -----------------------------------------
+
+// Whether [p, p + n) and [q, q + m) have a byte in common (a null one has none).
+static bool bytes_overlap(const void *p, uint64_t n, const void *q, uint64_t m) {
+    const auto a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+    return p && q && a < b + m && b < a + n;
+}
+
+static uint64_t mx_code_bytes(uint64_t rows, uint64_t cols, int32_t bits) { return rows * (cols * bits / 8); }
+static uint64_t mx_scale_bytes(uint64_t rows, uint64_t cols) { return rows * (cols / kva::kMxBlock); }
+static uint64_t mx_packed_size(uint64_t rows, uint64_t cols) {
+    const uint64_t padded = (rows + kva::kMxWeightTile - 1) / kva::kMxWeightTile * kva::kMxWeightTile;
+    return mx_code_bytes(padded, cols, 4) + mx_scale_bytes(padded, cols);
+}
+
+static int check_mx_bits(int32_t bits) {
+    if (bits != 8 && bits != 4) return fail(KVA_ERR_UNSUPPORTED, "%d-bit elements: 8 or 4", bits);
     return KVA_OK;
+}
+
+static int check_mx_shape(int32_t rows, int32_t cols, int32_t quantum) {
+    if (rows < 0) return fail(KVA_ERR_INVALID_ARG, "%d rows", rows);
+    if (cols <= 0 || cols % quantum != 0)
+        return fail(KVA_ERR_INVALID_ARG, "%d columns: a positive multiple of %d", cols, quantum);
+    return KVA_OK;
+}
+
+// The activations of a product by packed weights: given as codes and scales, or
+// as fp16 rows that the call takes to `bits` first, into the front of the
+// projection workspace, as many tokens at a time as half of it holds.
+struct MxInput {
+    const void *x, *scales;
+    int32_t bits;
+    size_t cols;
+    bool coded() const { return scales != nullptr; }
+    size_t row_codes() const { return cols * bits / 8; }
+    uint64_t bytes(uint64_t n) const { return n * cols * (coded() ? bits : 16) / 8; }
+    size_t codes_size(size_t n) const { return round_up(n * row_codes(), 256); }
+    // Workspace floats that n tokens' codes and scales take.
+    size_t held_floats(size_t n) const {
+        return coded() ? 0 : (codes_size(n) + round_up(n * (cols / kva::kMxBlock), 256)) / sizeof(float);
+    }
+};
+
+// Tokens of a launch.
+static int32_t mx_tokens_per_launch(const kva_cache *c, const MxInput &in, int32_t n_rows, int32_t n_tok) {
+    size_t n = static_cast<size_t>(n_tok);
+    if (!in.coded())
+        n = std::min(n, (c->part_floats * sizeof(float) / 2 - std::min<size_t>(512, c->part_floats)) /
+                            (in.row_codes() + in.cols / kva::kMxBlock));
+    n = std::min(n, c->part_floats / 2 / static_cast<size_t>(n_rows));
+    return static_cast<int32_t>(n);
+}
+
+// Tokens [t0, t0 + a.n_tok) of a product: quantised where they come in fp16,
+// then multiplied and finished.  a.part and m.x are set for them.
+static hipError_t run_mx(const kva_cache *c, const MxInput &in, kva::ProjectArgs &a, kva::MxProduct &m, bool heads,
+                         const kva::ProductPlan &plan, int32_t t0, hipStream_t s) {
+    const size_t n = a.n_tok;
+    if (in.coded()) {
+        m.x = static_cast<const uint8_t *>(in.x) + t0 * in.row_codes();
+        m.x_scales = static_cast<const uint8_t *>(in.scales) + t0 * (in.cols / kva::kMxBlock);
+        a.part = c->d_proj;
+    } else {
+        kva::MxRows r{};
+        r.x = static_cast<const uint16_t *>(in.x) + t0 * in.cols;
+        r.x_stride = static_cast<int64_t>(in.cols);
+        r.rows = a.n_tok;
+        r.cols = static_cast<int32_t>(in.cols);
+        r.codes = reinterpret_cast<uint8_t *>(c->d_proj);
+        r.scales = r.codes + in.codes_size(n);
+        if (const hipError_t e = kva::launch_mx_quantize(r, in.bits, s); e != hipSuccess) return e;
+        m.x = r.codes;
+        m.x_scales = r.scales;
+        a.part = c->d_proj + in.held_floats(n);
+    }
+    return kva::launch_mx_product(a, m, heads, plan, s);
+}
+
+static int mx_project_impl(kva_cache *c, int32_t layer, const MxInput &in, const void *w_q, const void *w_kv,
+                           const void *q_norm_w, const void *k_norm_w, const void *cos_tab, const void *sin_tab,
+                           int32_t table_rows, void *q_out, void *q_gate_out, void *kv_out, kva_stream_t stream) {
+    if (!c) return fail(KVA_ERR_INVALID_ARG, "cache is NULL");
+    int rc = check_layer(c, layer);
+    if (rc) return rc;
+    if (!c->step_valid) return fail(KVA_ERR_STATE, "no step begun (kva_step_begin)");
+    if ((rc = check_mx_bits(in.bits))) return rc;
+    if (c->st_n_tok == 0) return require_device(c);
+    if (!in.x || !w_q || !w_kv || !q_norm_w || !k_norm_w || !cos_tab || !sin_tab || !q_out)
+        return fail(KVA_ERR_INVALID_ARG, "NULL tensor pointer");
+    if (!aligned16(in.x) || !aligned16(in.scales) || !aligned16(w_q) || !aligned16(w_kv) || !aligned16(q_norm_w) ||
+        !aligned16(k_norm_w) || !aligned16(q_out) || !aligned16(q_gate_out) || !aligned16(kv_out))
+        return fail(KVA_ERR_MISALIGNED, "x, scales, weights, norm weights and outputs must be 16-byte aligned");
+    const auto hidden = static_cast<int32_t>(in.cols);
+    if ((rc = check_project(c, hidden, cos_tab, sin_tab, table_rows))) return rc;
+    kva::ProjectArgs a = project_args(c, hidden, q_norm_w, k_norm_w, cos_tab, sin_tab);
+    const uint64_t T = c->st_n_tok, q_bytes = T * c->cfg.num_heads * kva::kHeadDim * 2,
+                   kv_bytes = T * 2 * c->cfg.num_kv_heads * kva::kHeadDim * 2;
+    auto over_operand = [&](const void *out, uint64_t n) {
+        return bytes_overlap(out, n, in.x, in.bytes(T)) || bytes_overlap(out, n, in.scales, mx_scale_bytes(T, in.cols)) ||
+               bytes_overlap(out, n, w_q, mx_packed_size(a.n_a, in.cols)) ||
+               bytes_overlap(out, n, w_kv, mx_packed_size(a.n_b, in.cols));
+    };
+    if (over_operand(q_out, q_bytes) || over_operand(q_gate_out, q_bytes) || over_operand(kv_out, kv_bytes))
+        return fail(KVA_ERR_INVALID_ARG, "an output overlaps an operand");
+    a.n_tok = mx_tokens_per_launch(c, in, a.n_a + a.n_b, c->st_n_tok);
+    kva::MxProduct m{};
+    m.w_a = static_cast<const uint8_t *>(w_q);
+    m.w_b = static_cast<const uint8_t *>(w_kv);
+    m.bits = in.bits;
+    kva::ProductPlan plan{};
+    int32_t planned_for = a.n_tok;
+    if (a.n_tok < 1 ||
+        !kva::plan_mx(a, m, true, c->n_cu, c->part_floats - in.held_floats(a.n_tok), plan))
+        return fail(KVA_ERR_INVALID_ARG, "hidden %d exceeds the projection workspace (%zu floats)", hidden,
+                    c->part_floats);
+    c->last_product = plan;
+    if ((rc = check_rows8_capture(c))) return rc;
+    if ((rc = require_device(c))) return rc;
+    const auto s = static_cast<hipStream_t>(stream);
+    return run_project(c, layer, a, q_out, q_gate_out, kv_out, s, [&](kva::ProjectArgs &b, int32_t t0) {
+        if (b.n_tok != planned_for) {
+            planned_for = b.n_tok;
+            if (!kva::plan_mx(b, m, true, c->n_cu, c->part_floats - in.held_floats(b.n_tok), plan))
+                return hipErrorInvalidValue;
+        }
+        return run_mx(c, in, b, m, true, plan, t0, s);
+    });
+}
+
+static int mx_out_impl(kva_cache *c, const MxInput &in, int32_t n_tok, const void *w_o, int32_t n_out,
+                       const void *residual, void *out, kva_stream_t stream) {
+    if (!c) return fail(KVA_ERR_INVALID_ARG, "cache is NULL");
+    int rc = check_mx_bits(in.bits);
+    if (rc) return rc;
+    if (n_tok < 0) return fail(KVA_ERR_INVALID_ARG, "n_tok %d is negative", n_tok);
+    if (n_tok == 0) return require_device(c);
+    if (!in.x || !w_o || !out) return fail(KVA_ERR_INVALID_ARG, "NULL tensor pointer");
+    if (!aligned16(in.x) || !aligned16(in.scales) || !aligned16(w_o) || !aligned16(residual) || !aligned16(out))
+        return fail(KVA_ERR_MISALIGNED, "attn, scales, w_o, residual and out must be 16-byte aligned");
+    const auto q_dim = static_cast<int32_t>(in.cols);
+    if (q_dim <= 0 || q_dim % kva::kProjHiddenQuantum != 0)
+        return fail(KVA_ERR_INVALID_ARG, "q_dim %d must be a positive multiple of %d", q_dim,
+                    kva::kProjHiddenQuantum);
+    if (static_cast<int64_t>(kva::kProjTokens) * q_dim * 2 > INT32_MAX)
+        return fail(KVA_ERR_INVALID_ARG, "q_dim %d too large", q_dim);
+    if (n_out <= 0 || n_out % 16 != 0)
+        return fail(KVA_ERR_INVALID_ARG, "n_out %d must be a positive multiple of 16", n_out);
+    if (static_cast<int64_t>(n_tok) * n_out > INT32_MAX)
+        return fail(KVA_ERR_INVALID_ARG, "n_tok x n_out too large");
+    const uint64_t out_bytes = static_cast<uint64_t>(n_tok) * n_out * 2;
+    if (bytes_overlap(out, out_bytes, in.x, in.bytes(n_tok)) ||
+        bytes_overlap(out, out_bytes, in.scales, mx_scale_bytes(n_tok, in.cols)) ||
+        bytes_overlap(out, out_bytes, w_o, mx_packed_size(n_out, in.cols)))
+        return fail(KVA_ERR_INVALID_ARG, "out overlaps an operand");
+    if (residual != out && bytes_overlap(out, out_bytes, residual, out_bytes))
+        return fail(KVA_ERR_INVALID_ARG, "out overlaps a part of residual: it may be residual itself");
+    kva::ProjectArgs a{};
+    a.n_a = n_out;
+    a.hidden = q_dim;
+    a.ev_before = c->kev_before;
+    a.ev_after = c->kev_after;
+    a.n_tok = mx_tokens_per_launch(c, in, n_out, n_tok);
+    kva::MxProduct m{};
+    m.w_a = m.w_b = static_cast<const uint8_t *>(w_o);
+    m.bits = in.bits;
+    kva::ProductPlan plan{};
+    int32_t planned_for = a.n_tok;
+    if (a.n_tok < 1 ||
+        !kva::plan_mx(a, m, false, c->n_cu, c->part_floats - in.held_floats(a.n_tok), plan))
+        return fail(KVA_ERR_INVALID_ARG, "q_dim %d to n_out %d exceeds the projection workspace (%zu floats)", q_dim,
+                    n_out, c->part_floats);
+    c->last_product = plan;
+    if ((rc = require_device(c))) return rc;
+    const auto s = static_cast<hipStream_t>(stream);
+    const int32_t per = a.n_tok;
+    for (int32_t t0 = 0; t0 < n_tok; t0 += per) {
+        const size_t at0 = static_cast<size_t>(t0) * n_out;
+        a.n_tok = std::min(per, n_tok - t0);
+        a.y_out = static_cast<uint16_t *>(out) + at0;
+        a.residual = residual ? static_cast<const uint16_t *>(residual) + at0 : nullptr;
+        if (a.n_tok != planned_for) {
+            planned_for = a.n_tok;
+            if (!kva::plan_mx(a, m, false, c->n_cu, c->part_floats - in.held_floats(a.n_tok), plan))
+                return hip_fail(hipErrorInvalidValue, "plan of a product");
+        }
+        KVA_HIP(run_mx(c, in, a, m, false, plan, t0, s));
+    }
+    return KVA_OK;
+}
+
+int kva_mx_packed_bytes(int32_t rows, int32_t cols, size_t *bytes) {
+    if (!bytes) return fail(KVA_ERR_INVALID_ARG, "bytes is NULL");
+    if (int rc = check_mx_shape(rows, cols, kva::kProjHiddenQuantum)) return rc;
+    *bytes = mx_packed_size(rows, cols);
+    return KVA_OK;
+}
+
+int kva_mx_quantize(const void *x, int64_t x_stride, int32_t rows, int32_t cols, int32_t bits, void *codes,
+                    void *scales, kva_stream_t stream) {
+    int rc = check_mx_bits(bits);
+    if (!rc) rc = check_mx_shape(rows, cols, kva::kMxBlock);
+    if (rc) return rc;
+    if (x_stride < cols || x_stride % 8 != 0)
+        return fail(KVA_ERR_INVALID_ARG, "x_stride %lld: at least cols and a multiple of 8",
+                    static_cast<long long>(x_stride));
+    if (rows == 0) return KVA_OK;
+    if (!x || !codes || !scales) return fail(KVA_ERR_INVALID_ARG, "NULL pointer");
+    if (!aligned16(x) || !aligned16(codes) || !aligned16(scales))
+        return fail(KVA_ERR_MISALIGNED, "x, codes and scales must be 16-byte aligned");
+    const uint64_t x_bytes = (static_cast<uint64_t>(rows - 1) * x_stride + cols) * 2;
+    if (bytes_overlap(codes, mx_code_bytes(rows, cols, bits), x, x_bytes) ||
+        bytes_overlap(scales, mx_scale_bytes(rows, cols), x, x_bytes) ||
+        bytes_overlap(codes, mx_code_bytes(rows, cols, bits), scales, mx_scale_bytes(rows, cols)))
+        return fail(KVA_ERR_INVALID_ARG, "x, codes and scales overlap");
+    kva::MxRows a{};
+    a.x = static_cast<const uint16_t *>(x);
+    a.x_stride = x_stride;
+    a.rows = rows;
+    a.cols = cols;
+    a.codes = static_cast<uint8_t *>(codes);
+    a.scales = static_cast<uint8_t *>(scales);
+    KVA_HIP(kva::launch_mx_quantize(a, bits, static_cast<hipStream_t>(stream)));
+    return KVA_OK;
+}
+
+int kva_mx_dequantize(const void *codes, const void *scales, int32_t rows, int32_t cols, int32_t bits, void *y,
+                      kva_stream_t stream) {
+    int rc = check_mx_bits(bits);
+    if (!rc) rc = check_mx_shape(rows, cols, kva::kMxBlock);
+    if (rc) return rc;
+    if (rows == 0) return KVA_OK;
+    if (!codes || !scales || !y) return fail(KVA_ERR_INVALID_ARG, "NULL pointer");
+    if (!aligned16(codes) || !aligned16(scales) || !aligned16(y))
+        return fail(KVA_ERR_MISALIGNED, "codes, scales and y must be 16-byte aligned");
+    const uint64_t y_bytes = static_cast<uint64_t>(rows) * cols * 2;
+    if (bytes_overlap(y, y_bytes, codes, mx_code_bytes(rows, cols, bits)) ||
+        bytes_overlap(y, y_bytes, scales, mx_scale_bytes(rows, cols)))
+        return fail(KVA_ERR_INVALID_ARG, "y overlaps codes or scales");
+    kva::MxRows a{};
+    a.rows = rows;
+    a.cols = cols;
+    a.codes = static_cast<uint8_t *>(const_cast<void *>(codes));    // only read
+    a.scales = static_cast<uint8_t *>(const_cast<void *>(scales));
+    a.y = static_cast<uint16_t *>(y);
+    KVA_HIP(kva::launch_mx_dequantize(a, bits, static_cast<hipStream_t>(stream)));
+    return KVA_OK;
+}
+
+int kva_mx_pack_weights(const void *codes, const void *scales, int32_t rows, int32_t cols, void *packed,
+                        kva_stream_t stream) {
+    if (int rc = check_mx_shape(rows, cols, kva::kProjHiddenQuantum)) return rc;
+    if (rows == 0) return KVA_OK;
+    if (!codes || !scales || !packed) return fail(KVA_ERR_INVALID_ARG, "NULL pointer");
+    if (!aligned16(codes) || !aligned16(scales) || !aligned16(packed))
+        return fail(KVA_ERR_MISALIGNED, "codes, scales and packed must be 16-byte aligned");
+    if (bytes_overlap(packed, mx_packed_size(rows, cols), codes, mx_code_bytes(rows, cols, 4)) ||
+        bytes_overlap(packed, mx_packed_size(rows, cols), scales, mx_scale_bytes(rows, cols)))
+        return fail(KVA_ERR_INVALID_ARG, "packed overlaps codes or scales");
+    kva::MxPack a{};
+    a.codes = static_cast<const uint8_t *>(codes);
+    a.scales = static_cast<const uint8_t *>(scales);
+    a.rows = rows;
+    a.n_tiles = (static_cast<int64_t>(rows) + kva::kMxWeightTile - 1) / kva::kMxWeightTile;
+    a.cols = cols;
+    a.packed = static_cast<uint8_t *>(packed);
+    KVA_HIP(kva::launch_mx_pack(a, static_cast<hipStream_t>(stream)));
+    return KVA_OK;
+}
+
+int kva_add_rmsnorm(const void *hidden, const void *delta, const void *w, int32_t n_tok, int32_t cols, float eps,
+                    int32_t bits, void *out, void *scales, void *sum_out, kva_stream_t stream) {
+    if (bits != 16)
+        if (int rc = check_mx_bits(bits)) return rc;
+    if (int rc = check_mx_shape(n_tok, cols, kva::kMxBlock)) return rc;
+    if (cols > kva::kMxNormMax) return fail(KVA_ERR_UNSUPPORTED, "%d columns: at most %d", cols, kva::kMxNormMax);
+    if (!(eps >= 0.0f)) return fail(KVA_ERR_INVALID_ARG, "eps %g", static_cast<double>(eps));
+    if (n_tok == 0) return KVA_OK;
+    if (!hidden || !w || !out) return fail(KVA_ERR_INVALID_ARG, "NULL pointer");
+    if ((bits == 16) != (scales == nullptr))
+        return fail(KVA_ERR_INVALID_ARG, "scales go with 8- and 4-bit rows, and only with them");
+    if ((delta == nullptr) != (sum_out == nullptr))
+        return fail(KVA_ERR_INVALID_ARG, "sum_out goes with delta, and only with it");
+    if (!aligned16(hidden) || !aligned16(delta) || !aligned16(w) || !aligned16(out) || !aligned16(scales) ||
+        !aligned16(sum_out))
+        return fail(KVA_ERR_MISALIGNED, "pointers must be 16-byte aligned");
+    const uint64_t n = static_cast<uint64_t>(n_tok) * cols, rows16 = 2 * n, out_bytes = mx_code_bytes(n_tok, cols, bits),
+                   scale_bytes = mx_scale_bytes(n_tok, cols), w_bytes = 2 * static_cast<uint64_t>(cols);
+    // A row is read whole before it is written: the sum may take the place of
+    // either term.
+    auto apart = [&](const void *p, uint64_t size, bool in_place) {
+        return !(bytes_overlap(p, size, hidden, rows16) && !(in_place && p == hidden)) &&
+               !(bytes_overlap(p, size, delta, rows16) && !(in_place && p == delta)) && !bytes_overlap(p, size, w, w_bytes);
+    };
+    if (!apart(sum_out, rows16, true) || !apart(out, out_bytes, false) || !apart(scales, scale_bytes, false) ||
+        bytes_overlap(out, out_bytes, sum_out, rows16) || bytes_overlap(out, out_bytes, scales, scale_bytes) ||
+        bytes_overlap(scales, scale_bytes, sum_out, rows16))
+        return fail(KVA_ERR_INVALID_ARG, "outputs overlap each other or an input");
+    kva::MxNorm a{};
+    a.hidden = static_cast<const uint16_t *>(hidden);
+    a.delta = static_cast<const uint16_t *>(delta);
+    a.sum_out = static_cast<uint16_t *>(sum_out);
+    a.w = static_cast<const uint16_t *>(w);
+    a.out = out;
+    a.scales = static_cast<uint8_t *>(scales);
+    a.n_tok = n_tok;
+    a.cols = cols;
+    a.eps = eps;
+    KVA_HIP(kva::launch_add_rmsnorm(a, bits, static_cast<hipStream_t>(stream)));
+    return KVA_OK;
+}
+
+int kva_mx_project_append(kva_cache *c, int32_t layer, const void *x, const void *x_scales, int32_t bits,
+                          int32_t hidden, const void *w_q_packed, const void *w_kv_packed, const void *q_norm_w,
+                          const void *k_norm_w, const void *cos_tab, const void *sin_tab, int32_t table_rows,
+                          void *q_out, void *q_gate_out, void *kv_out, kva_stream_t stream) {
+    int rc = capture_check(c, stream);
+    if (rc) return capture_note(c, rc);
+    const MxInput in{x, x_scales, bits, static_cast<size_t>(std::max(hidden, 0))};
+    rc = mx_project_impl(c, layer, in, w_q_packed, w_kv_packed, q_norm_w, k_norm_w, cos_tab, sin_tab, table_rows,
+                         q_out, q_gate_out, kv_out, stream);
+    if (rc == KVA_OK && c->capturing && c->st_n_tok > 0)
+        c->cap_table_rows = c->cap_table_rows ? std::min(c->cap_table_rows, table_rows) : table_rows;
+    return capture_note(c, rc);
+}
+
+int kva_mx_out_project(kva_cache *c, const void *attn, const void *attn_scales, int32_t bits, int32_t n_tok,
+                       int32_t q_dim, const void *w_o_packed, int32_t n_out, const void *residual, void *out,
+                       kva_stream_t stream) {
+    int rc = capture_check(c, stream);
+    if (rc) return capture_note(c, rc);
+    const MxInput in{attn, attn_scales, bits, static_cast<size_t>(std::max(q_dim, 0))};
+    return capture_note(c, mx_out_impl(c, in, n_tok, w_o_packed, n_out, residual, out, stream));
 }
 
 int kva_get_project_path(const kva_cache *c, int32_t *path) {

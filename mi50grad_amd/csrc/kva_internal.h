@@ -140,6 +140,57 @@ hipError_t launch_out_project(ProjectArgs a, const ProductPlan &plan, hipStream_
 constexpr int kBigProjMaxTokens = 1 << 24;
 bool plan_gemm(const ProjectArgs &a, bool heads, int n_cu, size_t part_floats, ProductPlan &plan);
 hipError_t launch_gemm_project(const ProjectArgs &a, bool heads, const ProductPlan &plan, hipStream_t s);
+// The finish kernels alone: a.part holds a.splits partials.
+hipError_t launch_project_finish(const ProjectArgs &a, hipStream_t s);
+hipError_t launch_out_finish(const ProjectArgs &a, hipStream_t s);
+
+// ---- microscaled rows and products (k_mx.hip, k_mxgemm.hip) ----
+
+constexpr int kMxBlock = 32;          // elements of a scale
+constexpr int kMxWeightTile = 32;     // rows of a packed weight's tile
+constexpr int kMxNormMax = 32768;     // values of a normalised row, at most
+struct MxRows {
+    const uint16_t *x;        // quantize: [rows] of x_stride values
+    int64_t x_stride;
+    int64_t rows;
+    int32_t cols;
+    uint8_t *codes;           // [rows][cols * bits / 8]
+    uint8_t *scales;          // [rows][cols / 32]
+    uint16_t *y;              // dequantize: [rows][cols]
+};
+hipError_t launch_mx_quantize(const MxRows &a, int bits, hipStream_t s);
+hipError_t launch_mx_dequantize(const MxRows &a, int bits, hipStream_t s);
+// A packed weight: codes [row tiles][cols / 64][64 lanes][16], then scales
+// [row tiles][cols / 256][64 lanes][4]: of lane l, row l % 32 of the tile, block
+// l / 32 of each step of 64; the dword has the bytes of four steps.
+struct MxPack {
+    const uint8_t *codes, *scales;  // 4-bit rows
+    int64_t rows, n_tiles;
+    int32_t cols;
+    uint8_t *packed;
+};
+hipError_t launch_mx_pack(const MxPack &a, hipStream_t s);
+struct MxNorm {
+    const uint16_t *hidden;   // [n_tok][cols]
+    const uint16_t *delta;    // nullable
+    uint16_t *sum_out;        // hidden + delta (with delta)
+    const uint16_t *w;        // [cols]
+    void *out;                // fp16 or codes
+    uint8_t *scales;
+    int32_t n_tok, cols;
+    float eps;
+};
+hipError_t launch_add_rmsnorm(const MxNorm &a, int bits, hipStream_t s);
+// The operands of a product by packed weights, beside ProjectArgs' outputs
+// (its x, w_a and w_b are not used; hidden, n_a, n_b and n_tok are).
+struct MxProduct {
+    const uint8_t *x, *x_scales;
+    const uint8_t *w_a, *w_b; // packed
+    int32_t bits;             // of x
+};
+bool plan_mx(const ProjectArgs &a, const MxProduct &m, bool heads, int n_cu, size_t part_floats, ProductPlan &plan);
+hipError_t launch_mx_product(const ProjectArgs &a, const MxProduct &m, bool heads, const ProductPlan &plan,
+                             hipStream_t s);
 
 // Reference-compatible norm+RoPE on a contiguous [n_heads][head_dim] buffer.
 struct LegacyNormArgs {
