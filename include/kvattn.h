@@ -457,9 +457,10 @@ int kva_add_rmsnorm(const void *hidden, const void *delta, const void *w, int32_
  * of w_q_fused and w_kv_fused there.  x is microscaled rows of `bits`, codes
  * and x_scales (kva_add_rmsnorm's); with x_scales NULL fp16 rows [T][hidden],
  * which the call takes to `bits` as kva_mx_quantize does.  A projected value
- * is the fp32 sum of the elements' products, times both blocks' scales,
- * rounded to fp16; the rest, and every output, as there.  No output overlaps
- * an operand.  fp16 rows go through the cache's projection workspace.        */
+ * is the fp32 sum of the elements' products, times both blocks' scales; it is
+ * rounded to fp16 once, Q and K after their norm and RoPE (in kv_out as
+ * projected); the rest, and every output, as there.  No output overlaps an
+ * operand.  fp16 rows go through the cache's projection workspace.           */
 int kva_mx_project_append(kva_cache *cache, int32_t layer, const void *x, const void *x_scales,
                           int32_t bits, int32_t hidden, const void *w_q_packed, const void *w_kv_packed,
                           const void *q_norm_w, const void *k_norm_w, const void *cos_tab,
@@ -468,8 +469,8 @@ int kva_mx_project_append(kva_cache *cache, int32_t layer, const void *x, const 
 /* kva_out_project by 4-bit weights: out[t] = fp16(attn[t] . W_o^T +
  * residual[t]).  attn is fp16 rows [n_tok][q_dim], taken to `bits` on the way
  * (attn_scales NULL), or microscaled rows.  residual NULL, apart from out, or
- * out itself.  q_dim a multiple of 512, n_out of 16; a token's fp32 sums and
- * its row have to fit the cache's projection workspace
+ * out itself.  q_dim a multiple of 512, n_out of 16; a token's microscaled
+ * row has to fit half of the cache's projection workspace
  * (KVA_ERR_INVALID_ARG).                                                    */
 int kva_mx_out_project(kva_cache *cache, const void *attn, const void *attn_scales, int32_t bits,
                        int32_t n_tok, int32_t q_dim, const void *w_o_packed, int32_t n_out,

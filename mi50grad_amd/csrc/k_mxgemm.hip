@@ -6,8 +6,14 @@
 // summed in fp32.  Lane l holds of A row l % 32's block l / 32 of a step of 64
 // (16 bytes), of an 8-bit B token l % 32's bytes 16 (l / 32) .. +15 of either
 // block (the instruction's order for 8 bits), of a 4-bit B its block l / 32,
-// and of both one scale byte, of block l / 32.
+// and of both one scale byte, of block l / 32; the result's register 4 q + j
+// is token l % 32's row 8 q + 4 (l / 32) + j.
+#include <algorithm>
+#include <iterator>
+#include <type_traits>
+
 #include "k_mx.h"
+#include "k_normrope.h"
 #include "kva_internal.h"
 
 namespace kva {
@@ -16,69 +22,543 @@ namespace {
 typedef int int8v_t __attribute__((ext_vector_type(8)));
 typedef float float16_t __attribute__((ext_vector_type(16)));
 
-constexpr int kMxWaves = 4;
-
-template <int BITS, int SEL>
-__device__ __forceinline__ float16_t mx_mfma(int8v_t w, int8v_t x, float16_t c, uint32_t ws, uint32_t xs) {
-    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, c, 4, BITS == 8 ? 0 : 4, SEL, ws, 0, xs);
-}
-
-// A wave takes 32 weight rows and 32 tokens, straight from memory, and leaves
-// fp32 partials [token][row] for a finish kernel.
-template <int BITS>
-__global__ __launch_bounds__(64 * kMxWaves) void mx_part_kernel(ProjectArgs a, MxProduct m) {
-    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
-    const int N = a.n_a + a.n_b;
-    const int n_rt = (N + 31) / 32, n_mt = (a.n_tok + 31) / 32;
-    const int tile = blockIdx.x * kMxWaves + (threadIdx.x >> 6);
-    if (tile >= n_rt * n_mt) return;
-    const int rt = tile / n_mt, mt = tile - rt * n_mt;
-    const int K = a.hidden, steps = K / 64;
-    const int rta = a.n_a / 32;
-    const bool first = rt < rta || a.n_b == 0;
-    const uint8_t *wp = first ? m.w_a : m.w_b;
-    const int64_t wt = first ? rt : rt - rta, w_tiles = ((first ? a.n_a : a.n_b) + 31) / 32;
-    const uint8_t *wc = wp + wt * steps * 1024 + 16 * lane;
-    const uint8_t *wsc = wp + w_tiles * 16 * K + wt * (steps / 4) * 256 + 4 * lane;
-    const int t = min(32 * mt + col, a.n_tok - 1);
-    const uint8_t *xc = m.x + static_cast<size_t>(t) * (K * BITS / 8) + 16 * half;
-    const uint8_t *xsc = m.x_scales + static_cast<size_t>(t) * (K / 32) + half;
-    float16_t acc = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    auto step = [&](auto sel, int s, uint32_t ws) {
-        const uint4 w = *reinterpret_cast<const uint4 *>(wc + 1024 * s);
-        const uint4 x0 = *reinterpret_cast<const uint4 *>(xc + (BITS == 8 ? 64 : 32) * s);
-        uint4 x1 = make_uint4(0, 0, 0, 0);
-        if constexpr (BITS == 8) x1 = *reinterpret_cast<const uint4 *>(xc + 64 * s + 32);
-        const uint32_t xs = xsc[2 * s];
-        const int8v_t wv = {static_cast<int>(w.x), static_cast<int>(w.y), static_cast<int>(w.z), static_cast<int>(w.w), 0, 0, 0, 0};
-        const int8v_t xv = {static_cast<int>(x0.x), static_cast<int>(x0.y), static_cast<int>(x0.z), static_cast<int>(x0.w),
-                            static_cast<int>(x1.x), static_cast<int>(x1.y), static_cast<int>(x1.z), static_cast<int>(x1.w)};
-        acc = mx_mfma<BITS, decltype(sel)::value>(wv, xv, acc, ws, xs);
-    };
-    for (int q = 0; q < steps / 4; ++q) {
-        const uint32_t ws = *reinterpret_cast<const uint32_t *>(wsc + 256 * q);
-        step(std::integral_constant<int, 0>{}, 4 * q, ws);
-        step(std::integral_constant<int, 1>{}, 4 * q + 1, ws);
-        step(std::integral_constant<int, 2>{}, 4 * q + 2, ws);
-        step(std::integral_constant<int, 3>{}, 4 * q + 3, ws);
+template <int BITS, int WSEL, int XSEL>
+__device__ __forceinline__ float16_t mx_mfma(uint4 w, const uint4 (&x)[BITS == 8 ? 2 : 1], float16_t c, uint32_t ws,
+                                             uint32_t xs) {
+    const int8v_t wv = {static_cast<int>(w.x), static_cast<int>(w.y), static_cast<int>(w.z), static_cast<int>(w.w), 0, 0, 0, 0};
+    int8v_t xv = {static_cast<int>(x[0].x), static_cast<int>(x[0].y), static_cast<int>(x[0].z), static_cast<int>(x[0].w), 0, 0, 0, 0};
+    if constexpr (BITS == 8) {
+        xv[4] = static_cast<int>(x[1].x);
+        xv[5] = static_cast<int>(x[1].y);
+        xv[6] = static_cast<int>(x[1].z);
+        xv[7] = static_cast<int>(x[1].w);
     }
-    if (32 * mt + col >= a.n_tok) return;
-    float *part = a.part + static_cast<size_t>(32 * mt + col) * N + 32 * rt + 4 * half;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (32 * rt + 8 * i + 4 * half < N)
-            *reinterpret_cast<float4_t *>(part + 8 * i) = float4_t{acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]};
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wv, xv, c, 4, BITS == 8 ? 0 : 4, WSEL, static_cast<int>(ws),
+                                                           XSEL, static_cast<int>(xs));
 }
+
+__device__ __forceinline__ uint4 rsrc_b128(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff) {
+    const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, 0);
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+__device__ __forceinline__ float16_t zero16() {
+    return float16_t{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+}
+
+// The packed weight that row tile `rt` of the stacked rows lies in, and its
+// place there.
+struct MxTileAt {
+    const uint8_t *codes, *scales;  // of the tile
+};
+__device__ __forceinline__ MxTileAt mx_tile_at(const ProjectArgs &a, const MxProduct &m, int rt) {
+    const int rta = a.n_a / kMxWeightTile;
+    const bool first = rt < rta || a.n_b == 0;
+    const uint8_t *w = first ? m.w_a : m.w_b;
+    const int64_t t = first ? rt : rt - rta;
+    const int64_t tiles = ((first ? a.n_a : a.n_b) + kMxWeightTile - 1) / kMxWeightTile;
+    return {w + t * 16 * a.hidden, w + tiles * 16 * a.hidden + t * a.hidden};
+}
+
+// ---- up to 32 tokens ---------------------------------------------------------
+
+constexpr int kMxStreamWaves = 8;
+
+// A workgroup takes RT row tiles over the whole of hidden, an eighth of it per
+// wave (hidden is a multiple of 512: whole steps), straight from memory into
+// registers; the waves' sums meet in LDS.  No k is split among workgroups, so
+// with EPI_OUT the result is finished here; else fp32 rows go to a finish
+// kernel.
+template <int BITS, int RT, bool EPI_OUT>
+__global__ __launch_bounds__(64 * kMxStreamWaves) void mx_stream_kernel(ProjectArgs a, MxProduct m) {
+    constexpr int C = 4;  // steps of a chunk
+    constexpr int XV = BITS == 8 ? 2 : 1;
+    __shared__ float4_t red[kMxStreamWaves][RT][4][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    const int N = a.n_a + a.n_b, K = a.hidden;
+    const int rt0 = blockIdx.x * RT, n_rt = (N + kMxWeightTile - 1) / kMxWeightTile;
+    const int n = K / (64 * kMxStreamWaves), s0 = wave * n;  // this wave's steps
+    __amdgpu_buffer_rsrc_t rw[RT], rs[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const MxTileAt at = mx_tile_at(a, m, min(rt0 + i, n_rt - 1));
+        const bool in = rt0 + i < n_rt;
+        rw[i] = ro_rsrc(at.codes, in ? 16u * K : 0u);
+        rs[i] = ro_rsrc(at.scales, in ? static_cast<uint32_t>(K) : 0u);
+    }
+    const uint32_t x_row = static_cast<uint32_t>(K) * BITS / 8, s_row = static_cast<uint32_t>(K) / 32;
+    const auto rx = ro_rsrc(m.x, a.n_tok * x_row), rxs = ro_rsrc(m.x_scales, a.n_tok * s_row);
+    const uint32_t xo = col * x_row + 16 * half, xso = col * s_row + half;
+
+    float16_t acc[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) acc[i] = zero16();
+    struct Chunk {
+        uint4 w[RT][C], x[C][XV];
+        uint32_t ws[RT][C], xs[C];
+    };
+    auto load = [&](Chunk &c, int s, int left) {
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            if (j >= left) break;
+            const int st = s + j;
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                c.w[i][j] = rsrc_b128(rw[i], 16 * lane, 1024 * st);
+                c.ws[i][j] = __builtin_amdgcn_raw_buffer_load_b8(rs[i], 4 * lane, (st >> 2) * 256 + (st & 3), 0);
+            }
+            c.x[j][0] = rsrc_b128(rx, xo, st * (8 * BITS));
+            if constexpr (BITS == 8) c.x[j][1] = rsrc_b128(rx, xo + 32, st * 64);
+            c.xs[j] = __builtin_amdgcn_raw_buffer_load_b8(rxs, xso, 2 * st, 0);
+        }
+    };
+    auto multiply = [&](const Chunk &c, int left) {
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            if (j >= left) break;
+#pragma unroll
+            for (int i = 0; i < RT; ++i) acc[i] = mx_mfma<BITS, 0, 0>(c.w[i][j], c.x[j], acc[i], c.ws[i][j], c.xs[j]);
+        }
+    };
+    Chunk c0, c1;
+    load(c0, s0, n);
+    for (int s = 0; s < n; s += 2 * C) {
+        if (s + C < n) load(c1, s0 + s + C, n - s - C);
+        multiply(c0, n - s);
+        if (s + C >= n) break;
+        if (s + 2 * C < n) load(c0, s0 + s + 2 * C, n - s - 2 * C);
+        multiply(c1, n - s - C);
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            red[wave][i][q][lane] = float4_t{acc[i][4 * q], acc[i][4 * q + 1], acc[i][4 * q + 2], acc[i][4 * q + 3]};
+    __syncthreads();
+    // Eight threads finish a token's 32 rows of a tile.
+    for (int f = threadIdx.x; f < RT * 256; f += 64 * kMxStreamWaves) {
+        const int i = f >> 8, t = (f >> 3) & 31, rq = f & 7;
+        if (t >= a.n_tok) continue;
+        const int from = t + 32 * (rq & 1);
+        float4_t sum = red[0][i][rq >> 1][from];
+#pragma unroll
+        for (int w = 1; w < kMxStreamWaves; ++w) sum += red[w][i][rq >> 1][from];
+        const int row = 32 * (rt0 + i) + 4 * rq;
+        if (row >= N) continue;
+        const size_t at = static_cast<size_t>(t) * N + row;
+        if constexpr (EPI_OUT) {
+            if (a.residual) {
+                const uint2 r = ld8(a.residual + at);
+                sum += float4_t{lo_f(r.x), hi_f(r.x), lo_f(r.y), hi_f(r.y)};
+            }
+            *reinterpret_cast<uint2 *>(a.y_out + at) = make_uint2(pack_h2(sum[0], sum[1]), pack_h2(sum[2], sum[3]));
+        } else {
+            *reinterpret_cast<float4_t *>(a.part + at) = sum;
+        }
+    }
+}
+
+// ---- tiles -------------------------------------------------------------------
+
+enum MxEpilogue {
+    kMxHead,  // a tile is a head's rows: norm + RoPE, outputs, cache rows
+    kMxOut,   // out = fp16(sum + residual)
+    kMxPart,  // fp32 partials [split][token][row] for a finish kernel
+};
+
+// A tile of BM tokens x BN weight rows over WM x WN waves and S LDS stages of
+// KC values of k.
+template <int BITS_, int BM_, int BN_, int WM_, int WN_, int S_>
+struct MxTile {
+    static constexpr int BITS = BITS_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, S = S_;
+    static constexpr int kWaves = WM * WN;
+    static constexpr int KC = BITS == 8 ? 128 : 256;  // a row's 128-byte line
+    static constexpr int SPC = KC / 64;               // steps of a stage
+    static constexpr int kTM = BM / WM / 32, kTN = BN / WN / 32;  // MFMA tiles of a wave
+    static constexpr int XV = BITS == 8 ? 2 : 1;      // 16-byte pieces of a token's step
+    static constexpr int kStageX = BM * 128, kStageW = BN / 32 * SPC * 1024;
+    static constexpr int kPlanes = KC / 128;          // dwords of a token's scales
+    static constexpr int kStageXs = kPlanes * BM * 4, kStageWs = BN / 32 * 256;
+    static constexpr int kStage = kStageX + kStageW + kStageXs + kStageWs;
+    static constexpr int kLoadsX = kStageX / 1024 / kWaves, kLoadsW = kStageW / 1024 / kWaves;
+    static constexpr int kSmallX = kStageXs / 256, kSmall = kSmallX + kStageWs / 256;
+    static constexpr int kLoadsS = (kSmall + kWaves - 1) / kWaves;
+    static constexpr int kLoads = kLoadsX + kLoadsW + kLoadsS;
+    static_assert(BM % (32 * WM) == 0 && BN % (32 * WN) == 0 && BM % 64 == 0, "whole MFMA tiles and loads");
+    static_assert(kLoadsX * kWaves * 1024 == kStageX && kLoadsW * kWaves * 1024 == kStageW, "whole loads per wave");
+    static_assert(S >= 2 && kLoads * (S - 1) < 64, "vmcnt is six bits");
+    static_assert(S * kStage + 256 + 4 * 4 * BM <= 160 * 1024, "the ring, a sink and the token facts fit the LDS");
+};
+
+// The granule swizzle of a row of 128 bytes: the 16 rows that 16 lanes read
+// at one granule fall in distinct 16-byte bank groups.
+__device__ __forceinline__ int mx_swizzle(int r) { return ((r >> 1) ^ ((r & 1) << 2)) & 7; }
+
+template <class T, int EPI>
+struct MxShared {
+    uint8_t ring[T::S * T::kStage];
+    uint8_t sink[256];  // of loads that a wave makes only to keep its count
+    int32_t meta[EPI == kMxHead ? 4 : 1][EPI == kMxHead ? T::BM : 1];
+};
+
+__device__ __forceinline__ void word_to_lds_at(__amdgpu_buffer_rsrc_t r, uint32_t lds, uint32_t voff, uint32_t soff) {
+    touch_line(r, lds, voff, soff);
+}
+
+// Workgroup i runs on XCD i % 8: deal each XCD a contiguous run of n tiles.
+__device__ __forceinline__ int mx_deal(int i, int n) {
+    const int xcd = i & 7, q8 = n >> 3, r8 = n & 7;
+    return xcd * q8 + min(xcd, r8) + (i >> 3);
+}
+
+template <class T, int EPI>
+__global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, MxProduct m) {
+    constexpr int kTM = T::kTM, kTN = T::kTN, SPC = T::SPC, BITS = T::BITS, XV = T::XV;
+    __shared__ __attribute__((aligned(16))) MxShared<T, EPI> sh;
+    const int N = a.n_a + a.n_b, K = a.hidden;
+    const int n_rt = (N + T::BN - 1) / T::BN, n_mt = (a.n_tok + T::BM - 1) / T::BM;
+    const int splits = EPI == kMxPart ? a.splits : 1;
+    const int tau = mx_deal(blockIdx.x, n_rt * splits * n_mt);
+    // Token tiles fastest, then row tiles, then splits.
+    const int ws_at = __builtin_amdgcn_readfirstlane(tau / n_mt);
+    const int mt = __builtin_amdgcn_readfirstlane(tau - ws_at * n_mt);
+    const int split = EPI == kMxPart ? __builtin_amdgcn_readfirstlane(ws_at / n_rt) : 0;
+    const int rt = ws_at - split * n_rt;
+    const int t0 = mt * T::BM, n0 = rt * T::BN;
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+
+    if constexpr (EPI == kMxHead) {
+        for (int i = threadIdx.x; i < T::BM; i += 64 * T::kWaves) {
+            const int t = min(t0 + i, a.n_tok - 1);
+            const int seq = a.tok_seq[t], slot = a.tok_slot[t];
+            sh.meta[0][i] = a.tok_pos[t];
+            sh.meta[1][i] = seq;
+            sh.meta[2][i] = slot;
+            sh.meta[3][i] = a.table[static_cast<size_t>(seq) * a.table_stride + (slot >> 4)];
+        }
+    }
+
+    // The operands as buffers: rows past the last token and tiles past the
+    // last weight row read as zeros.
+    const uint32_t x_row = static_cast<uint32_t>(K) * BITS / 8, s_row = static_cast<uint32_t>(K) / 32;
+    const uint32_t toks = static_cast<uint32_t>(max(0, min(T::BM, a.n_tok - t0)));
+    const MxTileAt at = mx_tile_at(a, m, n0 / 32);
+    const uint32_t tiles = static_cast<uint32_t>((min(T::BN, N - n0) + 31) / 32);
+    const auto rx = ro_rsrc(m.x + static_cast<size_t>(t0) * x_row, toks * x_row);
+    const auto rxs = ro_rsrc(m.x_scales + static_cast<size_t>(t0) * s_row, toks * s_row);
+    const auto rw = ro_rsrc(at.codes, tiles * 16u * K), rws = ro_rsrc(at.scales, tiles * static_cast<uint32_t>(K));
+    const auto none = ro_rsrc(m.x, 0u);
+    const uint32_t lds0 = lds_addr(sh.ring), sink = lds_addr(sh.sink);
+    const int nc_all = K / T::KC;
+    const int cb = EPI == kMxPart ? __builtin_amdgcn_readfirstlane(split * nc_all / splits) : 0;
+    const int nc = EPI == kMxPart ? __builtin_amdgcn_readfirstlane((split + 1) * nc_all / splits) - cb : nc_all;
+
+    uint32_t xoff[T::kLoadsX], woff[T::kLoadsW], soff[T::kLoadsS];
+#pragma unroll
+    for (int j = 0; j < T::kLoadsX; ++j) {
+        const int row = 8 * (T::kWaves * j + wv) + (lane >> 3);
+        xoff[j] = row * x_row + 16 * ((lane & 7) ^ mx_swizzle(row));
+    }
+#pragma unroll
+    for (int j = 0; j < T::kLoadsW; ++j) {
+        const int q = T::kWaves * j + wv;
+        woff[j] = (q / SPC) * 16u * K + (q % SPC) * 1024u + 16 * lane;
+    }
+#pragma unroll
+    for (int j = 0; j < T::kLoadsS; ++j) {
+        const int q = T::kWaves * j + wv;
+        soff[j] = q < T::kSmallX ? (64 * (q % (T::BM / 64)) + lane) * s_row + 4 * (q / (T::BM / 64))
+                                 : (q - T::kSmallX) * static_cast<uint32_t>(K) + 4 * lane;
+    }
+    // A chunk past the end goes through an empty buffer: the same loads, no
+    // memory access, so every wave's load counter advances alike.
+    auto issue = [&](int c) {
+        const bool on = c < nc;
+        const uint32_t k = static_cast<uint32_t>(on ? cb + c : 0);
+        const uint32_t st = lds0 + (c % T::S) * T::kStage;
+        const auto ax = on ? rx : none, aw = on ? rw : none;
+#pragma unroll
+        for (int j = 0; j < T::kLoadsX; ++j) load_to_lds_at(ax, st + 1024 * (T::kWaves * j + wv), xoff[j], k * 128);
+#pragma unroll
+        for (int j = 0; j < T::kLoadsW; ++j)
+            load_to_lds_at(aw, st + T::kStageX + 1024 * (T::kWaves * j + wv), woff[j], k * (SPC * 1024));
+#pragma unroll
+        for (int j = 0; j < T::kLoadsS; ++j) {
+            const int q = T::kWaves * j + wv;
+            const bool of_x = q < T::kSmallX, any = q < T::kSmall;
+            word_to_lds_at(!on || !any ? none : of_x ? rxs : rws,
+                           any ? st + T::kStageX + T::kStageW + 256 * q : sink, soff[j],
+                           __builtin_amdgcn_readfirstlane(of_x ? k * (T::KC / 32) : k * T::KC / 256 * 256));
+        }
+    };
+
+    const int wm = wv / T::WN, wn = wv % T::WN;
+    float16_t acc[kTM][kTN];
+#pragma unroll
+    for (int i = 0; i < kTM; ++i)
+#pragma unroll
+        for (int j = 0; j < kTN; ++j) acc[i][j] = zero16();
+
+    struct Step {
+        uint4 x[kTM][XV], w[kTN];
+    };
+    auto read = [&](Step &o, const uint8_t *st, int s) {
+#pragma unroll
+        for (int j = 0; j < kTN; ++j)
+            o.w[j] = *reinterpret_cast<const uint4 *>(st + T::kStageX + ((wn * kTN + j) * SPC + s) * 1024 + 16 * lane);
+#pragma unroll
+        for (int i = 0; i < kTM; ++i) {
+            const int row = (wm * kTM + i) * 32 + col;
+            const uint8_t *r = st + row * 128;
+            const int z = mx_swizzle(row);
+            if constexpr (BITS == 8) {
+                o.x[i][0] = *reinterpret_cast<const uint4 *>(r + 16 * ((4 * s + half) ^ z));
+                o.x[i][1] = *reinterpret_cast<const uint4 *>(r + 16 * ((4 * s + 2 + half) ^ z));
+            } else {
+                o.x[i][0] = *reinterpret_cast<const uint4 *>(r + 16 * ((2 * s + half) ^ z));
+            }
+        }
+    };
+    // A chunk's scales: of each token tile a dword per 128 k with the bytes of
+    // this lane's blocks at 0 and 2, of each row tile the bytes of four steps.
+    struct Scales {
+        uint32_t x[kTM][T::kPlanes], w[kTN];
+    };
+    auto read_scales = [&](Scales &o, const uint8_t *st, int c) {
+        const uint32_t *xs = reinterpret_cast<const uint32_t *>(st + T::kStageX + T::kStageW);
+        const uint32_t *wsc = reinterpret_cast<const uint32_t *>(st + T::kStageX + T::kStageW + T::kStageXs);
+#pragma unroll
+        for (int i = 0; i < kTM; ++i)
+#pragma unroll
+            for (int p = 0; p < T::kPlanes; ++p) o.x[i][p] = xs[p * T::BM + (wm * kTM + i) * 32 + col] >> (8 * half);
+#pragma unroll
+        for (int j = 0; j < kTN; ++j) {
+            o.w[j] = wsc[(wn * kTN + j) * 64 + lane];
+            if constexpr (T::KC == 128) o.w[j] >>= 16 * (c & 1);
+        }
+    };
+    auto multiply = [&](auto s, const Step &o, const Scales &sc) {
+        constexpr int kS = decltype(s)::value;
+#pragma unroll
+        for (int i = 0; i < kTM; ++i)
+#pragma unroll
+            for (int j = 0; j < kTN; ++j)
+                acc[i][j] = mx_mfma<BITS, kS, 2 * (kS & 1)>(o.w[j], o.x[i], acc[i][j], sc.w[j], sc.x[i][kS >> 1]);
+    };
+#pragma unroll
+    for (int s = 0; s < T::S; ++s) issue(s);
+    wait_vm<T::kLoads * (T::S - 1)>();
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    Step o0, o1;
+    Scales sc, sc_next;
+    read(o0, sh.ring, 0);
+    read_scales(sc, sh.ring, cb);
+    for (int c = 0; c < nc; ++c) {
+        const uint8_t *st = sh.ring + (c % T::S) * T::kStage;
+        auto one = [&](auto s, Step &now, Step &then) {
+            constexpr int kS = decltype(s)::value;
+            if constexpr (kS + 1 < SPC) {
+                read(then, st, kS + 1);
+            } else {
+                // This wave has read all of chunk c, and chunk c + 1 has landed.
+                wait_vm_lds<T::kLoads * (T::S - 2)>();
+                __builtin_amdgcn_s_barrier();
+                __builtin_amdgcn_sched_barrier(0);
+                issue(c + T::S);
+                const uint8_t *next = sh.ring + ((c + 1) % T::S) * T::kStage;
+                read(then, next, 0);
+                read_scales(sc_next, next, cb + c + 1);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(s, now, sc);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        one(std::integral_constant<int, 0>{}, o0, o1);
+        one(std::integral_constant<int, 1>{}, o1, o0);
+        if constexpr (SPC == 4) {
+            one(std::integral_constant<int, 2>{}, o0, o1);
+            one(std::integral_constant<int, 3>{}, o1, o0);
+        }
+        sc = sc_next;
+    }
+    // Every load (the dummy ones past the end too) has landed before the LDS
+    // is handed on.
+    __builtin_amdgcn_s_waitcnt(0);
+
+    if constexpr (EPI == kMxPart || EPI == kMxOut) {
+        float *part = EPI == kMxPart ? a.part + static_cast<size_t>(split) * a.n_tok * N : nullptr;
+#pragma unroll
+        for (int i = 0; i < kTM; ++i) {
+            const int t = t0 + (wm * kTM + i) * 32 + col;
+            if (t >= a.n_tok) continue;
+#pragma unroll
+            for (int j = 0; j < kTN; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int row = n0 + (wn * kTN + j) * 32 + 8 * q + 4 * half;
+                    if (row >= N) continue;
+                    float4_t v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                    const size_t o = static_cast<size_t>(t) * N + row;
+                    if constexpr (EPI == kMxPart) {
+                        *reinterpret_cast<float4_t *>(part + o) = v;
+                    } else {
+                        if (a.residual) {
+                            const uint2 r = ld8(a.residual + o);
+                            v += float4_t{lo_f(r.x), hi_f(r.x), lo_f(r.y), hi_f(r.y)};
+                        }
+                        *reinterpret_cast<uint2 *>(a.y_out + o) = make_uint2(pack_h2(v[0], v[1]), pack_h2(v[2], v[3]));
+                    }
+                }
+        }
+    } else {
+        static_assert(T::BN == kHeadDim, "a head tile holds whole heads");
+        constexpr int kRow = kHeadDim + 4;  // floats of a token's strip row, padded against bank conflicts
+        static_assert(32 * T::WM * kRow * 4 <= T::S * T::kStage, "a strip of tokens fits the ring");
+        __syncthreads();
+        const int head = rt, H = a.num_heads, hkv = a.num_kv_heads;
+        const int hw = threadIdx.x >> 5, l32 = threadIdx.x & 31;
+        const bool is_q = head < H, is_gate = !is_q && head < 2 * H;
+        const int kv = head - 2 * H;  // K heads 0..hkv-1, then V heads
+        const bool rot = is_q || (!is_gate && kv < hkv);
+        float *strip = reinterpret_cast<float *>(sh.ring);
+        const uint4 wnorm = rot ? ld16((is_q ? a.q_w : a.k_w) + 8 * l32) : make_uint4(0, 0, 0, 0);
+        const int cl = a.half_rot > 0 ? min(l32, a.half_rot / 4 - 1) : 0;
+        // 32 tokens of every wave row at a time, in fp32: Q and K are rounded
+        // once, after norm and RoPE.
+#pragma unroll
+        for (int i = 0; i < kTM; ++i) {
+#pragma unroll
+            for (int j = 0; j < kTN; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<float4_t *>(strip + (wm * 32 + col) * kRow + (wn * kTN + j) * 32 + 8 * q + 4 * half) =
+                        float4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+            __syncthreads();
+            for (int sr = hw; sr < 32 * T::WM; sr += 2 * T::kWaves) {
+                const int r = ((sr >> 5) * kTM + i) * 32 + (sr & 31);
+                const int t = t0 + r;
+                if (t >= a.n_tok) continue;
+                NormRopeIn nin;
+                nin.w = wnorm;
+                nin.c = nin.s = make_uint2(0, 0);
+                if (rot && a.half_rot > 0) {
+                    const size_t off = static_cast<size_t>(sh.meta[0][r]) * a.half_rot;
+                    nin.c = ld8(a.cos_tab + off + 4 * cl);
+                    nin.s = ld8(a.sin_tab + off + 4 * cl);
+                }
+                const float4_t lo = *reinterpret_cast<const float4_t *>(strip + sr * kRow + 8 * l32);
+                const float4_t hi = *reinterpret_cast<const float4_t *>(strip + sr * kRow + 8 * l32 + 4);
+                const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                const uint4 y = make_uint4(pack_h2(x[0], x[1]), pack_h2(x[2], x[3]), pack_h2(x[4], x[5]), pack_h2(x[6], x[7]));
+                if (is_gate) {
+                    if (a.gate_out) st16(a.gate_out + (static_cast<size_t>(t) * H + head - H) * kHeadDim + 8 * l32, y);
+                    continue;
+                }
+                if (!is_q && a.kv_out)
+                    st16(a.kv_out + (static_cast<size_t>(t) * 2 * hkv + kv) * kHeadDim + 8 * l32, y);
+                const uint4 o = rot ? norm_rope_apply<32>(x, nin, a.half_rot, a.eps, l32) : y;
+                if (is_q) {
+                    st16(a.q_out + (static_cast<size_t>(t) * H + head) * kHeadDim + 8 * l32, o);
+                    continue;
+                }
+                const size_t row_base = (static_cast<size_t>(sh.meta[3][r]) * kBlockTokens + (sh.meta[2][r] & 15)) * hkv;
+                if (kv < hkv)
+                    st16(a.k_pool + (row_base + kv) * kHeadDim + 8 * l32, o);
+                else
+                    st16(a.v_pool + (row_base + kv - hkv) * kHeadDim + 8 * l32, y);
+            }
+            __syncthreads();  // the strip is read before the next 32 tokens overwrite it
+        }
+    }
+}
+
+template <class T, int EPI>
+hipError_t launch_mx_gemm(const ProjectArgs &a, const MxProduct &m, hipStream_t s) {
+    const int n_rt = (a.n_a + a.n_b + T::BN - 1) / T::BN, n_mt = (a.n_tok + T::BM - 1) / T::BM;
+    const int splits = EPI == kMxPart ? a.splits : 1;
+    hipLaunchKernelGGL((mx_gemm_kernel<T, EPI>), dim3(n_rt * splits * n_mt), dim3(64 * T::kWaves), 0, s, a, m);
+    return hipGetLastError();
+}
+
+template <int BITS>
+hipError_t launch_mx_stream(const ProjectArgs &a, const MxProduct &m, bool heads, hipStream_t s) {
+    const int n_rt = (a.n_a + a.n_b + kMxWeightTile - 1) / kMxWeightTile;
+    const dim3 block(64 * kMxStreamWaves);
+    if (heads) hipLaunchKernelGGL((mx_stream_kernel<BITS, 2, false>), dim3((n_rt + 1) / 2), block, 0, s, a, m);
+    else hipLaunchKernelGGL((mx_stream_kernel<BITS, 1, true>), dim3(n_rt), block, 0, s, a, m);
+    return hipGetLastError();
+}
+
+// The tiles, and what 256 values of k of each take on a full chip (us).
+using MxLaunch = hipError_t (*)(const ProjectArgs &, const MxProduct &, hipStream_t);
+struct MxForm {
+    int bm, bn;
+    float us;
+    MxLaunch head, out, part;
+};
+template <int BITS, int BM, int BN, int WM, int WN, int S>
+constexpr MxForm mx_form(float us) {
+    using T = MxTile<BITS, BM, BN, WM, WN, S>;
+    MxForm f{BM, BN, us, nullptr, launch_mx_gemm<T, kMxOut>, launch_mx_gemm<T, kMxPart>};
+    if constexpr (BN == kHeadDim) f.head = launch_mx_gemm<T, kMxHead>;
+    return f;
+}
+const MxForm kForms8[] = {
+    mx_form<8, 256, 256, 2, 2, 3>(4.0f),
+    mx_form<8, 128, 256, 2, 2, 3>(2.2f),
+    mx_form<8, 64, 256, 1, 4, 4>(1.4f),
+    mx_form<8, 128, 128, 2, 2, 4>(1.3f),
+    mx_form<8, 64, 128, 1, 4, 4>(0.9f),
+};
+const MxForm kForms4[] = {
+    mx_form<4, 256, 256, 2, 2, 2>(2.8f),
+    mx_form<4, 128, 256, 2, 2, 3>(1.6f),
+    mx_form<4, 64, 256, 1, 4, 3>(1.2f),
+    mx_form<4, 128, 128, 2, 2, 4>(1.1f),
+    mx_form<4, 64, 128, 1, 4, 4>(0.8f),
+};
 
 }  // namespace
 
 bool plan_mx(const ProjectArgs &a, const MxProduct &m, bool heads, int n_cu, size_t part_floats, ProductPlan &plan) {
+    const int T = a.n_tok, N = a.n_a + a.n_b;
     plan = ProductPlan{};
-    plan.partial = true;
-    plan.splits = 1;
-    plan.bm = plan.bn = 32;
     plan.form = plan.pair = -1;
-    return static_cast<size_t>(a.n_tok) * (a.n_a + a.n_b) <= part_floats;
+    plan.splits = 1;
+    if (T <= kMxStreamTokens) {
+        plan.stream = true;
+        plan.partial = heads;
+        return !heads || static_cast<size_t>(T) * N <= part_floats;
+    }
+    const MxForm *forms = m.bits == 8 ? kForms8 : kForms4;
+    const int nc = a.hidden / 256;
+    double best_us = 0;
+    for (int i = 0; i < static_cast<int>(std::size(kForms8)); ++i) {
+        const MxForm &f = forms[i];
+        if (heads && a.n_a % f.bn != 0) continue;  // a tile never straddles the two weights
+        const double tiles = static_cast<double>((N + f.bn - 1) / f.bn) * ((T + f.bm - 1) / f.bm);
+        for (int splits = 1; splits <= kGemmMaxSplits && splits <= nc; ++splits) {
+            const bool partial = splits > 1 || (heads && !f.head);
+            const double part = static_cast<double>(splits) * T * N;
+            if (partial && part > static_cast<double>(part_floats)) break;
+            const double rounds = static_cast<double>((static_cast<int64_t>(tiles * splits) + n_cu - 1) / n_cu);
+            double us = rounds * (3.0 + (nc + splits - 1) / splits * f.us);
+            if (partial) us += 4.0 + 8.0 * part / 5.0e6;
+            if (plan.form < 0 || us < best_us) {
+                plan.form = i;
+                plan.splits = splits;
+                plan.partial = partial;
+                best_us = us;
+            }
+        }
+    }
+    if (plan.form < 0) return false;
+    plan.bm = forms[plan.form].bm;
+    plan.bn = forms[plan.form].bn;
+    return true;
 }
 
 hipError_t launch_mx_product(const ProjectArgs &args, const MxProduct &m, bool heads, const ProductPlan &plan,
@@ -87,14 +567,16 @@ hipError_t launch_mx_product(const ProjectArgs &args, const MxProduct &m, bool h
     a.splits = plan.splits;
     hipError_t e = a.ev_before ? hipEventRecord(a.ev_before, s) : hipSuccess;
     if (e != hipSuccess) return e;
-    const int64_t tiles = static_cast<int64_t>((a.n_a + a.n_b + 31) / 32) * ((a.n_tok + 31) / 32);
-    const dim3 grid(static_cast<unsigned>((tiles + kMxWaves - 1) / kMxWaves)), block(64 * kMxWaves);
-    if (m.bits == 8) hipLaunchKernelGGL(mx_part_kernel<8>, grid, block, 0, s, a, m);
-    else hipLaunchKernelGGL(mx_part_kernel<4>, grid, block, 0, s, a, m);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
+    if (plan.stream) {
+        e = m.bits == 8 ? launch_mx_stream<8>(a, m, heads, s) : launch_mx_stream<4>(a, m, heads, s);
+    } else {
+        const MxForm &f = (m.bits == 8 ? kForms8 : kForms4)[plan.form];
+        e = (plan.partial ? f.part : heads ? f.head : f.out)(a, m, s);
+    }
+    if (e != hipSuccess) return e;
     if (a.ev_after && (e = hipEventRecord(a.ev_after, s)) != hipSuccess) return e;
     if (!plan.partial) return hipSuccess;
-    return heads ? launch_project_finish(a, s) : launch_out_finish(a, s);
+    return heads ? launch_project_finish(a, true, s) : launch_out_finish(a, s);
 }
 
 }  // namespace kva

@@ -63,19 +63,13 @@ __device__ __forceinline__ void rope_in_flat(NormRopeIn &in, const uint16_t *__r
     in.s = ld8((rot ? sin_row : w) + 4 * cl);
 }
 
-// Normalise + rotate one row held as 8 fp16 per lane.  LANES = head_dim / 8
-// lanes take part (lane < LANES); the butterfly stays inside them.
+// Normalise + rotate one row held as 8 values per lane, rounded to fp16 at the
+// end.  LANES = head_dim / 8 lanes take part (lane < LANES); the butterfly
+// stays inside them.
 template <int LANES>
-__device__ __forceinline__ uint4 norm_rope_apply(uint4 xin, const NormRopeIn &in, int half_rot, float eps,
+__device__ __forceinline__ uint4 norm_rope_apply(const float (&x)[8], const NormRopeIn &in, int half_rot, float eps,
                                                  int lane) {
 #pragma clang fp contract(off)
-    const uint32_t xw[4] = {xin.x, xin.y, xin.z, xin.w};
-    float x[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        x[2 * i] = lo_f(xw[i]);
-        x[2 * i + 1] = hi_f(xw[i]);
-    }
     float s = x[0] * x[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) {
@@ -122,6 +116,15 @@ __device__ __forceinline__ uint4 norm_rope_apply(uint4 xin, const NormRopeIn &in
     y.z = pack_h2(n[4], n[5]);
     y.w = pack_h2(n[6], n[7]);
     return y;
+}
+
+// The same of fp16 values.
+template <int LANES>
+__device__ __forceinline__ uint4 norm_rope_apply(uint4 xin, const NormRopeIn &in, int half_rot, float eps,
+                                                 int lane) {
+    const float x[8] = {lo_f(xin.x), hi_f(xin.x), lo_f(xin.y), hi_f(xin.y),
+                        lo_f(xin.z), hi_f(xin.z), lo_f(xin.w), hi_f(xin.w)};
+    return norm_rope_apply<LANES>(x, in, half_rot, eps, lane);
 }
 
 template <int LANES>

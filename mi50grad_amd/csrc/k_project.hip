@@ -181,8 +181,9 @@ __global__ __launch_bounds__(64 * WAVES) void proj_lds_kernel(ProjectArgs a) {
 // group per head row.  Head rows of a token: H query, H gate, Hkv key, Hkv
 // value heads (the order of the weight rows).  The token's metadata and
 // page id are workgroup-uniform, read through the scalar cache while the
-// partials are in flight.
-template <int S>
+// partials are in flight.  ONCE: Q and K are normalised and rotated from the
+// fp32 sums and rounded at the end alone.
+template <int S, bool ONCE>
 __global__ __launch_bounds__(256) void proj_finish_kernel(ProjectArgs a) {
     const int H = a.num_heads, hkv = a.num_kv_heads;
     const int rows_per_tok = 2 * H + 2 * hkv;
@@ -220,22 +221,25 @@ __global__ __launch_bounds__(256) void proj_finish_kernel(ProjectArgs a) {
     rope_in_flat(nin, w, a.cos_tab + static_cast<size_t>(pos) * half_rot, a.sin_tab + static_cast<size_t>(pos) * half_rot,
                  half_rot, lane);
     const int blk = ld_uniform(a.table + static_cast<size_t>(seq) * stride + (slot >> 4));
-    uint4 y;
-    {
-        float4_t lo = plo[0], hi = phi[0];
+    float4_t lo = plo[0], hi = phi[0];
 #pragma unroll
-        for (int s = 1; s < S; ++s) {
-            lo = s < splits ? lo + plo[s] : lo;
-            hi = s < splits ? hi + phi[s] : hi;
-        }
-        y.x = pack_h2(lo[0], lo[1]);
-        y.y = pack_h2(lo[2], lo[3]);
-        y.z = pack_h2(hi[0], hi[1]);
-        y.w = pack_h2(hi[2], hi[3]);
+    for (int s = 1; s < S; ++s) {
+        lo = s < splits ? lo + plo[s] : lo;
+        hi = s < splits ? hi + phi[s] : hi;
     }
+    const float sums[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    uint4 y;
+    y.x = pack_h2(lo[0], lo[1]);
+    y.y = pack_h2(lo[2], lo[3]);
+    y.z = pack_h2(hi[0], hi[1]);
+    y.w = pack_h2(hi[2], hi[3]);
+    auto norm_rope = [&] {
+        if constexpr (ONCE) return norm_rope_apply<32>(sums, nin, a.half_rot, a.eps, lane);
+        else return norm_rope_apply<32>(y, nin, a.half_rot, a.eps, lane);
+    };
 
     if (hr < H) {
-        const uint4 q = norm_rope_apply<32>(y, nin, a.half_rot, a.eps, lane);
+        const uint4 q = norm_rope();
         st16(a.q_out + (static_cast<size_t>(t) * H + hr) * kHeadDim + 8 * lane, q);
         return;
     }
@@ -247,7 +251,7 @@ __global__ __launch_bounds__(256) void proj_finish_kernel(ProjectArgs a) {
     if (a.kv_out) st16(a.kv_out + (static_cast<size_t>(t) * 2 * hkv + kv) * kHeadDim + 8 * lane, y);
     const size_t row_base = (static_cast<size_t>(blk) * kBlockTokens + (slot & 15)) * hkv;
     if (kv < hkv) {
-        const uint4 k = norm_rope_apply<32>(y, nin, a.half_rot, a.eps, lane);
+        const uint4 k = norm_rope();
         st16(a.k_pool + (row_base + kv) * kHeadDim + 8 * lane, k);
     } else {
         st16(a.v_pool + (row_base + kv - hkv) * kHeadDim + 8 * lane, y);
@@ -345,19 +349,25 @@ bool plan_product(const ProjectArgs &a, bool heads, int n_cu, size_t part_floats
     return true;
 }
 
-hipError_t launch_project_finish(const ProjectArgs &a, hipStream_t s) {
+hipError_t launch_project_finish(const ProjectArgs &a, bool once, hipStream_t s) {
     const int blocks_per_tok = (2 * a.num_heads + 2 * a.num_kv_heads + 7) / 8;
     const dim3 grid(static_cast<unsigned>(a.n_tok) * blocks_per_tok), block(256);
-    if (a.splits <= 2) hipLaunchKernelGGL(proj_finish_kernel<2>, grid, block, 0, s, a);
-    else if (a.splits <= 4) hipLaunchKernelGGL(proj_finish_kernel<4>, grid, block, 0, s, a);
-    else hipLaunchKernelGGL(proj_finish_kernel<kGemmMaxSplits>, grid, block, 0, s, a);
+    if (once) {
+        if (a.splits <= 1) hipLaunchKernelGGL((proj_finish_kernel<1, true>), grid, block, 0, s, a);
+        else if (a.splits <= 4) hipLaunchKernelGGL((proj_finish_kernel<4, true>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((proj_finish_kernel<kGemmMaxSplits, true>), grid, block, 0, s, a);
+    } else {
+        if (a.splits <= 2) hipLaunchKernelGGL((proj_finish_kernel<2, false>), grid, block, 0, s, a);
+        else if (a.splits <= 4) hipLaunchKernelGGL((proj_finish_kernel<4, false>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((proj_finish_kernel<kGemmMaxSplits, false>), grid, block, 0, s, a);
+    }
     return hipGetLastError();
 }
 
 hipError_t launch_project(ProjectArgs a, const ProductPlan &plan, hipStream_t s) {
     if (a.n_tok <= 0) return hipSuccess;
     const hipError_t e = launch_product(a, true, plan, s);
-    return e != hipSuccess || !plan.partial ? e : launch_project_finish(a, s);
+    return e != hipSuccess || !plan.partial ? e : launch_project_finish(a, false, s);
 }
 
 hipError_t launch_out_finish(const ProjectArgs &a, hipStream_t s) {

@@ -1478,13 +1478,11 @@ struct MxInput {
 };
 
 // Tokens of a launch.
-static int32_t mx_tokens_per_launch(const kva_cache *c, const MxInput &in, int32_t n_rows, int32_t n_tok) {
-    size_t n = static_cast<size_t>(n_tok);
-    if (!in.coded())
-        n = std::min(n, (c->part_floats * sizeof(float) / 2 - std::min<size_t>(512, c->part_floats)) /
-                            (in.row_codes() + in.cols / kva::kMxBlock));
-    n = std::min(n, c->part_floats / 2 / static_cast<size_t>(n_rows));
-    return static_cast<int32_t>(n);
+static int32_t mx_tokens_per_launch(const kva_cache *c, const MxInput &in, int32_t n_tok) {
+    const auto n = static_cast<size_t>(std::min(n_tok, kva::kBigProjMaxTokens));
+    if (in.coded()) return static_cast<int32_t>(n);
+    const size_t room = c->part_floats * sizeof(float) / 2 - 512;  // less what the codes' and scales' ends are padded by
+    return static_cast<int32_t>(std::min(n, room / (in.row_codes() + in.cols / kva::kMxBlock)));
 }
 
 // Tokens [t0, t0 + a.n_tok) of a product: quantised where they come in fp16,
@@ -1538,7 +1536,7 @@ static int mx_project_impl(kva_cache *c, int32_t layer, const MxInput &in, const
     };
     if (over_operand(q_out, q_bytes) || over_operand(q_gate_out, q_bytes) || over_operand(kv_out, kv_bytes))
         return fail(KVA_ERR_INVALID_ARG, "an output overlaps an operand");
-    a.n_tok = mx_tokens_per_launch(c, in, a.n_a + a.n_b, c->st_n_tok);
+    a.n_tok = mx_tokens_per_launch(c, in, c->st_n_tok);
     kva::MxProduct m{};
     m.w_a = static_cast<const uint8_t *>(w_q);
     m.w_b = static_cast<const uint8_t *>(w_kv);
@@ -1595,7 +1593,7 @@ static int mx_out_impl(kva_cache *c, const MxInput &in, int32_t n_tok, const voi
     a.hidden = q_dim;
     a.ev_before = c->kev_before;
     a.ev_after = c->kev_after;
-    a.n_tok = mx_tokens_per_launch(c, in, n_out, n_tok);
+    a.n_tok = mx_tokens_per_launch(c, in, n_tok);
     kva::MxProduct m{};
     m.w_a = m.w_b = static_cast<const uint8_t *>(w_o);
     m.bits = in.bits;

@@ -140,14 +140,16 @@ hipError_t launch_out_project(ProjectArgs a, const ProductPlan &plan, hipStream_
 constexpr int kBigProjMaxTokens = 1 << 24;
 bool plan_gemm(const ProjectArgs &a, bool heads, int n_cu, size_t part_floats, ProductPlan &plan);
 hipError_t launch_gemm_project(const ProjectArgs &a, bool heads, const ProductPlan &plan, hipStream_t s);
-// The finish kernels alone: a.part holds a.splits partials.
-hipError_t launch_project_finish(const ProjectArgs &a, hipStream_t s);
+// The finish kernels alone: a.part holds a.splits partials.  once: Q and K are
+// rounded only after norm and RoPE.
+hipError_t launch_project_finish(const ProjectArgs &a, bool once, hipStream_t s);
 hipError_t launch_out_finish(const ProjectArgs &a, hipStream_t s);
 
 // ---- microscaled rows and products (k_mx.hip, k_mxgemm.hip) ----
 
 constexpr int kMxBlock = 32;          // elements of a scale
 constexpr int kMxWeightTile = 32;     // rows of a packed weight's tile
+constexpr int kMxStreamTokens = 32;   // most tokens of the form that streams the weights past them
 constexpr int kMxNormMax = 32768;     // values of a normalised row, at most
 struct MxRows {
     const uint16_t *x;        // quantize: [rows] of x_stride values

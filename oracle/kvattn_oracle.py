@@ -132,8 +132,14 @@ def qknorm_rope_exact(x: np.ndarray, w: np.ndarray, cos_rows: np.ndarray,
     x: [n, head_dim] fp16.  w: [head_dim] fp16.  cos_rows/sin_rows:
     [n, half_rotary] fp16 (the table row of each vector's position).
     """
-    x = np.asarray(x, dtype=np.float16)
-    n, d = x.shape
+    return qknorm_rope_f32(np.asarray(x, dtype=np.float16).astype(np.float32), w, cos_rows, sin_rows, eps)
+
+
+def qknorm_rope_f32(xf: np.ndarray, w: np.ndarray, cos_rows: np.ndarray, sin_rows: np.ndarray,
+                    eps: float = RMS_EPS) -> np.ndarray:
+    """qknorm_rope_exact of float32 rows (fp32 sums that are rounded only at the end)."""
+    xf = np.asarray(xf, dtype=np.float32)
+    n, d = xf.shape
     assert d % 8 == 0 and (d // 8) & (d // 8 - 1) == 0, "head_dim/8 must be a power of two"
     cos_rows = np.asarray(cos_rows, dtype=np.float16)
     sin_rows = np.asarray(sin_rows, dtype=np.float16)
@@ -141,7 +147,6 @@ def qknorm_rope_exact(x: np.ndarray, w: np.ndarray, cos_rows: np.ndarray,
     cos_rows = cos_rows.reshape(n, half)
     sin_rows = sin_rows.reshape(n, half)
     assert 2 * half <= d
-    xf = x.astype(np.float32)
     sq = (xf * xf).reshape(n, d // 8, 8)
     s = sq[:, :, 0].copy()
     for i in range(1, 8):

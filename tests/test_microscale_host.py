@@ -174,5 +174,4 @@ def test_out_beyond_the_workspace():
     refused(INVALID, out, c, n=3, q_dim=fit + 1024)
     refused(NO_DEVICE, out, c, n=3, q_dim=fit + 1024, scales=1 << 46)
     refused(NO_DEVICE, out, c, n=3, q_dim=fit + 1024, bits=4)
-    refused(INVALID, out, c, n=3, n_out=4 * 64 * 4 * 256 // 2 + 16)
     c.destroy()
