@@ -11,6 +11,7 @@
 #include <algorithm>
 #include <iterator>
 #include <type_traits>
+#include <utility>
 
 #include "k_mx.h"
 #include "k_normrope.h"
@@ -58,6 +59,23 @@ __device__ __forceinline__ MxTileAt mx_tile_at(const ProjectArgs &a, const MxPro
     const int64_t t = first ? rt : rt - rta;
     const int64_t tiles = ((first ? a.n_a : a.n_b) + kMxWeightTile - 1) / kMxWeightTile;
     return {w + t * 16 * a.hidden, w + tiles * 16 * a.hidden + t * a.hidden};
+}
+
+// On the lambdas of the main loop: one that stays a call puts the registers
+// that it refers to into memory.
+#define KVA_INLINE __attribute__((always_inline))
+
+template <int V>
+using Int = std::integral_constant<int, V>;
+
+// f(Int<FROM>), ..., f(Int<TO - 1>).
+template <int FROM, class F, int... I>
+__device__ __forceinline__ void each_of(const F &f, std::integer_sequence<int, I...>) {
+    (f(Int<FROM + I>{}), ...);
+}
+template <int FROM, int TO, class F>
+__device__ __forceinline__ void each(const F &f) {
+    each_of<FROM>(f, std::make_integer_sequence<int, TO - FROM>{});
 }
 
 // ---- up to 32 tokens ---------------------------------------------------------
@@ -180,15 +198,16 @@ struct MxTile {
     static constexpr int kStageX = BM * 128, kStageW = BN / 32 * SPC * 1024;
     static constexpr int kPlanes = KC / 128;          // dwords of a token's scales
     static constexpr int kStageXs = kPlanes * BM * 4, kStageWs = BN / 32 * 256;
-    static constexpr int kStage = kStageX + kStageW + kStageXs + kStageWs;
     static constexpr int kLoadsX = kStageX / 1024 / kWaves, kLoadsW = kStageW / 1024 / kWaves;
     static constexpr int kSmallX = kStageXs / 256, kSmall = kSmallX + kStageWs / 256;
     static constexpr int kLoadsS = (kSmall + kWaves - 1) / kWaves;
     static constexpr int kLoads = kLoadsX + kLoadsW + kLoadsS;
+    // With room for what the waves load only to keep their count.
+    static constexpr int kStage = kStageX + kStageW + kStageXs + kStageWs + (kSmall % kWaves ? 256 : 0);
     static_assert(BM % (32 * WM) == 0 && BN % (32 * WN) == 0 && BM % 64 == 0, "whole MFMA tiles and loads");
     static_assert(kLoadsX * kWaves * 1024 == kStageX && kLoadsW * kWaves * 1024 == kStageW, "whole loads per wave");
     static_assert(S >= 2 && kLoads * (S - 1) < 64, "vmcnt is six bits");
-    static_assert(S * kStage + 256 + 4 * 4 * BM <= 160 * 1024, "the ring, a sink and the token facts fit the LDS");
+    static_assert(S * kStage + 4 * 4 * BM <= 160 * 1024, "the ring and the token facts fit the LDS");
 };
 
 // The granule swizzle of a row of 128 bytes: the 16 rows that 16 lanes read
@@ -198,7 +217,6 @@ __device__ __forceinline__ int mx_swizzle(int r) { return ((r >> 1) ^ ((r & 1) <
 template <class T, int EPI>
 struct MxShared {
     uint8_t ring[T::S * T::kStage];
-    uint8_t sink[256];  // of loads that a wave makes only to keep its count
     int32_t meta[EPI == kMxHead ? 4 : 1][EPI == kMxHead ? T::BM : 1];
 };
 
@@ -246,16 +264,17 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
     const uint32_t toks = static_cast<uint32_t>(max(0, min(T::BM, a.n_tok - t0)));
     const MxTileAt at = mx_tile_at(a, m, n0 / 32);
     const uint32_t tiles = static_cast<uint32_t>((min(T::BN, N - n0) + 31) / 32);
-    const auto rx = ro_rsrc(m.x + static_cast<size_t>(t0) * x_row, toks * x_row);
-    const auto rxs = ro_rsrc(m.x_scales + static_cast<size_t>(t0) * s_row, toks * s_row);
-    const auto rw = ro_rsrc(at.codes, tiles * 16u * K), rws = ro_rsrc(at.scales, tiles * static_cast<uint32_t>(K));
-    const auto none = ro_rsrc(m.x, 0u);
-    const uint32_t lds0 = lds_addr(sh.ring), sink = lds_addr(sh.sink);
-    const int nc_all = K / T::KC;
-    const int cb = EPI == kMxPart ? __builtin_amdgcn_readfirstlane(split * nc_all / splits) : 0;
-    const int nc = EPI == kMxPart ? __builtin_amdgcn_readfirstlane((split + 1) * nc_all / splits) - cb : nc_all;
+    const uint8_t *const x_at = m.x + static_cast<size_t>(t0) * x_row;
+    const uint8_t *const xs_at = m.x_scales + static_cast<size_t>(t0) * s_row;
+    const uint32_t x_size = toks * x_row, w_size = tiles * 16u * K;
+    const uint32_t lds0 = lds_addr(sh.ring);
+    // This split's chunks: slices of hidden are whole 256s.
+    constexpr int kPer = 256 / T::KC;
+    const int nc_all = K / 256;
+    const int cb = EPI == kMxPart ? __builtin_amdgcn_readfirstlane(split * nc_all / splits) * kPer : 0;
+    const int nc = EPI == kMxPart ? __builtin_amdgcn_readfirstlane((split + 1) * nc_all / splits) * kPer - cb : nc_all * kPer;
 
-    uint32_t xoff[T::kLoadsX], woff[T::kLoadsW], soff[T::kLoadsS];
+    uint32_t xoff[T::kLoadsX], woff[T::kLoadsW];
 #pragma unroll
     for (int j = 0; j < T::kLoadsX; ++j) {
         const int row = 8 * (T::kWaves * j + wv) + (lane >> 3);
@@ -266,31 +285,40 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
         const int q = T::kWaves * j + wv;
         woff[j] = (q / SPC) * 16u * K + (q % SPC) * 1024u + 16 * lane;
     }
+    // A small load brings 64 dwords of scales: of 64 tokens, of a row tile, or
+    // none, where a wave loads only to keep its count.
+    const uint8_t *sm_at[T::kLoadsS];
+    uint32_t sm_size[T::kLoadsS], sm_step[T::kLoadsS], sm_off[T::kLoadsS];
 #pragma unroll
     for (int j = 0; j < T::kLoadsS; ++j) {
         const int q = T::kWaves * j + wv;
-        soff[j] = q < T::kSmallX ? (64 * (q % (T::BM / 64)) + lane) * s_row + 4 * (q / (T::BM / 64))
-                                 : (q - T::kSmallX) * static_cast<uint32_t>(K) + 4 * lane;
+        const bool of_x = q < T::kSmallX;
+        sm_at[j] = of_x ? xs_at : at.scales;
+        sm_size[j] = of_x ? toks * s_row : q < T::kSmall ? tiles * static_cast<uint32_t>(K) : 0u;
+        sm_step[j] = of_x ? T::KC / 32 : 256;
+        sm_off[j] = of_x ? (64 * (q % (T::BM / 64)) + lane) * s_row + 4 * (q / (T::BM / 64))
+                         : (q - T::kSmallX) * static_cast<uint32_t>(K) + 4 * lane;
     }
-    // A chunk past the end goes through an empty buffer: the same loads, no
-    // memory access, so every wave's load counter advances alike.
-    auto issue = [&](int c) {
+    // Piece j of the loads of chunk c (the k-th of hidden) into the stage at
+    // `st`.  A chunk past the end goes through empty buffers: the same loads,
+    // no memory access, so every wave's load counter advances alike.
+    auto load = [&](auto piece, int c, uint32_t st) KVA_INLINE {
+        constexpr int j = decltype(piece)::value;
         const bool on = c < nc;
-        const uint32_t k = static_cast<uint32_t>(on ? cb + c : 0);
-        const uint32_t st = lds0 + (c % T::S) * T::kStage;
-        const auto ax = on ? rx : none, aw = on ? rw : none;
-#pragma unroll
-        for (int j = 0; j < T::kLoadsX; ++j) load_to_lds_at(ax, st + 1024 * (T::kWaves * j + wv), xoff[j], k * 128);
-#pragma unroll
-        for (int j = 0; j < T::kLoadsW; ++j)
-            load_to_lds_at(aw, st + T::kStageX + 1024 * (T::kWaves * j + wv), woff[j], k * (SPC * 1024));
-#pragma unroll
-        for (int j = 0; j < T::kLoadsS; ++j) {
-            const int q = T::kWaves * j + wv;
-            const bool of_x = q < T::kSmallX, any = q < T::kSmall;
-            word_to_lds_at(!on || !any ? none : of_x ? rxs : rws,
-                           any ? st + T::kStageX + T::kStageW + 256 * q : sink, soff[j],
-                           __builtin_amdgcn_readfirstlane(of_x ? k * (T::KC / 32) : k * T::KC / 256 * 256));
+        const uint32_t k = on ? static_cast<uint32_t>(cb + c) : 0u;
+        if constexpr (j < T::kLoadsX) {
+            load_to_lds_at(ro_rsrc(x_at, on ? x_size + 0u : 0u), st + 1024 * (T::kWaves * j + wv), xoff[j], k * 128);
+        } else if constexpr (j < T::kLoadsX + T::kLoadsW) {
+            constexpr int i = j - T::kLoadsX;
+            load_to_lds_at(ro_rsrc(at.codes, on ? w_size + 0u : 0u), st + T::kStageX + 1024 * (T::kWaves * i + wv),
+                           woff[i], k * (SPC * 1024));
+        } else {
+            constexpr int i = j - T::kLoadsX - T::kLoadsW;
+            constexpr uint32_t kPer = 256 / T::KC;
+            const uint32_t steps = sm_step[i] == 256 ? k / kPer : k + 0u;
+            word_to_lds_at(ro_rsrc(sm_at[i], on ? sm_size[i] + 0u : 0u),
+                           st + T::kStageX + T::kStageW + 256 * min(T::kWaves * i + wv, T::kSmall), sm_off[i],
+                           __builtin_amdgcn_readfirstlane(steps * sm_step[i]));
         }
     };
 
@@ -301,88 +329,113 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
 #pragma unroll
         for (int j = 0; j < kTN; ++j) acc[i][j] = zero16();
 
+    // Operands are read from LDS a step ahead, and a chunk's scales with its
+    // first step's: of each token tile a dword per 128 k (its bytes 0 and 2,
+    // shifted by this lane's half), of each row tile the bytes of four steps.
+    constexpr int kReads = kTN + kTM * XV, kScaleReads = kTM * T::kPlanes + kTN;
     struct Step {
         uint4 x[kTM][XV], w[kTN];
     };
-    auto read = [&](Step &o, const uint8_t *st, int s) {
-#pragma unroll
-        for (int j = 0; j < kTN; ++j)
-            o.w[j] = *reinterpret_cast<const uint4 *>(st + T::kStageX + ((wn * kTN + j) * SPC + s) * 1024 + 16 * lane);
-#pragma unroll
-        for (int i = 0; i < kTM; ++i) {
-            const int row = (wm * kTM + i) * 32 + col;
-            const uint8_t *r = st + row * 128;
-            const int z = mx_swizzle(row);
-            if constexpr (BITS == 8) {
-                o.x[i][0] = *reinterpret_cast<const uint4 *>(r + 16 * ((4 * s + half) ^ z));
-                o.x[i][1] = *reinterpret_cast<const uint4 *>(r + 16 * ((4 * s + 2 + half) ^ z));
-            } else {
-                o.x[i][0] = *reinterpret_cast<const uint4 *>(r + 16 * ((2 * s + half) ^ z));
-            }
-        }
-    };
-    // A chunk's scales: of each token tile a dword per 128 k with the bytes of
-    // this lane's blocks at 0 and 2, of each row tile the bytes of four steps.
     struct Scales {
         uint32_t x[kTM][T::kPlanes], w[kTN];
     };
-    auto read_scales = [&](Scales &o, const uint8_t *st, int c) {
-        const uint32_t *xs = reinterpret_cast<const uint32_t *>(st + T::kStageX + T::kStageW);
-        const uint32_t *wsc = reinterpret_cast<const uint32_t *>(st + T::kStageX + T::kStageW + T::kStageXs);
-#pragma unroll
-        for (int i = 0; i < kTM; ++i)
-#pragma unroll
-            for (int p = 0; p < T::kPlanes; ++p) o.x[i][p] = xs[p * T::BM + (wm * kTM + i) * 32 + col] >> (8 * half);
-#pragma unroll
-        for (int j = 0; j < kTN; ++j) {
-            o.w[j] = wsc[(wn * kTN + j) * 64 + lane];
-            if constexpr (T::KC == 128) o.w[j] >>= 16 * (c & 1);
+    auto read = [&](auto piece, Step &o, const uint8_t *st, int s) KVA_INLINE {
+        constexpr int p = decltype(piece)::value;
+        if constexpr (p < kTN) {
+            o.w[p] = *reinterpret_cast<const uint4 *>(st + T::kStageX + ((wn * kTN + p) * SPC + s) * 1024 + 16 * lane);
+        } else {
+            constexpr int i = (p - kTN) / XV, v = (p - kTN) % XV;
+            const int row = (wm * kTM + i) * 32 + col;
+            const int g = BITS == 8 ? 4 * s + 2 * v + half : 2 * s + half;
+            o.x[i][v] = *reinterpret_cast<const uint4 *>(st + row * 128 + 16 * (g ^ mx_swizzle(row)));
         }
     };
-    auto multiply = [&](auto s, const Step &o, const Scales &sc) {
-        constexpr int kS = decltype(s)::value;
-#pragma unroll
-        for (int i = 0; i < kTM; ++i)
-#pragma unroll
-            for (int j = 0; j < kTN; ++j)
-                acc[i][j] = mx_mfma<BITS, kS, 2 * (kS & 1)>(o.w[j], o.x[i], acc[i][j], sc.w[j], sc.x[i][kS >> 1]);
+    auto read_scale = [&](auto piece, Scales &o, const uint8_t *st) KVA_INLINE {
+        constexpr int p = decltype(piece)::value;
+        const uint32_t *xs = reinterpret_cast<const uint32_t *>(st + T::kStageX + T::kStageW);
+        if constexpr (p < kTN) {
+            o.w[p] = xs[T::kStageXs / 4 + (wn * kTN + p) * 64 + lane];
+        } else {
+            constexpr int i = (p - kTN) / T::kPlanes, pl = (p - kTN) % T::kPlanes;
+            o.x[i][pl] = xs[pl * T::BM + (wm * kTM + i) * 32 + col];
+        }
     };
+    // A step's products, with hook(k) after the k-th: what the wave issues
+    // there runs under the products instead of between two steps.
+    constexpr int kProducts = kTM * kTN;
+    auto multiply = [&](auto s, auto ws, const Step &o, const Scales &sc, const auto &hook) KVA_INLINE {
+        constexpr int kS = decltype(s)::value, kWs = decltype(ws)::value;
+        each<0, kProducts>([&](auto k) KVA_INLINE {
+            constexpr int i = decltype(k)::value / kTN, j = decltype(k)::value % kTN;
+            acc[i][j] = mx_mfma<BITS, kWs, 2 * (kS & 1)>(o.w[j], o.x[i], acc[i][j], sc.w[j], sc.x[i][kS >> 1]);
+            hook(k);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    // What comes after product k of n pieces spread over the first `over`.
+    auto spread = [](auto k, auto n, auto over, const auto &piece) KVA_INLINE {
+        constexpr int kK = decltype(k)::value, kN = decltype(n)::value, kOver = decltype(over)::value;
+        if constexpr (kK < kOver) each<kN * kK / kOver, kN * (kK + 1) / kOver>(piece);
+    };
+    // Reads come early, so that the last has arrived when its step begins.
+    using Early = Int<kProducts - kProducts / 4>;
+    using Whole = Int<kProducts>;
 #pragma unroll
-    for (int s = 0; s < T::S; ++s) issue(s);
+    for (int s = 0; s < T::S; ++s) each<0, T::kLoads>([&](auto j) KVA_INLINE { load(j, s, lds0 + s * T::kStage); });
     wait_vm<T::kLoads * (T::S - 1)>();
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
     Step o0, o1;
-    Scales sc, sc_next;
-    read(o0, sh.ring, 0);
-    read_scales(sc, sh.ring, cb);
-    for (int c = 0; c < nc; ++c) {
-        const uint8_t *st = sh.ring + (c % T::S) * T::kStage;
-        auto one = [&](auto s, Step &now, Step &then) {
+    Scales sc0, sc1;
+    each<0, kReads>([&](auto p) KVA_INLINE { read(p, o0, sh.ring, 0); });
+    each<0, kScaleReads>([&](auto p) KVA_INLINE { read_scale(p, sc0, sh.ring); });
+    uint32_t at0 = 0;  // this chunk's stage
+    // One chunk; PART: its place among the chunks that share a dword of weight scales.
+    auto chunk = [&](auto part, int c, Scales &sc, Scales &sc_next) KVA_INLINE {
+        constexpr int kPart = decltype(part)::value;
+        const uint32_t at1 = at0 + T::kStage == T::S * T::kStage ? 0 : at0 + T::kStage;
+        const uint8_t *st = sh.ring + at0, *next = sh.ring + at1;
+#pragma unroll
+        for (int i = 0; i < kTM; ++i)
+#pragma unroll
+            for (int p = 0; p < T::kPlanes; ++p) sc.x[i][p] >>= 8 * half;
+        auto one = [&](auto s, Step &now, Step &then) KVA_INLINE {
             constexpr int kS = decltype(s)::value;
+            using Ws = Int<kPart * SPC + kS>;
             if constexpr (kS + 1 < SPC) {
-                read(then, st, kS + 1);
+                multiply(s, Ws{}, now, sc, [&](auto k) KVA_INLINE { spread(k, Int<kReads>{}, Early{}, [&](auto p) KVA_INLINE { read(p, then, st, kS + 1); }); });
             } else {
                 // This wave has read all of chunk c, and chunk c + 1 has landed.
                 wait_vm_lds<T::kLoads * (T::S - 2)>();
                 __builtin_amdgcn_s_barrier();
                 __builtin_amdgcn_sched_barrier(0);
-                issue(c + T::S);
-                const uint8_t *next = sh.ring + ((c + 1) % T::S) * T::kStage;
-                read(then, next, 0);
-                read_scales(sc_next, next, cb + c + 1);
+                multiply(s, Ws{}, now, sc, [&](auto k) KVA_INLINE {
+                    spread(k, Int<kReads + kScaleReads>{}, Early{}, [&](auto p) KVA_INLINE {
+                        if constexpr (decltype(p)::value < kReads) read(p, then, next, 0);
+                        else read_scale(Int<decltype(p)::value - kReads>{}, sc_next, next);
+                    });
+                    spread(k, Int<T::kLoads>{}, Whole{}, [&](auto j) KVA_INLINE { load(j, c + T::S, lds0 + at0); });
+                });
             }
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(s, now, sc);
-            __builtin_amdgcn_sched_barrier(0);
         };
-        one(std::integral_constant<int, 0>{}, o0, o1);
-        one(std::integral_constant<int, 1>{}, o1, o0);
+        one(Int<0>{}, o0, o1);
+        one(Int<1>{}, o1, o0);
         if constexpr (SPC == 4) {
-            one(std::integral_constant<int, 2>{}, o0, o1);
-            one(std::integral_constant<int, 3>{}, o1, o0);
+            one(Int<2>{}, o0, o1);
+            one(Int<3>{}, o1, o0);
         }
-        sc = sc_next;
+        at0 = at1;
+    };
+    if constexpr (T::KC == 128) {  // chunks in twos: hidden and its slices are whole 256s
+        for (int c = 0; c < nc; c += 2) {
+            chunk(Int<0>{}, c, sc0, sc1);
+            chunk(Int<1>{}, c + 1, sc1, sc0);
+        }
+    } else {
+        for (int c = 0; c < nc; ++c) {
+            chunk(Int<0>{}, c, sc0, sc1);
+            sc0 = sc1;
+        }
     }
     // Every load (the dummy ones past the end too) has landed before the LDS
     // is handed on.
