@@ -43,6 +43,14 @@ __device__ __forceinline__ uint4 rsrc_b128(__amdgpu_buffer_rsrc_t r, uint32_t vo
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
+// A pointer that every lane holds alike, in scalar registers (a buffer's base).
+__device__ __forceinline__ const uint8_t *uniform(const uint8_t *p) {
+    const auto v = reinterpret_cast<uintptr_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+    return reinterpret_cast<const uint8_t *>(static_cast<uintptr_t>(hi) << 32 | lo);
+}
+
 __device__ __forceinline__ float16_t zero16() {
     return float16_t{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 }
@@ -195,34 +203,33 @@ struct MxTile {
     static constexpr int SPC = KC / 64;               // steps of a stage
     static constexpr int kTM = BM / WM / 32, kTN = BN / WN / 32;  // MFMA tiles of a wave
     static constexpr int XV = BITS == 8 ? 2 : 1;      // 16-byte pieces of a token's step
-    static constexpr int kStageX = BM * 128, kStageW = BN / 32 * SPC * 1024;
-    static constexpr int kPlanes = KC / 128;          // dwords of a token's scales
-    static constexpr int kStageXs = kPlanes * BM * 4, kStageWs = BN / 32 * 256;
+    static constexpr int kStageX = BM * 128, kStageW = BN / 32 * SPC * 1024, kStage = kStageX + kStageW;
+    static constexpr int kPlanes = KC / 128;          // dwords of a token's scales in a chunk
+    static constexpr int kParts = 512 / KC;           // chunks that share a load of scales
+    static constexpr int kSmall = (BM + BN) / 64;     // loads of 1 KB of scales, for 512 values of k
     static constexpr int kLoadsX = kStageX / 1024 / kWaves, kLoadsW = kStageW / 1024 / kWaves;
-    static constexpr int kSmallX = kStageXs / 256, kSmall = kSmallX + kStageWs / 256;
     static constexpr int kLoadsS = (kSmall + kWaves - 1) / kWaves;
-    static constexpr int kLoads = kLoadsX + kLoadsW + kLoadsS;
     // With room for what the waves load only to keep their count.
-    static constexpr int kStage = kStageX + kStageW + kStageXs + kStageWs + (kSmall % kWaves ? 256 : 0);
-    static_assert(BM % (32 * WM) == 0 && BN % (32 * WN) == 0 && BM % 64 == 0, "whole MFMA tiles and loads");
+    static constexpr int kScales = 1024 * (kSmall + (kSmall % kWaves ? 1 : 0));
+    // Scales of 512 arrive while those of earlier chunks are still read.
+    static constexpr int kScaleBufs = (S - 2) / kParts + 2;
+    static constexpr int kRing = S * kStage + kScaleBufs * kScales;
+    // Loads of a wave for chunk `part` of its 512, and for chunks [from, to).
+    static constexpr int loads(int part) { return kLoadsX + kLoadsW + (part % kParts == 0 ? kLoadsS : 0); }
+    static constexpr int loads(int from, int to) { return from < to ? loads(from) + loads(from + 1, to) : 0; }
+    // Of a chunk's loads, those of its first `steps` steps.
+    static constexpr int share(int part, int steps) { return loads(part) * steps / SPC; }
+    static_assert(BM % (32 * WM) == 0 && BN % (32 * WN) == 0 && BM % 64 == 0 && BN % 64 == 0,
+                  "whole MFMA tiles and loads");
     static_assert(kLoadsX * kWaves * 1024 == kStageX && kLoadsW * kWaves * 1024 == kStageW, "whole loads per wave");
-    static_assert(S >= 2 && kLoads * (S - 1) < 64, "vmcnt is six bits");
-    static_assert(S * kStage + 4 * 4 * BM <= 160 * 1024, "the ring and the token facts fit the LDS");
+    static_assert(S >= 2 && loads(0, S) < 64, "vmcnt is six bits");
+    static_assert(kRing <= 160 * 1024, "the ring fits the LDS");
+    static_assert(BM <= 64 * kWaves, "a thread a token");
 };
 
 // The granule swizzle of a row of 128 bytes: the 16 rows that 16 lanes read
 // at one granule fall in distinct 16-byte bank groups.
 __device__ __forceinline__ int mx_swizzle(int r) { return ((r >> 1) ^ ((r & 1) << 2)) & 7; }
-
-template <class T, int EPI>
-struct MxShared {
-    uint8_t ring[T::S * T::kStage];
-    int32_t meta[EPI == kMxHead ? 4 : 1][EPI == kMxHead ? T::BM : 1];
-};
-
-__device__ __forceinline__ void word_to_lds_at(__amdgpu_buffer_rsrc_t r, uint32_t lds, uint32_t voff, uint32_t soff) {
-    touch_line(r, lds, voff, soff);
-}
 
 // Workgroup i runs on XCD i % 8: deal each XCD a contiguous run of n tiles.
 __device__ __forceinline__ int mx_deal(int i, int n) {
@@ -233,7 +240,7 @@ __device__ __forceinline__ int mx_deal(int i, int n) {
 template <class T, int EPI>
 __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, MxProduct m) {
     constexpr int kTM = T::kTM, kTN = T::kTN, SPC = T::SPC, BITS = T::BITS, XV = T::XV;
-    __shared__ __attribute__((aligned(16))) MxShared<T, EPI> sh;
+    __shared__ __attribute__((aligned(16))) uint8_t ring[T::kRing];
     const int N = a.n_a + a.n_b, K = a.hidden;
     const int n_rt = (N + T::BN - 1) / T::BN, n_mt = (a.n_tok + T::BM - 1) / T::BM;
     const int splits = EPI == kMxPart ? a.splits : 1;
@@ -247,15 +254,14 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
 
-    if constexpr (EPI == kMxHead) {
-        for (int i = threadIdx.x; i < T::BM; i += 64 * T::kWaves) {
-            const int t = min(t0 + i, a.n_tok - 1);
-            const int seq = a.tok_seq[t], slot = a.tok_slot[t];
-            sh.meta[0][i] = a.tok_pos[t];
-            sh.meta[1][i] = seq;
-            sh.meta[2][i] = slot;
-            sh.meta[3][i] = a.table[static_cast<size_t>(seq) * a.table_stride + (slot >> 4)];
-        }
+    // The facts of the tile's tokens (RoPE position, slot, page), a thread a
+    // token: requested first, used last.
+    int3 fact = make_int3(0, 0, 0);
+    if (EPI == kMxHead && threadIdx.x < T::BM) {
+        const int t = min(t0 + static_cast<int>(threadIdx.x), a.n_tok - 1);
+        fact.x = a.tok_pos[t];
+        fact.y = a.tok_slot[t];
+        fact.z = a.table[static_cast<size_t>(a.tok_seq[t]) * a.table_stride + (fact.y >> 4)];
     }
 
     // The operands as buffers: rows past the last token and tiles past the
@@ -264,15 +270,16 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
     const uint32_t toks = static_cast<uint32_t>(max(0, min(T::BM, a.n_tok - t0)));
     const MxTileAt at = mx_tile_at(a, m, n0 / 32);
     const uint32_t tiles = static_cast<uint32_t>((min(T::BN, N - n0) + 31) / 32);
-    const uint8_t *const x_at = m.x + static_cast<size_t>(t0) * x_row;
+    const uint8_t *const x_at = uniform(m.x + static_cast<size_t>(t0) * x_row), *const w_at = uniform(at.codes);
     const uint8_t *const xs_at = m.x_scales + static_cast<size_t>(t0) * s_row;
-    const uint32_t x_size = toks * x_row, w_size = tiles * 16u * K;
-    const uint32_t lds0 = lds_addr(sh.ring);
-    // This split's chunks: slices of hidden are whole 256s.
-    constexpr int kPer = 256 / T::KC;
-    const int nc_all = K / 256;
-    const int cb = EPI == kMxPart ? __builtin_amdgcn_readfirstlane(split * nc_all / splits) * kPer : 0;
-    const int nc = EPI == kMxPart ? __builtin_amdgcn_readfirstlane((split + 1) * nc_all / splits) * kPer - cb : nc_all * kPer;
+    const uint32_t x_size = __builtin_amdgcn_readfirstlane(toks * x_row);
+    const uint32_t w_size = __builtin_amdgcn_readfirstlane(tiles * 16u * K);
+    const uint32_t lds0 = lds_addr(ring);
+    // This split's chunks: slices of hidden are whole 512s.
+    const int n512 = K / 512;
+    const int cb = EPI == kMxPart ? __builtin_amdgcn_readfirstlane(split * n512 / splits) * T::kParts : 0;
+    const int nc =
+        (EPI == kMxPart ? __builtin_amdgcn_readfirstlane((split + 1) * n512 / splits) : n512) * T::kParts - cb;
 
     uint32_t xoff[T::kLoadsX], woff[T::kLoadsW];
 #pragma unroll
@@ -285,23 +292,26 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
         const int q = T::kWaves * j + wv;
         woff[j] = (q / SPC) * 16u * K + (q % SPC) * 1024u + 16 * lane;
     }
-    // A small load brings 64 dwords of scales: of 64 tokens, of a row tile, or
-    // none, where a wave loads only to keep its count.
+    // A load of scales, for 512 values of k: 16 bytes of 64 tokens, or 512 of
+    // two row tiles, or none, where a wave loads only to keep its count.  (Four
+    // bytes of a token per chunk of 128 brought a line each time: a third of
+    // the L2's traffic.)
     const uint8_t *sm_at[T::kLoadsS];
     uint32_t sm_size[T::kLoadsS], sm_step[T::kLoadsS], sm_off[T::kLoadsS];
 #pragma unroll
     for (int j = 0; j < T::kLoadsS; ++j) {
-        const int q = T::kWaves * j + wv;
-        const bool of_x = q < T::kSmallX;
-        sm_at[j] = of_x ? xs_at : at.scales;
-        sm_size[j] = of_x ? toks * s_row : q < T::kSmall ? tiles * static_cast<uint32_t>(K) : 0u;
-        sm_step[j] = of_x ? T::KC / 32 : 256;
-        sm_off[j] = of_x ? (64 * (q % (T::BM / 64)) + lane) * s_row + 4 * (q / (T::BM / 64))
-                         : (q - T::kSmallX) * static_cast<uint32_t>(K) + 4 * lane;
+        const int q = T::kWaves * j + wv, qw = q - T::BM / 64;
+        const bool of_x = qw < 0;
+        sm_at[j] = uniform(of_x ? xs_at : at.scales);
+        sm_size[j] = __builtin_amdgcn_readfirstlane(of_x            ? toks * s_row
+                                                    : q < T::kSmall ? tiles * static_cast<uint32_t>(K)
+                                                                    : 0u);
+        sm_step[j] = of_x ? 16 : 512;
+        sm_off[j] = of_x ? (64 * q + lane) * s_row : (2 * qw + half) * static_cast<uint32_t>(K) + 16 * col;
     }
-    // Piece j of the loads of chunk c (the k-th of hidden) into the stage at
-    // `st`.  A chunk past the end goes through empty buffers: the same loads,
-    // no memory access, so every wave's load counter advances alike.
+    // Piece j of the loads of chunk c into the stage at `st`.  A chunk past the
+    // end goes through empty buffers: the same loads, no memory access, so
+    // every wave's load counter advances alike.
     auto load = [&](auto piece, int c, uint32_t st) KVA_INLINE {
         constexpr int j = decltype(piece)::value;
         const bool on = c < nc;
@@ -310,15 +320,14 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
             load_to_lds_at(ro_rsrc(x_at, on ? x_size + 0u : 0u), st + 1024 * (T::kWaves * j + wv), xoff[j], k * 128);
         } else if constexpr (j < T::kLoadsX + T::kLoadsW) {
             constexpr int i = j - T::kLoadsX;
-            load_to_lds_at(ro_rsrc(at.codes, on ? w_size + 0u : 0u), st + T::kStageX + 1024 * (T::kWaves * i + wv),
+            load_to_lds_at(ro_rsrc(w_at, on ? w_size + 0u : 0u), st + T::kStageX + 1024 * (T::kWaves * i + wv),
                            woff[i], k * (SPC * 1024));
         } else {
             constexpr int i = j - T::kLoadsX - T::kLoadsW;
-            constexpr uint32_t kPer = 256 / T::KC;
-            const uint32_t steps = sm_step[i] == 256 ? k / kPer : k + 0u;
-            word_to_lds_at(ro_rsrc(sm_at[i], on ? sm_size[i] + 0u : 0u),
-                           st + T::kStageX + T::kStageW + 256 * min(T::kWaves * i + wv, T::kSmall), sm_off[i],
-                           __builtin_amdgcn_readfirstlane(steps * sm_step[i]));
+            const uint32_t dst = T::S * T::kStage + c / T::kParts % T::kScaleBufs * T::kScales;
+            load_to_lds_at(ro_rsrc(sm_at[i], on ? sm_size[i] + 0u : 0u),
+                           lds0 + dst + 1024 * min(T::kWaves * i + wv, T::kSmall), sm_off[i],
+                           __builtin_amdgcn_readfirstlane(k / T::kParts * sm_step[i]));
         }
     };
 
@@ -350,14 +359,14 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
             o.x[i][v] = *reinterpret_cast<const uint4 *>(st + row * 128 + 16 * (g ^ mx_swizzle(row)));
         }
     };
-    auto read_scale = [&](auto piece, Scales &o, const uint8_t *st) KVA_INLINE {
-        constexpr int p = decltype(piece)::value;
-        const uint32_t *xs = reinterpret_cast<const uint32_t *>(st + T::kStageX + T::kStageW);
+    // Piece p of the scales of chunk `part` of its 512, which are at `at`.
+    auto read_scale = [&](auto piece, auto part, Scales &o, const uint8_t *from) KVA_INLINE {
+        constexpr int p = decltype(piece)::value, k = decltype(part)::value * T::KC;
         if constexpr (p < kTN) {
-            o.w[p] = xs[T::kStageXs / 4 + (wn * kTN + p) * 64 + lane];
+            o.w[p] = *reinterpret_cast<const uint32_t *>(from + T::BM * 16 + (wn * kTN + p) * 512 + k / 256 * 256 + 4 * lane);
         } else {
             constexpr int i = (p - kTN) / T::kPlanes, pl = (p - kTN) % T::kPlanes;
-            o.x[i][pl] = xs[pl * T::BM + (wm * kTM + i) * 32 + col];
+            o.x[i][pl] = *reinterpret_cast<const uint32_t *>(from + ((wm * kTM + i) * 32 + col) * 16 + 4 * (k / 128 + pl));
         }
     };
     // A step's products, with hook(k) after the k-th: what the wave issues
@@ -380,41 +389,51 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
     // Reads come early, so that the last has arrived when its step begins.
     using Early = Int<kProducts - kProducts / 4>;
     using Whole = Int<kProducts>;
-#pragma unroll
-    for (int s = 0; s < T::S; ++s) each<0, T::kLoads>([&](auto j) KVA_INLINE { load(j, s, lds0 + s * T::kStage); });
-    wait_vm<T::kLoads * (T::S - 1)>();
+    // Chunk c + S is loaded from c's last step on, when its stage is free, a
+    // share of it in each step until the next chunk's last: piled up in one
+    // step, four waves' loads hold up each other's products.
+    each<0, T::S - 1>([&](auto c) KVA_INLINE {
+        each<0, T::loads(decltype(c)::value)>([&](auto j) KVA_INLINE { load(j, c, lds0 + c * T::kStage); });
+    });
+    each<0, T::share(T::S - 1, 1)>([&](auto j) KVA_INLINE { load(j, T::S - 1, lds0 + (T::S - 1) * T::kStage); });
+    wait_vm<T::loads(1, T::S - 1) + T::share(T::S - 1, 1)>();
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
     Step o0, o1;
     Scales sc0, sc1;
-    each<0, kReads>([&](auto p) KVA_INLINE { read(p, o0, sh.ring, 0); });
-    each<0, kScaleReads>([&](auto p) KVA_INLINE { read_scale(p, sc0, sh.ring); });
-    uint32_t at0 = 0;  // this chunk's stage
-    // One chunk; PART: its place among the chunks that share a dword of weight scales.
+    each<0, kReads>([&](auto p) KVA_INLINE { read(p, o0, ring, 0); });
+    each<0, kScaleReads>([&](auto p) KVA_INLINE { read_scale(p, Int<0>{}, sc0, ring + T::S * T::kStage); });
+    uint32_t before = (T::S - 1) * T::kStage, at0 = 0;  // the last chunk's stage and this one's
+    // Chunk c, `part` of its 512.
     auto chunk = [&](auto part, int c, Scales &sc, Scales &sc_next) KVA_INLINE {
         constexpr int kPart = decltype(part)::value;
         const uint32_t at1 = at0 + T::kStage == T::S * T::kStage ? 0 : at0 + T::kStage;
-        const uint8_t *st = sh.ring + at0, *next = sh.ring + at1;
-#pragma unroll
-        for (int i = 0; i < kTM; ++i)
-#pragma unroll
-            for (int p = 0; p < T::kPlanes; ++p) sc.x[i][p] >>= 8 * half;
+        const uint8_t *st = ring + at0, *next = ring + at1;
+        const uint8_t *next_scales = ring + T::S * T::kStage + (c + 1) / T::kParts % T::kScaleBufs * T::kScales;
+        each<0, kTM>([&](auto i) KVA_INLINE { each<0, T::kPlanes>([&](auto p) KVA_INLINE { sc.x[i][p] >>= 8 * half; }); });
         auto one = [&](auto s, Step &now, Step &then) KVA_INLINE {
             constexpr int kS = decltype(s)::value;
-            using Ws = Int<kPart * SPC + kS>;
+            using Ws = Int<(kPart * SPC + kS) % 4>;
             if constexpr (kS + 1 < SPC) {
-                multiply(s, Ws{}, now, sc, [&](auto k) KVA_INLINE { spread(k, Int<kReads>{}, Early{}, [&](auto p) KVA_INLINE { read(p, then, st, kS + 1); }); });
+                multiply(s, Ws{}, now, sc, [&](auto k) KVA_INLINE {
+                    spread(k, Int<kReads>{}, Early{}, [&](auto p) KVA_INLINE { read(p, then, st, kS + 1); });
+                    constexpr int kPiece = T::share(kPart + T::S - 1, kS + 1), kEnd = T::share(kPart + T::S - 1, kS + 2);
+                    spread(k, Int<kEnd - kPiece>{}, Whole{}, [&](auto j) KVA_INLINE {
+                        load(Int<kPiece + decltype(j)::value>{}, c + T::S - 1, lds0 + before);
+                    });
+                });
             } else {
                 // This wave has read all of chunk c, and chunk c + 1 has landed.
-                wait_vm_lds<T::kLoads * (T::S - 2)>();
+                wait_vm_lds<T::loads(kPart + 2, kPart + T::S)>();
                 __builtin_amdgcn_s_barrier();
                 __builtin_amdgcn_sched_barrier(0);
                 multiply(s, Ws{}, now, sc, [&](auto k) KVA_INLINE {
                     spread(k, Int<kReads + kScaleReads>{}, Early{}, [&](auto p) KVA_INLINE {
                         if constexpr (decltype(p)::value < kReads) read(p, then, next, 0);
-                        else read_scale(Int<decltype(p)::value - kReads>{}, sc_next, next);
+                        else read_scale(Int<decltype(p)::value - kReads>{}, Int<(kPart + 1) % T::kParts>{}, sc_next, next_scales);
                     });
-                    spread(k, Int<T::kLoads>{}, Whole{}, [&](auto j) KVA_INLINE { load(j, c + T::S, lds0 + at0); });
+                    spread(k, Int<T::share(kPart + T::S, 1)>{}, Whole{},
+                           [&](auto j) KVA_INLINE { load(j, c + T::S, lds0 + at0); });
                 });
             }
         };
@@ -424,17 +443,15 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
             one(Int<2>{}, o0, o1);
             one(Int<3>{}, o1, o0);
         }
+        before = at0;
         at0 = at1;
     };
-    if constexpr (T::KC == 128) {  // chunks in twos: hidden and its slices are whole 256s
-        for (int c = 0; c < nc; c += 2) {
-            chunk(Int<0>{}, c, sc0, sc1);
-            chunk(Int<1>{}, c + 1, sc1, sc0);
-        }
-    } else {
-        for (int c = 0; c < nc; ++c) {
-            chunk(Int<0>{}, c, sc0, sc1);
-            sc0 = sc1;
+    for (int c = 0; c < nc; c += T::kParts) {
+        chunk(Int<0>{}, c, sc0, sc1);
+        chunk(Int<1>{}, c + 1, sc1, sc0);
+        if constexpr (T::kParts == 4) {
+            chunk(Int<2>{}, c + 2, sc0, sc1);
+            chunk(Int<3>{}, c + 3, sc1, sc0);
         }
     }
     // Every load (the dummy ones past the end too) has landed before the LDS
@@ -469,14 +486,21 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
     } else {
         static_assert(T::BN == kHeadDim, "a head tile holds whole heads");
         constexpr int kRow = kHeadDim + 4;  // floats of a token's strip row, padded against bank conflicts
-        static_assert(32 * T::WM * kRow * 4 <= T::S * T::kStage, "a strip of tokens fits the ring");
+        constexpr int kStrip = 32 * T::WM * kRow * 4;
+        static_assert(kStrip + 3 * 4 * T::BM <= T::kRing, "a strip of tokens and the tokens' facts fit the ring");
         __syncthreads();
+        int32_t *facts = reinterpret_cast<int32_t *>(ring + kStrip);
+        if (threadIdx.x < T::BM) {
+            facts[threadIdx.x] = fact.x;
+            facts[T::BM + threadIdx.x] = fact.y;
+            facts[2 * T::BM + threadIdx.x] = fact.z;
+        }
         const int head = rt, H = a.num_heads, hkv = a.num_kv_heads;
         const int hw = threadIdx.x >> 5, l32 = threadIdx.x & 31;
         const bool is_q = head < H, is_gate = !is_q && head < 2 * H;
         const int kv = head - 2 * H;  // K heads 0..hkv-1, then V heads
         const bool rot = is_q || (!is_gate && kv < hkv);
-        float *strip = reinterpret_cast<float *>(sh.ring);
+        float *strip = reinterpret_cast<float *>(ring);
         const uint4 wnorm = rot ? ld16((is_q ? a.q_w : a.k_w) + 8 * l32) : make_uint4(0, 0, 0, 0);
         const int cl = a.half_rot > 0 ? min(l32, a.half_rot / 4 - 1) : 0;
         // 32 tokens of every wave row at a time, in fp32: Q and K are rounded
@@ -498,7 +522,7 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
                 nin.w = wnorm;
                 nin.c = nin.s = make_uint2(0, 0);
                 if (rot && a.half_rot > 0) {
-                    const size_t off = static_cast<size_t>(sh.meta[0][r]) * a.half_rot;
+                    const size_t off = static_cast<size_t>(facts[r]) * a.half_rot;
                     nin.c = ld8(a.cos_tab + off + 4 * cl);
                     nin.s = ld8(a.sin_tab + off + 4 * cl);
                 }
@@ -517,7 +541,7 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
                     st16(a.q_out + (static_cast<size_t>(t) * H + head) * kHeadDim + 8 * l32, o);
                     continue;
                 }
-                const size_t row_base = (static_cast<size_t>(sh.meta[3][r]) * kBlockTokens + (sh.meta[2][r] & 15)) * hkv;
+                const size_t row_base = (static_cast<size_t>(facts[2 * T::BM + r]) * kBlockTokens + (facts[T::BM + r] & 15)) * hkv;
                 if (kv < hkv)
                     st16(a.k_pool + (row_base + kv) * kHeadDim + 8 * l32, o);
                 else
@@ -587,7 +611,7 @@ bool plan_mx(const ProjectArgs &a, const MxProduct &m, bool heads, int n_cu, siz
         return !heads || static_cast<size_t>(T) * N <= part_floats;
     }
     const MxForm *forms = m.bits == 8 ? kForms8 : kForms4;
-    const int nc = a.hidden / 256;
+    const int nc = a.hidden / 512;
     double best_us = 0;
     for (int i = 0; i < static_cast<int>(std::size(kForms8)); ++i) {
         const MxForm &f = forms[i];
@@ -598,7 +622,7 @@ bool plan_mx(const ProjectArgs &a, const MxProduct &m, bool heads, int n_cu, siz
             const double part = static_cast<double>(splits) * T * N;
             if (partial && part > static_cast<double>(part_floats)) break;
             const double rounds = static_cast<double>((static_cast<int64_t>(tiles * splits) + n_cu - 1) / n_cu);
-            double us = rounds * (3.0 + (nc + splits - 1) / splits * f.us);
+            double us = rounds * (3.0 + 2 * ((nc + splits - 1) / splits) * f.us);
             if (partial) us += 4.0 + 8.0 * part / 5.0e6;
             if (plan.form < 0 || us < best_us) {
                 plan.form = i;
