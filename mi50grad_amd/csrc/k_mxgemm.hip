@@ -51,6 +51,15 @@ __device__ __forceinline__ const uint8_t *uniform(const uint8_t *p) {
     return reinterpret_cast<const uint8_t *>(static_cast<uintptr_t>(hi) << 32 | lo);
 }
 
+// A barrier that waits for LDS alone: __syncthreads() would also wait until
+// every store has arrived, some 2 us.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("" ::: "memory");
+    wait_vm_lds<63>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 __device__ __forceinline__ float16_t zero16() {
     return float16_t{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 }
@@ -458,97 +467,129 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
     // is handed on.
     __builtin_amdgcn_s_waitcnt(0);
 
-    if constexpr (EPI == kMxPart || EPI == kMxOut) {
-        float *part = EPI == kMxPart ? a.part + static_cast<size_t>(split) * a.n_tok * N : nullptr;
-#pragma unroll
-        for (int i = 0; i < kTM; ++i) {
-            const int t = t0 + (wm * kTM + i) * 32 + col;
-            if (t >= a.n_tok) continue;
-#pragma unroll
-            for (int j = 0; j < kTN; ++j)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int row = n0 + (wn * kTN + j) * 32 + 8 * q + 4 * half;
-                    if (row >= N) continue;
-                    float4_t v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                    const size_t o = static_cast<size_t>(t) * N + row;
-                    if constexpr (EPI == kMxPart) {
-                        *reinterpret_cast<float4_t *>(part + o) = v;
-                    } else {
-                        if (a.residual) {
-                            const uint2 r = ld8(a.residual + o);
-                            v += float4_t{lo_f(r.x), hi_f(r.x), lo_f(r.y), hi_f(r.y)};
-                        }
-                        *reinterpret_cast<uint2 *>(a.y_out + o) = make_uint2(pack_h2(v[0], v[1]), pack_h2(v[2], v[3]));
-                    }
-                }
-        }
-    } else {
-        static_assert(T::BN == kHeadDim, "a head tile holds whole heads");
-        constexpr int kRow = kHeadDim + 4;  // floats of a token's strip row, padded against bank conflicts
-        constexpr int kStrip = 32 * T::WM * kRow * 4;
-        static_assert(kStrip + 3 * 4 * T::BM <= T::kRing, "a strip of tokens and the tokens' facts fit the ring");
-        __syncthreads();
-        int32_t *facts = reinterpret_cast<int32_t *>(ring + kStrip);
+    // The sums leave through LDS, 32 tokens of every wave row at a time, so that
+    // whole lines are stored (a lane's four rows of its token in place took 7 to
+    // 11 us a tile, 16 bytes of each line at once): LPR lanes a token's row,
+    // eight rows of the weight each.
+    constexpr int kRow = T::BN + 4;  // floats of a token's strip row, padded against bank conflicts
+    constexpr int kStripToks = 32 * T::WM, kStrip = kStripToks * kRow * 4;
+    constexpr int LPR = T::BN / 8, kGroups = 64 * T::kWaves / LPR, kPer = kStripToks / kGroups;
+    static_assert(kPer * kGroups == kStripToks, "whole rows per group");
+    static_assert(EPI != kMxHead || T::BN == kHeadDim, "a head tile holds whole heads");
+    static_assert(kStrip + 3 * 4 * T::BM <= T::kRing, "a strip of tokens and the tokens' facts fit the ring");
+    float *strip = reinterpret_cast<float *>(ring);
+    int32_t *facts = reinterpret_cast<int32_t *>(ring + kStrip);
+    const int grp = threadIdx.x / LPR, l = threadIdx.x % LPR;
+    const int n = n0 + 8 * l;  // this lane's first row
+    __syncthreads();
+    if constexpr (EPI == kMxHead) {
         if (threadIdx.x < T::BM) {
             facts[threadIdx.x] = fact.x;
             facts[T::BM + threadIdx.x] = fact.y;
             facts[2 * T::BM + threadIdx.x] = fact.z;
         }
-        const int head = rt, H = a.num_heads, hkv = a.num_kv_heads;
-        const int hw = threadIdx.x >> 5, l32 = threadIdx.x & 31;
-        const bool is_q = head < H, is_gate = !is_q && head < 2 * H;
-        const int kv = head - 2 * H;  // K heads 0..hkv-1, then V heads
-        const bool rot = is_q || (!is_gate && kv < hkv);
-        float *strip = reinterpret_cast<float *>(ring);
-        const uint4 wnorm = rot ? ld16((is_q ? a.q_w : a.k_w) + 8 * l32) : make_uint4(0, 0, 0, 0);
-        const int cl = a.half_rot > 0 ? min(l32, a.half_rot / 4 - 1) : 0;
-        // 32 tokens of every wave row at a time, in fp32: Q and K are rounded
-        // once, after norm and RoPE.
-#pragma unroll
-        for (int i = 0; i < kTM; ++i) {
-#pragma unroll
-            for (int j = 0; j < kTN; ++j)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
+        __syncthreads();
+    }
+    const int head = rt, H = a.num_heads, hkv = a.num_kv_heads;
+    const bool is_q = head < H, is_gate = !is_q && head < 2 * H;
+    const int kv = head - 2 * H;  // K heads 0..hkv-1, then V heads
+    const bool rot = EPI == kMxHead && (is_q || (!is_gate && kv < hkv));
+    const uint4 wnorm = rot ? ld16((is_q ? a.q_w : a.k_w) + 8 * l) : make_uint4(0, 0, 0, 0);
+    const int cl = a.half_rot > 0 ? min(l, a.half_rot / 4 - 1) : 0;
+    // Rows are stored, and residuals read, through buffers over the tile's
+    // tokens: those past the last fall out of range without a branch, and so
+    // do columns past the last row (far).  A null output is an empty buffer.
+    constexpr uint32_t far = 0x80000000u;
+    const void *to = EPI == kMxPart  ? static_cast<const void *>(a.part + (static_cast<size_t>(split) * a.n_tok + t0) * N)
+                     : EPI == kMxOut ? a.y_out + static_cast<size_t>(t0) * N
+                     : is_q          ? a.q_out + static_cast<size_t>(t0) * H * kHeadDim
+                     : is_gate       ? a.gate_out + (a.gate_out ? static_cast<size_t>(t0) * H * kHeadDim : 0)
+                                     : a.kv_out + (a.kv_out ? static_cast<size_t>(t0) * 2 * hkv * kHeadDim : 0);
+    const uint32_t line = EPI == kMxPart  ? 4u * N
+                          : EPI == kMxOut ? 2u * N
+                                          : 2u * kHeadDim * (is_q || is_gate ? H : 2 * hkv);
+    const uint32_t at_col = EPI == kMxPart  ? (n < N ? 4u * n : far)
+                            : EPI == kMxOut ? (n < N ? 2u * n : far)
+                                            : 2u * kHeadDim * (is_q ? head : is_gate ? head - H : kv) + 16u * l;
+    const uint8_t *to_at = uniform(static_cast<const uint8_t *>(to));
+    const auto rto = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t *>(to_at), 0, __builtin_amdgcn_readfirstlane(to_at ? toks * line : 0u), 0x00020000);
+    const uint8_t *res_at = uniform(reinterpret_cast<const uint8_t *>(a.residual ? a.residual + static_cast<size_t>(t0) * N : nullptr));
+    const auto rres = ro_rsrc(res_at, __builtin_amdgcn_readfirstlane(EPI == kMxOut && res_at ? toks * line : 0u));
+    // Row j of this lane's group in part i of the tile: its token.
+    auto token = [&](int i, int j) KVA_INLINE {
+        const int sr = grp + kGroups * j;
+        return ((sr >> 5) * kTM + i) * 32 + (sr & 31);
+    };
+    // What finishing part i reads, requested a part ahead: before the stores
+    // that would be waited for with it.
+    struct Ahead {
+        uint4 res[EPI == kMxOut ? kPer : 1];
+        uint2 c[EPI == kMxHead ? kPer : 1], s[EPI == kMxHead ? kPer : 1];
+    };
+    auto request = [&](Ahead &o, int i) KVA_INLINE {
+        if constexpr (EPI == kMxOut) {
+            each<0, kPer>([&](auto j) KVA_INLINE { o.res[j] = rsrc_b128(rres, token(i, j) * line + at_col, 0); });
+        } else if constexpr (EPI == kMxHead) {
+            each<0, kPer>([&](auto j) KVA_INLINE {
+                // Tokens past the last carry its position: inside the tables.
+                const size_t off = static_cast<size_t>(facts[token(i, j)]) * a.half_rot + 4 * cl;
+                const uint16_t *w = is_q ? a.q_w : a.k_w;  // without a rotary part: in bounds, not used
+                o.c[j] = ld8(a.half_rot > 0 ? a.cos_tab + off : w);
+                o.s[j] = ld8(a.half_rot > 0 ? a.sin_tab + off : w);
+            });
+        }
+    };
+    auto store = [&](uint4 v, uint32_t off) KVA_INLINE {
+        typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+        __builtin_amdgcn_raw_buffer_store_b128(u4_t{v.x, v.y, v.z, v.w}, rto, off, 0, 0);
+    };
+    Ahead now, then;
+    request(now, 0);
+#pragma unroll 1
+    for (int i = 0; i < kTM; ++i) {
+        each<0, kTM>([&](auto part) KVA_INLINE {
+            if (i != part) return;
+            each<0, kTN>([&](auto j) KVA_INLINE {
+                each<0, 4>([&](auto q) KVA_INLINE {
                     *reinterpret_cast<float4_t *>(strip + (wm * 32 + col) * kRow + (wn * kTN + j) * 32 + 8 * q + 4 * half) =
-                        float4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-            __syncthreads();
-            for (int sr = hw; sr < 32 * T::WM; sr += 2 * T::kWaves) {
-                const int r = ((sr >> 5) * kTM + i) * 32 + (sr & 31);
-                const int t = t0 + r;
-                if (t >= a.n_tok) continue;
-                NormRopeIn nin;
-                nin.w = wnorm;
-                nin.c = nin.s = make_uint2(0, 0);
-                if (rot && a.half_rot > 0) {
-                    const size_t off = static_cast<size_t>(facts[r]) * a.half_rot;
-                    nin.c = ld8(a.cos_tab + off + 4 * cl);
-                    nin.s = ld8(a.sin_tab + off + 4 * cl);
-                }
-                const float4_t lo = *reinterpret_cast<const float4_t *>(strip + sr * kRow + 8 * l32);
-                const float4_t hi = *reinterpret_cast<const float4_t *>(strip + sr * kRow + 8 * l32 + 4);
+                        float4_t{acc[part][j][4 * q], acc[part][j][4 * q + 1], acc[part][j][4 * q + 2], acc[part][j][4 * q + 3]};
+                });
+            });
+        });
+        lds_barrier();
+        request(then, min(i + 1, kTM - 1));
+        each<0, kPer>([&](auto j) KVA_INLINE {
+            const int r = token(i, j);
+            const uint32_t off = r * line + at_col;
+            const float *from = strip + (grp + kGroups * j) * kRow + 8 * l;
+            float4_t lo = *reinterpret_cast<const float4_t *>(from), hi = *reinterpret_cast<const float4_t *>(from + 4);
+            if constexpr (EPI == kMxPart) {
+                store(__builtin_bit_cast(uint4, lo), off);
+                store(__builtin_bit_cast(uint4, hi), off + 16);
+            } else if constexpr (EPI == kMxOut) {
+                // A lane reads its residual before it writes the same bytes, so
+                // out may be the residual.
+                const uint4 z = now.res[j];
+                lo += float4_t{lo_f(z.x), hi_f(z.x), lo_f(z.y), hi_f(z.y)};
+                hi += float4_t{lo_f(z.z), hi_f(z.z), lo_f(z.w), hi_f(z.w)};
+                store(make_uint4(pack_h2(lo[0], lo[1]), pack_h2(lo[2], lo[3]), pack_h2(hi[0], hi[1]), pack_h2(hi[2], hi[3])), off);
+            } else {
+                // In fp32 up to here: Q and K are rounded once, after norm and RoPE.
                 const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
                 const uint4 y = make_uint4(pack_h2(x[0], x[1]), pack_h2(x[2], x[3]), pack_h2(x[4], x[5]), pack_h2(x[6], x[7]));
-                if (is_gate) {
-                    if (a.gate_out) st16(a.gate_out + (static_cast<size_t>(t) * H + head - H) * kHeadDim + 8 * l32, y);
-                    continue;
+                uint4 o = y;
+                if (rot) o = norm_rope_apply<32>(x, NormRopeIn{wnorm, now.c[j], now.s[j]}, a.half_rot, a.eps, l);
+                store(is_q ? o : y, off);
+                if (kv >= 0 && t0 + r < a.n_tok) {
+                    const size_t row = (static_cast<size_t>(facts[2 * T::BM + r]) * kBlockTokens + (facts[T::BM + r] & 15)) * hkv;
+                    if (kv < hkv) st16(a.k_pool + (row + kv) * kHeadDim + 8 * l, o);
+                    else st16(a.v_pool + (row + kv - hkv) * kHeadDim + 8 * l, y);
                 }
-                if (!is_q && a.kv_out)
-                    st16(a.kv_out + (static_cast<size_t>(t) * 2 * hkv + kv) * kHeadDim + 8 * l32, y);
-                const uint4 o = rot ? norm_rope_apply<32>(x, nin, a.half_rot, a.eps, l32) : y;
-                if (is_q) {
-                    st16(a.q_out + (static_cast<size_t>(t) * H + head) * kHeadDim + 8 * l32, o);
-                    continue;
-                }
-                const size_t row_base = (static_cast<size_t>(facts[2 * T::BM + r]) * kBlockTokens + (facts[T::BM + r] & 15)) * hkv;
-                if (kv < hkv)
-                    st16(a.k_pool + (row_base + kv) * kHeadDim + 8 * l32, o);
-                else
-                    st16(a.v_pool + (row_base + kv - hkv) * kHeadDim + 8 * l32, y);
             }
-            __syncthreads();  // the strip is read before the next 32 tokens overwrite it
-        }
+        });
+        lds_barrier();  // the strip is read before the next tokens overwrite it
+        now = then;
     }
 }
 
