@@ -46,6 +46,7 @@ enum : int {
     kDppQuadXor1 = 0xB1,       // quad_perm [1,0,3,2]
     kDppQuadXor2 = 0x4E,       // quad_perm [2,3,0,1]
     kDppRowHalfMirror = 0x141, // lane i <-> 7-i inside each 8 lanes
+    kDppRowRor4 = 0x124,       // rotate a 16-lane row by 4
     kDppRowRor8 = 0x128,       // rotate a 16-lane row by 8
     kDppRowMirror = 0x140,     // lane i <-> 15-i inside each row
     kDppRowBcast15 = 0x142,    // lane 15 of a row -> all lanes of the next row

@@ -559,35 +559,61 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
         });
         lds_barrier();
         request(then, min(i + 1, kTM - 1));
-        each<0, kPer>([&](auto j) KVA_INLINE {
-            const int r = token(i, j);
-            const uint32_t off = r * line + at_col;
-            const float *from = strip + (grp + kGroups * j) * kRow + 8 * l;
-            float4_t lo = *reinterpret_cast<const float4_t *>(from), hi = *reinterpret_cast<const float4_t *>(from + 4);
-            if constexpr (EPI == kMxPart) {
-                store(__builtin_bit_cast(uint4, lo), off);
-                store(__builtin_bit_cast(uint4, hi), off + 16);
-            } else if constexpr (EPI == kMxOut) {
-                // A lane reads its residual before it writes the same bytes, so
-                // out may be the residual.
-                const uint4 z = now.res[j];
-                lo += float4_t{lo_f(z.x), hi_f(z.x), lo_f(z.y), hi_f(z.y)};
-                hi += float4_t{lo_f(z.z), hi_f(z.z), lo_f(z.w), hi_f(z.w)};
-                store(make_uint4(pack_h2(lo[0], lo[1]), pack_h2(lo[2], lo[3]), pack_h2(hi[0], hi[1]), pack_h2(hi[2], hi[3])), off);
+        if constexpr (EPI == kMxHead) {
+            // In fp32 up to here: Q and K are rounded once, after norm and RoPE.
+            // All rows are worked out before the first is stored, so that their
+            // sums across lanes run side by side.
+            uint4 y[kPer], o[kPer];
+            auto row = [&](int j, float (&x)[8]) KVA_INLINE {
+                const float *from = strip + (grp + kGroups * j) * kRow + 8 * l;
+                const float4_t lo = *reinterpret_cast<const float4_t *>(from), hi = *reinterpret_cast<const float4_t *>(from + 4);
+                x[0] = lo[0], x[1] = lo[1], x[2] = lo[2], x[3] = lo[3], x[4] = hi[0], x[5] = hi[1], x[6] = hi[2], x[7] = hi[3];
+                return make_uint4(pack_h2(x[0], x[1]), pack_h2(x[2], x[3]), pack_h2(x[4], x[5]), pack_h2(x[6], x[7]));
+            };
+            if (rot) {
+                each<0, kPer>([&](auto j) KVA_INLINE {
+                    float x[8];
+                    y[j] = row(j, x);
+                    o[j] = norm_rope_apply<32, true>(x, NormRopeIn{wnorm, now.c[j], now.s[j]}, a.half_rot, a.eps, l);
+                });
             } else {
-                // In fp32 up to here: Q and K are rounded once, after norm and RoPE.
-                const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                const uint4 y = make_uint4(pack_h2(x[0], x[1]), pack_h2(x[2], x[3]), pack_h2(x[4], x[5]), pack_h2(x[6], x[7]));
-                uint4 o = y;
-                if (rot) o = norm_rope_apply<32>(x, NormRopeIn{wnorm, now.c[j], now.s[j]}, a.half_rot, a.eps, l);
-                store(is_q ? o : y, off);
-                if (kv >= 0 && t0 + r < a.n_tok) {
-                    const size_t row = (static_cast<size_t>(facts[2 * T::BM + r]) * kBlockTokens + (facts[T::BM + r] & 15)) * hkv;
-                    if (kv < hkv) st16(a.k_pool + (row + kv) * kHeadDim + 8 * l, o);
-                    else st16(a.v_pool + (row + kv - hkv) * kHeadDim + 8 * l, y);
-                }
+                each<0, kPer>([&](auto j) KVA_INLINE {
+                    float x[8];
+                    y[j] = o[j] = row(j, x);
+                });
             }
-        });
+            if (is_q) {
+                each<0, kPer>([&](auto j) KVA_INLINE { store(o[j], token(i, j) * line + at_col); });
+            } else {
+                each<0, kPer>([&](auto j) KVA_INLINE { store(y[j], token(i, j) * line + at_col); });
+            }
+            if (kv >= 0) {
+                uint16_t *const pool = kv < hkv ? a.k_pool + kv * kHeadDim : a.v_pool + (kv - hkv) * kHeadDim;
+                each<0, kPer>([&](auto j) KVA_INLINE {
+                    const int r = token(i, j);
+                    const size_t at_row = static_cast<size_t>(facts[2 * T::BM + r]) * kBlockTokens + (facts[T::BM + r] & 15);
+                    if (t0 + r < a.n_tok) st16(pool + at_row * hkv * kHeadDim + 8 * l, o[j]);
+                });
+            }
+        } else {
+            each<0, kPer>([&](auto j) KVA_INLINE {
+                const uint32_t off = token(i, j) * line + at_col;
+                const float *from = strip + (grp + kGroups * j) * kRow + 8 * l;
+                float4_t lo = *reinterpret_cast<const float4_t *>(from), hi = *reinterpret_cast<const float4_t *>(from + 4);
+                if constexpr (EPI == kMxPart) {
+                    store(__builtin_bit_cast(uint4, lo), off);
+                    store(__builtin_bit_cast(uint4, hi), off + 16);
+                } else {
+                    // A lane reads its residual before it writes the same
+                    // bytes, so out may be the residual.
+                    const uint4 z = now.res[j];
+                    lo += float4_t{lo_f(z.x), hi_f(z.x), lo_f(z.y), hi_f(z.y)};
+                    hi += float4_t{lo_f(z.z), hi_f(z.z), lo_f(z.w), hi_f(z.w)};
+                    store(make_uint4(pack_h2(lo[0], lo[1]), pack_h2(lo[2], lo[3]), pack_h2(hi[0], hi[1]), pack_h2(hi[2], hi[3])),
+                          off);
+                }
+            });
+        }
         lds_barrier();  // the strip is read before the next tokens overwrite it
         now = then;
     }

@@ -63,10 +63,24 @@ __device__ __forceinline__ void rope_in_flat(NormRopeIn &in, const uint16_t *__r
     in.s = ld8((rot ? sin_row : w) + 4 * cl);
 }
 
+// The butterfly of 32 lanes by lane moves of the vector unit, the bits of the
+// one by __shfl_xor: once lanes 16 and 8 apart hold the same sum, a rotation by
+// 4 within 16 lanes brings the sum of lane ^ 4.  Every lane of the wave takes part.
+__device__ __forceinline__ float sum32_moves(float s) {
+#pragma clang fp contract(off)
+    float a = s, b = s;
+    swap16(a, b);
+    s = a + b;
+    s = s + dpp_f<kDppRowRor8>(s);
+    s = s + dpp_f<kDppRowRor4>(s);
+    s = s + dpp_f<kDppQuadXor2>(s);
+    return s + dpp_f<kDppQuadXor1>(s);
+}
+
 // Normalise + rotate one row held as 8 values per lane, rounded to fp16 at the
 // end.  LANES = head_dim / 8 lanes take part (lane < LANES); the butterfly
-// stays inside them.
-template <int LANES>
+// stays inside them.  MOVES: by sum32_moves.
+template <int LANES, bool MOVES = false>
 __device__ __forceinline__ uint4 norm_rope_apply(const float (&x)[8], const NormRopeIn &in, int half_rot, float eps,
                                                  int lane) {
 #pragma clang fp contract(off)
@@ -76,10 +90,15 @@ __device__ __forceinline__ uint4 norm_rope_apply(const float (&x)[8], const Norm
         const float sq = x[i] * x[i];
         s = s + sq;
     }
+    if constexpr (MOVES) {
+        static_assert(LANES == 32, "a half-wave per row");
+        s = sum32_moves(s);
+    } else {
 #pragma unroll
-    for (int off = LANES / 2; off >= 1; off >>= 1) {
-        const float other = __shfl_xor(s, off, 32);
-        s = s + other;
+        for (int off = LANES / 2; off >= 1; off >>= 1) {
+            const float other = __shfl_xor(s, off, 32);
+            s = s + other;
+        }
     }
     const float ms = s * (1.0f / static_cast<float>(LANES * 8));
     const float var = ms + eps;
