@@ -95,98 +95,146 @@ __device__ __forceinline__ void each(const F &f) {
     each_of<FROM>(f, std::make_integer_sequence<int, TO - FROM>{});
 }
 
+// The granule swizzle of a row of 128 bytes: the 16 rows that 16 lanes read
+// at one granule fall in distinct 16-byte bank groups.
+__device__ __forceinline__ int mx_swizzle(int r) { return ((r >> 1) ^ ((r & 1) << 2)) & 7; }
+
 // ---- up to 32 tokens ---------------------------------------------------------
 
 constexpr int kMxStreamWaves = 8;
 
-// A workgroup takes RT row tiles over the whole of hidden, an eighth of it per
-// wave (hidden is a multiple of 512: whole steps), straight from memory into
-// registers; the waves' sums meet in LDS.  No k is split among workgroups, so
-// with EPI_OUT the result is finished here; else fp32 rows go to a finish
-// kernel.
-template <int BITS, int RT, bool EPI_OUT>
+// A unit of the streaming form: 128 values of k of RT row tiles and of up to
+// 32 tokens, with their scales, in one of the wave's own S slots.
+template <int BITS_, int RT_>
+struct MxUnit {
+    static constexpr int BITS = BITS_, RT = RT_;
+    static constexpr int kXRow = 16 * BITS;           // bytes of a token
+    static constexpr int kX = 32 * kXRow, kW = RT * 2048, kXs = 256, kWs = RT * 256;
+    static constexpr int kSlot = kX + kW + kXs + kWs;
+    static constexpr int kLoads = kX / 1024 + kW / 1024 + 1 + RT;
+    static constexpr int S = 20 * 1024 / kSlot;       // the LDS shared by eight waves
+    static_assert(S >= 2 && kLoads * (S - 1) < 64, "one unit at least on its way, vmcnt is six bits");
+    static_assert(kMxStreamWaves * S * kSlot >= kMxStreamWaves * RT * 4096, "the waves' sums fit");
+};
+
+// A workgroup takes RT row tiles over the whole of hidden, a run of units per
+// wave, through loads that write the wave's own slots of LDS: no wave waits for
+// another, a token's row comes in whole lines (operands straight from memory
+// touch a line per token and instruction, four times as many: 32 tokens of 6144
+// -> 5120 took 12.6 us).  The waves' sums meet in LDS.  No k is split among
+// workgroups, so with OUT the result is finished here; else fp32 rows go to a
+// finish kernel.
+template <int BITS, int RT, bool OUT>
 __global__ __launch_bounds__(64 * kMxStreamWaves) void mx_stream_kernel(ProjectArgs a, MxProduct m) {
-    constexpr int C = 4;  // steps of a chunk
-    constexpr int XV = BITS == 8 ? 2 : 1;
-    __shared__ float4_t red[kMxStreamWaves][RT][4][64];
+    using U = MxUnit<BITS, RT>;
+    __shared__ __attribute__((aligned(16))) uint8_t ring[kMxStreamWaves][U::S * U::kSlot];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int N = a.n_a + a.n_b, K = a.hidden;
     const int rt0 = blockIdx.x * RT, n_rt = (N + kMxWeightTile - 1) / kMxWeightTile;
-    const int n = K / (64 * kMxStreamWaves), s0 = wave * n;  // this wave's steps
-    __amdgpu_buffer_rsrc_t rw[RT], rs[RT];
+    const int units = K / 128;
+    const int u0 = wave * units / kMxStreamWaves, n = (wave + 1) * units / kMxStreamWaves - u0;
+    const uint8_t *w_at[RT], *ws_at[RT];
+    uint32_t w_size[RT];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
         const MxTileAt at = mx_tile_at(a, m, min(rt0 + i, n_rt - 1));
-        const bool in = rt0 + i < n_rt;
-        rw[i] = ro_rsrc(at.codes, in ? 16u * K : 0u);
-        rs[i] = ro_rsrc(at.scales, in ? static_cast<uint32_t>(K) : 0u);
+        w_at[i] = uniform(at.codes);
+        ws_at[i] = uniform(at.scales);
+        w_size[i] = __builtin_amdgcn_readfirstlane(rt0 + i < n_rt ? static_cast<uint32_t>(K) : 0u);
     }
     const uint32_t x_row = static_cast<uint32_t>(K) * BITS / 8, s_row = static_cast<uint32_t>(K) / 32;
-    const auto rx = ro_rsrc(m.x, a.n_tok * x_row), rxs = ro_rsrc(m.x_scales, a.n_tok * s_row);
-    const uint32_t xo = col * x_row + 16 * half, xso = col * s_row + half;
-
+    // Loads of X: 1 KB of whole rows, granules swizzled so that the 16 rows that
+    // 16 lanes read at one fall in distinct banks.
+    constexpr int kLanes = U::kXRow / 16, kRows = 64 / kLanes;  // lanes of a row, rows of a load
+    auto swizzle = [](int r) { return BITS == 8 ? mx_swizzle(r) : (r >> 2) & 3; };
+    uint32_t xoff[U::kX / 1024];
+#pragma unroll
+    for (int j = 0; j < U::kX / 1024; ++j) {
+        const int row = kRows * j + lane / kLanes;
+        xoff[j] = row * x_row + 16 * ((lane % kLanes) ^ swizzle(row));
+    }
+    const uint32_t xs_off = col * s_row, lds0 = lds_addr(ring[wave]);
+    // Units past the wave's last go through empty buffers, so that every wait counts alike.
+    auto issue = [&](int i) {
+        const bool on = i < n;
+        const uint32_t u = on ? static_cast<uint32_t>(u0 + i) : 0u;
+        const uint32_t st = lds0 + i % U::S * U::kSlot;
+        const uint32_t toks = on ? static_cast<uint32_t>(a.n_tok) : 0u;
+#pragma unroll
+        for (int j = 0; j < RT; ++j) {
+            const auto rw = ro_rsrc(w_at[j], on ? w_size[j] * 16 : 0u), rs = ro_rsrc(ws_at[j], on ? w_size[j] + 0u : 0u);
+            load_to_lds_at(rw, st + U::kX + 2048 * j, 16 * lane, u * 2048);
+            load_to_lds_at(rw, st + U::kX + 2048 * j + 1024, 16 * lane + 1024, u * 2048);
+            touch_line(rs, st + U::kX + U::kW + U::kXs + 256 * j, 4 * lane, u / 2 * 256);
+        }
+        const auto rx = ro_rsrc(m.x, toks * x_row), rxs = ro_rsrc(m.x_scales, toks * s_row);
+#pragma unroll
+        for (int j = 0; j < U::kX / 1024; ++j) load_to_lds_at(rx, st + 1024 * j, xoff[j], u * U::kXRow);
+        touch_line(rxs, st + U::kX + U::kW, xs_off, u * 4);
+    };
     float16_t acc[RT];
 #pragma unroll
     for (int i = 0; i < RT; ++i) acc[i] = zero16();
-    struct Chunk {
-        uint4 w[RT][C], x[C][XV];
-        uint32_t ws[RT][C], xs[C];
-    };
-    auto load = [&](Chunk &c, int s, int left) {
+    for (int i = 0; i < U::S; ++i) issue(i);
+    for (int i = 0; i < n; ++i) {
+        wait_vm<U::kLoads *(U::S - 1)>();
+        __builtin_amdgcn_sched_barrier(0);
+        const uint8_t *st = ring[wave] + i % U::S * U::kSlot;
+        constexpr int XV = BITS == 8 ? 2 : 1;
+        uint4 x[2][XV], w[2][RT];
+        uint32_t ws[RT];
 #pragma unroll
-        for (int j = 0; j < C; ++j) {
-            if (j >= left) break;
-            const int st = s + j;
+        for (int s = 0; s < 2; ++s) {
 #pragma unroll
-            for (int i = 0; i < RT; ++i) {
-                c.w[i][j] = rsrc_b128(rw[i], 16 * lane, 1024 * st);
-                c.ws[i][j] = __builtin_amdgcn_raw_buffer_load_b8(rs[i], 4 * lane, (st >> 2) * 256 + (st & 3), 0);
+            for (int v = 0; v < XV; ++v) {
+                const int g = BITS == 8 ? 4 * s + 2 * v + half : 2 * s + half;
+                x[s][v] = *reinterpret_cast<const uint4 *>(st + col * U::kXRow + 16 * (g ^ swizzle(col)));
             }
-            c.x[j][0] = rsrc_b128(rx, xo, st * (8 * BITS));
-            if constexpr (BITS == 8) c.x[j][1] = rsrc_b128(rx, xo + 32, st * 64);
-            c.xs[j] = __builtin_amdgcn_raw_buffer_load_b8(rxs, xso, 2 * st, 0);
-        }
-    };
-    auto multiply = [&](const Chunk &c, int left) {
 #pragma unroll
-        for (int j = 0; j < C; ++j) {
-            if (j >= left) break;
-#pragma unroll
-            for (int i = 0; i < RT; ++i) acc[i] = mx_mfma<BITS, 0, 0>(c.w[i][j], c.x[j], acc[i], c.ws[i][j], c.xs[j]);
+            for (int j = 0; j < RT; ++j)
+                w[s][j] = *reinterpret_cast<const uint4 *>(st + U::kX + 2048 * j + 1024 * s + 16 * lane);
         }
-    };
-    Chunk c0, c1;
-    load(c0, s0, n);
-    for (int s = 0; s < n; s += 2 * C) {
-        if (s + C < n) load(c1, s0 + s + C, n - s - C);
-        multiply(c0, n - s);
-        if (s + C >= n) break;
-        if (s + 2 * C < n) load(c0, s0 + s + 2 * C, n - s - 2 * C);
-        multiply(c1, n - s - C);
+        const uint32_t xs = *reinterpret_cast<const uint32_t *>(st + U::kX + U::kW + 4 * lane) >> (8 * half);
+#pragma unroll
+        for (int j = 0; j < RT; ++j)
+            ws[j] = *reinterpret_cast<const uint32_t *>(st + U::kX + U::kW + U::kXs + 256 * j + 4 * lane) >> (16 * ((u0 + i) & 1));
+        // The slot has been read before it is loaded again.
+        wait_vm_lds<63>();
+        __builtin_amdgcn_sched_barrier(0);
+        issue(i + U::S);
+#pragma unroll
+        for (int j = 0; j < RT; ++j) {
+            acc[j] = mx_mfma<BITS, 0, 0>(w[0][j], x[0], acc[j], ws[j], xs);
+            acc[j] = mx_mfma<BITS, 1, 2>(w[1][j], x[1], acc[j], ws[j], xs);
+        }
     }
+    // Every load (the empty ones too) has landed before the LDS is handed on.
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    float4_t *red = reinterpret_cast<float4_t *>(ring);  // [wave][RT][4][64]
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            red[wave][i][q][lane] = float4_t{acc[i][4 * q], acc[i][4 * q + 1], acc[i][4 * q + 2], acc[i][4 * q + 3]};
+            red[((wave * RT + i) * 4 + q) * 64 + lane] =
+                float4_t{acc[i][4 * q], acc[i][4 * q + 1], acc[i][4 * q + 2], acc[i][4 * q + 3]};
     __syncthreads();
     // Eight threads finish a token's 32 rows of a tile.
     for (int f = threadIdx.x; f < RT * 256; f += 64 * kMxStreamWaves) {
         const int i = f >> 8, t = (f >> 3) & 31, rq = f & 7;
         if (t >= a.n_tok) continue;
-        const int from = t + 32 * (rq & 1);
-        float4_t sum = red[0][i][rq >> 1][from];
-#pragma unroll
-        for (int w = 1; w < kMxStreamWaves; ++w) sum += red[w][i][rq >> 1][from];
         const int row = 32 * (rt0 + i) + 4 * rq;
         if (row >= N) continue;
         const size_t at = static_cast<size_t>(t) * N + row;
-        if constexpr (EPI_OUT) {
-            if (a.residual) {
-                const uint2 r = ld8(a.residual + at);
-                sum += float4_t{lo_f(r.x), hi_f(r.x), lo_f(r.y), hi_f(r.y)};
-            }
+        uint2 r = make_uint2(0, 0);
+        if (OUT && a.residual) r = ld8(a.residual + at);
+        const int from = t + 32 * (rq & 1);
+        float4_t sum = red[(i * 4 + (rq >> 1)) * 64 + from];
+#pragma unroll
+        for (int w = 1; w < kMxStreamWaves; ++w) sum += red[((w * RT + i) * 4 + (rq >> 1)) * 64 + from];
+        if constexpr (OUT) {
+            sum += float4_t{lo_f(r.x), hi_f(r.x), lo_f(r.y), hi_f(r.y)};
             *reinterpret_cast<uint2 *>(a.y_out + at) = make_uint2(pack_h2(sum[0], sum[1]), pack_h2(sum[2], sum[3]));
         } else {
             *reinterpret_cast<float4_t *>(a.part + at) = sum;
@@ -235,10 +283,6 @@ struct MxTile {
     static_assert(kRing <= 160 * 1024, "the ring fits the LDS");
     static_assert(BM <= 64 * kWaves, "a thread a token");
 };
-
-// The granule swizzle of a row of 128 bytes: the 16 rows that 16 lanes read
-// at one granule fall in distinct 16-byte bank groups.
-__device__ __forceinline__ int mx_swizzle(int r) { return ((r >> 1) ^ ((r & 1) << 2)) & 7; }
 
 // Workgroup i runs on XCD i % 8: deal each XCD a contiguous run of n tiles.
 __device__ __forceinline__ int mx_deal(int i, int n) {
@@ -627,12 +671,13 @@ hipError_t launch_mx_gemm(const ProjectArgs &a, const MxProduct &m, hipStream_t 
     return hipGetLastError();
 }
 
-template <int BITS>
-hipError_t launch_mx_stream(const ProjectArgs &a, const MxProduct &m, bool heads, hipStream_t s) {
+// Two row tiles a workgroup where one would not fit the chip at once.
+template <int BITS, bool OUT>
+hipError_t launch_mx_stream(const ProjectArgs &a, const MxProduct &m, int n_cu, hipStream_t s) {
     const int n_rt = (a.n_a + a.n_b + kMxWeightTile - 1) / kMxWeightTile;
     const dim3 block(64 * kMxStreamWaves);
-    if (heads) hipLaunchKernelGGL((mx_stream_kernel<BITS, 2, false>), dim3((n_rt + 1) / 2), block, 0, s, a, m);
-    else hipLaunchKernelGGL((mx_stream_kernel<BITS, 1, true>), dim3(n_rt), block, 0, s, a, m);
+    if (n_rt > n_cu) hipLaunchKernelGGL((mx_stream_kernel<BITS, 2, OUT>), dim3((n_rt + 1) / 2), block, 0, s, a, m);
+    else hipLaunchKernelGGL((mx_stream_kernel<BITS, 1, OUT>), dim3(n_rt), block, 0, s, a, m);
     return hipGetLastError();
 }
 
@@ -705,14 +750,15 @@ bool plan_mx(const ProjectArgs &a, const MxProduct &m, bool heads, int n_cu, siz
     return true;
 }
 
-hipError_t launch_mx_product(const ProjectArgs &args, const MxProduct &m, bool heads, const ProductPlan &plan,
+hipError_t launch_mx_product(const ProjectArgs &args, const MxProduct &m, bool heads, int n_cu, const ProductPlan &plan,
                              hipStream_t s) {
     ProjectArgs a = args;
     a.splits = plan.splits;
     hipError_t e = a.ev_before ? hipEventRecord(a.ev_before, s) : hipSuccess;
     if (e != hipSuccess) return e;
     if (plan.stream) {
-        e = m.bits == 8 ? launch_mx_stream<8>(a, m, heads, s) : launch_mx_stream<4>(a, m, heads, s);
+        e = m.bits == 8 ? (heads ? launch_mx_stream<8, false> : launch_mx_stream<8, true>)(a, m, n_cu, s)
+                        : (heads ? launch_mx_stream<4, false> : launch_mx_stream<4, true>)(a, m, n_cu, s);
     } else {
         const MxForm &f = (m.bits == 8 ? kForms8 : kForms4)[plan.form];
         e = (plan.partial ? f.part : heads ? f.head : f.out)(a, m, s);

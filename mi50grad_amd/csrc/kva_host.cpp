@@ -1507,7 +1507,7 @@ static hipError_t run_mx(const kva_cache *c, const MxInput &in, kva::ProjectArgs
         m.x_scales = r.scales;
         a.part = c->d_proj + in.held_floats(n);
     }
-    return kva::launch_mx_product(a, m, heads, plan, s);
+    return kva::launch_mx_product(a, m, heads, c->n_cu, plan, s);
 }
 
 static int mx_project_impl(kva_cache *c, int32_t layer, const MxInput &in, const void *w_q, const void *w_kv,

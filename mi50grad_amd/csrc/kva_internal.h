@@ -191,7 +191,7 @@ struct MxProduct {
     int32_t bits;             // of x
 };
 bool plan_mx(const ProjectArgs &a, const MxProduct &m, bool heads, int n_cu, size_t part_floats, ProductPlan &plan);
-hipError_t launch_mx_product(const ProjectArgs &a, const MxProduct &m, bool heads, const ProductPlan &plan,
+hipError_t launch_mx_product(const ProjectArgs &a, const MxProduct &m, bool heads, int n_cu, const ProductPlan &plan,
                              hipStream_t s);
 
 // Reference-compatible norm+RoPE on a contiguous [n_heads][head_dim] buffer.
