@@ -469,8 +469,8 @@ int kva_mx_project_append(kva_cache *cache, int32_t layer, const void *x, const 
 /* kva_out_project by 4-bit weights: out[t] = fp16(attn[t] . W_o^T +
  * residual[t]).  attn is fp16 rows [n_tok][q_dim], taken to `bits` on the way
  * (attn_scales NULL), or microscaled rows.  residual NULL, apart from out, or
- * out itself.  q_dim a multiple of 512, n_out of 16; a token's microscaled
- * row has to fit half of the cache's projection workspace
+ * out itself.  q_dim a multiple of 512, n_out of 16, at most 1048576
+ * (KVA_ERR_UNSUPPORTED); a token's microscaled row has to fit half of the cache's projection workspace
  * (KVA_ERR_INVALID_ARG).                                                    */
 int kva_mx_out_project(kva_cache *cache, const void *attn, const void *attn_scales, int32_t bits,
                        int32_t n_tok, int32_t q_dim, const void *w_o_packed, int32_t n_out,

@@ -517,14 +517,13 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
     // eight rows of the weight each.
     constexpr int kRow = T::BN + 4;  // floats of a token's strip row, padded against bank conflicts
     constexpr int kStripToks = 32 * T::WM, kStrip = kStripToks * kRow * 4;
-    constexpr int LPR = T::BN / 8, kGroups = 64 * T::kWaves / LPR, kPer = kStripToks / kGroups;
-    static_assert(kPer * kGroups == kStripToks, "whole rows per group");
+    constexpr int LPR = T::BN / 8, kThreads = 64 * T::kWaves, kPer = kStripToks * LPR / kThreads;
+    static_assert(kPer * kThreads == kStripToks * LPR, "as many pieces for every thread");
     static_assert(EPI != kMxHead || T::BN == kHeadDim, "a head tile holds whole heads");
     static_assert(kStrip + 3 * 4 * T::BM <= T::kRing, "a strip of tokens and the tokens' facts fit the ring");
     float *strip = reinterpret_cast<float *>(ring);
     int32_t *facts = reinterpret_cast<int32_t *>(ring + kStrip);
-    const int grp = threadIdx.x / LPR, l = threadIdx.x % LPR;
-    const int n = n0 + 8 * l;  // this lane's first row
+    const int l = threadIdx.x % LPR;  // of a head's row, where it is the same for every piece
     __syncthreads();
     if constexpr (EPI == kMxHead) {
         if (threadIdx.x < T::BM) {
@@ -552,18 +551,23 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
     const uint32_t line = EPI == kMxPart  ? 4u * N
                           : EPI == kMxOut ? 2u * N
                                           : 2u * kHeadDim * (is_q || is_gate ? H : 2 * hkv);
-    const uint32_t at_col = EPI == kMxPart  ? (n < N ? 4u * n : far)
-                            : EPI == kMxOut ? (n < N ? 2u * n : far)
-                                            : 2u * kHeadDim * (is_q ? head : is_gate ? head - H : kv) + 16u * l;
+    const uint32_t head_col = 2u * kHeadDim * (is_q ? head : is_gate ? head - H : kv) + 16u * l;
     const uint8_t *to_at = uniform(static_cast<const uint8_t *>(to));
     const auto rto = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint8_t *>(to_at), 0, __builtin_amdgcn_readfirstlane(to_at ? toks * line : 0u), 0x00020000);
     const uint8_t *res_at = uniform(reinterpret_cast<const uint8_t *>(a.residual ? a.residual + static_cast<size_t>(t0) * N : nullptr));
     const auto rres = ro_rsrc(res_at, __builtin_amdgcn_readfirstlane(EPI == kMxOut && res_at ? toks * line : 0u));
-    // Row j of this lane's group in part i of the tile: its token.
+    // This thread's piece j of part i of the tile: its row of the strip, its
+    // token, and its place from there.
+    auto strip_row = [&](int j) KVA_INLINE { return static_cast<int>(threadIdx.x + kThreads * j) / LPR; };
     auto token = [&](int i, int j) KVA_INLINE {
-        const int sr = grp + kGroups * j;
+        const int sr = strip_row(j);
         return ((sr >> 5) * kTM + i) * 32 + (sr & 31);
+    };
+    auto lane_of = [&](int j) KVA_INLINE { return static_cast<int>(threadIdx.x + kThreads * j) % LPR; };
+    auto at_col = [&](int j) KVA_INLINE {
+        const int n = n0 + 8 * lane_of(j);  // its first row of the weight
+        return EPI == kMxHead ? head_col : n < N ? (EPI == kMxPart ? 4u : 2u) * n : far;
     };
     // What finishing part i reads, requested a part ahead: before the stores
     // that would be waited for with it.
@@ -573,7 +577,7 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
     };
     auto request = [&](Ahead &o, int i) KVA_INLINE {
         if constexpr (EPI == kMxOut) {
-            each<0, kPer>([&](auto j) KVA_INLINE { o.res[j] = rsrc_b128(rres, token(i, j) * line + at_col, 0); });
+            each<0, kPer>([&](auto j) KVA_INLINE { o.res[j] = rsrc_b128(rres, token(i, j) * line + at_col(j), 0); });
         } else if constexpr (EPI == kMxHead) {
             each<0, kPer>([&](auto j) KVA_INLINE {
                 // Tokens past the last carry its position: inside the tables.
@@ -609,7 +613,7 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
             // sums across lanes run side by side.
             uint4 y[kPer], o[kPer];
             auto row = [&](int j, float (&x)[8]) KVA_INLINE {
-                const float *from = strip + (grp + kGroups * j) * kRow + 8 * l;
+                const float *from = strip + strip_row(j) * kRow + 8 * l;
                 const float4_t lo = *reinterpret_cast<const float4_t *>(from), hi = *reinterpret_cast<const float4_t *>(from + 4);
                 x[0] = lo[0], x[1] = lo[1], x[2] = lo[2], x[3] = lo[3], x[4] = hi[0], x[5] = hi[1], x[6] = hi[2], x[7] = hi[3];
                 return make_uint4(pack_h2(x[0], x[1]), pack_h2(x[2], x[3]), pack_h2(x[4], x[5]), pack_h2(x[6], x[7]));
@@ -627,9 +631,9 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
                 });
             }
             if (is_q) {
-                each<0, kPer>([&](auto j) KVA_INLINE { store(o[j], token(i, j) * line + at_col); });
+                each<0, kPer>([&](auto j) KVA_INLINE { store(o[j], token(i, j) * line + at_col(j)); });
             } else {
-                each<0, kPer>([&](auto j) KVA_INLINE { store(y[j], token(i, j) * line + at_col); });
+                each<0, kPer>([&](auto j) KVA_INLINE { store(y[j], token(i, j) * line + at_col(j)); });
             }
             if (kv >= 0) {
                 uint16_t *const pool = kv < hkv ? a.k_pool + kv * kHeadDim : a.v_pool + (kv - hkv) * kHeadDim;
@@ -641,8 +645,8 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
             }
         } else {
             each<0, kPer>([&](auto j) KVA_INLINE {
-                const uint32_t off = token(i, j) * line + at_col;
-                const float *from = strip + (grp + kGroups * j) * kRow + 8 * l;
+                const uint32_t off = token(i, j) * line + at_col(j);
+                const float *from = strip + strip_row(j) * kRow + 8 * lane_of(j);
                 float4_t lo = *reinterpret_cast<const float4_t *>(from), hi = *reinterpret_cast<const float4_t *>(from + 4);
                 if constexpr (EPI == kMxPart) {
                     store(__builtin_bit_cast(uint4, lo), off);
@@ -681,37 +685,50 @@ hipError_t launch_mx_stream(const ProjectArgs &a, const MxProduct &m, int n_cu, 
     return hipGetLastError();
 }
 
-// The tiles, and what 256 values of k of each take on a full chip (us).
+// The tiles, and what they take (us): to start and end, and for 256 values of
+// k where a quarter of the CUs have a tile and where all do (the clock falls
+// with the load: at 5120 -> 14336 the matrix units are busy for 56 % of a clock
+// of 2.1 GHz).
 using MxLaunch = hipError_t (*)(const ProjectArgs &, const MxProduct &, hipStream_t);
 struct MxForm {
     int bm, bn;
-    float us;
+    float fixed, few, all;
     MxLaunch head, out, part;
 };
 template <int BITS, int BM, int BN, int WM, int WN, int S>
-constexpr MxForm mx_form(float us) {
+constexpr MxForm mx_form(float fixed, float few, float all) {
     using T = MxTile<BITS, BM, BN, WM, WN, S>;
-    MxForm f{BM, BN, us, nullptr, launch_mx_gemm<T, kMxOut>, launch_mx_gemm<T, kMxPart>};
+    MxForm f{BM, BN, fixed, few, all, nullptr, launch_mx_gemm<T, kMxOut>, nullptr};
     if constexpr (BN == kHeadDim) f.head = launch_mx_gemm<T, kMxHead>;
+    if constexpr (BM == 64 && BN == 128) f.part = launch_mx_gemm<T, kMxPart>;
     return f;
 }
 const MxForm kForms8[] = {
-    mx_form<8, 256, 256, 2, 2, 3>(4.0f),
-    mx_form<8, 128, 256, 2, 2, 3>(2.2f),
-    mx_form<8, 64, 256, 1, 4, 4>(1.4f),
-    mx_form<8, 128, 128, 2, 2, 4>(1.3f),
-    mx_form<8, 64, 128, 1, 4, 4>(0.9f),
+    mx_form<8, 256, 256, 2, 2, 3>(11.0f, 1.87f, 3.10f), mx_form<8, 128, 256, 2, 2, 4>(7.5f, 0.97f, 1.65f),
+    mx_form<8, 64, 256, 1, 4, 5>(5.2f, 0.61f, 0.94f),   mx_form<8, 128, 320, 2, 2, 4>(8.0f, 1.17f, 2.20f),
+    mx_form<8, 128, 128, 2, 2, 5>(5.5f, 0.65f, 0.95f),  mx_form<8, 64, 128, 1, 4, 6>(4.3f, 0.51f, 0.63f),
 };
 const MxForm kForms4[] = {
-    mx_form<4, 256, 256, 2, 2, 2>(2.8f),
-    mx_form<4, 128, 256, 2, 2, 3>(1.6f),
-    mx_form<4, 64, 256, 1, 4, 3>(1.2f),
-    mx_form<4, 128, 128, 2, 2, 4>(1.1f),
-    mx_form<4, 64, 128, 1, 4, 4>(0.8f),
+    mx_form<4, 256, 256, 2, 2, 2>(10.5f, 1.37f, 2.38f), mx_form<4, 128, 256, 2, 2, 3>(8.0f, 0.65f, 1.12f),
+    mx_form<4, 64, 256, 1, 4, 3>(5.4f, 0.46f, 0.61f),   mx_form<4, 128, 320, 2, 2, 2>(8.0f, 1.01f, 1.63f),
+    mx_form<4, 128, 128, 2, 2, 4>(4.9f, 0.42f, 0.69f),  mx_form<4, 64, 128, 1, 4, 6>(4.6f, 0.35f, 0.41f),
 };
+static_assert(std::size(kForms8) == std::size(kForms4), "one plan for both");
+
+// n tiles of `nc` 256s on n_cu CUs: rounds of the chip, the last as full as it is.
+double rounds_us(const MxForm &f, int64_t n, int nc, int n_cu) {
+    const int64_t whole = n / n_cu;
+    const double fill = static_cast<double>(n - whole * n_cu) / n_cu;
+    double us = whole * (f.fixed + static_cast<double>(nc) * f.all);
+    if (fill > 0) us += f.fixed + nc * (f.few + (f.all - f.few) * std::max(0.0, (fill - 0.25) / 0.75));
+    return us;
+}
 
 }  // namespace
 
+// Up to 32 tokens stream the weights past them; more take the tile, and split of
+// hidden, of the least estimated time.  A split adds its partials, written and
+// read back, and the finish launch.
 bool plan_mx(const ProjectArgs &a, const MxProduct &m, bool heads, int n_cu, size_t part_floats, ProductPlan &plan) {
     const int T = a.n_tok, N = a.n_a + a.n_b;
     plan = ProductPlan{};
@@ -723,19 +740,19 @@ bool plan_mx(const ProjectArgs &a, const MxProduct &m, bool heads, int n_cu, siz
         return !heads || static_cast<size_t>(T) * N <= part_floats;
     }
     const MxForm *forms = m.bits == 8 ? kForms8 : kForms4;
-    const int nc = a.hidden / 512;
+    const int n512 = a.hidden / 512;
     double best_us = 0;
     for (int i = 0; i < static_cast<int>(std::size(kForms8)); ++i) {
         const MxForm &f = forms[i];
         if (heads && a.n_a % f.bn != 0) continue;  // a tile never straddles the two weights
-        const double tiles = static_cast<double>((N + f.bn - 1) / f.bn) * ((T + f.bm - 1) / f.bm);
-        for (int splits = 1; splits <= kGemmMaxSplits && splits <= nc; ++splits) {
+        const int64_t tiles = static_cast<int64_t>((N + f.bn - 1) / f.bn) * ((T + f.bm - 1) / f.bm);
+        for (int splits = 1; splits <= kGemmMaxSplits && splits <= n512; ++splits) {
             const bool partial = splits > 1 || (heads && !f.head);
             const double part = static_cast<double>(splits) * T * N;
-            if (partial && part > static_cast<double>(part_floats)) break;
-            const double rounds = static_cast<double>((static_cast<int64_t>(tiles * splits) + n_cu - 1) / n_cu);
-            double us = rounds * (3.0 + 2 * ((nc + splits - 1) / splits) * f.us);
+            if (partial && (!f.part || part > static_cast<double>(part_floats))) break;
+            double us = rounds_us(f, tiles * splits, 2 * ((n512 + splits - 1) / splits), n_cu);
             if (partial) us += 4.0 + 8.0 * part / 5.0e6;
+            else if (heads) us += 0.02 * f.bm;  // norm, RoPE and three outputs' rows
             if (plan.form < 0 || us < best_us) {
                 plan.form = i;
                 plan.splits = splits;

@@ -1579,6 +1579,7 @@ static int mx_out_impl(kva_cache *c, const MxInput &in, int32_t n_tok, const voi
         return fail(KVA_ERR_INVALID_ARG, "q_dim %d too large", q_dim);
     if (n_out <= 0 || n_out % 16 != 0)
         return fail(KVA_ERR_INVALID_ARG, "n_out %d must be a positive multiple of 16", n_out);
+    if (n_out > kva::kMxMaxRows) return fail(KVA_ERR_UNSUPPORTED, "n_out %d: at most %d", n_out, kva::kMxMaxRows);
     if (static_cast<int64_t>(n_tok) * n_out > INT32_MAX)
         return fail(KVA_ERR_INVALID_ARG, "n_tok x n_out too large");
     const uint64_t out_bytes = static_cast<uint64_t>(n_tok) * n_out * 2;

@@ -286,6 +286,32 @@ def test_out_project_exact(device, bits, n_tok, q_dim, n_out, res):
     cache.destroy()
 
 
+# Every tile by its plan, with token and row remainders.
+@pytest.mark.parametrize("bits,n_tok,q_dim,n_out,tile,partial", [
+    (8, 37, 512, 48, (64, 128), 0), (4, 37, 512, 48, (64, 128), 0), (8, 45, 4096, 16, (64, 128), 1),
+    (4, 45, 4096, 16, (64, 128), 1), (8, 271, 512, 7184, (64, 256), 0), (4, 150, 1536, 14352, (64, 256), 0),
+    (8, 8190, 1024, 336, (128, 128), 0), (4, 271, 512, 7184, (128, 128), 0), (8, 283, 512, 14352, (128, 256), 0),
+    (4, 283, 512, 14352, (128, 256), 0), (8, 1310, 1536, 6160, (128, 320), 0), (4, 1310, 1536, 6160, (128, 320), 0),
+    (8, 1510, 1536, 7184, (256, 256), 0), (4, 1510, 1536, 7184, (256, 256), 0)])
+def test_out_project_each_tile(device, bits, n_tok, q_dim, n_out, tile, partial):
+    rng = np.random.default_rng(n_tok + n_out + bits)
+    say(f"mx_out_project tile {tile} partial={partial} {n_tok} tokens, {q_dim} -> {n_out}, {bits} bits")
+    cache = _any_cache()
+    x, w = _exact_rows(rng, n_tok, q_dim, bits), _exact_rows(rng, n_out, q_dim, 4)
+    r = rng.integers(-8, 9, (n_tok, n_out)).astype(np.float16)
+    guard = np.full((1, n_out), 77.0, np.float16)
+    out = device.array(np.concatenate([r, guard]))
+    cache.mx_out_project(device.array(x[0]), n_tok, q_dim, _pack(device, w), n_out, out, residual=out,
+                         attn_scales=device.array(x[1]), bits=bits)
+    device.synchronize()
+    plan = cache.product_plan()
+    assert (plan["tile_tokens"], plan["tile_rows"]) == tile and plan["partial"] == partial, plan
+    got = out.numpy()
+    assert np.array_equal(got[:n_tok], (mx.decode(*x, bits) @ mx.decode(*w, 4).T + r).astype(np.float16))
+    assert np.array_equal(_bits(got[n_tok:]), _bits(guard))
+    cache.destroy()
+
+
 @pytest.mark.parametrize("bits", [8, 4])
 @pytest.mark.parametrize("n_tok,q_dim,n_out", [(1, 6144, 5120), (7, 2048, 1040), (32, 6144, 5120), (181, 6144, 1040),
                                                (520, 4096, 528)])
@@ -444,6 +470,20 @@ def test_project_exact(device, bits, heads, kv, hidden, n_new):
     rope = [int(x) for x in rng.integers(0, 1024, sum(n_new))]
     r = _step(device, rng, heads, kv, hidden, lengths, n_new, bits, True, rope_pos=rope)
     _check_step(*r, heads, kv, lengths, n_new, True)
+    r[0].destroy()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("heads,kv,n_tok,hidden,tile,partial", [
+    (2, 1, 45, 2048, (64, 128), 1), (2, 1, 45, 512, (64, 256), 0), (24, 4, 283, 512, (128, 256), 0),
+    (16, 4, 813, 512, (256, 256), 0)])
+def test_project_each_tile(device, bits, heads, kv, n_tok, hidden, tile, partial):
+    rng = np.random.default_rng(n_tok + hidden + bits)
+    say(f"mx_project_append tile {tile} partial={partial} {n_tok} tokens, hidden {hidden}, {bits} bits")
+    r = _step(device, rng, heads, kv, hidden, [37], [n_tok], bits, True)
+    plan = r[0].product_plan()
+    assert (plan["tile_tokens"], plan["tile_rows"]) == tile and plan["partial"] == partial, plan
+    _check_step(*r, heads, kv, [37], [n_tok], True)
     r[0].destroy()
 
 

@@ -156,6 +156,8 @@ def test_out_refusals():
         refused(INVALID, out, c, q_dim=q_dim)
     for n_out in (0, -16, 8, 40):
         refused(INVALID, out, c, n_out=n_out)
+    refused(UNSUPPORTED, out, c, n_out=(1 << 20) + 16)
+    refused(NO_DEVICE, out, c, n_out=1 << 20)
     refused(INVALID, out, c, n=1 << 20, n_out=4096)
     refused(INVALID, out, c, q_dim=1 << 25)
     for kw in (dict(o=A), dict(o=A + 5 * 1024 - 16), dict(o=B + 16), dict(o=E, res=E + 16), dict(o=E, res=E - 16)):
