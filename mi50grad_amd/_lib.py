@@ -169,9 +169,17 @@ def check(rc: int, what: str) -> None:
         raise KvaError(rc, what, detail)
 
 
+_functions: dict = {}
+
+
 def call(name: str, *args) -> None:
     """Call ``name`` and raise KvaError on a nonzero return code."""
-    check(getattr(load(), name)(*args), name)
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(load(), name)
+    rc = fn(*args)
+    if rc != 0:
+        check(rc, name)
 
 
 def int_array(values) -> ctypes.Array:

@@ -103,13 +103,13 @@ __device__ __forceinline__ int mx_swizzle(int r) { return ((r >> 1) ^ ((r & 1) <
 
 constexpr int kMxStreamWaves = 8;
 
-// A unit of the streaming form: 128 values of k of RT row tiles and of up to
-// 32 tokens, with their scales, in one of the wave's own S slots.
-template <int BITS_, int RT_>
+// A unit of the streaming form: 128 values of k of RT row tiles and of TOK
+// tokens, with their scales, in one of the wave's own S slots.
+template <int BITS_, int RT_, int TOK_>
 struct MxUnit {
-    static constexpr int BITS = BITS_, RT = RT_;
+    static constexpr int BITS = BITS_, RT = RT_, TOK = TOK_;
     static constexpr int kXRow = 16 * BITS;           // bytes of a token
-    static constexpr int kX = 32 * kXRow, kW = RT * 2048, kXs = 256, kWs = RT * 256;
+    static constexpr int kX = TOK * kXRow < 1024 ? 1024 : TOK * kXRow, kW = RT * 2048, kXs = 256, kWs = RT * 256;
     static constexpr int kSlot = kX + kW + kXs + kWs;
     static constexpr int kLoads = kX / 1024 + kW / 1024 + 1 + RT;
     static constexpr int S = 20 * 1024 / kSlot;       // the LDS shared by eight waves
@@ -124,9 +124,9 @@ struct MxUnit {
 // -> 5120 took 12.6 us).  The waves' sums meet in LDS.  No k is split among
 // workgroups, so with OUT the result is finished here; else fp32 rows go to a
 // finish kernel.
-template <int BITS, int RT, bool OUT>
+template <int BITS, int RT, int TOK, bool OUT>
 __global__ __launch_bounds__(64 * kMxStreamWaves) void mx_stream_kernel(ProjectArgs a, MxProduct m) {
-    using U = MxUnit<BITS, RT>;
+    using U = MxUnit<BITS, RT, TOK>;
     __shared__ __attribute__((aligned(16))) uint8_t ring[kMxStreamWaves][U::S * U::kSlot];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
@@ -154,7 +154,9 @@ __global__ __launch_bounds__(64 * kMxStreamWaves) void mx_stream_kernel(ProjectA
         const int row = kRows * j + lane / kLanes;
         xoff[j] = row * x_row + 16 * ((lane % kLanes) ^ swizzle(row));
     }
-    const uint32_t xs_off = col * s_row, lds0 = lds_addr(ring[wave]);
+    // A column past TOK is a copy of one that is not, and not stored.
+    const int tok = col % TOK;
+    const uint32_t xs_off = tok * s_row, lds0 = lds_addr(ring[wave]);
     // Units past the wave's last go through empty buffers, so that every wait counts alike.
     auto issue = [&](int i) {
         const bool on = i < n;
@@ -189,7 +191,7 @@ __global__ __launch_bounds__(64 * kMxStreamWaves) void mx_stream_kernel(ProjectA
 #pragma unroll
             for (int v = 0; v < XV; ++v) {
                 const int g = BITS == 8 ? 4 * s + 2 * v + half : 2 * s + half;
-                x[s][v] = *reinterpret_cast<const uint4 *>(st + col * U::kXRow + 16 * (g ^ swizzle(col)));
+                x[s][v] = *reinterpret_cast<const uint4 *>(st + tok * U::kXRow + 16 * (g ^ swizzle(tok)));
             }
 #pragma unroll
             for (int j = 0; j < RT; ++j)
@@ -675,14 +677,21 @@ hipError_t launch_mx_gemm(const ProjectArgs &a, const MxProduct &m, hipStream_t 
     return hipGetLastError();
 }
 
-// Two row tiles a workgroup where one would not fit the chip at once.
-template <int BITS, bool OUT>
+template <int BITS, int TOK, bool OUT>
 hipError_t launch_mx_stream(const ProjectArgs &a, const MxProduct &m, int n_cu, hipStream_t s) {
     const int n_rt = (a.n_a + a.n_b + kMxWeightTile - 1) / kMxWeightTile;
     const dim3 block(64 * kMxStreamWaves);
-    if (n_rt > n_cu) hipLaunchKernelGGL((mx_stream_kernel<BITS, 2, OUT>), dim3((n_rt + 1) / 2), block, 0, s, a, m);
-    else hipLaunchKernelGGL((mx_stream_kernel<BITS, 1, OUT>), dim3(n_rt), block, 0, s, a, m);
+    // Two row tiles a workgroup where one would not fit the chip at once.
+    if (n_rt > n_cu) hipLaunchKernelGGL((mx_stream_kernel<BITS, 2, TOK, OUT>), dim3((n_rt + 1) / 2), block, 0, s, a, m);
+    else hipLaunchKernelGGL((mx_stream_kernel<BITS, 1, TOK, OUT>), dim3(n_rt), block, 0, s, a, m);
     return hipGetLastError();
+}
+
+// Up to 8 tokens leave the LDS to the weights: more of them on their way.
+template <int BITS>
+hipError_t launch_mx_stream(const ProjectArgs &a, const MxProduct &m, bool heads, int n_cu, hipStream_t s) {
+    if (heads) return (a.n_tok <= 8 ? launch_mx_stream<BITS, 8, false> : launch_mx_stream<BITS, 32, false>)(a, m, n_cu, s);
+    return (a.n_tok <= 8 ? launch_mx_stream<BITS, 8, true> : launch_mx_stream<BITS, 32, true>)(a, m, n_cu, s);
 }
 
 // The tiles, and what they take (us): to start and end, and for 256 values of
@@ -705,12 +714,12 @@ constexpr MxForm mx_form(float fixed, float few, float all) {
 }
 const MxForm kForms8[] = {
     mx_form<8, 256, 256, 2, 2, 3>(11.0f, 1.87f, 3.10f), mx_form<8, 128, 256, 2, 2, 4>(7.5f, 0.97f, 1.65f),
-    mx_form<8, 64, 256, 1, 4, 5>(5.2f, 0.61f, 0.94f),   mx_form<8, 128, 320, 2, 2, 4>(8.0f, 1.17f, 2.20f),
+    mx_form<8, 64, 256, 2, 2, 4>(5.2f, 0.61f, 0.94f),   mx_form<8, 128, 320, 2, 2, 4>(8.0f, 1.17f, 2.20f),
     mx_form<8, 128, 128, 2, 2, 5>(5.5f, 0.65f, 0.95f),  mx_form<8, 64, 128, 1, 4, 6>(4.3f, 0.51f, 0.63f),
 };
 const MxForm kForms4[] = {
     mx_form<4, 256, 256, 2, 2, 2>(10.5f, 1.37f, 2.38f), mx_form<4, 128, 256, 2, 2, 3>(8.0f, 0.65f, 1.12f),
-    mx_form<4, 64, 256, 1, 4, 3>(5.4f, 0.46f, 0.61f),   mx_form<4, 128, 320, 2, 2, 2>(8.0f, 1.01f, 1.63f),
+    mx_form<4, 64, 256, 2, 2, 3>(5.4f, 0.46f, 0.61f),   mx_form<4, 128, 320, 2, 2, 2>(8.0f, 1.01f, 1.63f),
     mx_form<4, 128, 128, 2, 2, 4>(4.9f, 0.42f, 0.69f),  mx_form<4, 64, 128, 1, 4, 6>(4.6f, 0.35f, 0.41f),
 };
 static_assert(std::size(kForms8) == std::size(kForms4), "one plan for both");
@@ -774,8 +783,7 @@ hipError_t launch_mx_product(const ProjectArgs &args, const MxProduct &m, bool h
     hipError_t e = a.ev_before ? hipEventRecord(a.ev_before, s) : hipSuccess;
     if (e != hipSuccess) return e;
     if (plan.stream) {
-        e = m.bits == 8 ? (heads ? launch_mx_stream<8, false> : launch_mx_stream<8, true>)(a, m, n_cu, s)
-                        : (heads ? launch_mx_stream<4, false> : launch_mx_stream<4, true>)(a, m, n_cu, s);
+        e = m.bits == 8 ? launch_mx_stream<8>(a, m, heads, n_cu, s) : launch_mx_stream<4>(a, m, heads, n_cu, s);
     } else {
         const MxForm &f = (m.bits == 8 ? kForms8 : kForms4)[plan.form];
         e = (plan.partial ? f.part : heads ? f.head : f.out)(a, m, s);

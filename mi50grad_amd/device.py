@@ -86,6 +86,11 @@ class DeviceArray:
         self.ptr = ptr if ptr is not None else dev.malloc(self.nbytes)
         self._owned = ptr is None
 
+    @property
+    def _as_parameter_(self) -> int:
+        """The address, where ctypes takes a pointer."""
+        return self.ptr
+
     @classmethod
     def from_host(cls, dev: GPUDevice, host: np.ndarray) -> "DeviceArray":
         host = np.ascontiguousarray(host)

@@ -275,16 +275,16 @@ class PagedKVCache:
         """project_append() by 4-bit weights (microscale.pack_weights): x is
         microscaled rows of `bits` with their x_scales, or FP16 rows (x_scales
         None) that the call takes to `bits`."""
-        _lib.call("kva_mx_project_append", self.handle, layer, _ptr(x), _ptr(x_scales), bits, hidden,
-                  _ptr(w_q_packed), _ptr(w_kv_packed), _ptr(q_norm_w), _ptr(k_norm_w), _ptr(cos_tab), _ptr(sin_tab),
-                  table_rows, _ptr(q_out), _ptr(q_gate_out), _ptr(kv_out), stream)
+        _lib.call("kva_mx_project_append", self.handle, layer, x, x_scales, bits, hidden,
+                  w_q_packed, w_kv_packed, q_norm_w, k_norm_w, cos_tab, sin_tab,
+                  table_rows, q_out, q_gate_out, kv_out, stream)
 
     def mx_out_project(self, attn, n_tok: int, q_dim: int, w_o_packed, n_out: int, out, residual=None,
                        attn_scales=None, bits: int = 8, stream=None) -> None:
         """out_project() by 4-bit weights: attn is FP16 rows that the call
         takes to `bits`, or microscaled rows of `bits` with attn_scales."""
-        _lib.call("kva_mx_out_project", self.handle, _ptr(attn), _ptr(attn_scales), bits, n_tok, q_dim,
-                  _ptr(w_o_packed), n_out, _ptr(residual), _ptr(out), stream)
+        _lib.call("kva_mx_out_project", self.handle, attn, attn_scales, bits, n_tok, q_dim,
+                  w_o_packed, n_out, residual, out, stream)
 
     def decode(self, layer: int, q, out, stream=None, gate=None, gate_stride: int = 0) -> None:
         """Decode attention; with `gate`, the output gate (out *= sigmoid(gate),

@@ -10,7 +10,7 @@ multiply: weights in 4 bits, quantised and packed once,
     pack_weights(codes, scales, rows, cols, packed)
 
 and activations in 8 or 4, per step.  Tensors are integer device addresses or
-``DeviceArray``s; no cache is needed.  The reference has no counterpart but its
+``DeviceArray``s (ctypes takes either); no cache is needed.  The reference has no counterpart but its
 engine's own RMSNorm launches (engine.py:3043-3139).
 """
 from __future__ import annotations
@@ -18,18 +18,17 @@ from __future__ import annotations
 import ctypes
 
 from . import _lib
-from .kv_cache import _ptr
 
 
 def quantize(x, rows: int, cols: int, bits: int, codes, scales, x_stride: int = 0, stream=None) -> None:
     """x [rows, cols] FP16 (x_stride values between rows; 0: cols) as codes
     [rows, cols * bits / 8] and scales [rows, cols / 32]."""
-    _lib.call("kva_mx_quantize", _ptr(x), x_stride or cols, rows, cols, bits, _ptr(codes), _ptr(scales), stream)
+    _lib.call("kva_mx_quantize", x, x_stride or cols, rows, cols, bits, codes, scales, stream)
 
 
 def dequantize(codes, scales, rows: int, cols: int, bits: int, y, stream=None) -> None:
     """The values of microscaled rows, y [rows, cols] FP16."""
-    _lib.call("kva_mx_dequantize", _ptr(codes), _ptr(scales), rows, cols, bits, _ptr(y), stream)
+    _lib.call("kva_mx_dequantize", codes, scales, rows, cols, bits, y, stream)
 
 
 def packed_bytes(rows: int, cols: int) -> int:
@@ -41,7 +40,7 @@ def packed_bytes(rows: int, cols: int) -> int:
 
 def pack_weights(codes, scales, rows: int, cols: int, packed, stream=None) -> None:
     """4-bit weight rows in the order that the products read."""
-    _lib.call("kva_mx_pack_weights", _ptr(codes), _ptr(scales), rows, cols, _ptr(packed), stream)
+    _lib.call("kva_mx_pack_weights", codes, scales, rows, cols, packed, stream)
 
 
 def add_rmsnorm(hidden, delta, w, n_tok: int, cols: int, eps: float, out, sum_out=None, scales=None, bits: int = 16,
@@ -49,5 +48,5 @@ def add_rmsnorm(hidden, delta, w, n_tok: int, cols: int, eps: float, out, sum_ou
     """sum_out = hidden + delta and out = its RMSNorm times w, as FP16 rows or
     (bits 8 or 4, with scales) microscaled ones; delta and sum_out None: the
     norm of hidden."""
-    _lib.call("kva_add_rmsnorm", _ptr(hidden), _ptr(delta), _ptr(w), n_tok, cols, eps, bits, _ptr(out), _ptr(scales),
-              _ptr(sum_out), stream)
+    _lib.call("kva_add_rmsnorm", hidden, delta, w, n_tok, cols, eps, bits, out, scales,
+              sum_out, stream)
