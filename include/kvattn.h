@@ -246,8 +246,8 @@ int kva_project_append(kva_cache *cache, int32_t layer, const void *x, int32_t h
 #define KVA_PROJECT_KERNELS 0
 #define KVA_PROJECT_PREFILL_GEMM 1
 int kva_get_project_path(const kva_cache *cache, int32_t *path);
-/* The launch of the last kva_project_append or kva_out_project on this cache
- * that passed its checks (its first, where it took several; on a host-only
+/* The launch of the last kva_project_append or kva_out_project (or of their
+ * kva_mx_ forms) on this cache that passed its checks (its first, where it took several; on a host-only
  * cache the one it would have made): tokens and weight rows of a GEMM tile
  * (0: weights streamed past x held in registers), tokens of the low tiles of
  * a launch of two heights (0: one height), slices that hidden was split
@@ -424,7 +424,7 @@ int kva_evict(kva_cache *cache, int32_t n_seqs, const int32_t *src_ids, const in
  * elements x/scale rounded to the nearest, ties to even; a block in which a
  * value is not finite is NaN.  Rows from elsewhere in this format are taken as
  * they are.  All of it but the products needs no cache and may be recorded
- * into a graph.  Pointers are 16-byte aligned and, where nothing else is said,
+ * into a graph; it takes at most 2^40 values a call.  Pointers are 16-byte aligned and, where nothing else is said,
  * outputs overlap no operand (KVA_ERR_INVALID_ARG).  bits is 8 or 4
  * (KVA_ERR_UNSUPPORTED).  The reference holds 4-bit weights for its other
  * layers as integers with an fp16 scale per group (its GPTQ form); its
@@ -508,8 +508,8 @@ int kva_get_decode_split(const kva_cache *cache, int32_t *split_tokens,
  * kva_event_elapsed_ms(before, after) is that kernel's own duration: the
  * decode kernel of kva_decode / kva_append_decode (without the combine
  * launch or the append), mq_kernel of kva_prefill / kva_tree_verify
- * (without its combine), the GEMM of kva_project_append / kva_out_project
- * (without the finish kernel).  A call that launches its main kernel more
+ * (without its combine), the GEMM of kva_project_append / kva_out_project and
+ * of their kva_mx_ forms (without the finish kernel or the rows' quantisation).  A call that launches its main kernel more
  * than once (chunked projections) records around each, so the events hold
  * the last.  Both NULL: off.  Refused while a graph is being recorded.     */
 int kva_kernel_events(kva_cache *cache, kva_event_t before, kva_event_t after);

@@ -147,9 +147,8 @@ __device__ __forceinline__ void load_to_lds_at(__amdgpu_buffer_rsrc_t r, uint32_
         : "memory", "m0");
 }
 
-// One dword per lane of a buffer to LDS (lane l's to lds + 4*l), read only to
-// bring its 128-byte line into the XCD's L2.
-__device__ __forceinline__ void touch_line(__amdgpu_buffer_rsrc_t r, uint32_t lds, uint32_t voff, uint32_t soff) {
+// The same of one dword per lane (lane l's to lds + 4*l).
+__device__ __forceinline__ void word_to_lds_at(__amdgpu_buffer_rsrc_t r, uint32_t lds, uint32_t voff, uint32_t soff) {
     asm volatile(
         "s_mov_b32 m0, %0\n\t"
         "s_nop 0\n\t"
@@ -157,6 +156,12 @@ __device__ __forceinline__ void touch_line(__amdgpu_buffer_rsrc_t r, uint32_t ld
         :
         : "s"(lds), "v"(voff), "s"(r), "s"(soff)
         : "memory", "m0");
+}
+
+// One dword per lane of a buffer to LDS, read only to bring its 128-byte line
+// into the XCD's L2.
+__device__ __forceinline__ void touch_line(__amdgpu_buffer_rsrc_t r, uint32_t lds, uint32_t voff, uint32_t soff) {
+    word_to_lds_at(r, lds, voff, soff);
 }
 
 // Wait until at most N of this wave's vector-memory operations are

@@ -168,12 +168,12 @@ __global__ __launch_bounds__(64 * kMxStreamWaves) void mx_stream_kernel(ProjectA
             const auto rw = ro_rsrc(w_at[j], on ? w_size[j] * 16 : 0u), rs = ro_rsrc(ws_at[j], on ? w_size[j] + 0u : 0u);
             load_to_lds_at(rw, st + U::kX + 2048 * j, 16 * lane, u * 2048);
             load_to_lds_at(rw, st + U::kX + 2048 * j + 1024, 16 * lane + 1024, u * 2048);
-            touch_line(rs, st + U::kX + U::kW + U::kXs + 256 * j, 4 * lane, u / 2 * 256);
+            word_to_lds_at(rs, st + U::kX + U::kW + U::kXs + 256 * j, 4 * lane, u / 2 * 256);
         }
         const auto rx = ro_rsrc(m.x, toks * x_row), rxs = ro_rsrc(m.x_scales, toks * s_row);
 #pragma unroll
         for (int j = 0; j < U::kX / 1024; ++j) load_to_lds_at(rx, st + 1024 * j, xoff[j], u * U::kXRow);
-        touch_line(rxs, st + U::kX + U::kW, xs_off, u * 4);
+        word_to_lds_at(rxs, st + U::kX + U::kW, xs_off, u * 4);
     };
     float16_t acc[RT];
 #pragma unroll

@@ -1453,6 +1453,14 @@ static int check_mx_bits(int32_t bits) {
     return KVA_OK;
 }
 
+// Rows that a kernel is launched over: a grid counts them in 31 bits.
+static int check_mx_size(int64_t rows, int64_t stride) {
+    if (stride > kva::kMxMaxValues || rows * stride > kva::kMxMaxValues)
+        return fail(KVA_ERR_UNSUPPORTED, "%lld rows of %lld values", static_cast<long long>(rows),
+                    static_cast<long long>(stride));
+    return KVA_OK;
+}
+
 static int check_mx_shape(int32_t rows, int32_t cols, int32_t quantum) {
     if (rows < 0) return fail(KVA_ERR_INVALID_ARG, "%d rows", rows);
     if (cols <= 0 || cols % quantum != 0)
@@ -1638,6 +1646,7 @@ int kva_mx_quantize(const void *x, int64_t x_stride, int32_t rows, int32_t cols,
     if (x_stride < cols || x_stride % 8 != 0)
         return fail(KVA_ERR_INVALID_ARG, "x_stride %lld: at least cols and a multiple of 8",
                     static_cast<long long>(x_stride));
+    if ((rc = check_mx_size(rows, x_stride))) return rc;
     if (rows == 0) return KVA_OK;
     if (!x || !codes || !scales) return fail(KVA_ERR_INVALID_ARG, "NULL pointer");
     if (!aligned16(x) || !aligned16(codes) || !aligned16(scales))
@@ -1662,6 +1671,7 @@ int kva_mx_dequantize(const void *codes, const void *scales, int32_t rows, int32
                       kva_stream_t stream) {
     int rc = check_mx_bits(bits);
     if (!rc) rc = check_mx_shape(rows, cols, kva::kMxBlock);
+    if (!rc) rc = check_mx_size(rows, cols);
     if (rc) return rc;
     if (rows == 0) return KVA_OK;
     if (!codes || !scales || !y) return fail(KVA_ERR_INVALID_ARG, "NULL pointer");
@@ -1683,7 +1693,9 @@ int kva_mx_dequantize(const void *codes, const void *scales, int32_t rows, int32
 
 int kva_mx_pack_weights(const void *codes, const void *scales, int32_t rows, int32_t cols, void *packed,
                         kva_stream_t stream) {
-    if (int rc = check_mx_shape(rows, cols, kva::kProjHiddenQuantum)) return rc;
+    int rc = check_mx_shape(rows, cols, kva::kProjHiddenQuantum);
+    if (!rc) rc = check_mx_size(rows, cols);
+    if (rc) return rc;
     if (rows == 0) return KVA_OK;
     if (!codes || !scales || !packed) return fail(KVA_ERR_INVALID_ARG, "NULL pointer");
     if (!aligned16(codes) || !aligned16(scales) || !aligned16(packed))

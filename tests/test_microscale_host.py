@@ -48,6 +48,12 @@ def test_quantize_refusals():
     refused(INVALID, ms.quantize, A, 4, 64, 8, B, B + 240)
     refused(INVALID, ms.dequantize, A, B, 4, 64, 8, A - 496)
     refused(INVALID, ms.dequantize, A, B, 4, 64, 8, B)
+    # more than 2^40 values
+    refused(UNSUPPORTED, ms.quantize, A, 1 << 21, 64, 8, 1 << 60, 1 << 61, x_stride=(1 << 19) + 8)
+    refused(UNSUPPORTED, ms.quantize, A, 1, 64, 8, B, C, x_stride=(1 << 40) + 8)
+    refused(UNSUPPORTED, ms.quantize, A, 2 ** 31 - 1, 64, 8, B, C, x_stride=2 ** 63 - 8)
+    refused(UNSUPPORTED, ms.dequantize, A, B, 2 ** 31 - 1, 1024, 8, C)
+    refused(UNSUPPORTED, ms.pack_weights, A, B, 2 ** 31 - 1, 1024, C)
     ms.quantize(None, 0, 64, 8, None, None)  # nothing to do
     ms.dequantize(None, None, 0, 64, 8, None)
 
