@@ -313,7 +313,8 @@ def test_out_project_each_tile(device, bits, n_tok, q_dim, n_out, tile, partial)
 
 
 @pytest.mark.parametrize("bits", [8, 4])
-@pytest.mark.parametrize("n_tok,q_dim,n_out", [(1, 6144, 5120), (7, 2048, 1040), (32, 6144, 5120), (181, 6144, 1040),
+@pytest.mark.parametrize("n_tok,q_dim,n_out", [(1, 6144, 5120), (7, 2048, 1040), (8, 512, 16), (3, 1536, 8208),
+                                               (9, 1024, 336), (32, 6144, 5120), (181, 6144, 1040),
                                                (520, 4096, 528)])
 def test_out_project_quantises_fp16_rows(device, bits, n_tok, q_dim, n_out):
     """fp16 rows give the bits that their microscaled rows give, and both are
@@ -323,6 +324,8 @@ def test_out_project_quantises_fp16_rows(device, bits, n_tok, q_dim, n_out):
     cache = _any_cache()
     x = (rng.standard_normal((n_tok, q_dim)) * 2.0 ** rng.integers(-3, 3, (n_tok, 1))).astype(np.float16)
     x[:, ::97] *= 10
+    x[0, 32:64] = 0
+    x[n_tok // 2, 64:96] *= 2.0 ** -14  # subnormal
     w = _random_rows(rng, n_out, q_dim, 4)
     r = rng.standard_normal((n_tok, n_out)).astype(np.float16)
     packed, dr = _pack(device, w), device.array(r)
@@ -337,6 +340,26 @@ def test_out_project_quantises_fp16_rows(device, bits, n_tok, q_dim, n_out):
     y, off = _product(mx.quantized(x, bits), mx.decode(*w, 4))
     y = y + r
     assert (np.abs(got - y) <= _half_step(y) + off).all()
+    cache.destroy()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("n_tok", [2, 8, 20])
+def test_fp16_rows_that_are_not_finite(device, bits, n_tok):
+    """A row with an infinity or NaN gives NaN, the others what they give without."""
+    rng = np.random.default_rng(n_tok + bits)
+    q_dim, n_out = 1024, 48
+    say(f"mx_out_project of fp16 rows that are not finite, {n_tok} tokens, {bits} bits")
+    cache = _any_cache()
+    v = rng.integers(-3, 4, (n_tok, q_dim)).astype(np.float16)  # exact in 4 and 8 bits
+    w = _exact_rows(rng, n_out, q_dim, 4)
+    y = v.astype(np.float64) @ mx.decode(*w, 4).T
+    v[0, 17], v[1, 1000] = np.nan, -np.inf
+    y[:2] = np.nan
+    out = device.empty((n_tok, n_out), np.float16)
+    cache.mx_out_project(device.array(v), n_tok, q_dim, _pack(device, w), n_out, out, bits=bits)
+    device.synchronize()
+    assert np.array_equal(out.numpy(), y.astype(np.float16), equal_nan=True)
     cache.destroy()
 
 
