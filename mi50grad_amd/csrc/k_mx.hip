@@ -1,7 +1,10 @@
 // Rows as microscaled rows and back, the order in which the products take
 // 4-bit weights, and the norm that leaves microscaled rows (gfx950).
 //
-// All of it streams memory: bytes read and written once at the rate of a copy.
+// All of it is bound by memory where there is enough: bytes are read and written
+// once, a lane taking 16 bytes of fp16 (a large copy runs at 4.8 TB/s here; what
+// the last kernel left in the caches is read faster).  A few rows take what a
+// launch takes, 1.4 to 2.5 us.
 #include "k_mx.h"
 #include "kva_internal.h"
 
@@ -19,7 +22,8 @@ __device__ __forceinline__ void half8_to_float(uint4 v, float (&x)[8]) {
     }
 }
 
-// A lane takes eight values of a row, four lanes a block.
+// A lane takes eight values of a row, four lanes a block.  5120 x 6144 to 4 bits:
+// 18.5 us, 4.3 TB/s (two pieces of a lane on their way: the same).
 template <int BITS>
 __global__ __launch_bounds__(kMxThreads) void mx_quantize_kernel(MxRows a) {
     const uint32_t per_row = a.cols / 8;
@@ -32,7 +36,8 @@ __global__ __launch_bounds__(kMxThreads) void mx_quantize_kernel(MxRows a) {
     mx_store_quad<BITS>(x, a.codes, a.scales, static_cast<size_t>(i) * 8);
 }
 
-// A lane gives eight values.
+// A lane gives eight values.  5120 x 6144 of 4 bits: 12.8 us, 6.2 TB/s, with the
+// codes in the caches; 8192 x 5120 of 8 bits: 20 us, 6.3 TB/s.
 template <int BITS>
 __global__ __launch_bounds__(kMxThreads) void mx_dequantize_kernel(MxRows a) {
     const int64_t i = static_cast<int64_t>(blockIdx.x) * kMxThreads + threadIdx.x;
@@ -62,7 +67,8 @@ __global__ __launch_bounds__(kMxThreads) void mx_dequantize_kernel(MxRows a) {
 // Weight rows in the order of the products' A operand (MxWeight): lane l of a
 // wave takes row l % 32's 16 bytes of block 2 * step + l / 32.  Rows past the
 // last are zeros.  A wave moves four steps (256 values of 32 rows), and with
-// them the dword of scales that each lane needs for those.
+// them the dword of scales that each lane needs for those.  Weights are packed
+// once: 12288 x 5120 in 23 us, 2.9 TB/s.
 __global__ __launch_bounds__(kMxThreads) void mx_pack_kernel(MxPack a) {
     const int lane = threadIdx.x & 63;
     const int n_quad = a.cols / 256;
@@ -92,7 +98,8 @@ __global__ __launch_bounds__(kMxThreads) void mx_pack_kernel(MxPack a) {
 // hidden + delta (rounded to fp16: the residual stream's type) and its norm,
 // x = s / sqrt(mean(s^2) + eps) * w over the rounded sums, rounded once to what
 // is asked for.  A workgroup takes a row and holds it in registers, so every
-// byte is read once; lanes past the row hold zeros.
+// byte is read once; lanes past the row hold zeros.  8192 x 5120 to 8 bits: 59
+// us, 5.0 TB/s; 2048 x 5120 to fp16: 14.5 us, 5.8 TB/s.
 template <int BITS, int PER>
 __global__ __launch_bounds__(1024) void add_rmsnorm_kernel(MxNorm a) {
     __shared__ float red[16];

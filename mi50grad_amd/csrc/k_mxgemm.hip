@@ -8,6 +8,24 @@
 // block (the instruction's order for 8 bits), of a 4-bit B its block l / 32,
 // and of both one scale byte, of block l / 32; the result's register 4 q + j
 // is token l % 32's row 8 q + 4 (l / 32) + j.
+//
+// Up to 32 tokens are bound by the weights, 17 bytes of each 32 values: 39 MB at
+// 5120 -> 14336 (a read of memory takes 6.6 us).  mx_stream_kernel takes 8.8 us
+// for one token and 10.5 to 12 for 32 of 8 bits, and 6.3 and 8.3 at 6144 -> 5120
+// (17 MB, 3.0 us), where 160 workgroups do not fill the chip.
+//
+// More tokens are bound by the matrix units, or rather by what clock the card's
+// power leaves them.  2048 tokens by mx_gemm_kernel, in us (and PFLOP/s), and a
+// library's plain product of the same types with fp16 outputs:
+//   5120 -> 14336, norm, RoPE and append   8 bits 134 (2.2)   4 bits 111 (2.7)
+//     plain product                               124                117
+//   6144 -> 5120 and a residual            8 bits  52 (2.5)   4 bits  51
+//     plain product                                62                 67
+// A tile of 256 x 256 starts in 2.3 us (its first stages) and ends in 7, or 13
+// as a head; between, its loads, LDS reads and products are interleaved step by
+// step, so that none of them waits in a row for the others.  Between 33 and some
+// 500 tokens the tiles do not fill the chip, and the latency of a chunk times
+// their number bounds: 181 tokens take 19 us, where the products would take 10.
 #include <algorithm>
 #include <iterator>
 #include <type_traits>
@@ -349,8 +367,8 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
     }
     // A load of scales, for 512 values of k: 16 bytes of 64 tokens, or 512 of
     // two row tiles, or none, where a wave loads only to keep its count.  (Four
-    // bytes of a token per chunk of 128 brought a line each time: a third of
-    // the L2's traffic.)
+    // bytes of a token per chunk of 128 would bring a line each time.  At 2048 x
+    // 14336 x 5120 that took the same: 145.7 us against 145.2.)
     const uint8_t *sm_at[T::kLoadsS];
     uint32_t sm_size[T::kLoadsS], sm_step[T::kLoadsS], sm_off[T::kLoadsS];
 #pragma unroll
@@ -681,13 +699,16 @@ template <int BITS, int TOK, bool OUT>
 hipError_t launch_mx_stream(const ProjectArgs &a, const MxProduct &m, int n_cu, hipStream_t s) {
     const int n_rt = (a.n_a + a.n_b + kMxWeightTile - 1) / kMxWeightTile;
     const dim3 block(64 * kMxStreamWaves);
-    // Two row tiles a workgroup where one would not fit the chip at once.
+    // Two row tiles a workgroup where one would not fit the chip at once: 5120 ->
+    // 14336 side by side, 9.9 us for one token and 11.4 for 32, by one 11.3 and 14.9.
     if (n_rt > n_cu) hipLaunchKernelGGL((mx_stream_kernel<BITS, 2, TOK, OUT>), dim3((n_rt + 1) / 2), block, 0, s, a, m);
     else hipLaunchKernelGGL((mx_stream_kernel<BITS, 1, TOK, OUT>), dim3(n_rt), block, 0, s, a, m);
     return hipGetLastError();
 }
 
-// Up to 8 tokens leave the LDS to the weights: more of them on their way.
+// Up to 8 tokens leave the LDS to the weights: more of them on their way.  One
+// token of 5120 -> 14336: 8.5 us, with room for 32 tokens 8.9; 8 and 9 tokens of
+// 8 bits take 9.1 and 10.5.
 template <int BITS>
 hipError_t launch_mx_stream(const ProjectArgs &a, const MxProduct &m, bool heads, int n_cu, hipStream_t s) {
     if (heads) return (a.n_tok <= 8 ? launch_mx_stream<BITS, 8, false> : launch_mx_stream<BITS, 32, false>)(a, m, n_cu, s);
@@ -696,8 +717,10 @@ hipError_t launch_mx_stream(const ProjectArgs &a, const MxProduct &m, bool heads
 
 // The tiles, and what they take (us): to start and end, and for 256 values of
 // k where a quarter of the CUs have a tile and where all do (the clock falls
-// with the load: at 5120 -> 14336 the matrix units are busy for 56 % of a clock
-// of 2.1 GHz).
+// with the load), measured tile by tile.  Side by side, 2048 tokens of 5120 ->
+// 14336 took 143.5 us by 256 x 256, 153 by 128 x 256 and 155 by a tile of 192 x
+// 256 that is not here; 6144 -> 5120 is 256 tiles of 128 x 320, but 320 of 128 x
+// 256, 64 of them in a second round.
 using MxLaunch = hipError_t (*)(const ProjectArgs &, const MxProduct &, hipStream_t);
 struct MxForm {
     int bm, bn;
@@ -737,7 +760,9 @@ double rounds_us(const MxForm &f, int64_t n, int nc, int n_cu) {
 
 // Up to 32 tokens stream the weights past them; more take the tile, and split of
 // hidden, of the least estimated time.  A split adds its partials, written and
-// read back, and the finish launch.
+// read back, and the finish launch.  At the border, 32 tokens streamed take 8.3
+// us at 6144 -> 5120, 33 by four splits and their finish 7.6 + 3.1; with norm and
+// RoPE at 5120 -> 14336 both need the finish, and take 12.2 and 11.4 before it.
 bool plan_mx(const ProjectArgs &a, const MxProduct &m, bool heads, int n_cu, size_t part_floats, ProductPlan &plan) {
     const int T = a.n_tok, N = a.n_a + a.n_b;
     plan = ProductPlan{};
