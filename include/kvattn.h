@@ -1,7 +1,8 @@
 /*
  * kvattn.h — C ABI of libkvattn.so, the MI355X (gfx950) full-attention
  * KV-cache path: paged FP16 or 8-bit K/V cache, fused QK-RMSNorm + RoPE + K/V append,
- * split-K GQA decode, chunked causal prefill and tree-verify attention.
+ * split-K GQA decode, chunked causal prefill and tree-verify attention, and
+ * the projections around it in fp16 or by microscaled 4-bit weights.
  *
  * Conventions (the reference's host wrappers use the same ones):
  *   - every pointer argument named q, k, v, out, x, w, cos_*, sin_*, *_base,
@@ -424,9 +425,9 @@ int kva_evict(kva_cache *cache, int32_t n_seqs, const int32_t *src_ids, const in
  * elements x/scale rounded to the nearest, ties to even; a block in which a
  * value is not finite is NaN.  Rows from elsewhere in this format are taken as
  * they are.  All of it but the products needs no cache and may be recorded
- * into a graph; it takes at most 2^40 values a call.  Pointers are 16-byte aligned and, where nothing else is said,
- * outputs overlap no operand (KVA_ERR_INVALID_ARG).  bits is 8 or 4
- * (KVA_ERR_UNSUPPORTED).  The reference holds 4-bit weights for its other
+ * into a graph; it takes at most 2^40 values a call.  Pointers are 16-byte
+ * aligned and, where nothing else is said, outputs overlap no operand
+ * (KVA_ERR_INVALID_ARG).  bits is 8 or 4 (KVA_ERR_UNSUPPORTED).  The reference holds 4-bit weights for its other
  * layers as integers with an fp16 scale per group (its GPTQ form); its
  * attention projections are fp16.                                           */
 /* x [rows][cols] fp16, x_stride values between rows (a multiple of 8, at least
@@ -470,8 +471,8 @@ int kva_mx_project_append(kva_cache *cache, int32_t layer, const void *x, const 
  * residual[t]).  attn is fp16 rows [n_tok][q_dim], taken to `bits` on the way
  * (attn_scales NULL), or microscaled rows.  residual NULL, apart from out, or
  * out itself.  q_dim a multiple of 512, n_out of 16, at most 1048576
- * (KVA_ERR_UNSUPPORTED); a token's microscaled row has to fit half of the cache's projection workspace
- * (KVA_ERR_INVALID_ARG).                                                    */
+ * (KVA_ERR_UNSUPPORTED); a token's microscaled row has to fit half of the
+ * cache's projection workspace (KVA_ERR_INVALID_ARG).                       */
 int kva_mx_out_project(kva_cache *cache, const void *attn, const void *attn_scales, int32_t bits,
                        int32_t n_tok, int32_t q_dim, const void *w_o_packed, int32_t n_out,
                        const void *residual, void *out, kva_stream_t stream);

@@ -10,8 +10,8 @@ multiply: weights in 4 bits, quantised and packed once,
     pack_weights(codes, scales, rows, cols, packed)
 
 and activations in 8 or 4, per step.  Tensors are integer device addresses or
-``DeviceArray``s (ctypes takes either); no cache is needed.  The reference has no counterpart but its
-engine's own RMSNorm launches (engine.py:3043-3139).
+``DeviceArray``s (ctypes takes either); no cache is needed.  The reference has
+no counterpart but its engine's own RMSNorm launches (engine.py:3043-3139).
 """
 from __future__ import annotations
 
