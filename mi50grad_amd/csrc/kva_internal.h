@@ -151,7 +151,9 @@ constexpr int kMxBlock = 32;          // elements of a scale
 constexpr int kMxWeightTile = 32;     // rows of a packed weight's tile
 constexpr int kMxStreamTokens = 32;   // most tokens of the form that streams the weights past them
 constexpr int kMxMaxRows = 1 << 20;   // rows of an output projection's weight, at most (a tile's offsets have 31 bits)
-constexpr int64_t kMxMaxValues = int64_t{1} << 40;  // of rows that are quantised, read or packed at once
+// Values of a call, at most: a launch counts its lanes, eight values each, in 32
+// bits.  And values between the first row and the last.
+constexpr int64_t kMxMaxValues = int64_t{1} << 34, kMxMaxSpan = int64_t{1} << 40;
 constexpr int kMxNormMax = 32768;     // values of a normalised row, at most
 struct MxRows {
     const uint16_t *x;        // quantize: [rows] of x_stride values
