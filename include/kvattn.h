@@ -425,7 +425,7 @@ int kva_evict(kva_cache *cache, int32_t n_seqs, const int32_t *src_ids, const in
  * elements x/scale rounded to the nearest, ties to even; a block in which a
  * value is not finite is NaN.  Rows from elsewhere in this format are taken as
  * they are.  All of it but the products needs no cache and may be recorded
- * into a graph; it takes at most 2^40 values a call.  Pointers are 16-byte
+ * into a graph; it takes at most 2^34 values a call.  Pointers are 16-byte
  * aligned and, where nothing else is said, outputs overlap no operand
  * (KVA_ERR_INVALID_ARG).  bits is 8 or 4 (KVA_ERR_UNSUPPORTED).  The reference holds 4-bit weights for its other
  * layers as integers with an fp16 scale per group (its GPTQ form); its

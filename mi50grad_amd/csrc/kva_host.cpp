@@ -1453,11 +1453,11 @@ static int check_mx_bits(int32_t bits) {
     return KVA_OK;
 }
 
-// Rows that a kernel is launched over: a grid counts them in 31 bits.
-static int check_mx_size(int64_t rows, int64_t stride) {
-    if (stride > kva::kMxMaxValues || rows * stride > kva::kMxMaxValues)
-        return fail(KVA_ERR_UNSUPPORTED, "%lld rows of %lld values", static_cast<long long>(rows),
-                    static_cast<long long>(stride));
+// Rows that a kernel is launched over.
+static int check_mx_size(int64_t rows, int64_t cols, int64_t stride) {
+    if (rows * cols > kva::kMxMaxValues || stride > kva::kMxMaxSpan || rows * stride > kva::kMxMaxSpan)
+        return fail(KVA_ERR_UNSUPPORTED, "%lld rows of %lld values, %lld apart", static_cast<long long>(rows),
+                    static_cast<long long>(cols), static_cast<long long>(stride));
     return KVA_OK;
 }
 
@@ -1646,7 +1646,7 @@ int kva_mx_quantize(const void *x, int64_t x_stride, int32_t rows, int32_t cols,
     if (x_stride < cols || x_stride % 8 != 0)
         return fail(KVA_ERR_INVALID_ARG, "x_stride %lld: at least cols and a multiple of 8",
                     static_cast<long long>(x_stride));
-    if ((rc = check_mx_size(rows, x_stride))) return rc;
+    if ((rc = check_mx_size(rows, cols, x_stride))) return rc;
     if (rows == 0) return KVA_OK;
     if (!x || !codes || !scales) return fail(KVA_ERR_INVALID_ARG, "NULL pointer");
     if (!aligned16(x) || !aligned16(codes) || !aligned16(scales))
@@ -1671,7 +1671,7 @@ int kva_mx_dequantize(const void *codes, const void *scales, int32_t rows, int32
                       kva_stream_t stream) {
     int rc = check_mx_bits(bits);
     if (!rc) rc = check_mx_shape(rows, cols, kva::kMxBlock);
-    if (!rc) rc = check_mx_size(rows, cols);
+    if (!rc) rc = check_mx_size(rows, cols, cols);
     if (rc) return rc;
     if (rows == 0) return KVA_OK;
     if (!codes || !scales || !y) return fail(KVA_ERR_INVALID_ARG, "NULL pointer");
@@ -1694,7 +1694,7 @@ int kva_mx_dequantize(const void *codes, const void *scales, int32_t rows, int32
 int kva_mx_pack_weights(const void *codes, const void *scales, int32_t rows, int32_t cols, void *packed,
                         kva_stream_t stream) {
     int rc = check_mx_shape(rows, cols, kva::kProjHiddenQuantum);
-    if (!rc) rc = check_mx_size(rows, cols);
+    if (!rc) rc = check_mx_size(rows, cols, cols);
     if (rc) return rc;
     if (rows == 0) return KVA_OK;
     if (!codes || !scales || !packed) return fail(KVA_ERR_INVALID_ARG, "NULL pointer");
@@ -1720,6 +1720,8 @@ int kva_add_rmsnorm(const void *hidden, const void *delta, const void *w, int32_
         if (int rc = check_mx_bits(bits)) return rc;
     if (int rc = check_mx_shape(n_tok, cols, kva::kMxBlock)) return rc;
     if (cols > kva::kMxNormMax) return fail(KVA_ERR_UNSUPPORTED, "%d columns: at most %d", cols, kva::kMxNormMax);
+    // A row has up to 64 lanes without values.
+    if (int rc = check_mx_size(n_tok, cols + 512, cols)) return rc;
     if (!(eps >= 0.0f)) return fail(KVA_ERR_INVALID_ARG, "eps %g", static_cast<double>(eps));
     if (n_tok == 0) return KVA_OK;
     if (!hidden || !w || !out) return fail(KVA_ERR_INVALID_ARG, "NULL pointer");

@@ -48,7 +48,7 @@ def test_quantize_refusals():
     refused(INVALID, ms.quantize, A, 4, 64, 8, B, B + 240)
     refused(INVALID, ms.dequantize, A, B, 4, 64, 8, A - 496)
     refused(INVALID, ms.dequantize, A, B, 4, 64, 8, B)
-    # more than 2^40 values
+    # more values, or further apart, than a call takes
     refused(UNSUPPORTED, ms.quantize, A, 1 << 21, 64, 8, 1 << 60, 1 << 61, x_stride=(1 << 19) + 8)
     refused(UNSUPPORTED, ms.quantize, A, 1, 64, 8, B, C, x_stride=(1 << 40) + 8)
     refused(UNSUPPORTED, ms.quantize, A, 2 ** 31 - 1, 64, 8, B, C, x_stride=2 ** 63 - 8)
@@ -98,6 +98,22 @@ def test_norm_refusals():
     refused(INVALID, norm, A, None, B, 4, 64, 1e-6, C, scales=C + 240, bits=8)
     refused(INVALID, norm, A, None, B, 4, 64, 1e-6, B, scales=C, bits=8)
     norm(None, None, None, 0, 64, 1e-6, None)
+
+
+def test_sizes_that_a_launch_cannot_count():
+    """Lanes, eight values each, are counted in 32 bits."""
+    rows, far = 1 << 20, (1 << 55, 1 << 56, 1 << 57)  # of 16384: 2^34 values
+    for bits in (8, 4):
+        refused(UNSUPPORTED, ms.quantize, far[0], rows + 1, 16384, bits, far[1], far[2])
+        refused(MISALIGNED, ms.quantize, far[0] + 8, rows, 16384, bits, far[1], far[2])
+        refused(UNSUPPORTED, ms.dequantize, far[0], far[1], rows + 1, 16384, bits, far[2])
+        refused(MISALIGNED, ms.dequantize, far[0] + 8, far[1], rows, 16384, bits, far[2])
+    refused(UNSUPPORTED, ms.pack_weights, far[0], far[1], rows + 1, 16384, far[2])
+    refused(MISALIGNED, ms.pack_weights, far[0] + 8, far[1], rows, 16384, far[2])
+    for cols in (32, 544, 5120, 32768):
+        most = (1 << 34) // (cols + 512)
+        refused(UNSUPPORTED, ms.add_rmsnorm, far[0], None, far[1], most + 1, cols, 1e-6, far[2])
+        refused(MISALIGNED, ms.add_rmsnorm, far[0] + 8, None, far[1], most, cols, 1e-6, far[2])
 
 
 def make(**kw):
