@@ -461,7 +461,8 @@ int kva_add_rmsnorm(const void *hidden, const void *delta, const void *w, int32_
  * is the fp32 sum of the elements' products, times both blocks' scales; it is
  * rounded to fp16 once, Q and K after their norm and RoPE (in kv_out as
  * projected); the rest, and every output, as there.  No output overlaps an
- * operand.  fp16 rows go through the cache's projection workspace.           */
+ * operand or another output.  fp16 rows go through the cache's projection
+ * workspace.                                                                */
 int kva_mx_project_append(kva_cache *cache, int32_t layer, const void *x, const void *x_scales,
                           int32_t bits, int32_t hidden, const void *w_q_packed, const void *w_kv_packed,
                           const void *q_norm_w, const void *k_norm_w, const void *cos_tab,

@@ -1537,13 +1537,20 @@ static int mx_project_impl(kva_cache *c, int32_t layer, const MxInput &in, const
     kva::ProjectArgs a = project_args(c, hidden, q_norm_w, k_norm_w, cos_tab, sin_tab);
     const uint64_t T = c->st_n_tok, q_bytes = T * c->cfg.num_heads * kva::kHeadDim * 2,
                    kv_bytes = T * 2 * c->cfg.num_kv_heads * kva::kHeadDim * 2;
+    const uint64_t norm_bytes = kva::kHeadDim * 2, tab_bytes = static_cast<uint64_t>(table_rows) * c->cfg.rotary_dim;
     auto over_operand = [&](const void *out, uint64_t n) {
+        if (bytes_overlap(out, n, q_norm_w, norm_bytes) || bytes_overlap(out, n, k_norm_w, norm_bytes) ||
+            bytes_overlap(out, n, cos_tab, tab_bytes) || bytes_overlap(out, n, sin_tab, tab_bytes))
+            return true;
         return bytes_overlap(out, n, in.x, in.bytes(T)) || bytes_overlap(out, n, in.scales, mx_scale_bytes(T, in.cols)) ||
                bytes_overlap(out, n, w_q, mx_packed_size(a.n_a, in.cols)) ||
                bytes_overlap(out, n, w_kv, mx_packed_size(a.n_b, in.cols));
     };
     if (over_operand(q_out, q_bytes) || over_operand(q_gate_out, q_bytes) || over_operand(kv_out, kv_bytes))
         return fail(KVA_ERR_INVALID_ARG, "an output overlaps an operand");
+    if (bytes_overlap(q_out, q_bytes, q_gate_out, q_bytes) || bytes_overlap(q_out, q_bytes, kv_out, kv_bytes) ||
+        bytes_overlap(q_gate_out, q_bytes, kv_out, kv_bytes))
+        return fail(KVA_ERR_INVALID_ARG, "outputs overlap each other");
     a.n_tok = mx_tokens_per_launch(c, in, c->st_n_tok);
     kva::MxProduct m{};
     m.w_a = static_cast<const uint8_t *>(w_q);

@@ -148,6 +148,16 @@ def test_project_refusals():
     # outputs over operands: 5 tokens, x 5 x 512 values
     for kw in (dict(q=A), dict(q=A + 5 * 1024 - 16), dict(gate=A), dict(kv=A), dict(q=B), dict(kv=C + 16)):
         refused(INVALID, project, c, **kw)
+    # norm weights of 512 bytes, tables of 4096 rows of 32, 5 tokens of 24 query heads and 8 K and V heads
+    for at in (1 << 44, (1 << 44) + 496, (1 << 45) + 4096 * 64 - 16):
+        for kw in (dict(q=at), dict(gate=at), dict(kv=at)):
+            refused(INVALID, project, c, **kw)
+    refused(NO_DEVICE, project, c, q=(1 << 44) + 512, gate=(1 << 45) + 4096 * 64)
+    q_bytes, kv_bytes = 5 * 24 * 512, 5 * 8 * 512
+    for kw in (dict(gate=E), dict(gate=E + q_bytes - 16), dict(kv=E + q_bytes - 16), dict(kv=E - kv_bytes + 16),
+               dict(gate=1 << 47, kv=(1 << 47) + 16)):
+        refused(INVALID, project, c, **kw)
+    refused(NO_DEVICE, project, c, gate=E + q_bytes, kv=E - kv_bytes)
     refused(NO_DEVICE, project, c, q=A + 5 * 1024)
     refused(NO_DEVICE, project, c, q=A + 5 * 512, scales=1 << 46)
     refused(INVALID, project, c, q=A + 5 * 512, scales=A + 5 * 512 + 16)
