@@ -13,7 +13,7 @@ import numpy as np
 import pytest
 
 from mi50grad_amd import microscale as ms
-from mi50grad_amd.device import Stream
+from mi50grad_amd.device import DeviceArray, Stream
 from mi50grad_amd.kv_cache import PagedKVCache
 from oracle import kvattn_oracle as orc
 from oracle import microscale_oracle as mx
@@ -700,3 +700,83 @@ def test_two_caches_on_two_streams(device):
         assert np.array_equal(outs[i].numpy(), (xs[i].astype(np.float64) @ mx.decode(*ws[i], 4).T).astype(np.float16))
         caches[i].destroy()
         streams[i].destroy()
+
+
+def _tail(a, shape, dtype, end=0):
+    """The last shape of values before `end` bytes of a device array's end."""
+    n = int(np.prod(shape)) * np.dtype(dtype).itemsize
+    return DeviceArray(a.dev, shape, dtype, ptr=a.ptr + a.nbytes - end - n)
+
+
+def test_rows_far_apart(device):
+    """Strides whose bytes pass 32 bits."""
+    rng = np.random.default_rng(31)
+    rows, cols, stride = 3, 96, 2 ** 31 + 8
+    say(f"quantize {rows} rows {stride} values apart")
+    x = rng.standard_normal((rows, cols)).astype(np.float16)
+    big = device.empty((rows - 1) * stride + cols, np.float16)
+    for r in range(rows):
+        DeviceArray(device, cols, np.float16, ptr=big.ptr + 2 * r * stride).copy_from(x[r])
+    codes, scales = device.empty((rows, cols), np.uint8), device.empty((rows, cols // 32), np.uint8)
+    ms.quantize(big, rows, cols, 8, codes, scales, x_stride=stride)
+    device.synchronize()
+    code, b = mx.encode(x, 8)
+    assert np.array_equal(codes.numpy(), code) and np.array_equal(scales.numpy(), b)
+    big.free()
+
+
+def test_more_than_32_bits_of_values(device):
+    """The last rows of 2^32 values and more: norm, quantise, and back."""
+    rng = np.random.default_rng(32)
+    cols, n = 2048, 2 ** 21 + 5
+    say(f"{n} rows of {cols}")
+    last = rng.standard_normal((5, cols)).astype(np.float16)
+    w = rng.uniform(0.5, 1.5, cols).astype(np.float16)
+    x = device.empty((n, cols), np.float16)
+    x.zero()
+    _tail(x, last.shape, np.float16).copy_from(last)
+    codes, scales = device.empty((n, cols), np.uint8), device.empty((n, cols // 32), np.uint8)
+    ms.quantize(x, n, cols, 8, codes, scales)
+    device.synchronize()
+    code, b = mx.encode(last, 8)
+    got, got_b = _tail(codes, (6, cols), np.uint8).numpy(), _tail(scales, (6, cols // 32), np.uint8).numpy()
+    assert np.array_equal(got[1:], code) and np.array_equal(got_b[1:], b)
+    assert not got[0].any()
+    ms.add_rmsnorm(x, None, device.array(w), n, cols, 1e-6, codes, scales=scales, bits=8)
+    device.synchronize()
+    norm = _tail(codes, (6, cols), np.uint8).numpy(), _tail(scales, (6, cols // 32), np.uint8).numpy()
+    few = device.empty((5, cols), np.uint8), device.empty((5, cols // 32), np.uint8)
+    ms.add_rmsnorm(device.array(last), None, device.array(w), 5, cols, 1e-6, few[0], scales=few[1], bits=8)
+    device.synchronize()
+    assert np.array_equal(norm[0][1:], few[0].numpy()) and np.array_equal(norm[1][1:], few[1].numpy())
+    assert not norm[0][0].any()
+    ms.dequantize(codes, scales, n, cols, 8, x)
+    device.synchronize()
+    y = _tail(x, (6, cols), np.float16).numpy()
+    assert np.array_equal(y, mx.decode(*norm, 8).astype(np.float16))
+    for a in (x, codes, scales):
+        a.free()
+
+
+def test_out_project_of_more_than_32_bits_of_codes(device):
+    """2^23 tokens and 5 more of 512: 4 GB of codes."""
+    rng = np.random.default_rng(33)
+    n, q_dim, n_out = 2 ** 23 + 5, 512, 16
+    say(f"mx_out_project of {n} rows")
+    cache = _any_cache()
+    codes, scales = device.empty((n, q_dim), np.uint8), device.empty((n, q_dim // 32), np.uint8)
+    codes.zero()
+    scales.zero()
+    c, s = _exact_rows(rng, 5, q_dim, 8)
+    _tail(codes, c.shape, np.uint8).copy_from(c)
+    _tail(scales, s.shape, np.uint8).copy_from(s)
+    w = _exact_rows(rng, n_out, q_dim, 4)
+    out = device.empty((n, n_out), np.float16)
+    cache.mx_out_project(codes, n, q_dim, _pack(device, w), n_out, out, attn_scales=scales)
+    device.synchronize()
+    y = _tail(out, (6, n_out), np.float16).numpy()
+    assert np.array_equal(y[1:], (mx.decode(c, s, 8) @ mx.decode(*w, 4).T).astype(np.float16))
+    assert not y[0].any()
+    for a in (codes, scales, out):
+        a.free()
+    cache.destroy()
