@@ -1438,7 +1438,7 @@ static int project_impl(kva_cache *c, int32_t layer, const void *x, int32_t hidd
 // Whether [p, p + n) and [q, q + m) have a byte in common (a null one has none).
 static bool bytes_overlap(const void *p, uint64_t n, const void *q, uint64_t m) {
     const auto a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
-    return p && q && a < b + m && b < a + n;
+    return p && q && n && m && a < b + m && b < a + n;
 }
 
 static uint64_t mx_code_bytes(uint64_t rows, uint64_t cols, int32_t bits) { return rows * (cols * bits / 8); }

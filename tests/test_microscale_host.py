@@ -168,6 +168,14 @@ def test_project_refusals():
     c.destroy()
 
 
+def test_project_without_rotary_dims():
+    """Tables are named but not read: they overlap nothing."""
+    c = make(rotary_dim=0)
+    c.begin_step([0], [1])
+    refused(NO_DEVICE, project, c, tabs=(E + 16, E + 32))
+    c.destroy()
+
+
 def out(c, x=A, n=5, q_dim=512, w=B, n_out=64, res=None, o=E, scales=None, bits=8):
     c.mx_out_project(x, n, q_dim, w, n_out, o, residual=res, attn_scales=scales, bits=bits)
 
