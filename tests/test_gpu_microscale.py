@@ -532,6 +532,38 @@ def test_project_of_fp16_rows(device, n_new):
     r[0].destroy()
 
 
+@pytest.mark.parametrize("rotary_dim", [0, 8, 72, 256])
+@pytest.mark.parametrize("n_tok,hidden", [(3, 512), (45, 2048), (45, 512)])
+def test_project_rotary_dims(device, rotary_dim, n_tok, hidden):
+    """Streamed, in parts of hidden and in one tile, the optional outputs left out."""
+    rng = np.random.default_rng(rotary_dim + n_tok)
+    heads, kv = 2, 1
+    say(f"mx_project_append rotary_dim {rotary_dim}, {n_tok} tokens, hidden {hidden}")
+    wq, wkv = (_exact_rows(rng, 2 * n * D, hidden, 4) for n in (heads, kv))
+    x = _exact_rows(rng, n_tok, hidden, 8)
+    qw, kw = ((1 + 0.1 * rng.standard_normal(D)).astype(np.float16) for _ in "qk")
+    angle = rng.uniform(0, 2 * np.pi, (64, rotary_dim // 2))
+    cos, sin = np.cos(angle).astype(np.float16), np.sin(angle).astype(np.float16)
+    tabs = [device.array(t if rotary_dim else np.zeros(8, np.float16)) for t in (cos, sin)]
+    cache = PagedKVCache(n_layers=1, max_seqs=1, max_blocks=8, max_blocks_per_seq=8, max_step_tokens=64,
+                         num_heads=heads, num_kv_heads=kv, rotary_dim=rotary_dim)
+    cache.reserve(0, n_tok)
+    cache.begin_step([0], [n_tok])
+    q = device.empty((n_tok, heads, D), np.float16)
+    cache.mx_project_append(0, device.array(x[0]), hidden, _pack(device, wq), _pack(device, wkv), device.array(qw),
+                            device.array(kw), *tabs, 64, q, x_scales=device.array(x[1]))
+    device.synchronize()
+    y = mx.decode(*x, 8) @ np.concatenate([mx.decode(*wq, 4), mx.decode(*wkv, 4)]).T
+    y = y.reshape(n_tok, -1, D)
+    rope = lambda v, w, n: orc.qknorm_rope_f32(  # noqa: E731
+        v.reshape(-1, D), w, np.repeat(cos[:n_tok], n, 0), np.repeat(sin[:n_tok], n, 0)).reshape(n_tok, n, D)
+    assert np.array_equal(_bits(q.numpy()), _bits(rope(y[:, :heads], qw, heads)))
+    k, v = cache.gather(0, 0, n_tok)
+    assert np.array_equal(_bits(k), _bits(rope(y[:, 2 * heads:2 * heads + kv], kw, kv)))
+    assert np.array_equal(v, y[:, 2 * heads + kv:].astype(np.float16))
+    cache.destroy()
+
+
 @pytest.mark.parametrize("n_new", [[1, 1], [33, 20]])
 def test_project_onto_the_8_bit_cache(device, n_new):
     """The rows that an 8-bit cache holds are those of an append of the fp16 cache's."""
