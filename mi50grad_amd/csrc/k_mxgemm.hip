@@ -17,7 +17,7 @@
 // More tokens are bound by the matrix units, or rather by what clock the card's
 // power leaves them.  2048 tokens by mx_gemm_kernel, in us (and PFLOP/s), and a
 // library's plain product of the same types with fp16 outputs:
-//   5120 -> 14336, norm, RoPE and append   8 bits 134 (2.2)   4 bits 111 (2.7)
+//   5120 -> 14336, norm, RoPE and append   8 bits 128 (2.3)   4 bits 107 (2.8)
 //     plain product                               124                117
 //   6144 -> 5120 and a residual            8 bits  52 (2.5)   4 bits  51
 //     plain product                                62                 67
@@ -317,12 +317,20 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
     const int N = a.n_a + a.n_b, K = a.hidden;
     const int n_rt = (N + T::BN - 1) / T::BN, n_mt = (a.n_tok + T::BM - 1) / T::BM;
     const int splits = EPI == kMxPart ? a.splits : 1;
-    const int tau = mx_deal(blockIdx.x, n_rt * splits * n_mt);
+    // With `by_kind` the first half of the workgroups takes Q and K heads, the
+    // second gate and V.
+    const bool by_kind = EPI == kMxHead && m.by_kind;
+    const int n_wg = n_rt * splits * n_mt / (by_kind ? 2 : 1), wg = blockIdx.x;
+    const bool second = by_kind && wg >= n_wg;
+    const int tau = mx_deal(second ? wg - n_wg : wg, n_wg);
     // Token tiles fastest, then row tiles, then splits.
     const int ws_at = __builtin_amdgcn_readfirstlane(tau / n_mt);
     const int mt = __builtin_amdgcn_readfirstlane(tau - ws_at * n_mt);
     const int split = EPI == kMxPart ? __builtin_amdgcn_readfirstlane(ws_at / n_rt) : 0;
-    const int rt = ws_at - split * n_rt;
+    const int H = a.num_heads, hkv = a.num_kv_heads;
+    const int rt = !by_kind      ? ws_at - split * n_rt
+                   : ws_at < H ? ws_at + (second ? H : 0)
+                                 : ws_at + H + (second ? hkv : 0);
     const int t0 = mt * T::BM, n0 = rt * T::BN;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
@@ -553,7 +561,7 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
         }
         __syncthreads();
     }
-    const int head = rt, H = a.num_heads, hkv = a.num_kv_heads;
+    const int head = rt;
     const bool is_q = head < H, is_gate = !is_q && head < 2 * H;
     const int kv = head - 2 * H;  // K heads 0..hkv-1, then V heads
     const bool rot = EPI == kMxHead && (is_q || (!is_gate && kv < hkv));
@@ -801,9 +809,10 @@ bool plan_mx(const ProjectArgs &a, const MxProduct &m, bool heads, int n_cu, siz
     return true;
 }
 
-hipError_t launch_mx_product(const ProjectArgs &args, const MxProduct &m, bool heads, int n_cu, const ProductPlan &plan,
+hipError_t launch_mx_product(const ProjectArgs &args, const MxProduct &product, bool heads, int n_cu, const ProductPlan &plan,
                              hipStream_t s) {
     ProjectArgs a = args;
+    MxProduct m = product;
     a.splits = plan.splits;
     hipError_t e = a.ev_before ? hipEventRecord(a.ev_before, s) : hipSuccess;
     if (e != hipSuccess) return e;
@@ -811,6 +820,12 @@ hipError_t launch_mx_product(const ProjectArgs &args, const MxProduct &m, bool h
         e = m.bits == 8 ? launch_mx_stream<8>(a, m, heads, n_cu, s) : launch_mx_stream<4>(a, m, heads, n_cu, s);
     } else {
         const MxForm &f = (m.bits == 8 ? kForms8 : kForms4)[plan.form];
+        // Tiles that are normalised end some 6 us later than the others, of which
+        // there are as many: where a CU takes a second tile, not two of them (5120
+        // -> 14336 of 2048 tokens side by side: 127.5 us against 131, in 4 bits 107
+        // against 111).  Tiles that all run at once keep the order of the heads
+        // (181 tokens: 19.5 us against 19.7).
+        m.by_kind = heads && static_cast<int64_t>((a.n_a + a.n_b) / f.bn) * ((a.n_tok + f.bm - 1) / f.bm) > n_cu;
         e = (plan.partial ? f.part : heads ? f.head : f.out)(a, m, s);
     }
     if (e != hipSuccess) return e;

@@ -193,6 +193,7 @@ struct MxProduct {
     const uint8_t *x, *x_scales;
     const uint8_t *w_a, *w_b; // packed
     int32_t bits;             // of x
+    bool by_kind;             // the order of a tile kernel's heads
 };
 bool plan_mx(const ProjectArgs &a, const MxProduct &m, bool heads, int n_cu, size_t part_floats, ProductPlan &plan);
 hipError_t launch_mx_product(const ProjectArgs &a, const MxProduct &m, bool heads, int n_cu, const ProductPlan &plan,

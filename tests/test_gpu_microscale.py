@@ -485,7 +485,8 @@ def _check_step(cache, kr, vr, got, y, off, qw, kw, tables, pos, heads, kv, leng
 @pytest.mark.parametrize("bits", [8, 4])
 @pytest.mark.parametrize("heads,kv,hidden,n_new", [
     (2, 1, 512, [1]), (24, 4, 5120, [1] * 32), (6, 3, 1024, [3, 1, 5]), (8, 1, 1536, [31]), (4, 4, 512, [20, 21]),
-    (24, 4, 512, [64]), (6, 1, 2560, [100, 81]), (2, 1, 512, [700]), (24, 4, 1024, [257, 1]), (8, 8, 512, [2048])])
+    (24, 4, 512, [64]), (6, 1, 2560, [100, 81]), (2, 1, 512, [700]), (24, 4, 1024, [257, 1]), (8, 8, 512, [2048]),
+    (24, 4, 512, [1000, 100]), (8, 4, 512, [2900])])  # the last two: more tiles than CUs
 def test_project_exact(device, bits, heads, kv, hidden, n_new):
     rng = np.random.default_rng(heads + hidden + sum(n_new) + bits)
     lengths = [int(x) for x in rng.integers(0, 60, len(n_new))]
