@@ -17,7 +17,7 @@
 // More tokens are bound by the matrix units, or rather by what clock the card's
 // power leaves them.  2048 tokens by mx_gemm_kernel, in us (and PFLOP/s), and a
 // library's plain product of the same types with fp16 outputs:
-//   5120 -> 14336, norm, RoPE and append   8 bits 128 (2.3)   4 bits 107 (2.8)
+//   5120 -> 14336, norm, RoPE and append   8 bits 127 (2.4)   4 bits 105 (2.9)
 //     plain product                               124                117
 //   6144 -> 5120 and a residual            8 bits  52 (2.5)   4 bits  51
 //     plain product                                62                 67
@@ -647,10 +647,24 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
                 return make_uint4(pack_h2(x[0], x[1]), pack_h2(x[2], x[3]), pack_h2(x[4], x[5]), pack_h2(x[6], x[7]));
             };
             if (rot) {
+                // A square root and a division take some 25 instructions: lane l
+                // takes row l % kPer's and hands them on (each lane all of its rows': 127.7
+                // us for 126.8 at 2048 tokens of 5120 -> 14336, in 4 bits 107.2 for 105.4).
+                static_assert((kPer & (kPer - 1)) == 0 && kPer <= LPR, "a lane a row");
+                float mine = 0.f;
                 each<0, kPer>([&](auto j) KVA_INLINE {
                     float x[8];
                     y[j] = row(j, x);
-                    o[j] = norm_rope_apply<32, true>(x, NormRopeIn{wnorm, now.c[j], now.s[j]}, a.half_rot, a.eps, l);
+                    const float sum = sum32_moves(sum_squares(x));
+                    mine = (l & (kPer - 1)) == j ? sum : mine;
+                });
+                const int inv = __builtin_bit_cast(int, inv_rms<32>(mine, a.eps));
+                each<0, kPer>([&](auto j) KVA_INLINE {
+                    float x[8];
+                    row(j, x);
+                    constexpr int kLane = decltype(j)::value << 5;  // of 32: lane j's
+                    const float by = __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(inv, kLane));
+                    o[j] = norm_rope_by(x, NormRopeIn{wnorm, now.c[j], now.s[j]}, a.half_rot, by, l);
                 });
             } else {
                 each<0, kPer>([&](auto j) KVA_INLINE {

@@ -77,12 +77,8 @@ __device__ __forceinline__ float sum32_moves(float s) {
     return s + dpp_f<kDppQuadXor1>(s);
 }
 
-// Normalise + rotate one row held as 8 values per lane, rounded to fp16 at the
-// end.  LANES = head_dim / 8 lanes take part (lane < LANES); the butterfly
-// stays inside them.  MOVES: by sum32_moves.
-template <int LANES, bool MOVES = false>
-__device__ __forceinline__ uint4 norm_rope_apply(const float (&x)[8], const NormRopeIn &in, int half_rot, float eps,
-                                                 int lane) {
+// A lane's share of a row's sum of squares.
+__device__ __forceinline__ float sum_squares(const float (&x)[8]) {
 #pragma clang fp contract(off)
     float s = x[0] * x[0];
 #pragma unroll
@@ -90,20 +86,23 @@ __device__ __forceinline__ uint4 norm_rope_apply(const float (&x)[8], const Norm
         const float sq = x[i] * x[i];
         s = s + sq;
     }
-    if constexpr (MOVES) {
-        static_assert(LANES == 32, "a half-wave per row");
-        s = sum32_moves(s);
-    } else {
-#pragma unroll
-        for (int off = LANES / 2; off >= 1; off >>= 1) {
-            const float other = __shfl_xor(s, off, 32);
-            s = s + other;
-        }
-    }
+    return s;
+}
+
+// What a row of 8 * LANES values is multiplied by, of its sum of squares.
+template <int LANES>
+__device__ __forceinline__ float inv_rms(float s, float eps) {
+#pragma clang fp contract(off)
     const float ms = s * (1.0f / static_cast<float>(LANES * 8));
     const float var = ms + eps;
-    const float inv = 1.0f / sqrtf(var);
+    return 1.0f / sqrtf(var);
+}
 
+// Normalise + rotate one row held as 8 values per lane, rounded to fp16 at the
+// end, by its inv_rms.
+__device__ __forceinline__ uint4 norm_rope_by(const float (&x)[8], const NormRopeIn &in, int half_rot, float inv,
+                                              int lane) {
+#pragma clang fp contract(off)
     const uint32_t ww[4] = {in.w.x, in.w.y, in.w.z, in.w.w};
     float n[8];
 #pragma unroll
@@ -135,6 +134,21 @@ __device__ __forceinline__ uint4 norm_rope_apply(const float (&x)[8], const Norm
     y.z = pack_h2(n[4], n[5]);
     y.w = pack_h2(n[6], n[7]);
     return y;
+}
+
+// The same from the row alone.  LANES = head_dim / 8 lanes take part (lane <
+// LANES); the butterfly stays inside them.
+template <int LANES>
+__device__ __forceinline__ uint4 norm_rope_apply(const float (&x)[8], const NormRopeIn &in, int half_rot, float eps,
+                                                 int lane) {
+#pragma clang fp contract(off)
+    float s = sum_squares(x);
+#pragma unroll
+    for (int off = LANES / 2; off >= 1; off >>= 1) {
+        const float other = __shfl_xor(s, off, 32);
+        s = s + other;
+    }
+    return norm_rope_by(x, in, half_rot, inv_rms<LANES>(s, eps), lane);
 }
 
 // The same of fp16 values.
