@@ -431,7 +431,8 @@ int kva_evict(kva_cache *cache, int32_t n_seqs, const int32_t *src_ids, const in
  * layers as integers with an fp16 scale per group (its GPTQ form); its
  * attention projections are fp16.                                           */
 /* x [rows][cols] fp16, x_stride values between rows (a multiple of 8, at least
- * cols), as microscaled rows.  cols a multiple of 32.                       */
+ * cols; rows * x_stride at most 2^40: KVA_ERR_UNSUPPORTED), as microscaled rows.
+ * cols a multiple of 32.                                                    */
 int kva_mx_quantize(const void *x, int64_t x_stride, int32_t rows, int32_t cols, int32_t bits,
                     void *codes, void *scales, kva_stream_t stream);
 /* The values of microscaled rows, y [rows][cols] fp16: rounded to it, so exact

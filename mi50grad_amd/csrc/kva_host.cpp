@@ -1455,7 +1455,8 @@ static int check_mx_bits(int32_t bits) {
 
 // Rows that a kernel is launched over.
 static int check_mx_size(int64_t rows, int64_t cols, int64_t stride) {
-    if (rows * cols > kva::kMxMaxValues || stride > kva::kMxMaxSpan || rows * stride > kva::kMxMaxSpan)
+    // By division: the product of rows and stride may pass 64 bits.
+    if (rows * cols > kva::kMxMaxValues || stride > kva::kMxMaxSpan / std::max<int64_t>(rows, 1))
         return fail(KVA_ERR_UNSUPPORTED, "%lld rows of %lld values, %lld apart", static_cast<long long>(rows),
                     static_cast<long long>(cols), static_cast<long long>(stride));
     return KVA_OK;

@@ -217,3 +217,15 @@ def test_out_beyond_the_workspace():
     refused(NO_DEVICE, out, c, n=3, q_dim=fit + 1024, scales=1 << 46)
     refused(NO_DEVICE, out, c, n=3, q_dim=fit + 1024, bits=4)
     c.destroy()
+
+
+def test_rows_whose_distance_no_64_bits_hold():
+    """Rows times stride past 2^63 (and past 2^64, where the product's low bits
+    are small again) is refused like any distance above 2^40."""
+    for rows in (2, 1 << 22, 1 << 23, 1 << 24, (1 << 24) + 1, 1 << 29):
+        refused(UNSUPPORTED, ms.quantize, A, rows, 32, 8, B, C, x_stride=1 << 40)
+    refused(UNSUPPORTED, ms.quantize, A, 1 << 29, 32, 4, B, C, x_stride=(1 << 35) + 8)
+    far = (1 << 55, 1 << 56, (1 << 57) + 8)
+    refused(MISALIGNED, ms.quantize, far[0], 1, 32, 8, far[1], far[2], x_stride=1 << 40)  # at the limit: the next check
+    refused(MISALIGNED, ms.quantize, far[0], 1 << 20, 32, 8, far[1], far[2], x_stride=1 << 20)
+    refused(UNSUPPORTED, ms.quantize, far[0], 1 << 20, 32, 8, far[1], far[2], x_stride=(1 << 20) + 8)
