@@ -1453,10 +1453,10 @@ static int check_mx_bits(int32_t bits) {
     return KVA_OK;
 }
 
-// Rows that a kernel is launched over.
-static int check_mx_size(int64_t rows, int64_t cols, int64_t stride) {
+// Rows that a kernel is launched over, with lanes for `idle` more values of each at most.
+static int check_mx_size(int64_t rows, int64_t cols, int64_t stride, int64_t idle = 0) {
     // By division: the product of rows and stride may pass 64 bits.
-    if (rows * cols > kva::kMxMaxValues || stride > kva::kMxMaxSpan / std::max<int64_t>(rows, 1))
+    if (rows * (cols + idle) > kva::kMxMaxValues || stride > kva::kMxMaxSpan / std::max<int64_t>(rows, 1))
         return fail(KVA_ERR_UNSUPPORTED, "%lld rows of %lld values, %lld apart", static_cast<long long>(rows),
                     static_cast<long long>(cols), static_cast<long long>(stride));
     return KVA_OK;
@@ -1729,7 +1729,7 @@ int kva_add_rmsnorm(const void *hidden, const void *delta, const void *w, int32_
     if (int rc = check_mx_shape(n_tok, cols, kva::kMxBlock)) return rc;
     if (cols > kva::kMxNormMax) return fail(KVA_ERR_UNSUPPORTED, "%d columns: at most %d", cols, kva::kMxNormMax);
     // A row has up to 64 lanes without values.
-    if (int rc = check_mx_size(n_tok, cols + 512, cols)) return rc;
+    if (int rc = check_mx_size(n_tok, cols, cols, 512)) return rc;
     if (!(eps >= 0.0f)) return fail(KVA_ERR_INVALID_ARG, "eps %g", static_cast<double>(eps));
     if (n_tok == 0) return KVA_OK;
     if (!hidden || !w || !out) return fail(KVA_ERR_INVALID_ARG, "NULL pointer");

@@ -229,3 +229,10 @@ def test_rows_whose_distance_no_64_bits_hold():
     refused(MISALIGNED, ms.quantize, far[0], 1, 32, 8, far[1], far[2], x_stride=1 << 40)  # at the limit: the next check
     refused(MISALIGNED, ms.quantize, far[0], 1 << 20, 32, 8, far[1], far[2], x_stride=1 << 20)
     refused(UNSUPPORTED, ms.quantize, far[0], 1 << 20, 32, 8, far[1], far[2], x_stride=(1 << 20) + 8)
+
+
+def test_a_refusal_names_the_sizes_it_was_given():
+    for cols in (32, 5120):
+        n = (1 << 34) // (cols + 512) + 1
+        with pytest.raises(KvaError, match=rf"{n} rows of {cols} values, {cols} apart"):
+            ms.add_rmsnorm(1 << 55, None, 1 << 56, n, cols, 1e-6, 1 << 57)
