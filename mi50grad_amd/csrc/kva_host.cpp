@@ -1348,11 +1348,11 @@ static kva::ProjectArgs project_args(const kva_cache *c, int32_t hidden, const v
 
 // The step's tokens through a projection, a.n_tok (the plan made for them) at a
 // time, and its rows into the cache.  launch(a, t0) takes a.n_tok tokens from
-// t0 on, planning anew where they are fewer.
+// t0 on, planning anew where they are fewer.  `path` is what the call reports.
 extern "C++" {
 template <class Launch>
 static int run_project(kva_cache *c, int32_t layer, kva::ProjectArgs &a, void *q_out, void *q_gate_out, void *kv_out,
-                       hipStream_t s, Launch launch) {
+                       int32_t path, hipStream_t s, Launch launch) {
     const size_t q_row = static_cast<size_t>(c->cfg.num_heads) * kva::kHeadDim,
                  kv_row = 2 * static_cast<size_t>(c->cfg.num_kv_heads) * kva::kHeadDim;
     // Onto an 8-bit cache the projection leaves its rows in token order (token t
@@ -1384,7 +1384,7 @@ static int run_project(kva_cache *c, int32_t layer, kva::ProjectArgs &a, void *q
         set_append_plan(c, layer, rows);
         KVA_HIP(launch_rows(c, layer, rows, false, s));
     }
-    c->last_proj_path = c->st_n_tok > kva::kProjTokens ? KVA_PROJECT_PREFILL_GEMM : KVA_PROJECT_KERNELS;
+    c->last_proj_path = path;
     return KVA_OK;
 }
 }  // extern "C++"
@@ -1423,7 +1423,8 @@ static int project_impl(kva_cache *c, int32_t layer, const void *x, int32_t hidd
     if ((rc = check_rows8_capture(c))) return rc;
     if ((rc = require_device(c))) return rc;
     const auto s = static_cast<hipStream_t>(stream);
-    return run_project(c, layer, a, q_out, q_gate_out, kv_out, s, [&](kva::ProjectArgs &b, int32_t t0) {
+    const int32_t path = c->st_n_tok > kva::kProjTokens ? KVA_PROJECT_PREFILL_GEMM : KVA_PROJECT_KERNELS;
+    return run_project(c, layer, a, q_out, q_gate_out, kv_out, path, s, [&](kva::ProjectArgs &b, int32_t t0) {
         b.x = static_cast<const uint16_t *>(x) + t0 * h;
         if (b.n_tok != planned_for) {
             planned_for = b.n_tok;
@@ -1567,7 +1568,8 @@ static int mx_project_impl(kva_cache *c, int32_t layer, const MxInput &in, const
     if ((rc = check_rows8_capture(c))) return rc;
     if ((rc = require_device(c))) return rc;
     const auto s = static_cast<hipStream_t>(stream);
-    return run_project(c, layer, a, q_out, q_gate_out, kv_out, s, [&](kva::ProjectArgs &b, int32_t t0) {
+    const int32_t path = plan.stream ? KVA_PROJECT_KERNELS : KVA_PROJECT_PREFILL_GEMM;
+    return run_project(c, layer, a, q_out, q_gate_out, kv_out, path, s, [&](kva::ProjectArgs &b, int32_t t0) {
         if (b.n_tok != planned_for) {
             planned_for = b.n_tok;
             if (!kva::plan_mx(b, m, true, c->n_cu, c->part_floats - in.held_floats(b.n_tok), plan))

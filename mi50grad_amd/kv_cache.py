@@ -240,7 +240,9 @@ class PagedKVCache:
     def project_path(self) -> str:
         """Which path the last project_append took: "kernels" (steps of up to
         64 tokens) or "prefill_gemm" (larger ones: one launch of GEMM tiles,
-        and a finish launch where hidden is split)."""
+        and a finish launch where hidden is split).  Of the last
+        mx_project_append: "kernels" where it streamed the weights (up to 32
+        tokens), "prefill_gemm" where it ran tiles."""
         p = ctypes.c_int32()
         _lib.call("kva_get_project_path", self.handle, ctypes.byref(p))
         return {0: "kernels", 1: "prefill_gemm"}[p.value]

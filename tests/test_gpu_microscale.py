@@ -813,3 +813,28 @@ def test_out_project_of_more_than_32_bits_of_codes(device):
     for a in (codes, scales, out):
         a.free()
     cache.destroy()
+
+
+# ---- which path ran -----------------------------------------------------------
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("n_tok,hidden,path", [(1, 512, "kernels"), (32, 512, "kernels"), (33, 512, "prefill_gemm"),
+                                               (45, 2048, "prefill_gemm"), (64, 512, "prefill_gemm"),
+                                               (65, 512, "prefill_gemm")])
+def test_project_path(device, bits, n_tok, hidden, path):
+    """Streamed weights up to 32 tokens, tiles above, whether a finish kernel follows them or not."""
+    say(f"project_path of {n_tok} tokens by 4-bit weights, hidden {hidden}, {bits} bits")
+    rng, heads, kv = np.random.default_rng(n_tok), 2, 1
+    cache = PagedKVCache(n_layers=1, max_seqs=1, max_blocks=8, max_blocks_per_seq=8, max_step_tokens=n_tok,
+                         num_heads=heads, num_kv_heads=kv)
+    cache.reserve(0, n_tok)
+    wq, wkv = (_pack(device, _exact_rows(rng, 2 * n * D, hidden, 4)) for n in (heads, kv))
+    tables, norm = Tables(device, n_tok), device.array(np.ones(D, np.float16))
+    x = [device.array(a) for a in _exact_rows(rng, n_tok, hidden, bits)]
+    cache.begin_step([0], [n_tok])
+    cache.mx_project_append(0, x[0], hidden, wq, wkv, norm, norm, tables.d_cos, tables.d_sin, tables.rows,
+                            device.empty((n_tok, heads, D), np.float16), x_scales=x[1], bits=bits)
+    device.synchronize()
+    assert cache.project_path() == path
+    assert (cache.product_plan()["tile_tokens"] == 0) == (path == "kernels")
+    cache.destroy()
