@@ -387,7 +387,9 @@ __global__ __launch_bounds__(64 * T::kWaves) void mx_gemm_kernel(ProjectArgs a, 
         sm_size[j] = __builtin_amdgcn_readfirstlane(of_x            ? toks * s_row
                                                     : q < T::kSmall ? tiles * static_cast<uint32_t>(K)
                                                                     : 0u);
-        sm_step[j] = of_x ? 16 : 512;
+        // An empty buffer is read at 0 alone: a range check may subtract the scalar
+        // offset from the size.
+        sm_step[j] = of_x ? 16 : q < T::kSmall ? 512 : 0;
         sm_off[j] = of_x ? (64 * q + lane) * s_row : (2 * qw + half) * static_cast<uint32_t>(K) + 16 * col;
     }
     // Piece j of the loads of chunk c into the stage at `st`.  A chunk past the
