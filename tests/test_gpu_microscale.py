@@ -838,3 +838,167 @@ def test_project_path(device, bits, n_tok, hidden, path):
     assert cache.project_path() == path
     assert (cache.product_plan()["tile_tokens"] == 0) == (path == "kernels")
     cache.destroy()
+
+
+# ---- fp16 rows into the projection, recorded steps of many tokens --------------
+
+@pytest.mark.parametrize("n_new", [[2, 1], [40], [300]])
+def test_project_of_fp16_rows_to_4_bits(device, n_new):
+    """fp16 rows whose values 4 bits hold exactly."""
+    rng = np.random.default_rng(sum(n_new) + 4)
+    lengths = [5] * len(n_new)
+    say(f"mx_project_append of fp16 rows to 4 bits, new {n_new}")
+    r = _step(device, rng, 6, 1, 1024, lengths, n_new, 4, True, fp16=True)
+    _check_step(*r, 6, 1, lengths, n_new, True)
+    r[0].destroy()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("n_new", [[500, 295], [771], [398]])
+def test_project_of_fp16_rows_in_parts(device, bits, n_new):
+    """More fp16 rows than a launch takes: half of the workspace, 2 MB for one
+    query and one KV head, holds 397 rows of 5280 bytes in 8 bits and 770 of 2720
+    in 4.  Some end with a launch of 1 to 32 tokens, which streams the weights."""
+    rng = np.random.default_rng(sum(n_new) + bits)
+    lengths = [int(x) for x in rng.integers(0, 60, len(n_new))]
+    say(f"mx_project_append of fp16 rows in parts, new {n_new}, {bits} bits")
+    rope = [int(x) for x in rng.integers(0, 1024, sum(n_new))]
+    r = _step(device, rng, 1, 1, 5120, lengths, n_new, bits, True, fp16=True, rope_pos=rope)
+    _check_step(*r, 1, 1, lengths, n_new, True)
+    r[0].destroy()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("n_new", [[2, 1], [33, 20], [500, 295]])
+def test_project_of_fp16_rows_onto_the_8_bit_cache(device, bits, n_new):
+    """In one launch and in parts: what the cache holds is an append of the fp16
+    cache's rows, and every output the same."""
+    rng = np.random.default_rng(sum(n_new) + bits)
+    heads, kv, hidden, T, B = 1, 1, 5120, sum(n_new), len(n_new)
+    say(f"mx_project_append of fp16 rows onto an 8-bit cache, new {n_new}, {bits} bits")
+    wq, wkv = (_pack(device, _exact_rows(rng, 2 * n * D, hidden, 4)) for n in (heads, kv))
+    x = device.array(rng.integers(-4, 5, (T, hidden)).astype(np.float16))
+    qw, kw = (device.array((1 + 0.1 * rng.standard_normal(D)).astype(np.float16)) for _ in "qk")
+    tables = Tables(device, 512)
+    got = []
+    for kv_bits in (16, 8, 8):
+        cache = PagedKVCache(n_layers=1, max_seqs=B, max_blocks=64, max_blocks_per_seq=32, max_step_tokens=1024,
+                             num_heads=heads, num_kv_heads=kv, kv_bits=kv_bits)
+        for b, n in enumerate(n_new):
+            cache.reserve(b, n)
+        cache.begin_step(list(range(B)), n_new)
+        out = [device.empty((T, n, D), np.float16) for n in (heads, heads, 2 * kv)]
+        k, v = device.empty((T, kv, D), np.float16), device.empty((T, kv, D), np.float16)
+        if len(got) < 2:
+            cache.mx_project_append(0, x, hidden, wq, wkv, qw, kw, tables.d_cos, tables.d_sin, 512, *out, bits=bits)
+        else:  # the fp16 cache's rows, appended
+            cache.append_rows(0, device.array(got[0][3]), device.array(got[0][4]))
+        cache.read_rows(0, list(range(B)), [0] * B, n_new, k, v)
+        device.synchronize()
+        got.append([a.numpy() for a in out + [k, v]])
+        cache.destroy()
+    for i in range(3):
+        assert np.array_equal(_bits(got[1][i]), _bits(got[0][i]))
+    for i in (3, 4):
+        assert np.array_equal(_bits(got[1][i]), _bits(got[2][i]))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("n_tok", [1, 9, 32, 45, 300])
+def test_project_of_random_fp16_rows(device, bits, n_tok):
+    """Rows that are rounded on the way: the product of what they are rounded
+    to, as test_project_random checks coded ones."""
+    rng = np.random.default_rng(n_tok + bits)
+    heads, kv, hidden = 3, 1, 2560
+    say(f"mx_project_append of random fp16 rows, {n_tok} tokens, {bits} bits")
+    cache, kr, vr = build_cache([7], [list(range(n_tok // 16 + 2))], extra_rows=[n_tok], rng=rng, num_heads=heads,
+                                num_kv_heads=kv)
+    x = (rng.standard_normal((n_tok, hidden)) * 2.0 ** rng.integers(-3, 3, (n_tok, 1))).astype(np.float16)
+    x[:, ::97] *= 10
+    wq, wkv = _random_rows(rng, 2 * heads * D, hidden, 4), _random_rows(rng, 2 * kv * D, hidden, 4)
+    qw, kw = ((1 + 0.1 * rng.standard_normal(D)).astype(np.float16) for _ in "qk")
+    tables = Tables(device, 1024)
+    cache.begin_step([0], [n_tok])
+    d = dict(q=device.empty((n_tok, heads, D), np.float16), g=device.empty((n_tok, heads, D), np.float16),
+             kv=device.empty((n_tok, 2, kv, D), np.float16))
+    cache.mx_project_append(0, device.array(x), hidden, _pack(device, wq), _pack(device, wkv), device.array(qw),
+                            device.array(kw), tables.d_cos, tables.d_sin, tables.rows, *d.values(), bits=bits)
+    device.synchronize()
+    got = {k: v.numpy() for k, v in d.items()}
+    y, off = _product(mx.quantized(x, bits), np.concatenate([mx.decode(*wq, 4), mx.decode(*wkv, 4)]))
+    _check_step(cache, kr, vr, got, y.reshape(n_tok, -1, D), off.reshape(n_tok, -1, D), qw, kw, tables,
+                list(range(7, 7 + n_tok)), heads, kv, [7], [n_tok], False)
+    cache.destroy()
+
+
+@pytest.mark.parametrize("coded", [True, False])
+@pytest.mark.parametrize("heads,kv,hidden,n_new", [(2, 1, 512, [25, 20]), (2, 1, 2048, [25, 20]), (1, 1, 5120, [410])])
+def test_a_recorded_prompt_step(device, heads, kv, hidden, n_new, coded):
+    """Norm, projection and output projection (of the gates) of more than 32
+    tokens, recorded and replayed, its own eager runs between: the eager bits.
+    Tiles that finish their rows, parts of hidden with a finish kernel, and (fp16
+    rows of 5120) more than one launch."""
+    rng = np.random.default_rng(hidden + coded)
+    B, T, steps = len(n_new), sum(n_new), 5
+    say(f"a recorded step of {n_new} tokens in 4 bits, {heads}/{kv} heads, hidden {hidden}, coded {coded}")
+    w = [_random_rows(rng, n * D, hidden, 4) for n in (2 * heads, 2 * kv)]
+    w.append(_random_rows(rng, hidden, 512, 4))
+    for a in w:
+        a[1][:] -= 6
+    packed = [_pack(device, a) for a in w]
+    norm, qw, kw = (device.array((1 + 0.1 * rng.standard_normal(n)).astype(np.float16)) for n in (hidden, D, D))
+    tables = Tables(device, 4096)
+    empty = lambda *s, t=np.float16: device.empty(s, t)  # noqa: E731
+    h, delta, x, gate, q = empty(T, hidden), empty(T, hidden), empty(T, hidden), empty(T, heads, D), empty(T, heads, D)
+    codes, scales = empty(T, hidden, t=np.uint8), empty(T, hidden // 32, t=np.uint8)
+    n_rows = T * heads * D // 512  # the gates as rows of 512
+    caches = [PagedKVCache(n_layers=1, max_seqs=B, max_blocks=256, max_blocks_per_seq=160, max_step_tokens=512,
+                           num_heads=heads, num_kv_heads=kv) for _ in range(2)]
+    for c in caches:
+        for b in range(B):
+            c.reserve(b, steps * n_new[b])
+
+    def run(cache, s):
+        if coded:
+            ms.add_rmsnorm(h, delta, norm, T, hidden, EPS, codes, sum_out=h, scales=scales, bits=8, stream=s)
+            cache.mx_project_append(0, codes, hidden, *packed[:2], qw, kw, tables.d_cos, tables.d_sin, tables.rows, q,
+                                    gate, x_scales=scales, stream=s)
+        else:
+            ms.add_rmsnorm(h, delta, norm, T, hidden, EPS, x, sum_out=h, stream=s)
+            cache.mx_project_append(0, x, hidden, *packed[:2], qw, kw, tables.d_cos, tables.d_sin, tables.rows, q,
+                                    gate, stream=s)
+        cache.mx_out_project(gate, n_rows, 512, packed[2], hidden, h, residual=h, stream=s)
+
+    stream = Stream()
+    s = stream.handle
+    graph = None
+    for step in range(steps):
+        h0, d0 = (rng.standard_normal((T, hidden)).astype(np.float16) for _ in "hd")
+        got = []
+        for i, c in enumerate(caches):
+            h.copy_from(h0)
+            delta.copy_from(d0)
+            q.zero()
+            gate.zero()
+            device.synchronize()
+            c.begin_step(list(range(B)), n_new, stream=s)
+            if i == 0:
+                run(c, s)
+            else:
+                if graph is None:
+                    graph = c.record_step(s)
+                    run(c, s)
+                    graph.end()
+                graph.launch()
+            stream.synchronize()
+            got.append([a.numpy() for a in (h, q, gate)])
+        for a, b in zip(*got):
+            assert np.isfinite(a).all() and a.any()
+            assert np.array_equal(_bits(a), _bits(b)), step
+    for b in range(B):
+        for a, g in zip(*(c.gather(0, b, steps * n_new[b]) for c in caches)):
+            assert np.array_equal(_bits(a), _bits(g))
+    graph.destroy()
+    for c in caches:
+        c.destroy()
+    stream.destroy()
