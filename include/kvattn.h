@@ -439,8 +439,9 @@ int kva_evict(kva_cache *cache, int32_t n_seqs, const int32_t *src_ids, const in
  * cols a multiple of 32.                                                    */
 int kva_mx_quantize(const void *x, int64_t x_stride, int32_t rows, int32_t cols, int32_t bits,
                     void *codes, void *scales, kva_stream_t stream);
-/* The values of microscaled rows, y [rows][cols] fp16: rounded to it, so exact
- * but below 2^-24 (largest magnitudes above 65504 become infinite).         */
+/* The values of microscaled rows, y [rows][cols] fp16: rounded to it once,
+ * ties to even: exact but where a value has bits below 2^-24 (magnitudes above
+ * 65504 become infinite).                                                   */
 int kva_mx_dequantize(const void *codes, const void *scales, int32_t rows, int32_t cols, int32_t bits,
                       void *y, kva_stream_t stream);
 /* 4-bit weight rows in the order that the products read, made once per weight:

@@ -68,7 +68,7 @@ __global__ __launch_bounds__(kMxThreads) void mx_dequantize_kernel(MxRows a) {
 // wave takes row l % 32's 16 bytes of block 2 * step + l / 32.  Rows past the
 // last are zeros.  A wave moves four steps (256 values of 32 rows), and with
 // them the dword of scales that each lane needs for those.  Weights are packed
-// once: 12288 x 5120 in 23 us, 2.9 TB/s.
+// once: 12288 x 5120 in 23 us, 2.9 TB/s, where a copy of as much takes 14.
 __global__ __launch_bounds__(kMxThreads) void mx_pack_kernel(MxPack a) {
     const int lane = threadIdx.x & 63;
     const int n_quad = a.cols / 256;

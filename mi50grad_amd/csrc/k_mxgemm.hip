@@ -12,11 +12,15 @@
 // Up to 32 tokens are bound by the weights, 17 bytes of each 32 values: 39 MB at
 // 5120 -> 14336 (a read of memory takes 6.6 us).  mx_stream_kernel takes 8.8 us
 // for one token and 10.5 to 12 for 32 of 8 bits, and 6.3 and 8.3 at 6144 -> 5120
-// (17 MB, 3.0 us), where 160 workgroups do not fill the chip.
+// (17 MB, 3.0 us), where 160 workgroups do not fill the chip.  Each workgroup
+// reads all of X, 32 tokens of 8 bits as many bytes as the weights; and of the 82
+// lines of 128 bytes that a unit of one row tile touches, 32 are for a token's
+// four bytes of scales each.
 //
 // More tokens are bound by the matrix units, or rather by what clock the card's
 // power leaves them.  2048 tokens by mx_gemm_kernel, in us (and PFLOP/s), and a
-// library's plain product of the same types with fp16 outputs:
+// library's plain product of the same types with fp16 outputs, on one box (the
+// first line takes 134 and 109 on a slower one):
 //   5120 -> 14336, norm, RoPE and append   8 bits 127 (2.4)   4 bits 105 (2.9)
 //     plain product                               124                117
 //   6144 -> 5120 and a residual            8 bits  52 (2.5)   4 bits  51
@@ -24,8 +28,9 @@
 // A tile of 256 x 256 starts in 2.3 us (its first stages) and ends in 7, or 13
 // as a head; between, its loads, LDS reads and products are interleaved step by
 // step, so that none of them waits in a row for the others.  Between 33 and some
-// 500 tokens the tiles do not fill the chip, and the latency of a chunk times
-// their number bounds: 181 tokens take 19 us, where the products would take 10.
+// 500 tokens the tiles do not fill the chip: 181 tokens are 168 tiles of 64 x 256
+// for 256 CUs and take 19 to 20 us, some 12 for 20 times 256 values and 7 to start
+// and end as a head, where the products spread over the chip would take 10.
 #include <algorithm>
 #include <iterator>
 #include <type_traits>
@@ -724,15 +729,16 @@ hipError_t launch_mx_stream(const ProjectArgs &a, const MxProduct &m, int n_cu, 
     const int n_rt = (a.n_a + a.n_b + kMxWeightTile - 1) / kMxWeightTile;
     const dim3 block(64 * kMxStreamWaves);
     // Two row tiles a workgroup where one would not fit the chip at once: 5120 ->
-    // 14336 side by side, 9.9 us for one token and 11.4 for 32, by one 11.3 and 14.9.
+    // 14336 side by side, the whole call 11.6 us for one token and 13.8 for 32, by
+    // one 13.4 and 16.9.
     if (n_rt > n_cu) hipLaunchKernelGGL((mx_stream_kernel<BITS, 2, TOK, OUT>), dim3((n_rt + 1) / 2), block, 0, s, a, m);
     else hipLaunchKernelGGL((mx_stream_kernel<BITS, 1, TOK, OUT>), dim3(n_rt), block, 0, s, a, m);
     return hipGetLastError();
 }
 
 // Up to 8 tokens leave the LDS to the weights: more of them on their way.  One
-// token of 5120 -> 14336: 8.5 us, with room for 32 tokens 8.9; 8 and 9 tokens of
-// 8 bits take 9.1 and 10.5.
+// token of 5120 -> 14336 side by side: the whole call 11.6 us, with room for 32
+// tokens 11.9; the product of 8 and 9 tokens of 8 bits takes 9.1 and 10.5.
 template <int BITS>
 hipError_t launch_mx_stream(const ProjectArgs &a, const MxProduct &m, bool heads, int n_cu, hipStream_t s) {
     if (heads) return (a.n_tok <= 8 ? launch_mx_stream<BITS, 8, false> : launch_mx_stream<BITS, 32, false>)(a, m, n_cu, s);
@@ -742,9 +748,9 @@ hipError_t launch_mx_stream(const ProjectArgs &a, const MxProduct &m, bool heads
 // The tiles, and what they take (us): to start and end, and for 256 values of
 // k where a quarter of the CUs have a tile and where all do (the clock falls
 // with the load), measured tile by tile.  Side by side, 2048 tokens of 5120 ->
-// 14336 took 143.5 us by 256 x 256, 153 by 128 x 256 and 155 by a tile of 192 x
-// 256 that is not here; 6144 -> 5120 is 256 tiles of 128 x 320, but 320 of 128 x
-// 256, 64 of them in a second round.
+// 14336 take 134 us by 256 x 256 and 152 by 128 x 256, of 4 bits 109 and 119;
+// 6144 -> 5120 is 256 tiles of 128 x 320, but 320 of 128 x 256, 64 of them in a
+// second round.
 using MxLaunch = hipError_t (*)(const ProjectArgs &, const MxProduct &, hipStream_t);
 struct MxForm {
     int bm, bn;

@@ -8,6 +8,8 @@ multiply: weights in 4 bits, quantised and packed once,
     quantize(w, rows, cols, 4, codes, scales)
     packed = dev.empty(packed_bytes(rows, cols), np.uint8)
     pack_weights(codes, scales, rows, cols, packed)
+    dev.synchronize()
+    codes.free(), scales.free()  # a DeviceArray is held until it is freed
 
 and activations in 8 or 4, per step.  Tensors are integer device addresses or
 ``DeviceArray``s (ctypes takes either); no cache is needed.  The reference has
