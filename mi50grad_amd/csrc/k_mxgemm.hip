@@ -19,7 +19,7 @@
 //
 // More tokens are bound by the matrix units, or rather by what clock the card's
 // power leaves them.  2048 tokens by mx_gemm_kernel, in us (and PFLOP/s), and a
-// library's plain product of the same types with fp16 outputs, on one box (the
+// library's plain product of the same types with fp16 outputs, on one card (the
 // first line takes 134 and 109 on a slower one):
 //   5120 -> 14336, norm, RoPE and append   8 bits 127 (2.4)   4 bits 105 (2.9)
 //     plain product                               124                117
